@@ -48,11 +48,15 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 2
+#define KDA_ABI_VERSION 3
 
 typedef struct CUstream_st *kda_stream_t; /* identical to cudaStream_t */
 
-enum kda_dtype { KDA_DTYPE_BF16 = 0, KDA_DTYPE_F16 = 1 };
+enum kda_dtype {
+  KDA_DTYPE_BF16 = 0,
+  KDA_DTYPE_F16 = 1,
+  KDA_DTYPE_F32 = 2, /* gates of the delta rule only (ABI version 3) */
+};
 
 enum kda_flags {
   /* Reference-exact state update U_c = K_c V_c^T (kernels/kda_kernel.py:294).
@@ -79,6 +83,7 @@ enum kda_status {
   KDA_ERR_WORKSPACE = 5,       /* workspace missing or too small */
   KDA_ERR_CUDA = 6,            /* a CUDA runtime call or launch failed */
   KDA_ERR_DEVICE_TIMEOUT = 64, /* device-side: a bounded wait expired (status word bit) */
+  KDA_ERR_DEVICE_INDEX = 128,  /* device-side: a state index or sequence offset out of range (status word bit) */
 };
 
 typedef struct kda_tensor {
@@ -198,6 +203,81 @@ const char *kda_kernel_name(int32_t kernel);
      clears what must start at zero on its own stream.  Calls that overlap on
      the GPU race on the array: serialise them (one stream, or events). */
 int kda_fwd_sm100_noalloc(const kda_fwd_params *p, kda_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * The gated delta rule (ABI version 3; no counterpart in the reference, whose
+ * scan only adds K^T V).  Per (sequence, value head), S [D, D] fp32 with rows =
+ * key channels, g the log decay (<= 0) and beta the write strength of a token:
+ *
+ *     S' = exp(g_t) S_{t-1}       u_t = beta_t (v_t - S'^T k_t)
+ *     S_t = S' + k_t u_t^T        o_t = scale * S_t^T q_t
+ *
+ * H value heads share Hk query/key heads in groups of H / Hk (value head h uses
+ * query/key head h / (H / Hk)).  g and beta may be bf16, f16 or f32; g below -110
+ * counts as -110 (exp is 0 in fp32 either way).
+ *
+ * Sequences: with cu_seqlens == NULL each of the B batch rows is one sequence
+ * of T tokens.  With cu_seqlens (device [nseq + 1], B == 1) sequence i is
+ * tokens [cu_seqlens[i], cu_seqlens[i + 1]); it may be empty.  Offsets are not
+ * trusted: out-of-order or out-of-range ones are clamped into order and range
+ * and set KDA_ERR_DEVICE_INDEX in *status.  Tokens outside every sequence get
+ * zero outputs and zero gradients, and never reach a result.
+ * -------------------------------------------------------------------- */
+typedef struct kda_delta_params {
+  int32_t B, H, Hk, T, D; /* D 64 or 128; H a multiple of Hk */
+  int32_t dtype;          /* KDA_DTYPE_BF16 or KDA_DTYPE_F16: q, k, v, o, dout, dq, dk, dv */
+  int32_t g_dtype, beta_dtype;
+  int32_t nseq;           /* sequences of cu_seqlens; ignored without it */
+  int32_t cu_int64;       /* cu_seqlens holds int64 (0: int32) */
+  float scale;
+  kda_tensor q, k, v;     /* [B, Hk, T, D], [B, Hk, T, D], [B, H, T, D]; layout rules as above */
+  const void *g, *beta;   /* [B, H, T] by the strides below */
+  int64_t g_stride_b, g_stride_h, g_stride_t;
+  int64_t beta_stride_b, beta_stride_h, beta_stride_t;
+  const void *cu_seqlens;
+  const float *state_in;  /* [sequences, H, D, D] contiguous; NULL -> zeros */
+  /* forward */
+  kda_tensor o;           /* [B, H, T, D] */
+  float *state_out;       /* [sequences, H, D, D]; NULL -> not written */
+  /* backward */
+  kda_tensor dout;        /* dL/do */
+  const float *dstate_out; /* dL/d(state_out); NULL -> zero */
+  kda_tensor dq, dk, dv;
+  void *dg, *dbeta;       /* [B, H, T] contiguous, in g's and beta's dtype */
+  float *dstate_in;       /* dL/d(state_in); NULL -> not written */
+  void *workspace;        /* 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t *status;
+} kda_delta_params;
+
+size_t kda_delta_fwd_workspace_bytes(const kda_delta_params *p);
+size_t kda_delta_bwd_workspace_bytes(const kda_delta_params *p);
+int kda_delta_fwd_sm100(const kda_delta_params *p, kda_stream_t stream);
+int kda_delta_bwd_sm100(const kda_delta_params *p, kda_stream_t stream);
+
+/* One new token for each of N rows: row n reads and updates state slots[n] of
+   the pool in place (slots == NULL: state n) and writes o[n].  A negative slot
+   marks a padded row: its o is zero and no state changes; a slot >= num_states
+   does the same and sets KDA_ERR_DEVICE_INDEX in *status.  Rows that name the
+   same slot are applied in row order.  q, k [N, Hk, D], v, o [N, H, D] with unit
+   inner stride, other strides multiples of 8, 16-byte aligned; each state [D, D]
+   contiguous fp32, 16-byte aligned, strides multiples of 4. */
+typedef struct kda_delta_step_params {
+  int32_t N, H, Hk, D, num_states;
+  int32_t dtype, g_dtype, beta_dtype;
+  float scale;
+  const void *q, *k, *v;
+  void *o;
+  const void *g, *beta; /* [N, H] */
+  int64_t q_stride_n, q_stride_h, k_stride_n, k_stride_h, v_stride_n, v_stride_h, o_stride_n, o_stride_h;
+  int64_t g_stride_n, g_stride_h, beta_stride_n, beta_stride_h;
+  float *state;
+  int64_t state_stride_n, state_stride_h;
+  const void *slots;    /* [N] or NULL */
+  int32_t slots_int64;  /* slots holds int64 (0: int32) */
+  int32_t *status;
+} kda_delta_step_params;
+int kda_delta_step_sm100(const kda_delta_step_params *p, kda_stream_t stream);
 
 #ifdef __cplusplus
 } /* extern "C" */

@@ -7,12 +7,17 @@ output_final_state) -> (y, final_state)``
     the extended scan (initial / final state, tensor decay), differentiable.
 ``kda_chunked_scan(q, k, v, gate, decay, chunk_size, use_triton) -> y``
     SimpleTrain's own dispatch signature (``kernels/kda_kernel.py:303``).
+``gated_delta_chunk(q, k, v, g, beta, scale, initial_state, cu_seqlens,
+output_final_state) -> (o, final_state)``
+    the gated delta rule over sequences (padded or packed), differentiable.
+``gated_delta_step(q, k, v, g, beta, state, state_indices, scale) -> o``
+    the same rule for one new token a row, on a pool of states in place.
 ``install()``
     make ``kernels.kda_kernel`` resolve to the drop-in module.
 ``device_status()``
     read device-side error bits (bounded waits that expired).
 """
-__all__ = ["kda_chunk", "kda_chunked_scan", "install", "device_status"]
+__all__ = ["kda_chunk", "kda_chunked_scan", "gated_delta_chunk", "gated_delta_step", "install", "device_status"]
 
 
 def __getattr__(name):
@@ -21,6 +26,9 @@ def __getattr__(name):
     if name in ("kda_chunk", "device_status"):
         from . import ops
         return getattr(ops, name)
+    if name in ("gated_delta_chunk", "gated_delta_step"):
+        from . import delta
+        return getattr(delta, name)
     if name in ("install", "kda_chunked_scan"):
         from . import kda_kernel
         return getattr(kda_kernel, name)

@@ -8,15 +8,16 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_double, c_int32, c_int64, c_size_t, c_uint32, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 # KDA_B200_LIB_DIR selects another build of both libraries (default: in-tree _lib/)
 LIB_DIR = os.environ.get("KDA_B200_LIB_DIR") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libkda_sm100.so")
 
 KDA_DTYPE_BF16 = 0
 KDA_DTYPE_F16 = 1
+KDA_DTYPE_F32 = 2
 KDA_FLAG_LITERAL = 1 << 0
 KDA_FLAG_PER_STEP = 1 << 1
 
@@ -28,14 +29,18 @@ KDA_ERR_BAD_LAYOUT = 4
 KDA_ERR_WORKSPACE = 5
 KDA_ERR_CUDA = 6
 KDA_ERR_DEVICE_TIMEOUT = 64
+KDA_ERR_DEVICE_INDEX = 128
 
 EXPORTED = (
     "kda_fwd_sm100", "kda_bwd_sm100", "kda_fwd_workspace_bytes", "kda_bwd_workspace_bytes",
     "kda_status_string", "kda_abi_version", "kda_launch_count", "kda_fwd_sm100_noalloc",
     "kda_trace_start", "kda_trace_read", "kda_trace_stop", "kda_kernel_name",
+    "kda_delta_fwd_sm100", "kda_delta_bwd_sm100", "kda_delta_fwd_workspace_bytes", "kda_delta_bwd_workspace_bytes",
+    "kda_delta_step_sm100",
     # include/st_fused_ops.h
     "st_silu_mul_fwd", "st_silu_mul_bwd", "st_rmsnorm_residual_fwd", "st_rmsnorm_residual_bwd",
     "st_rmsnorm_residual_bwd_scratch", "st_cross_entropy_fwd", "st_cross_entropy_bwd",
+    "st_token_logprobs_fwd", "st_token_logprobs_bwd",
 )
 NOALLOC_SCRATCH_BYTES = 32 << 20
 
@@ -70,6 +75,35 @@ class KdaBwdParams(ctypes.Structure):
         ("dstate_in", c_void_p), ("ddecay", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),
         ("status", c_void_p),
+    ]
+
+
+class KdaDeltaParams(ctypes.Structure):
+    _fields_ = [
+        ("B", c_int32), ("H", c_int32), ("Hk", c_int32), ("T", c_int32), ("D", c_int32),
+        ("dtype", c_int32), ("g_dtype", c_int32), ("beta_dtype", c_int32), ("nseq", c_int32), ("cu_int64", c_int32),
+        ("scale", c_float),
+        ("q", KdaTensor), ("k", KdaTensor), ("v", KdaTensor), ("g", c_void_p), ("beta", c_void_p),
+        ("g_stride_b", c_int64), ("g_stride_h", c_int64), ("g_stride_t", c_int64),
+        ("beta_stride_b", c_int64), ("beta_stride_h", c_int64), ("beta_stride_t", c_int64),
+        ("cu_seqlens", c_void_p), ("state_in", c_void_p),
+        ("o", KdaTensor), ("state_out", c_void_p),
+        ("dout", KdaTensor), ("dstate_out", c_void_p),
+        ("dq", KdaTensor), ("dk", KdaTensor), ("dv", KdaTensor), ("dg", c_void_p), ("dbeta", c_void_p),
+        ("dstate_in", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("status", c_void_p),
+    ]
+
+
+class KdaDeltaStepParams(ctypes.Structure):
+    _fields_ = [
+        ("N", c_int32), ("H", c_int32), ("Hk", c_int32), ("D", c_int32), ("num_states", c_int32),
+        ("dtype", c_int32), ("g_dtype", c_int32), ("beta_dtype", c_int32), ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("o", c_void_p), ("g", c_void_p), ("beta", c_void_p),
+        ("q_stride_n", c_int64), ("q_stride_h", c_int64), ("k_stride_n", c_int64), ("k_stride_h", c_int64),
+        ("v_stride_n", c_int64), ("v_stride_h", c_int64), ("o_stride_n", c_int64), ("o_stride_h", c_int64),
+        ("g_stride_n", c_int64), ("g_stride_h", c_int64), ("beta_stride_n", c_int64), ("beta_stride_h", c_int64),
+        ("state", c_void_p), ("state_stride_n", c_int64), ("state_stride_h", c_int64),
+        ("slots", c_void_p), ("slots_int64", c_int32), ("status", c_void_p),
     ]
 
 
@@ -108,6 +142,14 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
         fn.restype = c_int32
     lib.kda_kernel_name.argtypes = [c_int32]
     lib.kda_kernel_name.restype = c_char_p
+    for fn in (lib.kda_delta_fwd_sm100, lib.kda_delta_bwd_sm100):
+        fn.argtypes = [POINTER(KdaDeltaParams), c_void_p]
+        fn.restype = c_int32
+    for fn in (lib.kda_delta_fwd_workspace_bytes, lib.kda_delta_bwd_workspace_bytes):
+        fn.argtypes = [POINTER(KdaDeltaParams)]
+        fn.restype = c_size_t
+    lib.kda_delta_step_sm100.argtypes = [POINTER(KdaDeltaStepParams), c_void_p]
+    lib.kda_delta_step_sm100.restype = c_int32
     ver = lib.kda_abi_version()
     if ver != ABI_VERSION:
         raise ImportError(f"KDA library ABI version {ver} != binding version {ABI_VERSION}; rebuild")

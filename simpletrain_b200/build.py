@@ -84,7 +84,7 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> str:
 def _hash() -> str:
     h = hashlib.sha256()
     files = sources() + sorted(glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh")))
-    files.append(os.path.join(ROOT, "include", "kda_sm100.h"))
+    files += [os.path.join(ROOT, "include", n) for n in ("kda_sm100.h", "st_fused_ops.h")]
     for f in files:
         h.update(f.encode())
         with open(f, "rb") as fh:

@@ -334,6 +334,7 @@ const char *kda_status_string(int32_t s) {
     case KDA_ERR_WORKSPACE: return "workspace missing or too small";
     case KDA_ERR_CUDA: return "CUDA launch or runtime error";
     case KDA_ERR_DEVICE_TIMEOUT: return "device-side bounded wait expired";
+    case KDA_ERR_DEVICE_INDEX: return "a state index or sequence offset was out of range";
     default: return "unknown kda status";
   }
 }

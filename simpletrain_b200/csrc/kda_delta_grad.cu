@@ -1,0 +1,461 @@
+// The gated delta rule's gradients of q, k, g and beta, chunk by chunk, and its C-ABI
+// entry points.
+//
+// Mathematics, for one chunk and head with the state S before it, the gradient dS of the
+// state after it, U = T X, dX (the reverse scan's), e_ij = e^{gamma_i - gamma_j},
+// w_i = e^{gamma_63 - gamma_i}, G_i = e^{gamma_i}:
+//   M_ij = -(dX U^T)_ij beta_i e_ij (i > j)      (gradient of k_i.k_j)
+//   N_ij = scale (dO U^T)_ij e_ij (i >= j)       (gradient of q_i.k_j)
+//   dQ = N K + scale G (dO S^T)
+//   dK = M K + M^T K + N^T Q - G beta (dX S^T) + w (U dS^T)
+//   dbeta_i = dX_i.v_i - G_i t_i - sum_j (dX U^T)_ij e_ij k_i.k_j,   t_i = k_i.(dX S^T)_i
+// The gradient of gamma_i, row by row, is what those terms give through their e^gamma
+// factors; with y_i = w_i k_i.(U dS^T)_i,
+//   dgamma_i = q_i.dq_i + k_i.(M K)_i - k_i.(M^T K + N^T Q)_i - G_i beta_i t_i
+//   dg_t = sum_{i >= t} dgamma_i + sum_{j < t} y_j + e^{gamma_63} <S, dS>
+// (the y_j enter dgamma_j with a minus and dgamma_63 with a plus; summed this way nothing
+// cancels).
+//
+// One CTA per (chunk, query/key head) walks the value heads that share the head and sums
+// their dq and dk in registers, in order: no atomics, the result does not depend on the
+// launch.  Six products a head, all of them on tiles that are loaded once; the state and
+// its gradient take turns in one 64 KB buffer.  One CTA fills an SM's shared memory.
+#include "kda_delta_tc.cuh"
+
+namespace kda {
+namespace delta {
+namespace {
+
+template <int D>
+struct GradSmem {
+  static constexpr uint32_t kTile = 128 * D * 2;
+  static constexpr uint32_t KQ = 0, AH = KQ + kTile, AL = AH + kTile;  // [dX; dO] hi, lo (dO's lo rows: zeros)
+  static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U: per 64 columns [64 x 64] hi, lo
+  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S or dS: per 64 columns [D x 64] hi, lo
+  static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
+};
+
+template <int D, bool BF>
+__global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
+  using L = GradSmem<D>;
+  constexpr int NS = D / 64, W = D / 2;  // W: columns of a D-wide row that a thread owns
+  constexpr uint32_t tG1 = 0, tG2 = 64, tG5 = 128, tG6 = 256, tG3 = 0, tG4 = 384;
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ Ctl ctl;
+  __shared__ __align__(16) float gam[64];
+  __shared__ float sm_q[2][64], sm_k[2][64], sm_t[2][64], sm_y[2][64], sm_xv[2][64], sm_rs[2][64], sm_dot[8];
+  int64_t b, t0;
+  int rows;
+  if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
+  const int tid = threadIdx.x, row = tid & 127, half = tid >> 7, r64 = row & 63;
+  const bool upper = row >= 64;
+  const int hk = blockIdx.y, G_ = a.p.H / a.p.Hk;
+  const uint32_t sb = smem_u32(smem), lane_base = (uint32_t)((tid >> 5) & 3) << 21;
+  load_rows<D>(sb + L::KQ, 0, 16384, static_cast<const uint16_t *>(a.p.k.data) + b * a.p.k.stride_b + hk * a.p.k.stride_h + t0 * a.p.k.stride_t,
+               a.p.k.stride_t, rows);
+  load_rows<D>(sb + L::KQ, 64, 16384, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
+               a.p.q.stride_t, rows);
+  const uint32_t tmem = cta_begin(ctl, 512);
+  const uint32_t lane_t = tmem + lane_base;
+  uint32_t ph = 0, ph_load = 0;
+  float acc[W];
+#pragma unroll
+  for (int j = 0; j < W; ++j) acc[j] = 0.f;
+  // this thread's row of the [K; Q] tile against a D-wide row of values, W columns of it
+  auto kq_chunk = [&](int c) { return ld_shared_v4(sb + L::KQ + ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c)); };
+
+  for (int hh = 0; hh < G_; ++hh) {
+    const int h = hk * G_ + hh;
+    const size_t ch = (size_t)blockIdx.x * a.p.H + h;
+    const char *gS = a.w.S + ch * NS * (size_t)(D * 256), *gD = a.w.dS + ch * NS * (size_t)(D * 256);
+    if (tid == 0) {
+      const uint32_t bar = smem_u32(&ctl.load_bar);
+      mbar_arrive_expect_tx(bar, NS * (16384 + 16384 + D * 256));
+      for (int s = 0; s < NS; ++s) {
+        const char *x = a.w.dX + (ch * NS + s) * (size_t)16384;
+        bulk_load(sb + L::AH + s * 16384, x, 8192, bar);
+        bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, bar);
+      }
+      bulk_load(sb + L::U, a.w.U + ch * NS * (size_t)16384, NS * 16384, bar);
+      bulk_load(sb + L::S, gS, NS * D * 256, bar);
+    }
+    load_rows<D>(sb + L::AH, 64, 16384, static_cast<const uint16_t *>(a.p.dout.data) + b * a.p.dout.stride_b + h * a.p.dout.stride_h + t0 * a.p.dout.stride_t,
+                 a.p.dout.stride_t, rows);
+    if (upper)
+#pragma unroll
+      for (int c = 0; c < W / 8; ++c)
+        sts(sb + L::AL + ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c), make_uint4(0, 0, 0, 0));
+    if (tid < 64) gam[tid] = a.w.gam[ch * 64 + tid];
+    const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
+    const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
+    cp_async_wait();
+    publish();
+    mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
+    ph_load ^= 1;
+    __syncwarp();
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t id64 = idesc_f16(128, 64, BF, false, false), idD = idesc_f16(128, D, BF, false, false);
+      issue(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, D / 16, id64, false);
+      const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384}, uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
+      const KMajor sh{sb + L::S, D * 256}, sl{sb + L::S + D * 128, D * 256};
+      issue(tmem + tG2, ah, uh, D / 16, id64, false);
+      issue(tmem + tG2, ah, ul, D / 16, id64, true);
+      issue(tmem + tG2, al, uh, D / 16, id64, true);
+      issue(tmem + tG5, ah, sh, D / 16, idD, false);
+      issue(tmem + tG5, ah, sl, D / 16, idD, true);
+      issue(tmem + tG5, al, sh, D / 16, idD, true);
+      mma_commit(smem_u32(&ctl.mma_bar));
+    }
+    // meanwhile: <S, dS> (same place in both images), and dX . v
+    float dot = 0.f;
+    for (int e = tid; e < NS * D * 8; e += kThreads) {
+      const int s = e / (D * 8), o = e % (D * 8) * 16;
+      const uint32_t off = s * (D * 256) + o;
+      float x[8], y[8], z[8];
+      unpack8<BF>(ld_shared_v4(sb + L::S + off), x);
+      unpack8<BF>(ld_shared_v4(sb + L::S + off + D * 128), y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] += y[j];
+      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off), y);
+      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off + D * 128), z);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j] + z[j], dot);
+    }
+    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+    if ((tid & 31) == 0) sm_dot[tid >> 5] = dot;
+    if (!upper) {
+      float xv = 0.f;
+      if (r64 < rows) {
+        const uint16_t *vp = static_cast<const uint16_t *>(a.p.v.data) + b * a.p.v.stride_b + h * a.p.v.stride_h + (t0 + r64) * a.p.v.stride_t + half * W;
+#pragma unroll
+        for (int c = 0; c < W / 8; ++c) {
+          const uint32_t at = ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c);
+          float x[8], y[8], v[8];
+          unpack8<BF>(ld_shared_v4(sb + L::AH + at), x);
+          unpack8<BF>(ld_shared_v4(sb + L::AL + at), y);
+          unpack8<BF>(*reinterpret_cast<const uint4 *>(vp + 8 * c), v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
+        }
+      }
+      sm_xv[half][r64] = xv;
+    }
+    wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
+    // M, N over the dX / dO tiles (all their products are done); every thread is past its reads of them
+    float x[32];
+    {
+      float y[32];
+      tmem_ld32(lane_t + tG1 + 32 * half, x);
+      tmem_ld32(lane_t + tG2 + 32 * half, y);
+      float rs = 0.f;
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        const int col = 32 * half + j;
+        const float e = ex2f((gi - gam[col]) * kLog2e);
+        if (!upper) {
+          const float m = col < r64 ? -y[j] * e : 0.f;
+          rs = col < r64 ? fmaf(m, x[j], rs) : rs;
+          x[j] = m * bi;
+        } else {
+          x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
+        }
+      }
+      if (!upper) sm_rs[half][r64] = rs;
+    }
+    publish();
+    if (tid == 0) {
+      const uint32_t bar = smem_u32(&ctl.load_bar);
+      mbar_arrive_expect_tx(bar, NS * D * 256);
+      bulk_load(sb + L::S, gD, NS * D * 256, bar);  // the state's products and dot are done
+    }
+    store_split32<BF>(sb + L::MN, sb + L::MN + 16384, row, half, x);
+    publish();
+    if (tid == 0) {
+      tc_fence_after();
+      const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
+      const MNMajor kq{sb + L::KQ, 16384};
+      issue(tmem + tG3, KMajor{sb + L::MN, 0}, kq, 4, id3, false);
+      issue(tmem + tG3, KMajor{sb + L::MN + 16384, 0}, kq, 4, id3, true);
+      // 64 rows (k tokens); the other 64 are not used
+      issue(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, 8, id4, false);
+      issue(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, 8, id4, true);
+      mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
+      const uint32_t id6 = idesc_f16(128, D, BF, false, false);
+      const KMajor uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
+      const KMajor dh{sb + L::S, D * 256}, dl{sb + L::S + D * 128, D * 256};
+      issue(tmem + tG6, uh, dh, D / 16, id6, false);
+      issue(tmem + tG6, uh, dl, D / 16, id6, true);
+      issue(tmem + tG6, ul, dh, D / 16, id6, true);
+      mma_commit(smem_u32(&ctl.mma_bar));
+    }
+    ph_load ^= 1;
+    // meanwhile the terms through the state
+    float dq_dot = 0.f, t_dot = 0.f, k_dot = 0.f, y_dot = 0.f;
+#pragma unroll
+    for (int c0 = 0; c0 < W; c0 += 32) {
+      tmem_ld32(lane_t + tG5 + half * W + c0, x);
+      const float f = upper ? a.p.scale * Gi : -Gi * bi;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float k[8];
+        unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float v = f * x[8 * c + j];
+          t_dot = fmaf(k[j], upper ? v : x[8 * c + j], t_dot);
+          acc[c0 + 8 * c + j] += v;
+        }
+      }
+    }
+    wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
+#pragma unroll
+    for (int c0 = 0; c0 < W; c0 += 32) {
+      tmem_ld32(lane_t + tG3 + half * W + c0, x);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float k[8];
+        unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          dq_dot = fmaf(k[j], x[8 * c + j], dq_dot);
+          acc[c0 + 8 * c + j] += x[8 * c + j];
+        }
+      }
+      if (!upper) {
+        tmem_ld32(lane_t + tG4 + half * W + c0, x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float k[8];
+          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            k_dot = fmaf(k[j], x[8 * c + j], k_dot);
+            acc[c0 + 8 * c + j] += x[8 * c + j];
+          }
+        }
+        tmem_ld32(lane_t + tG6 + half * W + c0, x);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float k[8];
+          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float v = wi * x[8 * c + j];
+            y_dot = fmaf(k[j], v, y_dot);
+            acc[c0 + 8 * c + j] += v;
+          }
+        }
+      }
+    }
+    if (upper) {
+      sm_q[half][r64] = dq_dot + t_dot;
+    } else {
+      sm_k[half][r64] = dq_dot - k_dot;  // k.(M K) - k.(M^T K + N^T Q)
+      sm_t[half][r64] = t_dot;
+      sm_y[half][r64] = y_dot;
+    }
+    __syncthreads();
+    if (tid < 32) {
+      float f[2], y[2];
+      const float last = exp_fast(gam[63]);
+      float sd = 0.f;
+      for (int w = 0; w < 8; ++w) sd += sm_dot[w];
+      sd *= last;
+      for (int j = 0; j < 2; ++j) {
+        const int i = 2 * tid + j;
+        const float G = exp_fast(gam[i]), be = a.w.beta[ch * 64 + i], t = sm_t[0][i] + sm_t[1][i];
+        f[j] = (sm_q[0][i] + sm_q[1][i]) + (sm_k[0][i] + sm_k[1][i]) - G * be * t;
+        y[j] = sm_y[0][i] + sm_y[1][i];
+        if (i < rows)
+          store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype,
+                     (sm_xv[0][i] + sm_xv[1][i]) - G * t + (sm_rs[0][i] + sm_rs[1][i]));
+      }
+      // suffix sums of f, exclusive prefix sums of y
+      float sf = f[0] + f[1], py = y[0] + y[1];
+      for (int o = 1; o < 32; o <<= 1) {
+        const float u = __shfl_down_sync(0xffffffffu, sf, o), v = __shfl_up_sync(0xffffffffu, py, o);
+        if (tid + o < 32) sf += u;
+        if (tid >= o) py += v;
+      }
+      const float next = __shfl_down_sync(0xffffffffu, sf, 1), prev = __shfl_up_sync(0xffffffffu, py, 1);
+      const float s1 = f[1] + (tid < 31 ? next : 0.f), p0 = tid > 0 ? prev : 0.f;
+      if (2 * tid < rows) store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid, a.p.g_dtype, (f[0] + s1) + p0 + sd);
+      if (2 * tid + 1 < rows)
+        store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid + 1, a.p.g_dtype, s1 + (p0 + y[0]) + sd);
+    }
+    __syncthreads();
+  }
+  if (r64 < rows) {
+    const kda_tensor &o = upper ? a.p.dq : a.p.dk;
+    uint16_t *dst = static_cast<uint16_t *>(o.data) + b * o.stride_b + hk * o.stride_h + (t0 + r64) * o.stride_t + half * W;
+#pragma unroll
+    for (int c0 = 0; c0 < W; c0 += 32) {
+      float x[32];
+#pragma unroll
+      for (int j = 0; j < 32; ++j) x[j] = acc[c0 + j];
+      store_row32<BF>(dst + c0, x);
+    }
+  }
+  cta_end(tmem, 512);
+}
+
+template <int D, bool BF>
+cudaError_t run_grad(const Args &a, cudaStream_t st) {
+  constexpr uint32_t smem = GradSmem<D>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(grad_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  grad_kernel<D, BF><<<dim3((unsigned)a.max_chunks, (unsigned)a.p.Hk), kThreads, smem, st>>>(a);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_grad(const Args &a, cudaStream_t st) {
+  if (a.max_chunks == 0) return cudaSuccess;
+  const bool bf = a.p.dtype == KDA_DTYPE_BF16;
+  if (a.p.D == 64) return bf ? run_grad<64, true>(a, st) : run_grad<64, false>(a, st);
+  return bf ? run_grad<128, true>(a, st) : run_grad<128, false>(a, st);
+}
+
+}  // namespace delta
+}  // namespace kda
+
+// ------------------------------------------------------------------- C ABI --
+namespace {
+
+using kda::delta::Args;
+
+bool gate_ok(int32_t d) { return d == KDA_DTYPE_BF16 || d == KDA_DTYPE_F16 || d == KDA_DTYPE_F32; }
+
+int check_sizes(const kda_delta_params *p) {
+  if (p == nullptr) return KDA_ERR_NULL_ARGUMENT;
+  if (p->B < 0 || p->H < 0 || p->Hk < 0 || p->T < 0) return KDA_ERR_BAD_SHAPE;
+  if (p->D != 64 && p->D != 128) return KDA_ERR_UNSUPPORTED;
+  if (p->dtype != KDA_DTYPE_BF16 && p->dtype != KDA_DTYPE_F16) return KDA_ERR_UNSUPPORTED;
+  if (!gate_ok(p->g_dtype) || !gate_ok(p->beta_dtype)) return KDA_ERR_UNSUPPORTED;
+  if (p->B > 0 && p->H > 0 && (p->Hk == 0 || p->H % p->Hk)) return KDA_ERR_BAD_SHAPE;
+  if (p->cu_seqlens != nullptr && (p->B != 1 || p->nseq < 0)) return KDA_ERR_BAD_SHAPE;
+  if (p->H > 65535) return KDA_ERR_BAD_SHAPE;  // a grid dimension
+  const int64_t nseq = p->cu_seqlens != nullptr ? (int64_t)p->nseq + 1 : p->B;
+  if (nseq * p->H * 2 > 0x7fffffff) return KDA_ERR_BAD_SHAPE;
+  const int64_t chunks = p->cu_seqlens != nullptr ? (int64_t)p->T / 64 + p->nseq : (int64_t)p->B * (((int64_t)p->T + 63) / 64);
+  if (chunks > 0x7fffffff) return KDA_ERR_BAD_SHAPE;
+  return KDA_OK;
+}
+
+size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Sizes and workspace regions; returns the bytes needed (p->workspace may be NULL).
+size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
+  a->p = *p;
+  const bool packed = p->cu_seqlens != nullptr;
+  a->nseq = packed ? p->nseq : p->B;
+  a->per_seq = packed ? 0 : (int)(((int64_t)p->T + 63) / 64);
+  a->max_chunks = packed ? p->T / 64 + p->nseq : p->B * a->per_seq;
+  const size_t cells = (size_t)a->max_chunks * p->H, slices = cells * (p->D / 64);
+  char *base = static_cast<char *>(p->workspace);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char *r = base == nullptr ? nullptr : base + at;
+    at += align256(bytes);
+    return r;
+  };
+  a->w = {};
+  if (packed) {
+    a->w.bound = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
+    a->w.first = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
+  }
+  a->w.gam = reinterpret_cast<float *>(take(cells * 256));
+  a->w.beta = reinterpret_cast<float *>(take(cells * 256));
+  a->w.T = take(cells * kda::delta::kImgT);
+  if (backward) {
+    a->w.S = take(slices * p->D * 256);
+    a->w.dS = take(slices * p->D * 256);
+    a->w.U = take(slices * 16384);
+    a->w.dX = take(slices * 16384);
+  }
+  return at;
+}
+
+int check_view(const kda_tensor &t) {
+  if (t.data == nullptr) return KDA_ERR_NULL_ARGUMENT;
+  if (t.stride_d != 1 || (reinterpret_cast<uintptr_t>(t.data) & 15u)) return KDA_ERR_BAD_LAYOUT;
+  if ((t.stride_b % 8) || (t.stride_h % 8) || (t.stride_t % 8)) return KDA_ERR_BAD_LAYOUT;
+  return KDA_OK;
+}
+
+bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; }
+
+int check_common(const kda_delta_params *p, bool tokens) {
+  if (tokens) {
+    for (const kda_tensor *t : {&p->q, &p->k, &p->v})
+      if (const int rc = check_view(*t)) return rc;
+    if (p->g == nullptr || p->beta == nullptr) return KDA_ERR_NULL_ARGUMENT;
+  }
+  if (misaligned(p->state_in)) return KDA_ERR_BAD_LAYOUT;
+  return KDA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kda_delta_fwd_workspace_bytes(const kda_delta_params *p) {
+  Args a;
+  if (check_sizes(p) != KDA_OK) return 0;
+  return lay_out(p, false, &a);
+}
+
+size_t kda_delta_bwd_workspace_bytes(const kda_delta_params *p) {
+  Args a;
+  if (check_sizes(p) != KDA_OK) return 0;
+  return lay_out(p, true, &a);
+}
+
+int kda_delta_fwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
+  int rc = check_sizes(p);
+  if (rc != KDA_OK) return rc;
+  if (p->B == 0 || p->H == 0) return KDA_OK;
+  const bool tokens = p->T > 0;
+  if ((rc = check_common(p, tokens)) != KDA_OK) return rc;
+  if (tokens && (rc = check_view(p->o)) != KDA_OK) return rc;
+  if (misaligned(p->state_out)) return KDA_ERR_BAD_LAYOUT;
+  Args a;
+  const size_t need = lay_out(p, false, &a);
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
+    return KDA_ERR_WORKSPACE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = p->cu_seqlens != nullptr ? kda::delta::launch_plan(a, st) : cudaSuccess;
+  if (e == cudaSuccess) e = kda::delta::launch_prep(a, st);
+  if (e == cudaSuccess) e = kda::delta::launch_scan(a, false, st);
+  return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
+}
+
+int kda_delta_bwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
+  int rc = check_sizes(p);
+  if (rc != KDA_OK) return rc;
+  if (p->B == 0 || p->H == 0) return KDA_OK;
+  const bool tokens = p->T > 0;
+  if ((rc = check_common(p, tokens)) != KDA_OK) return rc;
+  if (tokens) {
+    for (const kda_tensor *t : {&p->dout, &p->dq, &p->dk, &p->dv})
+      if ((rc = check_view(*t)) != KDA_OK) return rc;
+    if (p->dg == nullptr || p->dbeta == nullptr) return KDA_ERR_NULL_ARGUMENT;
+  }
+  if (misaligned(p->dstate_out) || misaligned(p->dstate_in)) return KDA_ERR_BAD_LAYOUT;
+  Args a;
+  const size_t need = lay_out(p, true, &a);
+  if (need > 0 && (p->workspace == nullptr || p->workspace_bytes < need || (reinterpret_cast<uintptr_t>(p->workspace) & 255u)))
+    return KDA_ERR_WORKSPACE;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e = p->cu_seqlens != nullptr ? kda::delta::launch_plan(a, st) : cudaSuccess;
+  if (e == cudaSuccess) e = kda::delta::launch_prep(a, st);
+  if (e == cudaSuccess) e = kda::delta::launch_scan(a, true, st);
+  if (e == cudaSuccess) e = kda::delta::launch_rev(a, st);
+  if (e == cudaSuccess) e = kda::delta::launch_grad(a, st);
+  return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
+}
+
+}  // extern "C"

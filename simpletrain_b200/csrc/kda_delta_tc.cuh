@@ -1,0 +1,285 @@
+// Pieces shared by the gated delta rule's kernels: arguments, sequence and chunk
+// bookkeeping, tile loads, the two-term operand split, and MMA issue.
+//
+// Every kernel is one CTA of 256 threads that alternates between tcgen05 products
+// issued by one thread and epilogues by all: thread t owns tensor-memory lane t % 128
+// (an output row) and one half (t / 128) of the columns, so per-token factors are
+// per-thread scalars.  Products have M = 128: the 64 rows of a chunk's k tile are
+// stacked on the 64 of its q tile (and T on P T, dX on dO), or, for the state, rows
+// are the key channels.
+//
+// Two-term operands.  A value x that is not an input is handed to the tensor cores as
+// hi + lo, hi = round16(x), lo = round16(x - hi): 16 bits of mantissa in bf16, 22 in
+// fp16, against 8 and 11 in one term.  A product of two such values is issued as
+// hi*hi + hi*lo + lo*hi into one fp32 accumulator.  With single terms the state,
+// which feeds on itself chunk after chunk, was 2.5e-3 from the 64-bit recurrence;
+// with two it is 4e-6, and the tensor pipe is not what bounds these kernels.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/kda_sm100.h"
+#include "kda_internal.h"
+#include "tc_common.cuh"
+
+namespace kda {
+namespace delta {
+
+using namespace kda::tc;
+
+constexpr int kChunk = 64;
+constexpr int kThreads = 256;
+constexpr int kImgT = 32768;  // T / PT image of a (chunk, head): [128 x 64] hi, then lo
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
+
+// Workspace regions (device pointers) of one call.
+struct Work {
+  int *bound;      // [nseq + 1] sequence offsets, clamped into order and range (packed sequences only)
+  int *first;      // [nseq + 1] first chunk of each sequence
+  float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
+  float *beta;     // [chunk][H][64]
+  char *T;         // [chunk][H] images of T over P T
+  char *S, *dS;    // [chunk][H][D / 64] images of the state before / the state gradient after the chunk: [D x 64] hi, lo
+  char *U, *dX;    // [chunk][H][D / 64] images of the chunk's u rows / their gradient before T^T: [64 x 64] hi, lo
+};
+
+struct Args {
+  kda_delta_params p;
+  Work w;
+  int nseq;       // sequences (batch rows, or those of cu_seqlens)
+  int per_seq;    // chunks of a batch row (without cu_seqlens)
+  int max_chunks; // upper bound of the chunks over all sequences
+};
+
+struct Seq {
+  int64_t b, t0;  // batch row and first token
+  int len, chunk0;
+};
+
+__device__ __forceinline__ Seq get_seq(const Args &a, int n) {
+  if (a.p.cu_seqlens == nullptr) return {n, 0, a.p.T, n * a.per_seq};
+  const int lo = a.w.bound[n];
+  return {0, lo, a.w.bound[n + 1] - lo, a.w.first[n]};
+}
+
+// Chunk u as (sequence, first token in it, rows); false past the last chunk.
+__device__ __forceinline__ bool get_chunk(const Args &a, int u, int64_t *b, int64_t *t, int *rows) {
+  if (a.p.cu_seqlens == nullptr) {
+    const int n = u / a.per_seq, c = u - n * a.per_seq;
+    *b = n;
+    *t = (int64_t)c * kChunk;
+    *rows = min(kChunk, a.p.T - c * kChunk);
+    return true;
+  }
+  if (u >= a.w.first[a.nseq]) return false;
+  int lo = 0, hi = a.nseq;  // first[lo] <= u < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.w.first[mid] <= u) lo = mid; else hi = mid;
+  }
+  const int c = u - a.w.first[lo], s0 = a.w.bound[lo];
+  *b = 0;
+  *t = (int64_t)s0 + (int64_t)c * kChunk;
+  *rows = min(kChunk, a.w.bound[lo + 1] - s0 - c * kChunk);
+  return true;
+}
+
+__device__ __forceinline__ float ex2f(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float exp_fast(float x) { return ex2f(x * kLog2e); }
+
+__device__ __forceinline__ float load_gate(const void *p, int64_t i, int dtype) {
+  if (dtype == KDA_DTYPE_F32) return static_cast<const float *>(p)[i];
+  return unpack2((uint32_t) static_cast<const uint16_t *>(p)[i], dtype == KDA_DTYPE_BF16).x;
+}
+__device__ __forceinline__ void store_gate(void *p, int64_t i, int dtype, float v) {
+  if (dtype == KDA_DTYPE_F32)
+    static_cast<float *>(p)[i] = v;
+  else
+    static_cast<uint16_t *>(p)[i] = (uint16_t)(pack2(v, 0.f, dtype == KDA_DTYPE_BF16) & 0xffffu);
+}
+
+// ------------------------------------------------------------- tile loads --
+// 16 bytes to shared memory, zeros where `live` is false (the source is not read then)
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// `rows` live rows (of 64) of a [T, D] view at `base` into tile rows [row0, row0 + 64)
+// of D/64 swizzled [128 x 64] blocks `block` bytes apart; rows past `rows` become zeros.
+template <int D>
+__device__ __forceinline__ void load_rows(uint32_t tile, int row0, uint32_t block, const uint16_t *base, int64_t stride_t,
+                                          int rows) {
+  constexpr int P = D / 8;
+#pragma unroll
+  for (int i = 0; i < 64 * P / kThreads; ++i) {
+    const int p = threadIdx.x + i * kThreads, r = p / P, c = p % P, tr = row0 + r;
+    const bool live = r < rows;
+    cp_async16(tile + (c >> 3) * block + tr * 128 + (((c & 7) ^ (tr & 7)) << 4), base + (live ? r * stride_t : 0) + c * 8,
+               live);
+  }
+}
+
+// contiguous bytes global -> shared, counted on an mbarrier (sizes and addresses are multiples of 16)
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
+               "r"(src), "r"(bytes)
+               : "memory");
+}
+
+// ------------------------------------------------------------ hi/lo split --
+template <bool BF>
+__device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+  hi = pack2(a, b, BF);
+  const float2 h = unpack2(hi, BF);
+  lo = pack2(a - h.x, b - h.y, BF);
+}
+
+// Eight consecutive columns (16-byte chunk c16) of row `row` of a swizzled tile, as hi and lo.
+template <bool BF>
+__device__ __forceinline__ void split8(const float *x, uint4 &hi, uint4 &lo) {
+  split2<BF>(x[0], x[1], hi.x, lo.x);
+  split2<BF>(x[2], x[3], hi.y, lo.y);
+  split2<BF>(x[4], x[5], hi.z, lo.z);
+  split2<BF>(x[6], x[7], hi.w, lo.w);
+}
+__device__ __forceinline__ uint32_t chunk_at(int row, int c16) {
+  return (uint32_t)(row * 128 + (((c16 ^ row) & 7) << 4));
+}
+__device__ __forceinline__ void sts(uint32_t addr, const uint4 &v) { st_shared_v4(addr, v.x, v.y, v.z, v.w); }
+
+// 32 columns (chunks 4*half ..) of a row into the hi and lo tiles
+template <bool BF>
+__device__ __forceinline__ void store_split32(uint32_t hi_tile, uint32_t lo_tile, int row, int half, const float (&x)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 h, l;
+    split8<BF>(x + 8 * c, h, l);
+    const uint32_t at = chunk_at(row, 4 * half + c);
+    sts(hi_tile + at, h);
+    sts(lo_tile + at, l);
+  }
+}
+// the same into an image in global memory
+template <bool BF>
+__device__ __forceinline__ void store_split32(char *hi_tile, char *lo_tile, int row, int half, const float (&x)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint4 h, l;
+    split8<BF>(x + 8 * c, h, l);
+    const uint32_t at = chunk_at(row, 4 * half + c);
+    *reinterpret_cast<uint4 *>(hi_tile + at) = h;
+    *reinterpret_cast<uint4 *>(lo_tile + at) = l;
+  }
+}
+template <bool BF>
+__device__ __forceinline__ void unpack8(const uint4 &v, float *f) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = unpack2(w[i], BF);
+    f[2 * i] = p.x;
+    f[2 * i + 1] = p.y;
+  }
+}
+template <bool BF>
+__device__ __forceinline__ void store_row32(uint16_t *dst, const float (&x)[32]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    reinterpret_cast<uint4 *>(dst)[c] = make_uint4(pack2(x[8 * c], x[8 * c + 1], BF), pack2(x[8 * c + 2], x[8 * c + 3], BF),
+                                                   pack2(x[8 * c + 4], x[8 * c + 5], BF), pack2(x[8 * c + 6], x[8 * c + 7], BF));
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&x)[32]) {
+  uint32_t r[32];
+  tmem_ld_32x32b_x32(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&x)[32]) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(x[i]);
+  tmem_st_32x32b_x32(taddr, r);
+}
+
+// -------------------------------------------------------------- MMA issue --
+// Operand views of a swizzled tile: K-major (rows are M or N, 64-column blocks `block`
+// bytes apart along K) or MN-major (rows are K, 64-column blocks `block` bytes apart
+// along M or N).  Step ks covers K elements [16 ks, 16 ks + 16).
+struct KMajor {
+  uint32_t at, block;
+  __device__ __forceinline__ uint64_t desc(int ks) const { return sdesc_k(at + (ks >> 2) * block + (ks & 3) * 32); }
+};
+struct MNMajor {
+  uint32_t at, block;
+  __device__ __forceinline__ uint64_t desc(int ks) const { return sdesc_mn(at + ks * 2048, block); }
+};
+template <typename A, typename B>
+__device__ __forceinline__ void issue(uint32_t d, const A &a, const B &b, int steps, uint32_t idesc, bool accumulate) {
+  for (int ks = 0; ks < steps; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
+}
+
+// --------------------------------------------------------- CTA scaffolding --
+struct Ctl {
+  uint64_t mma_bar, load_bar;
+  uint32_t tmem;
+  int abort;
+};
+
+// Barriers and tensor memory; returns the tensor-memory base.
+__device__ __forceinline__ uint32_t cta_begin(Ctl &ctl, uint32_t cols) {
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&ctl.mma_bar), 1);
+    mbar_init(smem_u32(&ctl.load_bar), 1);
+    mbar_fence_init();
+    ctl.abort = 0;
+  }
+  if (threadIdx.x < 32) {
+    tmem_alloc(smem_u32(&ctl.tmem), cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return *reinterpret_cast<volatile uint32_t *>(&ctl.tmem);
+}
+__device__ __forceinline__ void cta_end(uint32_t tmem, uint32_t cols) {
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x < 32) tmem_dealloc(tmem, cols);
+}
+// Writes of this thread to shared and tensor memory before the barrier are seen by the
+// products that thread 0 issues after it.
+__device__ __forceinline__ void publish() {
+  fence_async_smem();
+  tc_fence_before();
+  __syncthreads();
+}
+__device__ __forceinline__ void wait_bar(uint64_t &bar, uint32_t &phase, Ctl &ctl, int32_t *status) {
+  mbar_wait(smem_u32(&bar), phase, status, &ctl.abort);
+  phase ^= 1;
+  __syncwarp();
+  tc_fence_after();
+}
+
+// launchers (kda_delta_scan.cu, kda_delta_grad.cu)
+cudaError_t launch_plan(const Args &a, cudaStream_t st);
+cudaError_t launch_prep(const Args &a, cudaStream_t st);
+cudaError_t launch_scan(const Args &a, bool store, cudaStream_t st);
+cudaError_t launch_rev(const Args &a, cudaStream_t st);
+cudaError_t launch_grad(const Args &a, cudaStream_t st);
+
+}  // namespace delta
+}  // namespace kda

@@ -1,0 +1,577 @@
+// Log probabilities of given tokens, entropies and top alternatives of rows of
+// logits, with the gradient (C ABI in include/st_fused_ops.h).
+//
+// Mathematics, in base 2 so that each element costs one ex2: y = c * logit with
+// c = log2(e) / temperature, m = max y, s = sum 2^(y-m), w = sum 2^(y-m) (y-m):
+//   lse = ln2 (m + log2 s)      logprob = ln2 (y_token - m - log2 s)
+//   entropy = ln2 (log2 s - w / s)
+//   dlogit_v = (a ([v = token] - p_v) - b p_v (ln p_v + entropy)) / temperature
+// One pass over the row keeps a running (m, s, w) per thread, rescaled when a
+// vector raises the maximum; the triples are merged across the block and, where
+// a cluster of CTAs shares a row, across the cluster through distributed shared
+// memory (no workspace, no atomics on global memory).
+//
+// Top alternatives: a thread's maximum over its elements comes out of the same
+// pass.  The k-th largest of the block's thread maxima bounds the block's k-th
+// largest element from below, so a second sweep (of L2: the row was just read)
+// keeps only elements at or above it, a little over k of them, and ranks those by
+// (value, then lowest index).  When more than kCand elements tie at or above the
+// bound (constant rows, rows with fewer than k finite values) they are selected
+// one by one instead, a sweep each.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "../../include/st_fused_ops.h"
+#include "kda_internal.h"
+#include "tc_common.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+using kda::tc::pack2;
+using kda::tc::unpack2;
+
+constexpr int kBlock = 256;
+constexpr int kWarps = kBlock / 32;
+constexpr int kTopMax = 32;
+constexpr int kCand = 1024;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// y - m below this contributes 2^-300 = 0 in fp32; a floor keeps 0 * (y - m) finite for y = -inf
+constexpr float kFloor = -300.f;
+
+enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int DT>
+struct Elem {
+  static constexpr int kBytes = DT == kF32 ? 4 : 2;
+  static constexpr int kVec = 16 / kBytes;
+  static __device__ __forceinline__ float load(const char *row, int64_t i) {
+    if (DT == kF32) return reinterpret_cast<const float *>(row)[i];
+    return unpack2((uint32_t) reinterpret_cast<const uint16_t *>(row)[i], DT == kBF16).x;
+  }
+  static __device__ __forceinline__ void store(char *row, int64_t i, float v) {
+    if (DT == kF32)
+      reinterpret_cast<float *>(row)[i] = v;
+    else
+      reinterpret_cast<uint16_t *>(row)[i] = (uint16_t)(pack2(v, 0.f, DT == kBF16) & 0xffffu);
+  }
+  static __device__ __forceinline__ void unpack(const uint4 &v, float (&f)[kVec]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (DT == kF32) {
+        f[i] = __uint_as_float(w[i]);
+      } else {
+        const float2 p = unpack2(w[i], DT == kBF16);
+        f[2 * i] = p.x;
+        f[(2 * i + 1) % kVec] = p.y;
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float (&f)[kVec]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (DT == kF32)
+        w[i] = __float_as_uint(f[i]);
+      else
+        w[i] = pack2(f[2 * i], f[(2 * i + 1) % kVec], DT == kBF16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+// The part of a row that one CTA of the row's cluster owns: scalar elements
+// [lo, body), 16-byte vectors from element `body`, scalar elements [tail, hi).
+// Rows need only be element-aligned.
+struct Slice {
+  int64_t lo, body, nvec, tail, hi;
+};
+
+template <int DT>
+__device__ __forceinline__ Slice slice_of(const char *row, int64_t V, int rank, int parts) {
+  using E = Elem<DT>;
+  const int64_t mis = (int64_t)(reinterpret_cast<uintptr_t>(row) & 15u) / E::kBytes;
+  int64_t head = mis ? E::kVec - mis : 0;
+  if (head > V) head = V;
+  const int64_t nv = (V - head) / E::kVec;
+  const int64_t v0 = nv * rank / parts, v1 = nv * (rank + 1) / parts;
+  Slice s;
+  s.body = head + v0 * E::kVec;
+  s.nvec = v1 - v0;
+  s.lo = rank == 0 ? 0 : s.body;
+  s.tail = s.body + s.nvec * E::kVec;
+  s.hi = rank == parts - 1 ? V : s.tail;
+  return s;
+}
+
+// fn(index, value) for every element of the slice, spread over the block.
+template <int DT, typename F>
+__device__ __forceinline__ void for_each(const char *row, const Slice &sl, F fn) {
+  using E = Elem<DT>;
+  const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
+  for (int64_t i = threadIdx.x; i < sl.nvec; i += kBlock) {
+    float f[E::kVec];
+    E::unpack(__ldg(v4 + i), f);
+#pragma unroll
+    for (int k = 0; k < E::kVec; ++k) fn(sl.body + i * E::kVec + k, f[k]);
+  }
+  for (int64_t i = sl.lo + threadIdx.x; i < sl.body; i += kBlock) fn(i, E::load(row, i));
+  for (int64_t i = sl.tail + threadIdx.x; i < sl.hi; i += kBlock) fn(i, E::load(row, i));
+}
+
+// running (m, s, w); m = -inf means "nothing but -inf yet" (s = w = 0)
+struct Stat {
+  float m, s, w;
+};
+
+__device__ __forceinline__ Stat merge(const Stat &a, const Stat &b) {
+  const float M = fmaxf(a.m, b.m);
+  if (M == -INFINITY) return {M, a.s + b.s, a.w + b.w};  // sums are 0, or NaN from a NaN logit
+  const float da = fmaxf(a.m - M, kFloor), db = fmaxf(b.m - M, kFloor);
+  const float fa = ex2(da), fb = ex2(db);
+  return {M, a.s * fa + b.s * fb, (a.w + da * a.s) * fa + (b.w + db * b.s) * fb};
+}
+
+__device__ __forceinline__ void add1(Stat &t, float y) {
+  if (y > t.m) {
+    const float d = fmaxf(t.m - y, kFloor), f = ex2(d);
+    t.w = (t.w + d * t.s) * f;
+    t.s *= f;
+    t.m = y;
+  }
+  if (t.m != -INFINITY || y != y) {
+    const float d = y - t.m, e = ex2(d);
+    t.s += e;
+    t.w = fmaf(e, fmaxf(d, kFloor), t.w);
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c) {
+  using E = Elem<DT>;
+  Stat t{-INFINITY, 0.f, 0.f};
+  const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
+  auto vec = [&](const uint4 &raw) {
+    float f[E::kVec];
+    E::unpack(raw, f);
+    float mv = f[0], any = f[0];
+#pragma unroll
+    for (int k = 1; k < E::kVec; ++k) {
+      mv = fmaxf(mv, f[k]);
+      any += f[k];
+    }
+    mv *= c;
+    if (mv > t.m) {
+      const float d = fmaxf(t.m - mv, kFloor), fct = ex2(d);
+      t.w = (t.w + d * t.s) * fct;
+      t.s *= fct;
+      t.m = mv;
+    }
+    if (t.m == -INFINITY) {
+      if (any != any) t.s = t.w = NAN;  // a NaN among -infinities
+      return;
+    }
+    float s = 0.f, w = 0.f;
+#pragma unroll
+    for (int k = 0; k < E::kVec; ++k) {
+      const float d = fmaf(f[k], c, -t.m), e = ex2(d);
+      s += e;
+      w = fmaf(e, fmaxf(d, kFloor), w);
+    }
+    t.s += s;
+    t.w += w;
+  };
+  int64_t i = threadIdx.x;
+  for (; i + 3 * kBlock < sl.nvec; i += 4 * kBlock) {  // four loads in flight a thread
+    uint4 r[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r[j] = __ldg(v4 + i + j * kBlock);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vec(r[j]);
+  }
+  for (; i < sl.nvec; i += kBlock) vec(__ldg(v4 + i));
+  for (int64_t j = sl.lo + threadIdx.x; j < sl.body; j += kBlock) add1(t, c * E::load(row, j));
+  for (int64_t j = sl.tail + threadIdx.x; j < sl.hi; j += kBlock) add1(t, c * E::load(row, j));
+  return t;
+}
+
+// (value, index) order: larger value first, then the lower index
+__device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
+__device__ __forceinline__ float sort_key(float x) { return x == x ? x : -INFINITY; }
+
+struct Shared {
+  Stat part[kWarps];
+  Stat total;         // this CTA's
+  float tmax[kBlock];
+  float bound;
+  int count;
+  float cand_v[kCand];
+  int cand_i[kCand];
+  float top_v[kTopMax];  // this CTA's best k, in order
+  int top_i[kTopMax];
+  float red_v[kWarps];
+  int red_i[kWarps];
+};
+
+// This CTA's best k of its slice into sh.top_*, in order; missing places get (-inf, INT_MAX).
+// thread_max is the thread's largest c * logit (c > 0, and rounding keeps the order: a logit
+// at or above the k-th largest has c * logit at or above the bound).
+template <int DT>
+__device__ void local_top(const char *row, const Slice &sl, float c, float thread_max, int k, Shared &sh) {
+  const int tid = threadIdx.x;
+  sh.tmax[tid] = thread_max;
+  if (tid < kTopMax) {
+    sh.top_v[tid] = -INFINITY;
+    sh.top_i[tid] = 0x7fffffff;
+  }
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  int rank = 0;
+  for (int j = 0; j < kBlock; ++j) rank += before(sh.tmax[j], j, thread_max, tid) ? 1 : 0;
+  if (rank == k - 1) sh.bound = thread_max;
+  __syncthreads();
+  const float bound = sh.bound;
+  for_each<DT>(row, sl, [&](int64_t i, float x) {
+    x = sort_key(x);
+    if (c * x >= bound) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) {
+        sh.cand_v[at] = x;
+        sh.cand_i[at] = (int)i;
+      }
+    }
+  });
+  __syncthreads();
+  const int n = sh.count;
+  if (n <= kCand) {
+    for (int a = tid; a < n; a += kBlock) {
+      const float v = sh.cand_v[a];
+      const int id = sh.cand_i[a];
+      int r = 0;
+      for (int j = 0; j < n && r < k; ++j) r += before(sh.cand_v[j], sh.cand_i[j], v, id) ? 1 : 0;
+      if (r < k) {
+        sh.top_v[r] = v;
+        sh.top_i[r] = id;
+      }
+    }
+    __syncthreads();
+    return;
+  }
+  float last_v = INFINITY;
+  int last_i = -1;
+  for (int r = 0; r < k; ++r) {  // the best element behind the last one chosen
+    float bv = -INFINITY;
+    int bi = 0x7fffffff;
+    for_each<DT>(row, sl, [&](int64_t i, float x) {
+      x = sort_key(x);
+      if (before(last_v, last_i, x, (int)i) && before(x, (int)i, bv, bi)) {
+        bv = x;
+        bi = (int)i;
+      }
+    });
+    for (int o = 16; o > 0; o >>= 1) {
+      const float v2 = __shfl_xor_sync(0xffffffffu, bv, o);
+      const int i2 = __shfl_xor_sync(0xffffffffu, bi, o);
+      if (before(v2, i2, bv, bi)) {
+        bv = v2;
+        bi = i2;
+      }
+    }
+    if ((tid & 31) == 0) {
+      sh.red_v[tid >> 5] = bv;
+      sh.red_i[tid >> 5] = bi;
+    }
+    __syncthreads();
+    bv = sh.red_v[0];
+    bi = sh.red_i[0];
+    for (int j = 1; j < kWarps; ++j)
+      if (before(sh.red_v[j], sh.red_i[j], bv, bi)) {
+        bv = sh.red_v[j];
+        bi = sh.red_i[j];
+      }
+    __syncthreads();
+    if (tid == 0) {
+      sh.top_v[r] = bv;
+      sh.top_i[r] = bi;
+    }
+    last_v = bv;
+    last_i = bi;
+  }
+  __syncthreads();
+}
+
+struct FwdArgs {
+  const char *logits;
+  int64_t row_bytes, V;
+  const int64_t *tokens;
+  int64_t ignore_index;
+  float c;  // log2(e) / temperature
+  float *logprob, *entropy, *lse, *top_logprob;
+  int64_t *top_id;
+  int k;
+};
+
+template <int DT, bool CLUSTER>
+__global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
+  __shared__ Shared sh;
+  const int tid = threadIdx.x;
+  int rank = 0, parts = 1;
+  if (CLUSTER) {
+    rank = (int)cg::this_cluster().block_rank();
+    parts = (int)cg::this_cluster().num_blocks();
+  }
+  const int64_t r = blockIdx.x / parts;
+  const char *row = a.logits + r * a.row_bytes;
+  const Slice sl = slice_of<DT>(row, a.V, rank, parts);
+  Stat t = sweep<DT>(row, sl, a.c);
+  if (a.k > 0) {
+    local_top<DT>(row, sl, a.c, t.m, a.k, sh);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    const Stat u{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o),
+                 __shfl_xor_sync(0xffffffffu, t.w, o)};
+    t = merge(t, u);
+  }
+  if ((tid & 31) == 0) sh.part[tid >> 5] = t;
+  __syncthreads();
+  t = sh.part[0];
+  for (int i = 1; i < kWarps; ++i) t = merge(t, sh.part[i]);
+  if (CLUSTER) {
+    cg::cluster_group cl = cg::this_cluster();
+    if (tid == 0) sh.total = t;
+    cl.sync();
+    if (rank == 0)
+      for (int p = 1; p < parts; ++p) t = merge(t, *cl.map_shared_rank(&sh.total, p));
+  }
+  if (rank == 0) {
+    const float l2 = log2f(t.s);
+    const bool empty = t.m == -INFINITY && t.s == 0.f;  // no finite logit in the row
+    if (tid == 0) {
+      const int64_t tok = a.tokens[r];
+      float lp;
+      if (tok == a.ignore_index)
+        lp = 0.f;
+      else if (tok < 0 || tok >= a.V)
+        lp = NAN;
+      else if (empty)
+        lp = -INFINITY;
+      else
+        lp = (fmaf(Elem<DT>::load(row, tok), a.c, -t.m) - l2) * kLn2;
+      a.logprob[r] = lp;
+      a.entropy[r] = empty ? 0.f : (l2 - t.w / t.s) * kLn2;
+      a.lse[r] = empty ? -INFINITY : (t.m + l2) * kLn2;
+    }
+    if (a.k > 0) {
+      // candidates: the CTAs' ordered lists, at most 8 x kTopMax = kBlock of them
+      float v = -INFINITY;
+      int id = 0x7fffffff;
+      const int n = parts * a.k;
+      if (tid < n) {
+        const Shared *src = &sh;
+        if (CLUSTER) src = cg::this_cluster().map_shared_rank(&sh, tid / a.k);
+        v = src->top_v[tid % a.k];
+        id = src->top_i[tid % a.k];
+      }
+      sh.cand_v[tid] = v;
+      sh.cand_i[tid] = id;
+      __syncthreads();
+      if (tid < n) {
+        int pos = 0;
+        for (int j = 0; j < n; ++j) pos += before(sh.cand_v[j], sh.cand_i[j], v, id) ? 1 : 0;
+        if (pos < a.k && id != 0x7fffffff) {
+          a.top_logprob[r * a.k + pos] = empty ? -INFINITY : (fmaf(v, a.c, -t.m) - l2) * kLn2;
+          a.top_id[r * a.k + pos] = id;
+        }
+      }
+    }
+  }
+  if (CLUSTER) cg::this_cluster().sync();  // no CTA leaves while rank 0 reads its shared memory
+}
+
+struct BwdArgs {
+  const char *logits;
+  int64_t row_bytes, V;
+  const int64_t *tokens;
+  int64_t ignore_index;
+  float c, inv_t;
+  const float *entropy, *lse, *dlogprob, *dentropy;
+  char *dlogits;  // [N, V] contiguous
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
+  using E = Elem<DT>;
+  const int64_t r = blockIdx.x;
+  const char *row = g.logits + r * g.row_bytes;
+  char *out = g.dlogits + r * g.V * E::kBytes;
+  const int64_t tok = g.tokens[r];
+  const bool counted = tok != g.ignore_index;
+  const float lse = g.lse[r];
+  const bool empty = lse == -INFINITY;
+  // a token outside [0, V): its log probability is NaN, and so is the row's gradient through it
+  const float a = !counted ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
+  const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r], l2 = lse * kLog2e;
+  const float base = -a - b * H, slope = -b * kLn2;
+  auto grad = [&](int64_t i, float x) {
+    const float d = fmaf(x, g.c, -l2), p = ex2(d);
+    float v = p * fmaf(slope, fmaxf(d, kFloor), base);
+    if (i == tok) v += a;
+    return empty ? 0.f : v;
+  };
+  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  if (!same) {
+    for (int64_t i = threadIdx.x + (int64_t)blockIdx.y * kBlock; i < g.V; i += (int64_t)kBlock * gridDim.y)
+      E::store(out, i, grad(i, E::load(row, i)));
+    return;
+  }
+  const Slice sl = slice_of<DT>(row, g.V, blockIdx.y, gridDim.y);
+  const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
+  uint4 *o4 = reinterpret_cast<uint4 *>(out + sl.body * E::kBytes);
+  for (int64_t i = threadIdx.x; i < sl.nvec; i += kBlock) {
+    float f[E::kVec];
+    E::unpack(__ldg(v4 + i), f);
+#pragma unroll
+    for (int k = 0; k < E::kVec; ++k) f[k] = grad(sl.body + i * E::kVec + k, f[k]);
+    o4[i] = E::pack(f);
+  }
+  for (int64_t i = sl.lo + threadIdx.x; i < sl.body; i += kBlock) E::store(out, i, grad(i, E::load(row, i)));
+  for (int64_t i = sl.tail + threadIdx.x; i < sl.hi; i += kBlock) E::store(out, i, grad(i, E::load(row, i)));
+}
+
+int sm_count() {
+  int dev = 0, n = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+  return n > 0 ? n : 1;
+}
+
+// CTAs that share a row: enough to give every SM two CTAs, each with at least
+// 4096 elements, up to the portable cluster size.
+int parts_of(int64_t N, int64_t V) {
+  const int64_t want = 2 * (int64_t)sm_count();
+  int p = 1;
+  while (p < 8 && N * p * 2 <= want && V / (p * 2) >= 4096) p *= 2;
+  return p;
+}
+
+template <int DT>
+cudaError_t launch_fwd(const FwdArgs &a, int64_t N, cudaStream_t st) {
+  const int parts = parts_of(N, a.V);
+  if (parts == 1) {
+    logprobs_fwd_kernel<DT, false><<<(unsigned)N, kBlock, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(N * parts));
+  cfg.blockDim = dim3(kBlock);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = parts;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<DT, true>, a);
+  return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int DT>
+cudaError_t launch_bwd(const BwdArgs &a, int64_t N, cudaStream_t st) {
+  const int64_t want = 4 * (int64_t)sm_count();
+  int64_t py = (want + N - 1) / N;
+  const int64_t most = (a.V + 8191) / 8192;
+  if (py > most) py = most;
+  if (py < 1) py = 1;
+  logprobs_bwd_kernel<DT><<<dim3((unsigned)N, (unsigned)py), kBlock, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+int check(int64_t N, int64_t V, int64_t stride, float temperature, int32_t dtype) {
+  if (N < 0 || V <= 0 || N > 0x7fffffff / 8 || V > 0x7ffffffe || (N > 1 && stride < V)) return KDA_ERR_BAD_SHAPE;
+  if (!(temperature > 0.f) || temperature > 3.4e38f) return KDA_ERR_UNSUPPORTED;
+  if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return KDA_ERR_UNSUPPORTED;
+  return KDA_OK;
+}
+
+bool element_aligned(const void *p, int32_t dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & (dtype == kF32 ? 3u : 1u)) == 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprob, float *entropy,
+                          float *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
+                          float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream) {
+  int rc = check(N, V, row_stride, temperature, dtype);
+  if (rc != KDA_OK) return rc;
+  if (top_k < 0 || top_k > V) return KDA_ERR_BAD_SHAPE;
+  if (top_k > kTopMax) return KDA_ERR_UNSUPPORTED;
+  if (N == 0) return KDA_OK;
+  if (!logits || !tokens || !logprob || !entropy || !lse || (top_k > 0 && (!top_logprob || !top_id)))
+    return KDA_ERR_NULL_ARGUMENT;
+  if (!element_aligned(logits, dtype)) return KDA_ERR_BAD_LAYOUT;
+  FwdArgs a{};
+  a.logits = static_cast<const char *>(logits);
+  a.row_bytes = row_stride * (dtype == kF32 ? 4 : 2);
+  a.V = V;
+  a.tokens = tokens;
+  a.ignore_index = ignore_index;
+  a.c = kLog2e / temperature;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.lse = lse;
+  a.top_logprob = top_logprob;
+  a.top_id = top_id;
+  a.k = top_k;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == kBF16  ? launch_fwd<kBF16>(a, N, st)
+                        : dtype == kF16 ? launch_fwd<kF16>(a, N, st)
+                                        : launch_fwd<kF32>(a, N, st);
+  kda::count_launches(1);
+  return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
+}
+
+int st_token_logprobs_bwd(const void *logits, int64_t row_stride, const int64_t *tokens, const float *entropy,
+                          const float *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
+                          int64_t V, float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream) {
+  int rc = check(N, V, row_stride, temperature, dtype);
+  if (rc != KDA_OK) return rc;
+  if (N == 0) return KDA_OK;
+  if (!logits || !tokens || !entropy || !lse || !dlogprob || !dentropy || !dlogits) return KDA_ERR_NULL_ARGUMENT;
+  if (!element_aligned(logits, dtype) || !element_aligned(dlogits, dtype)) return KDA_ERR_BAD_LAYOUT;
+  BwdArgs a{};
+  a.logits = static_cast<const char *>(logits);
+  a.row_bytes = row_stride * (dtype == kF32 ? 4 : 2);
+  a.V = V;
+  a.tokens = tokens;
+  a.ignore_index = ignore_index;
+  a.inv_t = 1.f / temperature;
+  a.c = kLog2e / temperature;
+  a.entropy = entropy;
+  a.lse = lse;
+  a.dlogprob = dlogprob;
+  a.dentropy = dentropy;
+  a.dlogits = static_cast<char *>(dlogits);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == kBF16  ? launch_bwd<kBF16>(a, N, st)
+                        : dtype == kF16 ? launch_bwd<kF16>(a, N, st)
+                                        : launch_bwd<kF32>(a, N, st);
+  kda::count_launches(1);
+  return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
+}
+
+}  // extern "C"

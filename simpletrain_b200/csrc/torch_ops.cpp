@@ -1,9 +1,12 @@
 // torch dispatcher ops over the C ABIs of include/kda_sm100.h and
 // include/st_fused_ops.h:
 //   kda_b200::chunk_fwd / chunk_bwd            -> kda_fwd_sm100 / kda_bwd_sm100
+//   kda_b200::delta_fwd / delta_bwd            -> kda_delta_fwd_sm100 / kda_delta_bwd_sm100
+//   kda_b200::delta_step                       -> kda_delta_step_sm100
 //   st_b200::silu_mul / silu_mul_bwd           -> st_silu_mul_fwd / _bwd
 //   st_b200::rmsnorm_residual / _bwd           -> st_rmsnorm_residual_fwd / _bwd
 //   st_b200::cross_entropy / cross_entropy_bwd -> st_cross_entropy_fwd / _bwd
+//   st_b200::token_logprobs / _bwd             -> st_token_logprobs_fwd / _bwd
 //
 // The schemas and CUDA implementations live here, in C++, so a call costs a
 // dispatcher hop and a few caching-allocator allocations instead of a Python
@@ -207,6 +210,181 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> chunk_bwd(
   return {dq, dk, dv, dg, ddecay, ds0};
 }
 
+// ------------------------------------------------------ the gated delta rule
+int32_t gate_code(const Tensor &t, const char *n) {
+  if (t.scalar_type() == at::kFloat) return KDA_DTYPE_F32;
+  if (t.scalar_type() == at::kBFloat16) return KDA_DTYPE_BF16;
+  if (t.scalar_type() == at::kHalf) return KDA_DTYPE_F16;
+  TORCH_CHECK(false, n, " must be float32, bfloat16 or float16");
+}
+
+// 32-bit sizes of the C ABI
+int32_t small(int64_t n) {
+  TORCH_CHECK(n >= 0 && n <= 0x7fffffff, "delta rule: a size of ", std::to_string(n), " is out of range");
+  return (int32_t)n;
+}
+
+bool index64(const Tensor &t, const char *n, const at::Device &dev) {
+  TORCH_CHECK(t.dim() == 1 && (t.scalar_type() == at::kInt || t.scalar_type() == at::kLong) && t.device() == dev, n,
+              " must be a one-dimensional int32 or int64 tensor on q's device");
+  return t.scalar_type() == at::kLong;
+}
+
+// Sizes, inputs and gates of a chunked call; `hold` keeps what the pointers need alive.
+kda_delta_params delta_params(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g, const Tensor &beta,
+                              double scale, const optional<Tensor> &s0, const optional<Tensor> &cu,
+                              std::vector<Tensor> &hold) {
+  TORCH_CHECK(q_.is_cuda(), "the KDA sm_100a kernels need CUDA tensors (there is no CPU path)");
+  TORCH_CHECK(q_.dim() == 4 && v_.dim() == 4 && k_.sizes() == q_.sizes(), "q, k must be [B, Hk, T, D], v [B, H, T, D]");
+  TORCH_CHECK(q_.size(0) == v_.size(0) && q_.size(2) == v_.size(2) && q_.size(3) == v_.size(3),
+              "q and v must have the same batch, tokens and head dim");
+  TORCH_CHECK(g.sizes() == v_.sizes().slice(0, 3) && beta.sizes() == g.sizes(), "g and beta must be [B, H, T]");
+  for (const Tensor *t : {&k_, &v_, &g, &beta})
+    TORCH_CHECK(t->device() == q_.device(), "all tensors must be on q's device");
+  TORCH_CHECK(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(), "k and v must have q's dtype");
+  const Tensor q = prep(q_), k = prep(k_), v = prep(v_);
+  kda_delta_params p{};
+  p.B = small(v.size(0)); p.H = small(v.size(1)); p.Hk = small(q.size(1)); p.T = small(v.size(2)); p.D = small(v.size(3));
+  p.dtype = dtype_code(q);
+  p.g_dtype = gate_code(g, "g");
+  p.beta_dtype = gate_code(beta, "beta");
+  p.scale = (float)scale;
+  p.q = desc(&q); p.k = desc(&k); p.v = desc(&v);
+  p.g = ptr(&g);
+  p.beta = ptr(&beta);
+  p.g_stride_b = g.stride(0); p.g_stride_h = g.stride(1); p.g_stride_t = g.stride(2);
+  p.beta_stride_b = beta.stride(0); p.beta_stride_h = beta.stride(1); p.beta_stride_t = beta.stride(2);
+  int64_t seqs = p.B;
+  if (cu.has_value()) {
+    p.cu_int64 = index64(*cu, "cu_seqlens", q.device()) ? 1 : 0;
+    TORCH_CHECK(cu->numel() >= 1 && p.B == 1, "cu_seqlens needs at least one offset and a batch of 1");
+    const Tensor c = cu->contiguous();
+    p.cu_seqlens = c.data_ptr();
+    seqs = c.numel() - 1;
+    p.nseq = small(seqs);
+    hold.push_back(c);
+  }
+  if (s0.has_value()) {
+    TORCH_CHECK(s0->scalar_type() == at::kFloat && s0->device() == q.device() &&
+                    s0->sizes() == at::IntArrayRef({seqs, (int64_t)p.H, (int64_t)p.D, (int64_t)p.D}),
+                "initial_state must be float32 [sequences, H, D, D] on q's device");
+    Tensor s = s0->contiguous();
+    if (reinterpret_cast<uintptr_t>(s.data_ptr()) % 16) s = s.clone();
+    p.state_in = static_cast<const float *>(ptr(&s));
+    hold.push_back(s);
+  }
+  for (const Tensor &t : {q, k, v, g, beta}) hold.push_back(t);
+  p.status = status_word(q.device()).data_ptr<int32_t>();
+  return p;
+}
+
+int64_t delta_seqs(const kda_delta_params &p) { return p.cu_seqlens != nullptr ? p.nseq : p.B; }
+
+std::tuple<Tensor, Tensor> delta_fwd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                                     const Tensor &beta, double scale, const optional<Tensor> &s0,
+                                     const optional<Tensor> &cu, bool want_state) {
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
+  std::vector<Tensor> hold;
+  kda_delta_params p = delta_params(q, k, v, g, beta, scale, s0, cu, hold);
+  const Tensor o = prep(empty_in_order_of(v));
+  const auto f32 = q.options().dtype(at::kFloat);
+  const Tensor s_out = want_state ? at::empty({delta_seqs(p), p.H, p.D, p.D}, f32) : at::empty({0}, f32);
+  p.o = desc(&o);
+  p.state_out = static_cast<float *>(ptr(&s_out));
+  p.workspace_bytes = kda_delta_fwd_workspace_bytes(&p);
+  const Tensor ws = at::empty({(int64_t)p.workspace_bytes}, q.options().dtype(at::kByte));
+  p.workspace = ptr(&ws);
+  check(kda_delta_fwd_sm100(&p, c10::cuda::getCurrentCUDAStream(q.device().index()).stream()), "kda_delta_fwd_sm100");
+  return {o, s_out};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> delta_bwd(
+    const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta, double scale,
+    const optional<Tensor> &s0, const optional<Tensor> &cu, const Tensor &dout_, const optional<Tensor> &ds_T,
+    bool need_ds0) {
+  c10::cuda::OptionalCUDAGuard guard;
+  if (q.is_cuda()) guard.set_device(q.device());
+  std::vector<Tensor> hold;
+  kda_delta_params p = delta_params(q, k, v, g, beta, scale, s0, cu, hold);
+  TORCH_CHECK(dout_.sizes() == v.sizes() && dout_.device() == q.device(), "dout must have v's shape and device");
+  const Tensor dout = prep(dout_.scalar_type() == q.scalar_type() ? dout_ : dout_.to(q.scalar_type()));
+  const Tensor dq = prep(empty_in_order_of(q)), dk = prep(empty_in_order_of(k)), dv = prep(empty_in_order_of(v));
+  const Tensor dg = at::empty(g.sizes(), g.options()), dbeta = at::empty(beta.sizes(), beta.options());
+  const auto f32 = q.options().dtype(at::kFloat);
+  const Tensor ds0 = need_ds0 ? at::empty({delta_seqs(p), p.H, p.D, p.D}, f32) : at::empty({0}, f32);
+  optional<Tensor> dsT;
+  if (ds_T.has_value() && ds_T->numel() > 0) {
+    TORCH_CHECK(ds_T->sizes() == at::IntArrayRef({delta_seqs(p), (int64_t)p.H, (int64_t)p.D, (int64_t)p.D}) &&
+                    ds_T->device() == q.device(), "the final state's gradient has the wrong shape or device");
+    dsT = ds_T->contiguous().to(at::kFloat);
+    if (reinterpret_cast<uintptr_t>(dsT->data_ptr()) % 16) dsT = dsT->clone();
+    p.dstate_out = static_cast<const float *>(ptr(&*dsT));
+  }
+  p.dout = desc(&dout);
+  p.dq = desc(&dq); p.dk = desc(&dk); p.dv = desc(&dv);
+  p.dg = ptr(&dg);
+  p.dbeta = ptr(&dbeta);
+  p.dstate_in = static_cast<float *>(ptr(&ds0));
+  p.workspace_bytes = kda_delta_bwd_workspace_bytes(&p);
+  const Tensor ws = at::empty({(int64_t)p.workspace_bytes}, q.options().dtype(at::kByte));
+  p.workspace = ptr(&ws);
+  check(kda_delta_bwd_sm100(&p, c10::cuda::getCurrentCUDAStream(q.device().index()).stream()), "kda_delta_bwd_sm100");
+  return {dq, dk, dv, dg, dbeta, ds0};
+}
+
+Tensor delta_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Tensor &g, const Tensor &beta,
+                  Tensor &state, const optional<Tensor> &slots, double scale) {
+  TORCH_CHECK(q_.is_cuda(), "the KDA sm_100a kernels need CUDA tensors (there is no CPU path)");
+  TORCH_CHECK(q_.dim() == 3 && v_.dim() == 3 && k_.sizes() == q_.sizes() && q_.size(0) == v_.size(0) &&
+                  q_.size(2) == v_.size(2), "q, k must be [N, Hk, D], v [N, H, D]");
+  TORCH_CHECK(g.sizes() == v_.sizes().slice(0, 2) && beta.sizes() == g.sizes(), "g and beta must be [N, H]");
+  for (const Tensor *t : {&k_, &v_, &g, &beta, const_cast<const Tensor *>(&state)})
+    TORCH_CHECK(t->device() == q_.device(), "all tensors must be on q's device");
+  TORCH_CHECK(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type(), "k and v must have q's dtype");
+  const int64_t N = v_.size(0), H = v_.size(1), D = v_.size(2);
+  TORCH_CHECK(state.dim() == 4 && state.scalar_type() == at::kFloat && state.size(1) == H && state.size(2) == D &&
+                  state.size(3) == D, "state must be float32 [states, H, D, D]");
+  TORCH_CHECK(state.numel() == 0 ||
+                  (state.stride(3) == 1 && state.stride(2) == D && state.stride(0) % 4 == 0 && state.stride(1) % 4 == 0 &&
+                   (state.size(0) == 1 || state.stride(0) >= D * D) && (H == 1 || state.stride(1) >= D * D) &&
+                   reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0),
+              "state is updated in place: each [D, D] must be contiguous, 16-byte aligned and apart from the others");
+  c10::cuda::CUDAGuard guard(q_.device());
+  const Tensor q = prep(q_), k = prep(k_), v = prep(v_);
+  Tensor o = at::empty({N, H, D}, v.options());
+  kda_delta_step_params p{};
+  p.N = small(N); p.H = small(H); p.Hk = small(q.size(1)); p.D = small(D); p.num_states = small(state.size(0));
+  p.dtype = dtype_code(q);
+  p.g_dtype = gate_code(g, "g");
+  p.beta_dtype = gate_code(beta, "beta");
+  p.scale = (float)scale;
+  p.q = ptr(&q); p.k = ptr(&k); p.v = ptr(&v); p.o = ptr(&o); p.g = ptr(&g); p.beta = ptr(&beta);
+  // a dimension of one element is never stepped over, whatever stride it reports
+  auto st = [](const Tensor &t, int i) { return t.size(i) == 1 ? (int64_t)0 : t.stride(i); };
+  p.q_stride_n = st(q, 0); p.q_stride_h = st(q, 1);
+  p.k_stride_n = st(k, 0); p.k_stride_h = st(k, 1);
+  p.v_stride_n = st(v, 0); p.v_stride_h = st(v, 1);
+  p.o_stride_n = st(o, 0); p.o_stride_h = st(o, 1);
+  p.g_stride_n = g.stride(0); p.g_stride_h = g.stride(1);
+  p.beta_stride_n = beta.stride(0); p.beta_stride_h = beta.stride(1);
+  p.state = static_cast<float *>(ptr(&state));
+  p.state_stride_n = st(state, 0);
+  p.state_stride_h = st(state, 1);
+  Tensor idx;
+  if (slots.has_value()) {
+    p.slots_int64 = index64(*slots, "state_indices", q.device()) ? 1 : 0;
+    TORCH_CHECK(slots->size(0) == N, "state_indices must be [N]");
+    idx = slots->contiguous();
+    p.slots = ptr(&idx);
+  } else {
+    TORCH_CHECK(N <= state.size(0), "without state_indices there must be a state for each row");
+  }
+  p.status = status_word(q.device()).data_ptr<int32_t>();
+  check(kda_delta_step_sm100(&p, c10::cuda::getCurrentCUDAStream(q.device().index()).stream()), "kda_delta_step_sm100");
+  return o;
+}
+
 // The status word the kernels write (Python reads and clears it).
 Tensor status(int64_t device) { return status_word(at::Device(at::kCUDA, (c10::DeviceIndex)device)); }
 
@@ -295,6 +473,55 @@ Tensor cross_entropy_bwd(const Tensor &logits_, const Tensor &labels_, const Ten
   return dlogits;
 }
 
+int32_t logit_code(const Tensor &t) {
+  TORCH_CHECK(t.is_cuda(), "the sm_100a fused ops need CUDA tensors (there is no CPU path)");
+  return t.scalar_type() == at::kFloat ? (int32_t)ST_DTYPE_F32 : dtype_code(t);
+}
+
+// rows of V contiguous elements, any distance apart
+Tensor logit_rows(const Tensor &t) {
+  return (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) ? t : t.contiguous();
+}
+int64_t row_stride(const Tensor &t) { return t.size(0) <= 1 ? t.size(1) : t.stride(0); }
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &logits_, const Tensor &tokens_,
+                                                                  int64_t top_k, double temperature,
+                                                                  int64_t ignore_index) {
+  TORCH_CHECK(logits_.dim() == 2, "token_logprobs: logits must be [N, V]");
+  TORCH_CHECK(tokens_.dim() == 1 && tokens_.size(0) == logits_.size(0) && tokens_.device() == logits_.device() &&
+                  (tokens_.scalar_type() == at::kLong || tokens_.scalar_type() == at::kInt),
+              "token_logprobs: tokens must be int32 or int64 [N] on the logits' device");
+  const int32_t dt = logit_code(logits_);
+  const int64_t N = logits_.size(0), V = logits_.size(1);
+  TORCH_CHECK(top_k >= 0 && top_k <= 32 && top_k <= V, "token_logprobs: top_k must be in [0, min(32, V)], got ",
+              std::to_string(top_k));
+  c10::cuda::CUDAGuard guard(logits_.device());
+  const Tensor logits = logit_rows(logits_), tokens = tokens_.contiguous().to(at::kLong);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  Tensor lp = at::empty({N}, f32), ent = at::empty({N}, f32), lse = at::empty({N}, f32);
+  Tensor top = at::empty({N, top_k}, f32), ids = at::empty({N, top_k}, tokens.options());
+  check(st_token_logprobs_fwd(logits.data_ptr(), row_stride(logits), tokens.data_ptr<int64_t>(), lp.data_ptr<float>(),
+                              ent.data_ptr<float>(), lse.data_ptr<float>(), static_cast<float *>(ptr(&top)),
+                              static_cast<int64_t *>(ptr(&ids)), (int32_t)top_k, N, V, (float)temperature, ignore_index,
+                              dt, stream_of(logits)),
+        "st_token_logprobs_fwd");
+  return {lp, ent, lse, top, ids};
+}
+
+Tensor token_logprobs_bwd(const Tensor &logits_, const Tensor &tokens_, const Tensor &ent_, const Tensor &lse_,
+                          const Tensor &dlp_, const Tensor &dent_, double temperature, int64_t ignore_index) {
+  c10::cuda::CUDAGuard guard(logits_.device());
+  const int64_t N = logits_.size(0), V = logits_.size(1);
+  const Tensor logits = logit_rows(logits_), tokens = tokens_.contiguous().to(at::kLong), ent = ent_.contiguous(),
+               lse = lse_.contiguous(), dlp = dlp_.contiguous().to(at::kFloat), dent = dent_.contiguous().to(at::kFloat);
+  Tensor dlogits = at::empty({N, V}, logits.options());
+  check(st_token_logprobs_bwd(logits.data_ptr(), row_stride(logits), tokens.data_ptr<int64_t>(), ent.data_ptr<float>(),
+                              lse.data_ptr<float>(), dlp.data_ptr<float>(), dent.data_ptr<float>(), dlogits.data_ptr(), N,
+                              V, (float)temperature, ignore_index, logit_code(logits), stream_of(logits)),
+        "st_token_logprobs_bwd");
+  return dlogits;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(st_b200, m) {
@@ -304,6 +531,12 @@ TORCH_LIBRARY(st_b200, m) {
   m.def("rmsnorm_residual_bwd(Tensor x, Tensor weight, Tensor rstd, Tensor dy) -> (Tensor, Tensor)");
   m.def("cross_entropy(Tensor logits, Tensor labels, bool want_probs) -> (Tensor, Tensor, Tensor)");
   m.def("cross_entropy_bwd(Tensor logits, Tensor labels, Tensor lse, Tensor dloss) -> Tensor");
+  m.def(
+      "token_logprobs(Tensor logits, Tensor tokens, int top_k, float temperature, int ignore_index) "
+      "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "token_logprobs_bwd(Tensor logits, Tensor tokens, Tensor entropy, Tensor lse, Tensor dlogprob, Tensor dentropy, "
+      "float temperature, int ignore_index) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(st_b200, CUDA, m) {
@@ -313,6 +546,8 @@ TORCH_LIBRARY_IMPL(st_b200, CUDA, m) {
   m.impl("rmsnorm_residual_bwd", &rmsnorm_residual_bwd);
   m.impl("cross_entropy", &cross_entropy);
   m.impl("cross_entropy_bwd", &cross_entropy_bwd);
+  m.impl("token_logprobs", &token_logprobs);
+  m.impl("token_logprobs_bwd", &token_logprobs_bwd);
 }
 
 TORCH_LIBRARY(kda_b200, m) {
@@ -324,11 +559,23 @@ TORCH_LIBRARY(kda_b200, m) {
       "Tensor? s0, Tensor? s_T, Tensor? ds_T, int chunk, int mode, bool need_ddecay, bool need_ds0) "
       "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("status_word(int device) -> Tensor");
+  m.def(
+      "delta_fwd(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, float scale, Tensor? s0, Tensor? cu_seqlens, "
+      "bool want_state) -> (Tensor, Tensor)");
+  m.def(
+      "delta_bwd(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, float scale, Tensor? s0, Tensor? cu_seqlens, "
+      "Tensor dout, Tensor? ds_T, bool need_ds0) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "delta_step(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) state, Tensor? state_indices, "
+      "float scale) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(kda_b200, CUDA, m) {
   m.impl("chunk_fwd", &chunk_fwd);
   m.impl("chunk_bwd", &chunk_bwd);
+  m.impl("delta_fwd", &delta_fwd);
+  m.impl("delta_bwd", &delta_bwd);
+  m.impl("delta_step", &delta_step);
 }
 
 TORCH_LIBRARY_IMPL(kda_b200, CompositeExplicitAutograd, m) { m.impl("status_word", &status); }

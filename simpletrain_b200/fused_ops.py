@@ -14,8 +14,17 @@ rejected (there is no CPU path).
 * ``fused_cross_entropy(logits[N, V], labels[N])`` -> ``(mean NLL, softmax)``;
   gradients flow through the loss (the softmax output is a plain tensor, as
   in the reference, which returns it for inspection / distillation).
+
+An addition beside them, over the same rows of logits:
+
+* ``token_logprobs(logits[N, V], tokens[N], top_k=..., temperature=...)`` ->
+  log probabilities of given tokens, entropies and top alternatives, without
+  a softmax in memory; gradients flow through the log probabilities and the
+  entropies.
 """
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 
@@ -156,6 +165,82 @@ def cross_entropy_loss(logits: Tensor, labels: Tensor) -> Tensor:
 def fused_cross_entropy(logits: Tensor, labels: Tensor, *, use_triton: bool = True) -> tuple[Tensor, Tensor]:
     """kernels/fused_ops.py:297-307, differentiable through the loss."""
     return cross_entropy_triton(logits, labels)
+
+
+# ------------------------------------------------------- token log probabilities
+class TokenLogprobs(NamedTuple):
+    logprob: Tensor       # [N] fp32
+    entropy: Tensor       # [N] fp32
+    top_logprobs: Tensor  # [N, top_k] fp32
+    top_ids: Tensor       # [N, top_k] int64
+
+
+@torch.library.register_fake("st_b200::token_logprobs")
+def _(logits, tokens, top_k, temperature, ignore_index):
+    N = logits.shape[0]
+    f32 = torch.float32
+    return (logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=f32),
+            logits.new_empty((N, top_k), dtype=f32), logits.new_empty((N, top_k), dtype=torch.int64))
+
+
+@torch.library.register_fake("st_b200::token_logprobs_bwd")
+def _(logits, tokens, entropy, lse, dlogprob, dentropy, temperature, ignore_index):
+    return logits.new_empty(logits.shape)
+
+
+def _lp_setup(ctx, inputs, output):
+    logits, tokens, _, temperature, ignore_index = inputs
+    _, entropy, lse, _, _ = output
+    ctx.save_for_backward(logits, tokens, entropy, lse)
+    ctx.temperature, ctx.ignore_index = temperature, ignore_index
+
+
+def _lp_backward(ctx, dlogprob, dentropy, _dlse, _dtop, _dids):
+    logits, tokens, entropy, lse = ctx.saved_tensors
+    if dlogprob is None:
+        dlogprob = torch.zeros_like(lse)
+    if dentropy is None:
+        dentropy = torch.zeros_like(lse)
+    return torch.ops.st_b200.token_logprobs_bwd(logits, tokens, entropy, lse, dlogprob, dentropy, ctx.temperature,
+                                                ctx.ignore_index), None, None, None, None
+
+
+torch.library.register_autograd("st_b200::token_logprobs", _lp_backward, setup_context=_lp_setup)
+
+
+def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperature: float = 1.0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """Log probabilities of given tokens, entropies and top alternatives of rows of logits.
+
+    logits: ``[N, V]`` bf16, fp16 or fp32, rows any distance apart (a slice of a
+    padded vocabulary is read in place); tokens: ``[N]`` int32 or int64.  With
+    ``x = logits / temperature`` and ``p = softmax(x)``:
+
+    * ``logprob[n] = log p[tokens[n]]``; 0 (and no gradient) where the token is
+      ``ignore_index``, NaN where it is otherwise outside ``[0, V)``.
+    * ``entropy[n] = -sum_v p_v log p_v``.
+    * ``top_logprobs, top_ids [N, top_k]`` (top_k <= 32): the largest logits in
+      order, the lower index first among equal ones; plain tensors without gradient.
+
+    A row of nothing but -infinity has ``logprob = -inf``, entropy 0 and gradient
+    0; a NaN or +infinity makes the row's values NaN.  Sums are fp32.
+    """
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [N, V] with V > 0, got {tuple(logits.shape)}")
+    if tokens.shape != logits.shape[:1]:
+        raise ValueError(f"tokens must be [N] = [{logits.shape[0]}], got {tuple(tokens.shape)}")
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
+        raise TypeError("tokens must be int32 or int64 on the logits' device")
+    if not 0 <= top_k <= min(32, logits.shape[1]):
+        raise ValueError(f"top_k must be in [0, min(32, V)], got {top_k}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    _need_cuda(logits, tokens)
+    lp, ent, _, top, ids = torch.ops.st_b200.token_logprobs(logits, tokens, int(top_k), float(temperature),
+                                                            int(ignore_index))
+    return TokenLogprobs(lp, ent, top.detach(), ids)
 
 
 def _supported_arch() -> bool:
