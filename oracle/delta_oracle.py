@@ -17,7 +17,7 @@ def delta_recurrence(q, k, v, g, beta, scale, state=None):
         u = beta[:, t, None] * (v[:, t] - torch.einsum("hkv,hk->hv", S, k[:, t]))
         S = S + k[:, t, :, None] * u[:, None, :]
         o.append(scale * torch.einsum("hkv,hk->hv", S, q[:, t]))
-    return (torch.stack(o, 1) if T else torch.zeros_like(v)), S
+    return (torch.stack(o, 1) if T else v * 1), S
 
 
 def gated_delta(q, k, v, g, beta, scale, state=None, bounds=None):

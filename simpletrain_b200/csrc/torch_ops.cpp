@@ -43,7 +43,8 @@ bool abi_layout_ok(const Tensor &t) {
   return true;
 }
 
-Tensor prep(const Tensor &t) { return abi_layout_ok(t) ? t : t.contiguous(); }
+// (a copy of a contiguous tensor whose base is misaligned: contiguous() would hand it back)
+Tensor prep(const Tensor &t) { return abi_layout_ok(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
 // New [B, H, T, D] tensor in the dimension order of `like`: its strides when
 // they are dense, else [B, T, H, D] memory when `like` is time-major (the KDA

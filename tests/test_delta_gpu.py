@@ -108,3 +108,317 @@ CASES = [
 def test_forward_and_gradients(B, H, Hk, T, D, dtype, gate, state):
     x = make(B, H, Hk, T, D, dtype, gate, state=state)
     compare(*run_both(x, D))
+
+
+def packed(lens, lead=0, tail=0, dtype=torch.int32):
+    ends = [lead]
+    for n in lens:
+        ends.append(ends[-1] + n)
+    return torch.tensor(ends, dtype=dtype, device=DEV), list(zip(ends[:-1], ends[1:])), ends[-1] + tail
+
+
+@pytest.mark.parametrize("lens,lead,tail,H,Hk,D,dtype,index", [
+    ([70, 1, 0, 64, 129], 0, 0, 2, 2, 64, torch.bfloat16, torch.int32),
+    ([0, 3, 200], 5, 9, 4, 2, 128, torch.bfloat16, torch.int64),
+    ([1] * 40 + [0] * 3, 0, 70, 2, 1, 64, torch.float16, torch.int32),
+    ([0], 0, 17, 1, 1, 128, torch.bfloat16, torch.int32),
+    ([128], 0, 0, 2, 1, 128, torch.float16, torch.int32),
+])
+def test_packed_sequences(lens, lead, tail, H, Hk, D, dtype, index):
+    cu, bounds, T = packed(lens, lead, tail, index)
+    x = make(1, H, Hk, T, D, dtype, torch.float32, seed=1, state=True, n=len(lens))
+    with torch.no_grad():  # what lies outside the sequences is never used
+        for n in ("q", "k", "v", "do"):
+            x[n][:, :, :lead] = torch.nan
+            x[n][:, :, T - tail:T] = torch.nan
+            x[n][:, :, T - tail:T] = torch.inf if n == "v" else torch.nan
+        for n in ("g", "beta"):
+            x[n][:, :, :lead] = torch.nan
+            x[n][:, :, T - tail:T] = torch.nan
+    got, exp = run_both(x, D, cu, bounds)
+    out = torch.ones(T, dtype=torch.bool, device=DEV)
+    for lo, hi in bounds:
+        out[lo:hi] = False
+    for t in (got[0], *got[2:7]):
+        assert (t[:, :, out] == 0).all()
+    compare(got, exp)
+
+
+def test_packed_rows_equal_their_own_calls():
+    """A sequence's results do not depend on what it is packed with."""
+    from simpletrain_b200 import gated_delta_chunk
+    cu, bounds, T = packed([100, 64, 37])
+    x = make(1, 2, 2, T, 128, torch.bfloat16, torch.float32, seed=2)
+    x["v"][:, :, 100:164] = torch.nan  # a broken sequence between two others
+    o, s = gated_delta_chunk(*(x[n] for n in NAMES), cu_seqlens=cu)
+    for i, (lo, hi) in enumerate(bounds):
+        oi, si = gated_delta_chunk(*(x[n][:, :, lo:hi] for n in NAMES))
+        if i != 1:
+            assert torch.equal(o[:, :, lo:hi], oi) and torch.equal(s[i], si[0])
+    assert torch.isnan(o[:, :, 100:164]).any()
+
+
+@pytest.mark.parametrize("raw", [[0, 90, 40, 130], [-5, 20, 130, 131], [0, 10 ** 12, 60, 130], [200, 300, 400, 500]])
+def test_bad_offsets_are_clamped_and_reported(raw):
+    from simpletrain_b200 import _ffi, device_status, gated_delta_chunk
+    T = 130
+    x = make(1, 2, 2, T, 64, torch.bfloat16, torch.float32)
+    clamped, most = [], 0
+    for r in raw:
+        most = max(most, min(max(r, 0), T))
+        clamped.append(most)
+    leaf = [x[n].requires_grad_(True) for n in NAMES]
+    results = []
+    for offsets in (raw, clamped):
+        o, s = gated_delta_chunk(*leaf, cu_seqlens=torch.tensor(offsets, device=DEV))
+        results.append((o, s, *torch.autograd.grad(o, leaf, x["do"])))
+        assert device_status() == (_ffi.KDA_ERR_DEVICE_INDEX if offsets is raw else 0)
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("case", ["plain", "fused", "sliced", "broadcast", "misaligned"])
+def test_layouts(case):
+    """Results do not depend on strides; broadcast inputs get the sum of their gradients."""
+    from simpletrain_b200 import gated_delta_chunk
+    B, H, T, D = 2, 2, 75, 64
+    x = make(B, H, H, T, D, torch.bfloat16, torch.float32, seed=3)
+    base = {n: x[n].contiguous() for n in (*NAMES, "do")}
+    if case == "broadcast":
+        base["k"] = base["k"][:, :1].expand(B, H, T, D).contiguous()
+        base["beta"] = base["beta"][:1].expand(B, H, T).contiguous()
+    want = {n: base[n].clone().requires_grad_(True) for n in NAMES}
+    o, s = gated_delta_chunk(*want.values())
+    dw = torch.autograd.grad(o, list(want.values()), base["do"])
+    if case == "plain":
+        got = {n: base[n].clone().transpose(1, 2).contiguous().transpose(1, 2) for n in NAMES}
+    elif case == "fused":
+        proj = torch.stack([base[n].transpose(1, 2) for n in "qkv"], 2)  # [B, T, 3, H, D]
+        got = dict(zip("qkv", (t.transpose(1, 2) for t in proj.unbind(2))), g=base["g"], beta=base["beta"])
+    elif case == "sliced":
+        got = {n: torch.cat([torch.full_like(base[n][:, :, :3], 9.0), base[n]], 2)[:, :, 3:] for n in NAMES}
+    elif case == "broadcast":
+        got = dict(base, k=base["k"][:, :1].expand(B, H, T, D), beta=base["beta"][:1].expand(B, H, T))
+    else:
+        got = {n: torch.cat([base[n].flatten()[:1], base[n].flatten()])[1:].view_as(base[n]) for n in NAMES}
+    leaf = {n: got[n].detach().requires_grad_(True) for n in NAMES}
+    o2, s2 = gated_delta_chunk(*(leaf[n] for n in NAMES))
+    assert torch.equal(o, o2) and torch.equal(s, s2)
+    dg = torch.autograd.grad(o2, [leaf[n] for n in NAMES], base["do"].transpose(2, 3).contiguous().transpose(2, 3))
+    for n, a, b in zip(NAMES, dw, dg):
+        assert torch.equal(a, b), n
+
+
+def test_strong_and_absent_decay():
+    """Resets (g far below 0, -inf), no decay at all, beta 0, 1 and 2."""
+    x = make(1, 2, 2, 150, 64, torch.bfloat16, torch.float32, seed=4, state=True)
+    x["g"][:, 0] = 0.0
+    x["g"][:, 1, 40] = -1e4
+    x["g"][:, 1, 90:93] = -torch.inf
+    x["g"][:, 1, 127] = -60.0
+    x["beta"][:, 0, 10:20] = 0.0
+    x["beta"][:, 0, 30:60] = 1.0
+    x["beta"][:, 0, 70:80] = 2.0
+    got, exp = run_both(x, 64)
+    # the gradient of a decay that is 0 in fp32 is 0; the formula's e^g at -inf and -1e4 is 0 too
+    compare(got, exp)
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the library's own forward, through the fp32 state."""
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(1, 2, 1, 100, 64, torch.float16, torch.float32, seed=5, state=True)
+    gen = torch.Generator().manual_seed(9)
+    for name in ("g", "beta", "s0"):  # fp32 inputs: they can be moved by a small step exactly
+        d = torch.randn(x[name].shape, generator=gen).to(DEV)
+        d = d / d.norm()
+        leaf = x[name].detach().clone().requires_grad_(True)
+
+        def loss(y):
+            a = dict(x)
+            a[name] = y
+            _, s = gated_delta_chunk(*(a[n] for n in NAMES), initial_state=a["s0"])
+            return (s.double() * x["dsT"].double()).sum()
+
+        (grad,) = torch.autograd.grad(loss(leaf), leaf)
+        # the state is smooth on the scale of 1: a central difference of step h is off by h^2 / 6 of a third
+        # derivative of the same size as the first, plus 2^-17 |s| |ds| / h of the forward's own error
+        h = 0.05
+        with torch.no_grad():
+            diff = (loss(x[name] + h * d) - loss(x[name] - h * d)) / (2 * h)
+            size = gated_delta_chunk(*(x[n] for n in NAMES), initial_state=x["s0"])[1].norm() * x["dsT"].norm()
+        allowed = h * h / 6 * 6 * grad.norm() + 2.0 ** -17 * size / h / 8
+        assert (diff - (grad.double() * d.double()).sum()).abs() <= allowed, name
+
+
+@pytest.mark.parametrize("T,B", [(0, 2), (5, 0)])
+def test_empty(T, B):
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(B, 2, 2, T, 64, torch.bfloat16, torch.float32, state=True)
+    s0 = x["s0"].requires_grad_(True)
+    leaf = [x[n].requires_grad_(True) for n in NAMES]
+    o, s = gated_delta_chunk(*leaf, initial_state=s0)
+    assert o.shape == (B, 2, T, 64) and torch.equal(s, s0)
+    grads = torch.autograd.grad([o, s], leaf + [s0], [x["do"], x["dsT"]])
+    assert torch.equal(grads[-1], x["dsT"]) and grads[0].shape == x["q"].shape
+    cu = torch.zeros(1, dtype=torch.int32, device=DEV)  # no sequence at all
+    if B == 2:
+        y = make(1, 2, 2, 9, 64, torch.bfloat16, torch.float32)
+        o, s = gated_delta_chunk(*(y[n] for n in NAMES), cu_seqlens=cu)
+        assert (o == 0).all() and s.shape == (0, 2, 64, 64)
+
+
+def test_long_sequence_and_state_handed_over():
+    """A long stream, and the same stream in two calls with the state between them."""
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(1, 2, 2, 5003, 64, torch.bfloat16, torch.float32, seed=6, decay=5.0)
+    o, s = gated_delta_chunk(*(x[n] for n in NAMES))
+    ref, s_ref = gated_delta(*(x[n].double() for n in NAMES), 64 ** -0.5)
+    check("o", o, as_result(ref, o))
+    check("s", s, as_result(s_ref, s))
+    cut = 64 * 31
+    o1, s1 = gated_delta_chunk(*(x[n][:, :, :cut] for n in NAMES))
+    o2, s2 = gated_delta_chunk(*(x[n][:, :, cut:] for n in NAMES), initial_state=s1)
+    assert torch.equal(torch.cat([o1, o2], 2), o) and torch.equal(s2, s)
+
+
+def test_repeats_streams_and_capture():
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(2, 4, 2, 200, 128, torch.bfloat16, torch.bfloat16, seed=7)
+    y = make(2, 4, 2, 200, 128, torch.bfloat16, torch.bfloat16, seed=8)
+
+    def step(z):
+        leaf = [z[n].detach().requires_grad_(True) for n in NAMES]
+        o, s = gated_delta_chunk(*leaf)
+        return (o.detach(), s.detach(), *torch.autograd.grad(o, leaf, z["do"]))
+
+    first, other = step(x), step(y)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):  # two calls at once
+        for i, (st, z) in enumerate(zip(streams, (x, y))):
+            with torch.cuda.stream(st):
+                got[i] = step(z)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for z in (x, y):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(step(z))
+        graphs.append(graph)
+    for graph in graphs:  # replayed side by side
+        with torch.cuda.stream(streams[graphs.index(graph)]):
+            graph.replay()
+    torch.cuda.synchronize()
+    for want, a, b in zip((first, other), got, outs):
+        for w, u, v in zip(want, a, b):
+            assert torch.equal(w, u) and torch.equal(w, v)
+
+
+# ------------------------------------------------------------------- step --
+def step_inputs(N, H, Hk, D, states, dtype, gate=torch.float32, seed=0):
+    x = make(1, H, Hk, N, D, dtype, gate, seed=seed)
+    a = {n: x[n][0].transpose(0, 1) for n in NAMES}  # [N, heads, ...] views
+    gen = torch.Generator().manual_seed(seed + 100)
+    a["state"] = (0.3 * torch.randn(states, H, D, D, generator=gen)).to(DEV)
+    return a
+
+
+def step_ref(a, slots, scale, rows=None):
+    """float64, rows in order."""
+    H, Hk = a["v"].shape[1], a["q"].shape[1]
+    st = a["state"].double().clone()
+    o = torch.zeros(a["v"].shape, dtype=torch.float64, device=DEV)
+    for n, s in enumerate(slots):
+        if 0 <= s < st.shape[0]:
+            q, k = (a[m][n].double().repeat_interleave(H // Hk, 0) for m in "qk")
+            S = st[s] * a["g"][n].double().exp()[:, None, None]
+            u = a["beta"][n].double()[:, None] * (a["v"][n].double() - torch.einsum("hkv,hk->hv", S, k))
+            S = S + k[:, :, None] * u[:, None]
+            st[s], o[n] = S, scale * torch.einsum("hkv,hk->hv", S, q)
+    return o, st
+
+
+@pytest.mark.parametrize("N,H,Hk,D,states,dtype,gate,slots", [
+    (1, 1, 1, 64, 1, torch.bfloat16, torch.float32, None),
+    (3, 4, 2, 128, 5, torch.bfloat16, torch.bfloat16, None),
+    (5, 2, 2, 128, 7, torch.float16, torch.float32, [6, 0, 3, 2, 5]),
+    (7, 3, 1, 64, 4, torch.bfloat16, torch.float16, [2, -1, 2, 0, 2, -7, 0]),   # the same state more than once, padding
+    (300, 2, 1, 64, 12, torch.bfloat16, torch.float32, [(7 * i) % 13 - 1 for i in range(300)]),
+])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_step(N, H, Hk, D, states, dtype, gate, slots, index):
+    from simpletrain_b200 import device_status, gated_delta_step
+    a = step_inputs(N, H, Hk, D, states, dtype, gate)
+    idx = None if slots is None else torch.tensor(slots, dtype=index, device=DEV)
+    o_ref, s_ref = step_ref(a, range(N) if slots is None else slots, D ** -0.5)
+    before = a["state"].clone()
+    o = gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], a["state"], state_indices=idx)
+    assert device_status() == 0
+    check("o", o, as_result(o_ref, o))
+    check("state", a["state"], as_result(s_ref, a["state"]))
+    used = set(range(N) if slots is None else slots)
+    for s in set(range(states)) - used:
+        assert torch.equal(a["state"][s], before[s])
+
+
+def test_step_on_a_strided_pool_and_bad_indices():
+    from simpletrain_b200 import _ffi, device_status, gated_delta_step
+    a = step_inputs(4, 2, 2, 64, 6, torch.bfloat16)
+    layers = torch.randn(6, 3, 2, 64, 64, generator=torch.Generator().manual_seed(1)).to(DEV)  # [slot, layer, H, D, D]
+    keep = layers.clone()
+    a["state"] = layers[:, 1]
+    slots = [4, 6, 1, 2 ** 33]  # two of them name no state
+    o_ref, s_ref = step_ref(a, slots, 0.5)
+    o = gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], layers[:, 1], scale=0.5,
+                         state_indices=torch.tensor(slots, device=DEV))
+    assert device_status() == _ffi.KDA_ERR_DEVICE_INDEX
+    check("o", o, as_result(o_ref, o))
+    check("state", layers[:, 1], as_result(s_ref, layers))
+    assert torch.equal(layers[:, 0], keep[:, 0]) and torch.equal(layers[:, 2], keep[:, 2])
+    assert (o[1] == 0).all() and (o[3] == 0).all()
+    with pytest.raises(RuntimeError):  # one state for all rows cannot be updated in place
+        gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], layers[:1, 0].expand(4, 2, 64, 64))
+
+
+def test_prefill_steps_and_scores_agree():
+    """Prefill, single steps with the tokens' log probabilities, and the chunked form over the whole
+    sequence with its gradient: the three operators as a serving and a training loop use them."""
+    from simpletrain_b200 import gated_delta_chunk, gated_delta_step
+    from simpletrain_b200.fused_ops import token_logprobs
+    B, H, T, D, V, cut = 3, 2, 90, 64, 211, 70
+    x = make(B, H, 1, T, D, torch.bfloat16, torch.float32, seed=11)
+    gen = torch.Generator().manual_seed(12)
+    head = (torch.randn(H * D, V, generator=gen) * 0.2).to(torch.bfloat16).to(DEV)
+    tok = torch.randint(0, V, (B, T), generator=gen).to(DEV)
+    leaf = [x[n].detach().requires_grad_(True) for n in NAMES]
+    o, _ = gated_delta_chunk(*leaf)
+    logits = o.transpose(1, 2).reshape(B * T, H * D) @ head
+    score = token_logprobs(logits, tok.view(-1), top_k=4, temperature=0.8)
+    grads = torch.autograd.grad(score.logprob.mean() + 0.01 * score.entropy.mean(), leaf)
+    pool = torch.zeros(5, H, D, D, device=DEV)
+    slots = torch.tensor([4, 0, 2], device=DEV)
+    with torch.no_grad():
+        _, s = gated_delta_chunk(*(x[n][:, :, :cut] for n in NAMES))
+        pool[slots] = s
+        for t in range(cut, T):
+            ot = gated_delta_step(*(x[n][:, :, t] for n in NAMES), pool, state_indices=slots)
+            # chunked and stepped o differ by a rounding of the 16-bit output each at most
+            want = o[:, :, t]
+            assert (ot.double() - want.double()).norm() <= 2 * tol(torch.bfloat16) * want.double().norm()
+            r = token_logprobs(ot.reshape(B, H * D) @ head, tok[:, t], top_k=4, temperature=0.8)
+            full = score.logprob.view(B, T)[:, t]
+            # logits: a sum of H D products, o and the head's result each off by half a bf16 step
+            size = (ot.reshape(B, H * D).float().norm(dim=1) * head.float().norm(dim=0).max()).max().item()
+            assert (r.logprob - full).abs().max() <= 2 * 3 * 2.0 ** -8 * size / 0.8
+    # the gradients against the definitions in float64, from the same logits' gradient
+    ref = [x[n].double().requires_grad_(True) for n in NAMES]
+    o64, _ = gated_delta(*ref, D ** -0.5)
+    again = logits.detach().requires_grad_(True)
+    r = token_logprobs(again, tok.view(-1), temperature=0.8)
+    (dlogits,) = torch.autograd.grad(r.logprob.mean() + 0.01 * r.entropy.mean(), again)
+    do = (dlogits @ head.t()).view(B, T, H, D).transpose(1, 2)
+    want = torch.autograd.grad(o64, ref, do.double())
+    for n, a, b in zip(NAMES, grads, want):
+        check(n, a, as_result(b, a))
