@@ -96,15 +96,15 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
     if (tid == 0) {
       tc_fence_after();
       const uint32_t id64 = idesc_f16(128, 64, BF, false, false), idD = idesc_f16(128, D, BF, false, false);
-      issue(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, D / 16, id64, false);
+      issue<D / 16>(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, id64, false);
       const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384}, uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
       const KMajor sh{sb + L::S, D * 256}, sl{sb + L::S + D * 128, D * 256};
-      issue(tmem + tG2, ah, uh, D / 16, id64, false);
-      issue(tmem + tG2, ah, ul, D / 16, id64, true);
-      issue(tmem + tG2, al, uh, D / 16, id64, true);
-      issue(tmem + tG5, ah, sh, D / 16, idD, false);
-      issue(tmem + tG5, ah, sl, D / 16, idD, true);
-      issue(tmem + tG5, al, sh, D / 16, idD, true);
+      issue<D / 16>(tmem + tG2, ah, uh, id64, false);
+      issue<D / 16>(tmem + tG2, ah, ul, id64, true);
+      issue<D / 16>(tmem + tG2, al, uh, id64, true);
+      issue<D / 16>(tmem + tG5, ah, sh, idD, false);
+      issue<D / 16>(tmem + tG5, ah, sl, idD, true);
+      issue<D / 16>(tmem + tG5, al, sh, idD, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     // meanwhile: <S, dS> (same place in both images), and dX . v
@@ -175,18 +175,18 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
       tc_fence_after();
       const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
       const MNMajor kq{sb + L::KQ, 16384};
-      issue(tmem + tG3, KMajor{sb + L::MN, 0}, kq, 4, id3, false);
-      issue(tmem + tG3, KMajor{sb + L::MN + 16384, 0}, kq, 4, id3, true);
+      issue<4>(tmem + tG3, KMajor{sb + L::MN, 0}, kq, id3, false);
+      issue<4>(tmem + tG3, KMajor{sb + L::MN + 16384, 0}, kq, id3, true);
       // 64 rows (k tokens); the other 64 are not used
-      issue(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, 8, id4, false);
-      issue(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, 8, id4, true);
+      issue<8>(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, id4, false);
+      issue<8>(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, id4, true);
       mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
       const uint32_t id6 = idesc_f16(128, D, BF, false, false);
       const KMajor uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
       const KMajor dh{sb + L::S, D * 256}, dl{sb + L::S + D * 128, D * 256};
-      issue(tmem + tG6, uh, dh, D / 16, id6, false);
-      issue(tmem + tG6, uh, dl, D / 16, id6, true);
-      issue(tmem + tG6, ul, dh, D / 16, id6, true);
+      issue<D / 16>(tmem + tG6, uh, dh, id6, false);
+      issue<D / 16>(tmem + tG6, uh, dl, id6, true);
+      issue<D / 16>(tmem + tG6, ul, dh, id6, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     ph_load ^= 1;

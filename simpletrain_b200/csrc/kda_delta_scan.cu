@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
   uint32_t ph = 0;
   if (tid == 0) {
     tc_fence_after();
-    issue(tmem, KMajor{sb + KQ, 16384}, KMajor{sb + KQ, 16384}, D / 16, idesc_f16(128, 64, BF, false, false), false);
+    issue<D / 16>(tmem, KMajor{sb + KQ, 16384}, KMajor{sb + KQ, 16384}, idesc_f16(128, 64, BF, false, false), false);
     mma_commit(smem_u32(&ctl.mma_bar));
   }
   if (tid < 64) {
@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
     const uint32_t id = idesc_f16(128, 64, BF, false, true);
     const KMajor ph_{sb + TT, 0}, pl{sb + TT + 16384, 0};
     const MNMajor th{sb + TT, 0}, tl{sb + TT + 16384, 0};
-    issue(tmem + 64, ph_, th, 4, id, false);
-    issue(tmem + 64, ph_, tl, 4, id, true);
-    issue(tmem + 64, pl, th, 4, id, true);
+    issue<4>(tmem + 64, ph_, th, id, false);
+    issue<4>(tmem + 64, ph_, tl, id, true);
+    issue<4>(tmem + 64, pl, th, id, true);
     mma_commit(smem_u32(&ctl.mma_bar));
   }
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
@@ -271,6 +271,19 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
   for (int64_t r = threadIdx.x; r < rows; r += kThreads)
     store_gate(p, (int64_t)h * a.p.T + (r < lo ? r : r - lo + hi), dtype, 0.f);
 }
+
+// gamma and beta of a chunk, for one thread's row
+struct Gates {
+  float gi, gl, bi;
+  __device__ __forceinline__ Gates(const Args &a, int chunk, int h, int row, bool live) : gi(0.f), gl(0.f), bi(0.f) {
+    if (live) {
+      const size_t at = ((size_t)chunk * a.p.H + h) * 64;
+      gi = a.w.gam[at + row];
+      gl = a.w.gam[at + 63];
+      bi = a.w.beta[at + row];
+    }
+  }
+};
 
 template <int D>
 struct ScanSmem {
@@ -332,10 +345,19 @@ __global__ void __launch_bounds__(kThreads, 2) scan_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(x + j) = *reinterpret_cast<const float4 *>(a.p.state_in + st_off + j);
   }
+  Gates gates(a, s.chunk0, h, r64, nc > 0);
   for (int c = 0; c < nc; ++c) {
     const int rows = min(kChunk, s.len - c * kChunk);
     const size_t ch = (size_t)(s.chunk0 + c) * a.p.H + h;
-    const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
+    const float gi = gates.gi, gl = gates.gl, bi = gates.bi;
+    if (c + 1 < nc) {  // the next chunk: gates on their way, rows into L2
+      const int next = min(kChunk, s.len - (c + 1) * kChunk);
+      gates = Gates(a, s.chunk0 + c + 1, h, r64, true);
+      prefetch_rows<D>(kb + (int64_t)(c + 1) * kChunk * a.p.k.stride_t, a.p.k.stride_t, next);
+      if (!STORE) prefetch_rows<D>(qb + (int64_t)(c + 1) * kChunk * a.p.q.stride_t, a.p.q.stride_t, next);
+      if (half == 0 && !upper && r64 < next)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(vb + (int64_t)(c + 1) * kChunk * a.p.v.stride_t));
+    }
     uint4 vraw[4];
     if (!upper) {
 #pragma unroll
@@ -360,8 +382,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_kernel(const Args a) {
     if (tid == 0) {
       tc_fence_after();
       const uint32_t id = idesc_f16(128, 64, BF, false, true);
-      issue(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SH, 0}, D / 16, id, false);
-      issue(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SL, 0}, D / 16, id, true);
+      issue<D / 16>(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SH, 0}, id, false);
+      issue<D / 16>(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SL, 0}, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
@@ -386,9 +408,9 @@ __global__ void __launch_bounds__(kThreads, 2) scan_kernel(const Args a) {
       const uint32_t id = idesc_f16(128, 64, BF, false, true);
       const KMajor th{sb + L::T, 0}, tl{sb + L::T + 16384, 0};
       const MNMajor xh{sb + L::B, 0}, xl{sb + L::B + 8192, 0};
-      issue(tmem + 128, th, xh, 4, id, false);
-      issue(tmem + 128, th, xl, 4, id, true);
-      issue(tmem + 128, tl, xh, 4, id, true);
+      issue<4>(tmem + 128, th, xh, id, false);
+      issue<4>(tmem + 128, th, xl, id, true);
+      issue<4>(tmem + 128, tl, xh, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     ph_load ^= 1;
@@ -418,8 +440,8 @@ __global__ void __launch_bounds__(kThreads, 2) scan_kernel(const Args a) {
       // D = 64: the second half of the 128 output rows reads other bytes of shared memory and is not used
       const uint32_t id = idesc_f16(128, 64, BF, true, true);
       const MNMajor kt{sb + L::KQ, 16384};
-      issue(tmem, kt, MNMajor{sb + L::B, 0}, 4, id, true);
-      issue(tmem, kt, MNMajor{sb + L::B + 8192, 0}, 4, id, true);
+      issue<4>(tmem, kt, MNMajor{sb + L::B, 0}, id, true);
+      issue<4>(tmem, kt, MNMajor{sb + L::B + 8192, 0}, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
@@ -498,10 +520,18 @@ __global__ void __launch_bounds__(kThreads, 2) rev_kernel(const Args a) {
   if (row < D && a.p.dstate_out != nullptr)
 #pragma unroll
     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(x + j) = *reinterpret_cast<const float4 *>(a.p.dstate_out + st_off + j);
+  Gates gates(a, s.chunk0 + nc - 1, h, r64, nc > 0);
   for (int c = nc - 1; c >= 0; --c) {
     const int rows = min(kChunk, s.len - c * kChunk);
     const size_t ch = (size_t)(s.chunk0 + c) * a.p.H + h;
-    const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
+    const float gi = gates.gi, gl = gates.gl, bi = gates.bi;
+    if (c > 0) {  // the chunk before: gates on their way, rows into L2
+      gates = Gates(a, s.chunk0 + c - 1, h, r64, true);
+      prefetch_rows<D>(kb + (int64_t)(c - 1) * kChunk * a.p.k.stride_t, a.p.k.stride_t, kChunk);
+      prefetch_rows<D>(qb + (int64_t)(c - 1) * kChunk * a.p.q.stride_t, a.p.q.stride_t, kChunk);
+      if (half == 0 && upper)
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(db + (int64_t)(c - 1) * kChunk * a.p.dout.stride_t));
+    }
     uint4 draw[4];
     if (upper) {
 #pragma unroll
@@ -527,8 +557,8 @@ __global__ void __launch_bounds__(kThreads, 2) rev_kernel(const Args a) {
     if (tid == 0) {
       tc_fence_after();
       const uint32_t id = idesc_f16(128, 64, BF, false, true);
-      issue(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SH, 0}, D / 16, id, false);
-      issue(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SL, 0}, D / 16, id, true);
+      issue<D / 16>(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SH, 0}, id, false);
+      issue<D / 16>(tmem + 64, KMajor{sb + L::KQ, 16384}, MNMajor{sb + L::SL, 0}, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
@@ -547,9 +577,9 @@ __global__ void __launch_bounds__(kThreads, 2) rev_kernel(const Args a) {
       const uint32_t id = idesc_f16(128, 64, BF, true, true);
       const MNMajor th{sb + L::T, 16384}, tl{sb + L::T + 16384, 0};
       const MNMajor bh{sb + L::BH, 0}, bl{sb + L::BL, 0};
-      issue(tmem + 128, th, bh, 8, id, false);
-      issue(tmem + 128, tl, bh, 8, id, true);
-      issue(tmem + 128, th, bl, 4, id, true);
+      issue<8>(tmem + 128, th, bh, id, false);
+      issue<8>(tmem + 128, tl, bh, id, true);
+      issue<4>(tmem + 128, th, bl, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     ph_load ^= 1;
@@ -578,8 +608,8 @@ __global__ void __launch_bounds__(kThreads, 2) rev_kernel(const Args a) {
       tc_fence_after();
       const uint32_t id = idesc_f16(128, 64, BF, true, true);
       const MNMajor kq{sb + L::KQ, 16384};
-      issue(tmem, kq, MNMajor{sb + L::BH, 0}, 8, id, true);
-      issue(tmem, kq, MNMajor{sb + L::BL, 0}, 8, id, true);
+      issue<8>(tmem, kq, MNMajor{sb + L::BH, 0}, id, true);
+      issue<8>(tmem, kq, MNMajor{sb + L::BL, 0}, id, true);
       mma_commit(smem_u32(&ctl.mma_bar));
     }
     wait_bar(ctl.mma_bar, ph, ctl, a.p.status);

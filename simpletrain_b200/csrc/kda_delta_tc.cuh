@@ -126,6 +126,14 @@ __device__ __forceinline__ void load_rows(uint32_t tile, int row0, uint32_t bloc
   }
 }
 
+// Bring the 128-byte lines of `rows` rows of a [T, D] view into L2 ahead of their loads.
+template <int D>
+__device__ __forceinline__ void prefetch_rows(const uint16_t *base, int64_t stride_t, int rows) {
+  constexpr int LINES = D / 64;
+  const int r = threadIdx.x / LINES, c = threadIdx.x % LINES;
+  if (r < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + r * stride_t + c * 64));
+}
+
 // contiguous bytes global -> shared, counted on an mbarrier (sizes and addresses are multiples of 16)
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -216,18 +224,23 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&x)[32]) 
 // -------------------------------------------------------------- MMA issue --
 // Operand views of a swizzled tile: K-major (rows are M or N, 64-column blocks `block`
 // bytes apart along K) or MN-major (rows are K, 64-column blocks `block` bytes apart
-// along M or N).  Step ks covers K elements [16 ks, 16 ks + 16).
+// along M or N).  Step ks covers K elements [16 ks, 16 ks + 16).  One thread issues all
+// products, so a step costs it an add to the descriptor's address field, no more.
 struct KMajor {
-  uint32_t at, block;
-  __device__ __forceinline__ uint64_t desc(int ks) const { return sdesc_k(at + (ks >> 2) * block + (ks & 3) * 32); }
+  uint64_t base;
+  uint32_t block;
+  __device__ __forceinline__ KMajor(uint32_t at, uint32_t block_) : base(sdesc_k(at)), block(block_ >> 4) {}
+  __device__ __forceinline__ uint64_t desc(int ks) const { return base + (uint64_t)((ks >> 2) * block + (ks & 3) * 2); }
 };
 struct MNMajor {
-  uint32_t at, block;
-  __device__ __forceinline__ uint64_t desc(int ks) const { return sdesc_mn(at + ks * 2048, block); }
+  uint64_t base;
+  __device__ __forceinline__ MNMajor(uint32_t at, uint32_t block_) : base(sdesc_mn(at, block_)) {}
+  __device__ __forceinline__ uint64_t desc(int ks) const { return base + (uint64_t)(ks * 128); }
 };
-template <typename A, typename B>
-__device__ __forceinline__ void issue(uint32_t d, const A &a, const B &b, int steps, uint32_t idesc, bool accumulate) {
-  for (int ks = 0; ks < steps; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
+template <int STEPS, typename A, typename B>
+__device__ __forceinline__ void issue(uint32_t d, const A &a, const B &b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int ks = 0; ks < STEPS; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
 }
 
 // --------------------------------------------------------- CTA scaffolding --
