@@ -30,8 +30,8 @@ template <int D>
 struct GradSmem {
   static constexpr uint32_t kTile = 128 * D * 2;
   static constexpr uint32_t KQ = 0, AH = KQ + kTile, AL = AH + kTile;  // [dX; dO] hi, lo (dO's lo rows: zeros)
-  static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U: per 64 columns [64 x 64] hi, lo
-  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S or dS: per 64 columns [D x 64] hi, lo
+  static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U^T: [D x 64] hi, lo
+  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S^T or dS^T: hi, lo, each D / 64 blocks [D x 64]
   static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
 };
 
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
   for (int hh = 0; hh < G_; ++hh) {
     const int h = hk * G_ + hh;
     const size_t ch = (size_t)blockIdx.x * a.p.H + h;
-    const char *gS = a.w.S + ch * NS * (size_t)(D * 256), *gD = a.w.dS + ch * NS * (size_t)(D * 256);
+    const char *gS = a.w.S + ch * (size_t)(D * D * 4), *gD = a.w.dS + ch * (size_t)(D * D * 4);
     if (tid == 0) {
       const uint32_t bar = smem_u32(&ctl.load_bar);
       mbar_arrive_expect_tx(bar, NS * (16384 + 16384 + D * 256));
@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
         bulk_load(sb + L::AH + s * 16384, x, 8192, bar);
         bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, bar);
       }
-      bulk_load(sb + L::U, a.w.U + ch * NS * (size_t)16384, NS * 16384, bar);
+      bulk_load(sb + L::U, a.w.U + ch * (size_t)(D * 256), D * 256, bar);
       bulk_load(sb + L::S, gS, NS * D * 256, bar);
     }
     load_rows<D>(sb + L::AH, 64, 16384, static_cast<const uint16_t *>(a.p.dout.data) + b * a.p.dout.stride_b + h * a.p.dout.stride_h + t0 * a.p.dout.stride_t,
@@ -95,13 +95,15 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
     __syncwarp();
     if (tid == 0) {
       tc_fence_after();
-      const uint32_t id64 = idesc_f16(128, 64, BF, false, false), idD = idesc_f16(128, D, BF, false, false);
+      const uint32_t id64 = idesc_f16(128, 64, BF, false, false), id64t = idesc_f16(128, 64, BF, false, true);
+      const uint32_t idD = idesc_f16(128, D, BF, false, true);
       issue<D / 16>(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, id64, false);
-      const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384}, uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
-      const KMajor sh{sb + L::S, D * 256}, sl{sb + L::S + D * 128, D * 256};
-      issue<D / 16>(tmem + tG2, ah, uh, id64, false);
-      issue<D / 16>(tmem + tG2, ah, ul, id64, true);
-      issue<D / 16>(tmem + tG2, al, uh, id64, true);
+      const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384};
+      const MNMajor uh{sb + L::U, 0}, ul{sb + L::U + D * 128, 0};
+      const MNMajor sh{sb + L::S, D * 128}, sl{sb + L::S + D * D * 2, D * 128};
+      issue<D / 16>(tmem + tG2, ah, uh, id64t, false);
+      issue<D / 16>(tmem + tG2, ah, ul, id64t, true);
+      issue<D / 16>(tmem + tG2, al, uh, id64t, true);
       issue<D / 16>(tmem + tG5, ah, sh, idD, false);
       issue<D / 16>(tmem + tG5, ah, sl, idD, true);
       issue<D / 16>(tmem + tG5, al, sh, idD, true);
@@ -109,16 +111,15 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
     }
     // meanwhile: <S, dS> (same place in both images), and dX . v
     float dot = 0.f;
-    for (int e = tid; e < NS * D * 8; e += kThreads) {
-      const int s = e / (D * 8), o = e % (D * 8) * 16;
-      const uint32_t off = s * (D * 256) + o;
+    for (int e = tid; e < D * D / 8; e += kThreads) {
+      const uint32_t off = e * 16;
       float x[8], y[8], z[8];
       unpack8<BF>(ld_shared_v4(sb + L::S + off), x);
-      unpack8<BF>(ld_shared_v4(sb + L::S + off + D * 128), y);
+      unpack8<BF>(ld_shared_v4(sb + L::S + off + D * D * 2), y);
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] += y[j];
       unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off), y);
-      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off + D * 128), z);
+      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off + D * D * 2), z);
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j] + z[j], dot);
     }
@@ -181,9 +182,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
       issue<8>(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, id4, false);
       issue<8>(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, id4, true);
       mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
-      const uint32_t id6 = idesc_f16(128, D, BF, false, false);
-      const KMajor uh{sb + L::U, 16384}, ul{sb + L::U + 8192, 16384};
-      const KMajor dh{sb + L::S, D * 256}, dl{sb + L::S + D * 128, D * 256};
+      const uint32_t id6 = idesc_f16(128, D, BF, true, true);
+      // 64 rows (tokens); the other 64 read bytes behind and are not used
+      const MNMajor uh{sb + L::U, D * 128}, ul{sb + L::U + D * 128, D * 128};
+      const MNMajor dh{sb + L::S, D * 128}, dl{sb + L::S + D * D * 2, D * 128};
       issue<D / 16>(tmem + tG6, uh, dh, id6, false);
       issue<D / 16>(tmem + tG6, uh, dl, id6, true);
       issue<D / 16>(tmem + tG6, ul, dh, id6, true);
@@ -354,7 +356,7 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->nseq = packed ? p->nseq : p->B;
   a->per_seq = packed ? 0 : (int)(((int64_t)p->T + 63) / 64);
   a->max_chunks = packed ? p->T / 64 + p->nseq : p->B * a->per_seq;
-  const size_t cells = (size_t)a->max_chunks * p->H, slices = cells * (p->D / 64);
+  const size_t cells = (size_t)a->max_chunks * p->H;
   char *base = static_cast<char *>(p->workspace);
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -371,10 +373,10 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
   a->w.T = take(cells * kda::delta::kImgT);
   if (backward) {
-    a->w.S = take(slices * p->D * 256);
-    a->w.dS = take(slices * p->D * 256);
-    a->w.U = take(slices * 16384);
-    a->w.dX = take(slices * 16384);
+    a->w.S = take(cells * p->D * p->D * 4);
+    a->w.dS = take(cells * p->D * p->D * 4);
+    a->w.U = take(cells * p->D * 256);
+    a->w.dX = take(cells * p->D * 256);
   }
   return at;
 }

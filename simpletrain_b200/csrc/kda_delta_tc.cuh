@@ -41,8 +41,10 @@ struct Work {
   float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
   float *beta;     // [chunk][H][64]
   char *T;         // [chunk][H] images of T over P T
-  char *S, *dS;    // [chunk][H][D / 64] images of the state before / the state gradient after the chunk: [D x 64] hi, lo
-  char *U, *dX;    // [chunk][H][D / 64] images of the chunk's u rows / their gradient before T^T: [64 x 64] hi, lo
+  char *S, *dS;    // [chunk][H] images of the state before / the state gradient after the chunk, transposed:
+                   // hi, then lo, each D / 64 blocks [D value rows x 64 key channels]
+  char *U;         // [chunk][H] images of the chunk's u rows, transposed: [D value rows x 64 tokens] hi, then lo
+  char *dX;        // [chunk][H][D / 64] images of the gradient of X: [64 tokens x 64] hi, then lo
 };
 
 struct Args {
@@ -241,6 +243,22 @@ template <int STEPS, typename A, typename B>
 __device__ __forceinline__ void issue(uint32_t d, const A &a, const B &b, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int ks = 0; ks < STEPS; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
+}
+
+// The same with the first operand in tensor memory: rows = lanes, two consecutive K
+// elements a column, so a step is eight columns.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+template <int STEPS, typename B>
+__device__ __forceinline__ void issue_ts(uint32_t d, uint32_t a, const B &b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int ks = 0; ks < STEPS; ++ks) mma_f16_ts(d, a + 8 * ks, b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
 }
 
 // --------------------------------------------------------- CTA scaffolding --
