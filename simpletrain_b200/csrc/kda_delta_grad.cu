@@ -31,7 +31,7 @@ struct GradSmem {
   static constexpr uint32_t kTile = 128 * D * 2;
   static constexpr uint32_t KQ = 0, AH = KQ + kTile, AL = AH + kTile;  // [dX; dO] hi, lo (dO's lo rows: zeros)
   static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U^T: [D x 64] hi, lo
-  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S^T or dS^T: hi, lo, each D / 64 blocks [D x 64]
+  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S^T or dS^T: hi, lo
   static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
 };
 
@@ -93,14 +93,14 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
     mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
     ph_load ^= 1;
     __syncwarp();
-    if (tid == 0) {
+    if (warp_leader()) {
       tc_fence_after();
       const uint32_t id64 = idesc_f16(128, 64, BF, false, false), id64t = idesc_f16(128, 64, BF, false, true);
       const uint32_t idD = idesc_f16(128, D, BF, false, true);
       issue<D / 16>(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, id64, false);
       const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384};
-      const MNMajor uh{sb + L::U, 0}, ul{sb + L::U + D * 128, 0};
-      const MNMajor sh{sb + L::S, D * 128}, sl{sb + L::S + D * D * 2, D * 128};
+      const MNPlain uh{sb + L::U, D}, ul{sb + L::U + D * 128, D};
+      const MNPlain sh{sb + L::S, D}, sl{sb + L::S + D * D * 2, D};
       issue<D / 16>(tmem + tG2, ah, uh, id64t, false);
       issue<D / 16>(tmem + tG2, ah, ul, id64t, true);
       issue<D / 16>(tmem + tG2, al, uh, id64t, true);
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
     }
     store_split32<BF>(sb + L::MN, sb + L::MN + 16384, row, half, x);
     publish();
-    if (tid == 0) {
+    if (warp_leader()) {
       tc_fence_after();
       const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
       const MNMajor kq{sb + L::KQ, 16384};
@@ -184,8 +184,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
       mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
       const uint32_t id6 = idesc_f16(128, D, BF, true, true);
       // 64 rows (tokens); the other 64 read bytes behind and are not used
-      const MNMajor uh{sb + L::U, D * 128}, ul{sb + L::U + D * 128, D * 128};
-      const MNMajor dh{sb + L::S, D * 128}, dl{sb + L::S + D * D * 2, D * 128};
+      const MNPlain uh{sb + L::U, D}, ul{sb + L::U + D * 128, D};
+      const MNPlain dh{sb + L::S, D}, dl{sb + L::S + D * D * 2, D};
       issue<D / 16>(tmem + tG6, uh, dh, id6, false);
       issue<D / 16>(tmem + tG6, uh, dl, id6, true);
       issue<D / 16>(tmem + tG6, ul, dh, id6, true);
@@ -381,10 +381,12 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   return at;
 }
 
-int check_view(const kda_tensor &t) {
+int check_view(const kda_tensor &t, int64_t B, int64_t H, int64_t T) {
   if (t.data == nullptr) return KDA_ERR_NULL_ARGUMENT;
   if (t.stride_d != 1 || (reinterpret_cast<uintptr_t>(t.data) & 15u)) return KDA_ERR_BAD_LAYOUT;
   if ((t.stride_b % 8) || (t.stride_h % 8) || (t.stride_t % 8)) return KDA_ERR_BAD_LAYOUT;
+  // a dimension that is stepped over has a stride (TMA maps have no broadcast)
+  if ((B > 1 && t.stride_b <= 0) || (H > 1 && t.stride_h <= 0) || (T > 1 && t.stride_t <= 0)) return KDA_ERR_BAD_LAYOUT;
   return KDA_OK;
 }
 
@@ -392,8 +394,9 @@ bool misaligned(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) !
 
 int check_common(const kda_delta_params *p, bool tokens) {
   if (tokens) {
-    for (const kda_tensor *t : {&p->q, &p->k, &p->v})
-      if (const int rc = check_view(*t)) return rc;
+    for (const kda_tensor *t : {&p->q, &p->k})
+      if (const int rc = check_view(*t, p->B, p->Hk, p->T)) return rc;
+    if (const int rc = check_view(p->v, p->B, p->H, p->T)) return rc;
     if (p->g == nullptr || p->beta == nullptr) return KDA_ERR_NULL_ARGUMENT;
   }
   if (misaligned(p->state_in)) return KDA_ERR_BAD_LAYOUT;
@@ -422,7 +425,7 @@ int kda_delta_fwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
   if (p->B == 0 || p->H == 0) return KDA_OK;
   const bool tokens = p->T > 0;
   if ((rc = check_common(p, tokens)) != KDA_OK) return rc;
-  if (tokens && (rc = check_view(p->o)) != KDA_OK) return rc;
+  if (tokens && (rc = check_view(p->o, p->B, p->H, p->T)) != KDA_OK) return rc;
   if (misaligned(p->state_out)) return KDA_ERR_BAD_LAYOUT;
   Args a;
   const size_t need = lay_out(p, false, &a);
@@ -442,8 +445,10 @@ int kda_delta_bwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
   const bool tokens = p->T > 0;
   if ((rc = check_common(p, tokens)) != KDA_OK) return rc;
   if (tokens) {
-    for (const kda_tensor *t : {&p->dout, &p->dq, &p->dk, &p->dv})
-      if ((rc = check_view(*t)) != KDA_OK) return rc;
+    for (const kda_tensor *t : {&p->dout, &p->dv})
+      if ((rc = check_view(*t, p->B, p->H, p->T)) != KDA_OK) return rc;
+    for (const kda_tensor *t : {&p->dq, &p->dk})
+      if ((rc = check_view(*t, p->B, p->Hk, p->T)) != KDA_OK) return rc;
     if (p->dg == nullptr || p->dbeta == nullptr) return KDA_ERR_NULL_ARGUMENT;
   }
   if (misaligned(p->dstate_out) || misaligned(p->dstate_in)) return KDA_ERR_BAD_LAYOUT;

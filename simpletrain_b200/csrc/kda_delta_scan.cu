@@ -17,6 +17,7 @@
 // products a chunk: with the state, with T (or its transpose), and the state update, which
 // accumulates on the state in tensor memory.
 #include "kda_delta_tc.cuh"
+#include "tmap.h"
 
 namespace kda {
 namespace delta {
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
   cp_async_wait();
   publish();
   uint32_t ph = 0;
-  if (tid == 0) {
+  if (warp_leader()) {
     tc_fence_after();
     issue<D / 16>(tmem, KMajor{sb + KQ, 16384}, KMajor{sb + KQ, 16384}, idesc_f16(128, 64, BF, false, false), false);
     mma_commit(smem_u32(&ctl.mma_bar));
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
     store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
   }
   publish();
-  if (tid == 0) {
+  if (warp_leader()) {
     tc_fence_after();
     // rows 64..127: P T (rows 0..63, T T, are not read)
     const uint32_t id = idesc_f16(128, 64, BF, false, true);
@@ -282,13 +283,12 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // state on the first product alone: its operands, not its arithmetic, set the time.
 //
 // Warps: 8 walk the dependent chain (a value channel a thread, half the columns each), 4
-// turn finished tiles into output or workspace rows, 3 load, one issues the products.
-// Loads run one chunk ahead in two stages.
+// turn finished tiles into output or workspace rows, one starts the loads, one issues the
+// products.  TMA brings the tiles two chunks ahead.
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
-constexpr int kScanThreads = 512;
-constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 15;  // the chain: warps 0 .. 7
-constexpr int kLoaders = 32 * (kMmaWarp - kLoadWarp);
+constexpr int kScanThreads = 448;
+constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 13;  // the chain: warps 0 .. 7
 
 // Per-token factors of a chunk, one array a factor: beta, -beta e^gamma, e^{gamma_63 - gamma}, scale e^gamma.
 struct Factors {
@@ -298,16 +298,15 @@ struct Factors {
 
 template <int D, int MODE>
 struct ScanSmem {
-  static constexpr uint32_t KQ = 0, V = 128 * D * 2, T = V + 64 * D * 2, kStage = T + kImgT;
-  static constexpr uint32_t OUT = 2 * kStage;  // outputs: [64 x D]; reverse: dX hi and lo
-  static constexpr uint32_t kTile = 64 * D * 2;
-  static constexpr uint32_t QS = OUT + 2 * kTile;  // reverse: Q' hi and lo
-  static constexpr uint32_t kBytes = MODE == kOut ? OUT + kTile : (MODE == kRev ? QS + 2 * kTile : OUT);
+  static constexpr uint32_t kTile = 64 * D * 2;  // [64 tokens x D], D / 64 swizzled blocks of 8 KB
+  static constexpr uint32_t K = 0, Q = kTile, V = 2 * kTile, T = 3 * kTile, kStage = T + kImgT;
+  static constexpr uint32_t OUT = 2 * kStage;  // outputs: o; reverse: dX hi, dX lo, dV
+  static constexpr uint32_t kBytes = OUT + (MODE == kOut ? kTile : (MODE == kRev ? 3 * kTile : 0));
 };
 
 struct ScanBars {
-  uint64_t full[2], tfull[2], empty[2];
-  uint64_t s_ready, ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
+  uint64_t full[2], empty[2];
+  uint64_t tail, s_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
 };
 
 // tensor-memory columns
@@ -323,29 +322,30 @@ __device__ __forceinline__ void tmem_split32(uint32_t hi_at, uint32_t lo_at, con
   tmem_st_32x32b_x16_nowait(lo_at, l);
 }
 
-// rows of a [T, D] view into D / 64 swizzled [64 x 64] blocks `block` bytes apart, by the loading threads
-template <int D>
-__device__ __forceinline__ void load_tile(uint32_t tile, uint32_t block, const uint16_t *base, int64_t stride_t, int rows,
-                                             int t) {
-  constexpr int P = D / 8;
-#pragma unroll 4
-  for (int p = t; p < 64 * P; p += kLoaders) {
-    const int r = p / P, c = p % P;
-    const bool live = r < rows;
-    cp_async16(tile + (c >> 3) * block + r * 128 + (((c & 7) ^ (r & 7)) << 4), base + (live ? r * stride_t : 0) + c * 8, live);
-  }
-}
-
 __device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r0), "r"(r1), "r"(r2),
                "r"(r3)
                : "memory");
 }
 
+// 16 x 256b fragments (64 columns of 16 lanes) times a per-column factor, rounded and stored
+// transposed: rows of the swizzled tile are columns (tokens), 16-byte runs are lanes (value channels).
+struct TileOut {
+  int quad, mat, rho;
+  __device__ __forceinline__ explicit TileOut(int quad_) : quad(quad_), mat((threadIdx.x & 31) >> 3), rho(threadIdx.x & 7) {}
+  __device__ __forceinline__ void put(uint32_t tile, int hh, int j, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) const {
+    const int m0 = 32 * quad + 16 * hh + 8 * (mat & 1), tok = 8 * (j + (mat >> 1)) + rho;
+    stmatrix_x4_trans(tile + (uint32_t)((m0 >> 6) * 8192) + chunk_at(tok, (m0 & 63) >> 3), r0, r1, r2, r3);
+  }
+};
+
 template <int D, bool BF, int MODE>
-__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
+__global__ void __launch_bounds__(kScanThreads, 1)
+    scan_kernel(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq,
+                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo) {
   using L = ScanSmem<D, MODE>;
   constexpr int Q = D / 32;  // warps that own live tensor-memory lanes, of four
+  constexpr int NB = D / 64;
   constexpr bool REV = MODE == kRev;
   extern __shared__ __align__(1024) char smem[];
   __shared__ ScanBars bars;
@@ -374,14 +374,15 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
   const uint32_t sb = smem_u32(smem);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&bars.full[i]), kLoaders);
-      mbar_init(smem_u32(&bars.tfull[i]), 1);
+      mbar_init(smem_u32(&bars.full[i]), 32);
       mbar_init(smem_u32(&bars.empty[i]), MODE == kStore ? 1 : 1 + Q);
+      mbar_init(smem_u32(&bars.s_ready[i]), 2 * Q);
     }
-    for (uint64_t *b : {&bars.s_ready, &bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
+    for (uint64_t *b : {&bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
     for (uint64_t *b : {&bars.ks_done, &bars.u_done, &bars.s_done, &bars.o_done}) mbar_init(smem_u32(b), 1);
     mbar_init(smem_u32(&bars.out_free), Q);
-    mbar_init(smem_u32(&bars.qs_ready), kLoaders);
+    mbar_init(smem_u32(&bars.qs_ready), Q);
+    mbar_init(smem_u32(&bars.tail), 32);
     mbar_fence_init();
     abort_flag = 0;
   }
@@ -393,7 +394,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(&tmem_slot);
-  auto wait = [&](uint64_t &b, uint32_t parity) { mbar_wait(smem_u32(&b), parity, a.p.status, &abort_flag); };
+  auto wait = [&](uint64_t &b, uint32_t parity) {
+    mbar_wait(smem_u32(&b), parity, a.p.status, &abort_flag);
+    __syncwarp();
+  };
   auto arrive_warp = [&](uint64_t &b) {  // after this warp's tensor-memory accesses
     tc_fence_before();
     __syncwarp();
@@ -404,6 +408,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
   const int nc = (s.len + kChunk - 1) / kChunk;
   auto chunk_of = [&](int it) { return REV ? nc - 1 - it : it; };
   auto cell = [&](int it) { return (size_t)(s.chunk0 + chunk_of(it)) * a.p.H + h; };
+  auto rows_of = [&](int it) { return min(kChunk, s.len - chunk_of(it) * kChunk); };
+  // a stage's tiles have landed (and, in a sequence's ragged chunk, the rows behind its end are zeros)
+  auto wait_full = [&](int it) {
+    wait(bars.full[it & 1], (it >> 1) & 1);
+    if (rows_of(it) < kChunk) wait(bars.tail, 0);
+  };
 
   if (warp < kOutWarp) {
     // ------------------------------------------------------------- the chain --
@@ -420,13 +430,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
       for (int i = 0; i < 8; ++i) vcol[i] = (uint32_t)((dv >> 6) * 8192 + i * 128 + ((((dv >> 3) ^ i) & 7) << 4) + (dv & 7) * 2);
       for (int it = 0; it < nc; ++it) {
         const int st = it & 1;
-        wait(bars.full[st], (it >> 1) & 1);
+        wait_full(it);
         const float last = fac[st].last[0];
         if (it > 0) {
-          wait(bars.s_done, (it - 1) & 1);
           if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
+          wait(bars.s_done, (it - 1) & 1);
         }
-        __syncwarp();
         tc_fence_after();
 #pragma unroll
         for (int c0 = 0; c0 < W; c0 += 32) {
@@ -442,9 +451,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(x[j] * last);
           tmem_st_32x32b_x32_nowait(tl + cS + half * W + c0, r);
+          tmem_wait_st();
+          arrive_warp(bars.s_ready[c0 / 32]);
         }
-        tmem_wait_st();
-        arrive_warp(bars.s_ready);
         float v[32];
         if (!REV) {  // V^T: this value channel of 32 tokens
           const uint32_t vt = sb + st * L::kStage + L::V + half * 4096;
@@ -456,7 +465,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
           }
         }
         wait(bars.ks_done, it & 1);
-        __syncwarp();
         tc_fence_after();
         {
           float x[32];
@@ -468,7 +476,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
           arrive_warp(bars.x_ready);
         }
         wait(bars.u_done, it & 1);
-        __syncwarp();
         tc_fence_after();
         {
           float x[32];
@@ -485,7 +492,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
       float *dst = REV ? a.p.dstate_in : (MODE == kOut ? a.p.state_out : nullptr);
       if (dst != nullptr) {
         if (nc > 0) wait(bars.s_done, (nc - 1) & 1);
-        __syncwarp();
         tc_fence_after();
 #pragma unroll
         for (int c0 = 0; c0 < W; c0 += 32) {
@@ -503,242 +509,281 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const Args a) {
     if (quad < Q) {
       const uint32_t tl = tmem + ((uint32_t)quad << 21);
       const int t = tid - kOutWarp * 32;  // 0 .. 32 Q - 1
-      const int mat = lane >> 3, rho = lane & 7;
-      // address of the 16-byte run that this lane gives stmatrix for columns (tokens) 8 j .. 8 j + 15, lanes 16 hh ..
-      auto st_at = [&](uint32_t tile, int hh, int j) {
-        const int m0 = 32 * quad + 16 * hh + 8 * (mat & 1), tok = 8 * (j + (mat >> 1)) + rho;
-        return tile + (uint32_t)((m0 >> 6) * 8192) + chunk_at(tok, (m0 & 63) >> 3);
+      const int row = 32 * quad + lane, q2 = 2 * (lane & 3);
+      const TileOut tile(quad);
+      const kda_tensor &ot = REV ? a.p.dv : a.p.o;
+      // a [64 x D] tile of o or dV from shared memory, once all warps have written it (store_tile ends the wait
+      // for its reads; the caller's next tile starts with tile_free)
+      auto store_tile = [&](uint32_t at, int it) {
+        const int c = chunk_of(it), rows = rows_of(it);
+        fence_async_smem();
+        named_bar_sync(1, 32 * Q);
+        if (rows == kChunk) {
+          if (t == 0)
+            for (int b = 0; b < NB; ++b) tma_store_4d(&mo, at + 8192 * b, 64 * b, (int)(s.t0 + (int64_t)c * kChunk), h, (int)s.b);
+        } else {  // what lies behind a packed sequence is another's
+          uint16_t *ob = static_cast<uint16_t *>(ot.data) + s.b * ot.stride_b + h * ot.stride_h + (s.t0 + (int64_t)c * kChunk) * ot.stride_t;
+          for (int e = t; e < rows * (D / 8); e += 32 * Q) {
+            const int r = e / (D / 8), g = e % (D / 8);
+            *reinterpret_cast<uint4 *>(ob + r * ot.stride_t + 8 * g) = ld_shared_v4(at + (g >> 3) * 8192 + chunk_at(r, g & 7));
+          }
+        }
+      };
+      auto tile_free = [&]() {
+        if (t == 0) tma_store_wait_read0();
+        named_bar_sync(1, 32 * Q);
       };
       for (int it = 0; it < nc; ++it) {
-        const int st = it & 1, c = chunk_of(it), rows = min(kChunk, s.len - c * kChunk);
+        const int st = it & 1;
         if (MODE == kOut) {
+          wait_full(it);
           wait(bars.o_done, it & 1);
-          __syncwarp();
           tc_fence_after();
-          const int q2 = 2 * (lane & 3);
+          uint32_t pk[2][16];  // [16-lane half][column block j, row half]
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
             uint32_t qs[32], o[32];
             tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, qs);
             tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR3, o);
-            uint32_t pk[16];  // [column block j][row half]
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float f0 = fac[st].sg[8 * j + q2], f1 = fac[st].sg[8 * j + q2 + 1];
 #pragma unroll
               for (int e = 0; e < 2; ++e)
-                pk[2 * j + e] = pack2(fmaf(f0, __uint_as_float(qs[4 * j + 2 * e]), __uint_as_float(o[4 * j + 2 * e])),
-                                      fmaf(f1, __uint_as_float(qs[4 * j + 2 * e + 1]), __uint_as_float(o[4 * j + 2 * e + 1])), BF);
+                pk[hh][2 * j + e] = pack2(fmaf(f0, __uint_as_float(qs[4 * j + 2 * e]), __uint_as_float(o[4 * j + 2 * e])),
+                                          fmaf(f1, __uint_as_float(qs[4 * j + 2 * e + 1]), __uint_as_float(o[4 * j + 2 * e + 1])), BF);
             }
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-              stmatrix_x4_trans(st_at(sb + L::OUT, hh, j), pk[2 * j], pk[2 * j + 1], pk[2 * j + 2], pk[2 * j + 3]);
           }
           arrive_warp(bars.out_free);
           if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
-          named_bar_sync(1, 32 * Q);
-          uint16_t *ob = static_cast<uint16_t *>(a.p.o.data) + s.b * a.p.o.stride_b + h * a.p.o.stride_h +
-                         (s.t0 + (int64_t)c * kChunk) * a.p.o.stride_t;
-#pragma unroll 4
-          for (int e = t; e < 64 * (D / 8); e += 32 * Q) {
-            const int r = e / (D / 8), g = e % (D / 8);
-            if (r < rows)
-              *reinterpret_cast<uint4 *>(ob + r * a.p.o.stride_t + 8 * g) = ld_shared_v4(sb + L::OUT + (g >> 3) * 8192 + chunk_at(r, g & 7));
-          }
-          named_bar_sync(1, 32 * Q);
+          tile_free();
+#pragma unroll
+          for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+            for (int j = 0; j < 8; j += 2)
+              tile.put(sb + L::OUT, hh, j, pk[hh][2 * j], pk[hh][2 * j + 1], pk[hh][2 * j + 2], pk[hh][2 * j + 3]);
+          store_tile(sb + L::OUT, it);
+          if (t == 0) tma_store_commit();
         } else {
+          if (REV) {  // Q' product's first operand: scale e^gamma dO, transposed, in two terms
+            wait_full(it);
+            if (it > 0) wait(bars.s_done, (it - 1) & 1);  // the last one is used
+            const uint32_t vt = sb + st * L::kStage + L::V + (row >> 6) * 8192 + (row & 7) * 2;
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              float x[32];
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                uint16_t u;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + (32 * b + j) * 128 + ((((row >> 3) ^ j) & 7) << 4)));
+                x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * b + j];
+              }
+              tmem_split32<BF>(tl + cR3 + 16 * b, tl + cR3 + 32 + 16 * b, x);
+            }
+            tmem_wait_st();
+            arrive_warp(bars.qs_ready);
+          }
           // the state (reverse: its gradient) as the chain split it
-          wait(bars.s_ready, it & 1);
-          __syncwarp();
+          char *img = (REV ? a.w.dS : a.w.S) + cell(it) * (size_t)(D * D * 4) + row * 16;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) wait(bars.s_ready[b], it & 1);
           tc_fence_after();
-          char *img = (REV ? a.w.dS : a.w.S) + cell(it) * (size_t)(D * D * 4);
-          const int row = 32 * quad + lane;
 #pragma unroll
           for (int part = 0; part < 2; ++part)
 #pragma unroll
-            for (int b = 0; b < D / 64; ++b) {
+            for (int b = 0; b < NB; ++b) {
               uint32_t r[32];
               tmem_ld_32x32b_x32(tl + (part ? cSL : cSH) + 32 * b, r);
-              char *dst = img + part * (D * D * 2) + b * (D * 128);
 #pragma unroll
               for (int g = 0; g < 8; ++g)
-                *reinterpret_cast<uint4 *>(dst + chunk_at(row, g)) = make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+                *reinterpret_cast<uint4 *>(img + part * (D * D * 2) + (8 * b + g) * (D * 16)) =
+                    make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
             }
           wait(bars.u_done, it & 1);
-          __syncwarp();
           tc_fence_after();
           if (MODE == kStore) {  // U^T
-            char *ui = a.w.U + cell(it) * (size_t)(D * 256);
+            char *ui = a.w.U + cell(it) * (size_t)(D * 256) + row * 16;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               float x[32];
               tmem_ld32(tl + cR1 + 32 * b, x);
-              store_split32<BF>(ui, ui + D * 128, row, b, x);
+              if (b == 1) arrive_warp(bars.out_free);
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                uint4 hi, lo;
+                split8<BF>(x + 8 * g, hi, lo);
+                *reinterpret_cast<uint4 *>(ui + (4 * b + g) * (D * 16)) = hi;
+                *reinterpret_cast<uint4 *>(ui + D * 128 + (4 * b + g) * (D * 16)) = lo;
+              }
             }
-            arrive_warp(bars.out_free);
           } else {  // dX, and dV = beta dX
+            tile_free();
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
               uint32_t x[32], hi[16], lo[16];
               tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, x);
+              if (hh == 1) arrive_warp(bars.out_free);
 #pragma unroll
               for (int i = 0; i < 16; ++i) split2<BF>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), hi[i], lo[i]);
 #pragma unroll
               for (int j = 0; j < 8; j += 2) {
-                stmatrix_x4_trans(st_at(sb + L::OUT, hh, j), hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
-                stmatrix_x4_trans(st_at(sb + L::OUT + L::kTile, hh, j), lo[2 * j], lo[2 * j + 1], lo[2 * j + 2], lo[2 * j + 3]);
+                tile.put(sb + L::OUT, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
+                tile.put(sb + L::OUT + L::kTile, hh, j, lo[2 * j], lo[2 * j + 1], lo[2 * j + 2], lo[2 * j + 3]);
               }
-            }
-            arrive_warp(bars.out_free);
-            named_bar_sync(1, 32 * Q);
-            char *xi = a.w.dX + cell(it) * (size_t)(D * 256);
-            uint16_t *vb = static_cast<uint16_t *>(a.p.dv.data) + s.b * a.p.dv.stride_b + h * a.p.dv.stride_h +
-                           (s.t0 + (int64_t)c * kChunk) * a.p.dv.stride_t;
-#pragma unroll 2
-            for (int e = t; e < 64 * (D / 8); e += 32 * Q) {
-              const int r = e / (D / 8), g = e % (D / 8);
-              const uint32_t off = chunk_at(r, g & 7);
-              const uint4 xh = ld_shared_v4(sb + L::OUT + (g >> 3) * 8192 + off);
-              const uint4 xl = ld_shared_v4(sb + L::OUT + L::kTile + (g >> 3) * 8192 + off);
-              *reinterpret_cast<uint4 *>(xi + (g >> 3) * 16384 + off) = xh;
-              *reinterpret_cast<uint4 *>(xi + (g >> 3) * 16384 + 8192 + off) = xl;
-              if (r < rows) {
-                const float be = fac[st].beta[r];
-                float y[8], z[8];
-                unpack8<BF>(xh, y);
-                unpack8<BF>(xl, z);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = be * (y[j] + z[j]);
-                *reinterpret_cast<uint4 *>(vb + r * a.p.dv.stride_t + 8 * g) =
-                    make_uint4(pack2(y[0], y[1], BF), pack2(y[2], y[3], BF), pack2(y[4], y[5], BF), pack2(y[6], y[7], BF));
+              for (int j = 0; j < 8; ++j) {
+                const float f0 = fac[st].beta[8 * j + q2], f1 = fac[st].beta[8 * j + q2 + 1];
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  hi[2 * j + e] = pack2(f0 * __uint_as_float(x[4 * j + 2 * e]), f1 * __uint_as_float(x[4 * j + 2 * e + 1]), BF);
               }
+#pragma unroll
+              for (int j = 0; j < 8; j += 2)
+                tile.put(sb + L::OUT + 2 * L::kTile, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
             }
-            named_bar_sync(1, 32 * Q);
+            __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
+            store_tile(sb + L::OUT + 2 * L::kTile, it);
+            if (t == 0) {  // the dX tiles are the images
+              char *xi = a.w.dX + cell(it) * (size_t)(D * 256);
+              for (int b = 0; b < NB; ++b) {
+                bulk_store(xi + b * 16384, sb + L::OUT + b * 8192, 8192);
+                bulk_store(xi + b * 16384 + 8192, sb + L::OUT + L::kTile + b * 8192, 8192);
+              }
+              tma_store_commit();
+            }
           }
         }
       }
+      if (t == 0) tma_store_wait_all();
     }
-  } else if (warp < kMmaWarp) {
+  } else if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ loads --
-    const int t = tid - kLoadWarp * 32;
-    const uint16_t *kb = static_cast<const uint16_t *>(a.p.k.data) + s.b * a.p.k.stride_b + hk * a.p.k.stride_h + s.t0 * a.p.k.stride_t;
-    const uint16_t *qb = static_cast<const uint16_t *>(a.p.q.data) + s.b * a.p.q.stride_b + hk * a.p.q.stride_h + s.t0 * a.p.q.stride_t;
-    const kda_tensor &vt = REV ? a.p.dout : a.p.v;
-    const uint16_t *vb = static_cast<const uint16_t *>(vt.data) + s.b * vt.stride_b + h * vt.stride_h + s.t0 * vt.stride_t;
+    constexpr uint32_t kBytes = (MODE == kStore ? 2 : 3) * L::kTile + (MODE == kStore ? 16384 : kImgT);
     auto load = [&](int it) {
-      const int st = it & 1, c = chunk_of(it), rows = min(kChunk, s.len - c * kChunk);
-      const int64_t r0 = (int64_t)c * kChunk;
-      const uint32_t base = sb + st * L::kStage;
-      if (it >= 2) wait(bars.empty[st], ((it >> 1) - 1) & 1);
-      __syncwarp();
-      load_tile<D>(base + L::KQ, 16384, kb + r0 * a.p.k.stride_t, a.p.k.stride_t, rows, t);
-      if (MODE != kStore) load_tile<D>(base + L::KQ + 8192, 16384, qb + r0 * a.p.q.stride_t, a.p.q.stride_t, rows, t);
-      load_tile<D>(base + L::V, 8192, vb + r0 * vt.stride_t, vt.stride_t, rows, t);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (t == 0) {
-        mbar_arrive_expect_tx(smem_u32(&bars.tfull[st]), kImgT);
-        bulk_load(base + L::T, a.w.T + cell(it) * kImgT, kImgT, smem_u32(&bars.tfull[st]));
-      }
-      if (t < 64) {
-        const size_t at = cell(it) * 64;
-        const float gi = a.w.gam[at + t], gl = a.w.gam[at + 63], be = a.w.beta[at + t], G = exp_fast(gi);
-        fac[st].beta[t] = be;
-        fac[st].bg[t] = -be * G;
-        fac[st].w[t] = exp_fast(gl - gi);
-        fac[st].sg[t] = a.p.scale * G;
-        if (t == 0) fac[st].last[0] = exp_fast(gl);
-      }
-    };
-    if (nc > 0) load(0);
-    for (int it = 0; it < nc; ++it) {
       const int st = it & 1;
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_async_smem();
-      mbar_arrive(smem_u32(&bars.full[st]));
-      if (REV) {
-        // Q' = scale e^gamma Q in two terms, once its last use (the previous chunk's update) is over
-        if (it > 0) wait(bars.s_done, (it - 1) & 1);
-        wait(bars.full[st], (it >> 1) & 1);
-        __syncwarp();
-#pragma unroll 4
-        for (int e = t; e < 64 * (D / 8); e += kLoaders) {
-          const int r = e / (D / 8), g = e % (D / 8);
-          const uint32_t off = (g >> 3) * 8192 + chunk_at(r, g & 7);
-          float x[8];
-          unpack8<BF>(ld_shared_v4(sb + st * L::kStage + L::KQ + 8192 + (g >> 3) * 16384 + chunk_at(r, g & 7)), x);
-          const float f = fac[st].sg[r];
+      const uint32_t base = sb + st * L::kStage, bar = smem_u32(&bars.full[st]);
+      if (it >= 2) wait(bars.empty[st], ((it >> 1) - 1) & 1);
+      if (lane == 0) {
+        const int t0 = (int)(s.t0 + (int64_t)chunk_of(it) * kChunk), b = (int)s.b;
+        mbar_expect_tx(bar, kBytes);
+        for (int i = 0; i < NB; ++i) {
+          tma_load_4d(base + L::K + 8192 * i, &mk, bar, 64 * i, t0, hk, b);
+          if (MODE != kStore) tma_load_4d(base + L::Q + 8192 * i, &mq, bar, 64 * i, t0, hk, b);
+          tma_load_4d(base + L::V + 8192 * i, &mv, bar, 64 * i, t0, h, b);
+        }
+        const char *img = a.w.T + cell(it) * kImgT;
+        if (MODE == kStore) {  // T alone
+          bulk_load(base + L::T, img, 8192, bar);
+          bulk_load(base + L::T + 16384, img + 16384, 8192, bar);
+        } else {
+          bulk_load(base + L::T, img, kImgT, bar);
+        }
+      }
+      const size_t at = cell(it) * 64;
+      const float gl = a.w.gam[at + 63];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] *= f;
-          uint4 hi, lo;
-          split8<BF>(x, hi, lo);
-          sts(sb + L::QS + off, hi);
-          sts(sb + L::QS + L::kTile + off, lo);
+      for (int i = lane; i < 64; i += 32) {
+        const float gi = a.w.gam[at + i], be = a.w.beta[at + i], G = exp_fast(gi);
+        fac[st].beta[i] = be;
+        fac[st].bg[i] = -be * G;
+        fac[st].w[i] = exp_fast(gl - gi);
+        fac[st].sg[i] = a.p.scale * G;
+      }
+      if (lane == 0) fac[st].last[0] = exp_fast(gl);
+      mbar_arrive(bar);
+      __syncwarp();
+    };
+    for (int it = 0; it < nc + 1; ++it) {
+      if (it < nc) load(it);
+      // a ragged chunk has landed: zeros behind its end
+      if (it > 0 && rows_of(it - 1) < kChunk) {
+        const int st = (it - 1) & 1, rows = rows_of(it - 1);
+        wait(bars.full[st], ((it - 1) >> 1) & 1);
+        for (int tl = 0; tl < 3; ++tl) {
+          if (MODE == kStore && tl == 1) continue;
+          const uint32_t base = sb + st * L::kStage + tl * L::kTile;
+          for (int e = lane; e < (kChunk - rows) * (D / 8); e += 32) {
+            const int r = rows + e / (D / 8), g = e % (D / 8);
+            sts(base + (g >> 3) * 8192 + chunk_at(r, g & 7), make_uint4(0, 0, 0, 0));
+          }
         }
         fence_async_smem();
-        mbar_arrive(smem_u32(&bars.qs_ready));
+        mbar_arrive(smem_u32(&bars.tail));
       }
-      if (it + 1 < nc) load(it + 1);
     }
-  } else if (lane == 0) {
+  } else if (elect_one()) {
     // ---------------------------------------------------------------- products --
+    auto wait = [&](uint64_t &b, uint32_t parity) { mbar_wait(smem_u32(&b), parity, a.p.status, &abort_flag); };
     const uint32_t id_k = idesc_f16(128, 64, BF, false, false), id_mn = idesc_f16(128, 64, BF, false, true);
-    const uint32_t id_u = idesc_f16(128, D, BF, false, true);          // update: N = key channels
-    const uint32_t id_a64 = idesc_f16(128, 64, BF, true, true), id_aD = idesc_f16(128, D, BF, true, true);  // dO^T from shared memory
+    const uint32_t id_u = idesc_f16(128, D, BF, false, true);   // update: N = key channels
+    const uint32_t id_a64 = idesc_f16(128, 64, BF, true, true);  // dO^T from shared memory
     for (int it = 0; it < nc; ++it) {
       const int st = it & 1;
       const uint32_t base = sb + st * L::kStage;
+      const KMajor k_rows(base + L::K, 8192), q_rows(base + L::Q, 8192);
+      const MNMajor k_cols(base + L::K, 8192), q_cols(base + L::Q, 8192);
       wait(bars.full[st], (it >> 1) & 1);
-      wait(bars.s_ready, it & 1);
+      if (rows_of(it) < kChunk) wait(bars.tail, 0);
+      // key channels in the order in which the chain hands them over: quarters 0 and 2, then 1 and 3
+      wait(bars.s_ready[0], it & 1);
       tc_fence_after();
-      const KMajor k_rows(base + L::KQ, 16384), q_rows(base + L::KQ + 8192, 16384);
-      const MNMajor k_cols(base + L::KQ, 16384);
-      issue_ts<D / 16>(tmem + cR1, tmem + cSH, k_rows, id_k, false);
-      issue_ts<D / 16>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+      constexpr int H4 = D / 32;  // steps of half the key channels
+      issue_ts<0, 2>(tmem + cR1, tmem + cSH, k_rows, id_k, false);
+      issue_ts<0, 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+      issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+      issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+      if (D == 128) {
+        wait(bars.s_ready[1], it & 1);
+        tc_fence_after();
+        issue_ts<2, 4>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+        issue_ts<2, 4>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+        issue_ts<6, 8>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+        issue_ts<6, 8>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+      }
       mma_commit(smem_u32(&bars.ks_done));
       if (MODE == kOut) {
         if (it > 0) wait(bars.out_free, (it - 1) & 1);
         tc_fence_after();
-        issue_ts<D / 16>(tmem + cR2, tmem + cSH, q_rows, id_k, false);
-        issue_ts<D / 16>(tmem + cR2, tmem + cSL, q_rows, id_k, true);
+        issue_ts<0, D / 16>(tmem + cR2, tmem + cSH, q_rows, id_k, false);
+        issue_ts<0, D / 16>(tmem + cR2, tmem + cSL, q_rows, id_k, true);
       }
-      wait(bars.tfull[st], (it >> 1) & 1);
-      if (REV) {
-        // dO^T [64 value channels a block] against P T and Q'
+      if (REV) {  // dO^T P T
         const MNMajor dO(base + L::V, 8192);
-        issue<4>(tmem + cR2, dO, MNMajor(base + L::T + 8192, 0), id_a64, false);
-        issue<4>(tmem + cR2, dO, MNMajor(base + L::T + 16384 + 8192, 0), id_a64, true);
-        wait(bars.qs_ready, it & 1);
-        tc_fence_after();
-        issue<4>(tmem + cS, dO, MNMajor(sb + L::QS, 8192), id_aD, true);
-        issue<4>(tmem + cS, dO, MNMajor(sb + L::QS + L::kTile, 8192), id_aD, true);
+        issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 8192, 0), id_a64, false);
+        issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 16384 + 8192, 0), id_a64, true);
       }
       wait(bars.x_ready, it & 1);
       tc_fence_after();
       if (REV) {
         const MNMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
-        issue_ts<4>(tmem + cR2, tmem + cXH, th, id_mn, true);
-        issue_ts<4>(tmem + cR2, tmem + cXH, tl, id_mn, true);
-        issue_ts<4>(tmem + cR2, tmem + cXL, th, id_mn, true);
+        issue_ts<0, 4>(tmem + cR2, tmem + cXH, th, id_mn, true);
+        issue_ts<0, 4>(tmem + cR2, tmem + cXH, tl, id_mn, true);
+        issue_ts<0, 4>(tmem + cR2, tmem + cXL, th, id_mn, true);
+        mma_commit(smem_u32(&bars.u_done));
+        wait(bars.qs_ready, it & 1);
+        tc_fence_after();
+        issue_ts<0, 4>(tmem + cS, tmem + cR3, q_cols, id_u, true);
+        issue_ts<0, 4>(tmem + cS, tmem + cR3 + 32, q_cols, id_u, true);
       } else {
         const KMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
-        issue_ts<4>(tmem + cR1, tmem + cXH, th, id_k, false);
-        issue_ts<4>(tmem + cR1, tmem + cXH, tl, id_k, true);
-        issue_ts<4>(tmem + cR1, tmem + cXL, th, id_k, true);
+        issue_ts<0, 4>(tmem + cR1, tmem + cXH, th, id_k, false);
+        issue_ts<0, 4>(tmem + cR1, tmem + cXH, tl, id_k, true);
+        issue_ts<0, 4>(tmem + cR1, tmem + cXL, th, id_k, true);
+        mma_commit(smem_u32(&bars.u_done));
       }
-      mma_commit(smem_u32(&bars.u_done));
       if (MODE == kOut) {
         const KMajor ph(base + L::T + 8192, 0), pl(base + L::T + 16384 + 8192, 0);
-        issue_ts<4>(tmem + cR3, tmem + cXH, ph, id_k, false);
-        issue_ts<4>(tmem + cR3, tmem + cXH, pl, id_k, true);
-        issue_ts<4>(tmem + cR3, tmem + cXL, ph, id_k, true);
+        issue_ts<0, 4>(tmem + cR3, tmem + cXH, ph, id_k, false);
+        issue_ts<0, 4>(tmem + cR3, tmem + cXH, pl, id_k, true);
+        issue_ts<0, 4>(tmem + cR3, tmem + cXL, ph, id_k, true);
         mma_commit(smem_u32(&bars.o_done));
       }
       wait(bars.up_ready, it & 1);
       tc_fence_after();
       const uint32_t up = tmem + (MODE == kOut ? cSH : cXH);
-      issue_ts<4>(tmem + cS, up, k_cols, id_u, true);
-      issue_ts<4>(tmem + cS, up + 32, k_cols, id_u, true);
+      issue_ts<0, 4>(tmem + cS, up, k_cols, id_u, true);
+      issue_ts<0, 4>(tmem + cS, up + 32, k_cols, id_u, true);
       mma_commit(smem_u32(&bars.s_done));
       mma_commit(smem_u32(&bars.empty[st]));
     }
@@ -764,12 +809,32 @@ constexpr uint32_t prep_smem() {
   return ((kq > mat ? kq : mat) + 1023) / 1024 * 1024 + kImgT;
 }
 
+template <int D, bool BF, int MODE>
+cudaError_t run_scan_mode(const Args &a, cudaStream_t st) {
+  const kda_delta_params &p = a.p;
+  CUtensorMap m[4] = {};
+  if (a.max_chunks > 0 && p.T > 0) {
+    auto view = [](const kda_tensor &t) { return View{t.data, t.stride_b, t.stride_h, t.stride_t, t.stride_d}; };
+    const kda_tensor &v = MODE == kRev ? p.dout : p.v, &o = MODE == kRev ? p.dv : (MODE == kOut ? p.o : p.v);
+    if (!make_tmap_bhtd(&m[0], view(p.k), p.B, p.Hk, p.T, D, BF) || !make_tmap_bhtd(&m[1], view(p.q), p.B, p.Hk, p.T, D, BF) ||
+        !make_tmap_bhtd(&m[2], view(v), p.B, p.H, p.T, D, BF) || !make_tmap_bhtd(&m[3], view(o), p.B, p.H, p.T, D, BF))
+      return cudaErrorInvalidValue;
+  }
+  constexpr uint32_t smem = ScanSmem<D, MODE>::kBytes;
+  cudaError_t e = cudaFuncSetAttribute(scan_kernel<D, BF, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)((a.nseq + (p.cu_seqlens != nullptr ? 1 : 0)) * p.H));
+  if (grid.x == 0) return cudaSuccess;
+  scan_kernel<D, BF, MODE><<<grid, kScanThreads, smem, st>>>(a, m[0], m[1], m[2], m[3]);
+  count_launches(1);
+  return cudaGetLastError();
+}
+
 template <int D, bool BF>
 cudaError_t run_scan(const Args &a, int mode, cudaStream_t st) {
-  const dim3 grid((unsigned)((a.nseq + (a.p.cu_seqlens != nullptr ? 1 : 0)) * a.p.H));
-  if (mode == kOut) return run(scan_kernel<D, BF, kOut>, grid, kScanThreads, ScanSmem<D, kOut>::kBytes, a, st);
-  if (mode == kStore) return run(scan_kernel<D, BF, kStore>, grid, kScanThreads, ScanSmem<D, kStore>::kBytes, a, st);
-  return run(scan_kernel<D, BF, kRev>, grid, kScanThreads, ScanSmem<D, kRev>::kBytes, a, st);
+  if (mode == kOut) return run_scan_mode<D, BF, kOut>(a, st);
+  if (mode == kStore) return run_scan_mode<D, BF, kStore>(a, st);
+  return run_scan_mode<D, BF, kRev>(a, st);
 }
 
 cudaError_t scan(const Args &a, int mode, cudaStream_t st) {

@@ -41,9 +41,9 @@ struct Work {
   float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
   float *beta;     // [chunk][H][64]
   char *T;         // [chunk][H] images of T over P T
-  char *S, *dS;    // [chunk][H] images of the state before / the state gradient after the chunk, transposed:
-                   // hi, then lo, each D / 64 blocks [D value rows x 64 key channels]
-  char *U;         // [chunk][H] images of the chunk's u rows, transposed: [D value rows x 64 tokens] hi, then lo
+  char *S, *dS;    // [chunk][H] images of the state before / the state gradient after the chunk, transposed: hi,
+                   // then lo, each D / 8 runs of [D value rows x 8 key channels]
+  char *U;         // [chunk][H] images of the chunk's u rows, transposed: hi, then lo, each 8 runs of [D value rows x 8 tokens]
   char *dX;        // [chunk][H][D / 64] images of the gradient of X: [64 tokens x 64] hi, then lo
 };
 
@@ -136,6 +136,10 @@ __device__ __forceinline__ void prefetch_rows(const uint16_t *base, int64_t stri
   if (r < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + r * stride_t + c * 64));
 }
 
+// Announce bytes to an mbarrier's phase without arriving on it.
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 // contiguous bytes global -> shared, counted on an mbarrier (sizes and addresses are multiples of 16)
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -149,11 +153,22 @@ __device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t byt
 }
 
 // ------------------------------------------------------------ hi/lo split --
+// lo = round16(x - hi), the difference by a mixed-precision fma that takes hi as it is packed
 template <bool BF>
 __device__ __forceinline__ void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
   hi = pack2(a, b, BF);
-  const float2 h = unpack2(hi, BF);
-  lo = pack2(a - h.x, b - h.y, BF);
+  float x, y;
+  if (BF)
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBF80;\n\t"
+        "fma.rn.f32.bf16 %0, l, m, %3;\n\tfma.rn.f32.bf16 %1, h, m, %4;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(hi), "f"(a), "f"(b));
+  else
+    asm("{\n\t.reg .b16 l, h, m;\n\tmov.b32 {l, h}, %2;\n\tmov.b16 m, 0xBC00;\n\t"
+        "fma.rn.f32.f16 %0, l, m, %3;\n\tfma.rn.f32.f16 %1, h, m, %4;\n\t}"
+        : "=f"(x), "=f"(y)
+        : "r"(hi), "f"(a), "f"(b));
+  lo = pack2(x, y, BF);
 }
 
 // Eight consecutive columns (16-byte chunk c16) of row `row` of a swizzled tile, as hi and lo.
@@ -239,26 +254,49 @@ struct MNMajor {
   __device__ __forceinline__ MNMajor(uint32_t at, uint32_t block_) : base(sdesc_mn(at, block_)) {}
   __device__ __forceinline__ uint64_t desc(int ks) const { return base + (uint64_t)(ks * 128); }
 };
+// MN-major without swizzle, the order in which the scans write their images: 16-byte runs of
+// eight M or N elements, one K row after the other (`rows` rows a run of 8 elements).
+struct MNPlain {
+  uint64_t base;
+  __device__ __forceinline__ MNPlain(uint32_t at, uint32_t rows)
+      : base((uint64_t)((at >> 4) & 0x3FFFu) | (uint64_t)8 << 16 | (uint64_t)(rows & 0x3FFFu) << 32 | (uint64_t)1 << 46) {}
+  __device__ __forceinline__ uint64_t desc(int ks) const { return base + (uint64_t)(ks * 16); }
+};
 template <int STEPS, typename A, typename B>
 __device__ __forceinline__ void issue(uint32_t d, const A &a, const B &b, uint32_t idesc, bool accumulate) {
 #pragma unroll
   for (int ks = 0; ks < STEPS; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
 }
 
-// The same with the first operand in tensor memory: rows = lanes, two consecutive K
-// elements a column, so a step is eight columns.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// One lane of a converged warp.  A branch on it tells the compiler that a single thread
+// issues, and a product then costs 27 cycles to issue against 46 behind a branch on the
+// lane number and 64 when every product is predicated (M = 128, N = 64, K = 16).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+// the thread that issues a CTA's products
+__device__ __forceinline__ bool warp_leader() { return threadIdx.x < 32 && elect_one(); }
+// first operand in tensor memory: rows = lanes, two consecutive K elements a column
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-template <int STEPS, typename B>
+// products with steps [K0, K1) of B and of A (tensor memory, eight columns a step)
+template <int K0, int K1, typename B>
 __device__ __forceinline__ void issue_ts(uint32_t d, uint32_t a, const B &b, uint32_t idesc, bool accumulate) {
 #pragma unroll
-  for (int ks = 0; ks < STEPS; ++ks) mma_f16_ts(d, a + 8 * ks, b.desc(ks), idesc, (accumulate || ks > 0) ? 1u : 0u);
+  for (int ks = K0; ks < K1; ++ks) mma_f16_ts(d, a + 8 * ks, b.desc(ks), idesc, (accumulate || ks > K0) ? 1u : 0u);
+}
+template <int K0, int K1, typename A, typename B>
+__device__ __forceinline__ void issue_ss(uint32_t d, const A &a, const B &b, uint32_t idesc, bool accumulate) {
+#pragma unroll
+  for (int ks = K0; ks < K1; ++ks) mma_f16(d, a.desc(ks), b.desc(ks), idesc, (accumulate || ks > K0) ? 1u : 0u);
 }
 
 // --------------------------------------------------------- CTA scaffolding --

@@ -39,7 +39,7 @@ bool abi_layout_ok(const Tensor &t) {
   if (t.stride(-1) != 1 && t.size(-1) != 1) return false;
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
   for (int64_t i = 0; i + 1 < t.dim(); ++i)
-    if (t.size(i) != 1 && t.stride(i) % 8) return false;
+    if (t.size(i) != 1 && (t.stride(i) % 8 || t.stride(i) == 0)) return false;  // a broadcast dimension has no TMA map
   return true;
 }
 
