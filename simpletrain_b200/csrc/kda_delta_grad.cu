@@ -16,287 +16,351 @@
 // (the y_j enter dgamma_j with a minus and dgamma_63 with a plus; summed this way nothing
 // cancels).
 //
-// One CTA per (chunk, query/key head) walks the value heads that share the head and sums
-// their dq and dk in registers, in order: no atomics, the result does not depend on the
-// launch.  Six products a head, all of them on tiles that are loaded once; the state and
-// its gradient take turns in one 64 KB buffer.  One CTA fills an SM's shared memory.
+// A CTA takes (chunk, query/key head) cells in turn, walks the value heads that share the
+// head and sums their dq and dk in registers, in order: no atomics, the result does not
+// depend on the launch.  The tiles of one value head fill an SM's shared memory, so the
+// next head's are brought into L2 meanwhile; 16 warps, a token row and a quarter of the
+// columns a thread, work off the products.
 #include "kda_delta_tc.cuh"
 
 namespace kda {
 namespace delta {
 namespace {
 
+constexpr int kGradThreads = 512;
+
 template <int D>
 struct GradSmem {
   static constexpr uint32_t kTile = 128 * D * 2;
   static constexpr uint32_t KQ = 0, AH = KQ + kTile, AL = AH + kTile;  // [dX; dO] hi, lo (dO's lo rows: zeros)
-  static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U^T: [D x 64] hi, lo
-  static constexpr uint32_t kBytes = S + 4 * D * D;                    // S^T or dS^T: hi, lo
+  static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U^T: hi, lo
+  static constexpr uint32_t DH = S + 4 * D * D;                        // S^T hi, lo, then dS^T lo over S^T hi; dS^T hi
+  static constexpr uint32_t RED = D == 128 ? AL : DH + 2 * D * D;      // per-row sums (4 KB): where lo tiles are done with
+  static constexpr uint32_t kBytes = DH + 2 * D * D + (D == 128 ? 0 : 4096);
   static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
 };
 
+__device__ __forceinline__ void prefetch_l2(const void *p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
+}
+
+// N consecutive fp32 columns of this warp's lanes
+template <int N>
+__device__ __forceinline__ void tmem_ldn(uint32_t taddr, float (&x)[N]) {
+  static_assert(N == 16 || N == 32, "");
+  if constexpr (N == 32) {
+    tmem_ld32(taddr, x);
+  } else {
+    uint32_t r[16];
+    tmem_ld_32x32b_x16(taddr, r);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+  }
+}
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads, 1) grad_kernel(const Args a) {
+__global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   using L = GradSmem<D>;
-  constexpr int NS = D / 64, W = D / 2;  // W: columns of a D-wide row that a thread owns
+  constexpr int NS = D / 64, W = D / 4;  // W: columns of a D-wide row that a thread owns
   constexpr uint32_t tG1 = 0, tG2 = 64, tG5 = 128, tG6 = 256, tG3 = 0, tG4 = 384;
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
+  __shared__ uint64_t bar_g2, bar_s, bar_d;
   __shared__ __align__(16) float gam[64];
-  __shared__ float sm_q[2][64], sm_k[2][64], sm_t[2][64], sm_y[2][64], sm_xv[2][64], sm_rs[2][64], sm_dot[8];
-  int64_t b, t0;
-  int rows;
-  if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
-  const int tid = threadIdx.x, row = tid & 127, half = tid >> 7, r64 = row & 63;
+  __shared__ float sm_dot[16];
+  typedef float Rows[4][64];  // [quarter][row]
+  Rows &sm_f = *reinterpret_cast<Rows *>(smem + L::RED), &sm_t = (&sm_f)[1], &sm_y = (&sm_f)[2], &sm_d = (&sm_f)[3];
+  const int tid = threadIdx.x, row = tid & 127, part = tid >> 7, r64 = row & 63;
   const bool upper = row >= 64;
-  const int hk = blockIdx.y, G_ = a.p.H / a.p.Hk;
+  const int G_ = a.p.H / a.p.Hk;
   const uint32_t sb = smem_u32(smem), lane_base = (uint32_t)((tid >> 5) & 3) << 21;
-  load_rows<D>(sb + L::KQ, 0, 16384, static_cast<const uint16_t *>(a.p.k.data) + b * a.p.k.stride_b + hk * a.p.k.stride_h + t0 * a.p.k.stride_t,
-               a.p.k.stride_t, rows);
-  load_rows<D>(sb + L::KQ, 64, 16384, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
-               a.p.q.stride_t, rows);
+  if (tid == 0) {
+    mbar_init(smem_u32(&bar_g2), 1);
+    mbar_init(smem_u32(&bar_s), 1);
+    mbar_init(smem_u32(&bar_d), 1);
+  }
   const uint32_t tmem = cta_begin(ctl, 512);
   const uint32_t lane_t = tmem + lane_base;
-  uint32_t ph = 0, ph_load = 0;
-  float acc[W];
-#pragma unroll
-  for (int j = 0; j < W; ++j) acc[j] = 0.f;
-  // this thread's row of the [K; Q] tile against a D-wide row of values, W columns of it
-  auto kq_chunk = [&](int c) { return ld_shared_v4(sb + L::KQ + ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c)); };
+  uint32_t ph = 0;  // every barrier completes once a value head (bar_g2 twice)
+  // this thread's W columns of its row of the [K; Q] tile, eight at a time
+  auto kq_chunk = [&](int c) { return ld_shared_v4(sb + L::KQ + ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c)); };
+  auto rows_at = [](const kda_tensor &x, int64_t b, int64_t hd, int64_t t) {
+    return static_cast<uint16_t *>(x.data) + b * x.stride_b + hd * x.stride_h + t * x.stride_t;
+  };
 
-  for (int hh = 0; hh < G_; ++hh) {
-    const int h = hk * G_ + hh;
-    const size_t ch = (size_t)blockIdx.x * a.p.H + h;
-    const char *gS = a.w.S + ch * (size_t)(D * D * 4), *gD = a.w.dS + ch * (size_t)(D * D * 4);
-    if (tid == 0) {
-      const uint32_t bar = smem_u32(&ctl.load_bar);
-      mbar_arrive_expect_tx(bar, NS * (16384 + 16384 + D * 256));
-      for (int s = 0; s < NS; ++s) {
-        const char *x = a.w.dX + (ch * NS + s) * (size_t)16384;
-        bulk_load(sb + L::AH + s * 16384, x, 8192, bar);
-        bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, bar);
+  for (int u = blockIdx.x; u < a.max_chunks * a.p.Hk; u += gridDim.x) {
+    const int cidx = u / a.p.Hk, hk = u % a.p.Hk;
+    int64_t b, t0;
+    int rows;
+    if (!get_chunk(a, cidx, &b, &t0, &rows)) break;  // the last chunks of the bound do not exist
+    auto load64 = [&](uint32_t tile, int row0, const uint16_t *src, int64_t stride) {
+      constexpr int P = D / 8;
+#pragma unroll
+      for (int i = 0; i < 64 * P / kGradThreads; ++i) {
+        const int p = tid + i * kGradThreads, r = p / P, c = p % P, tr = row0 + r;
+        cp_async16(tile + (c >> 3) * 16384 + chunk_at(tr, c & 7), src + (r < rows ? r * stride : 0) + c * 8, r < rows);
       }
-      bulk_load(sb + L::U, a.w.U + ch * (size_t)(D * 256), D * 256, bar);
-      bulk_load(sb + L::S, gS, NS * D * 256, bar);
-    }
-    load_rows<D>(sb + L::AH, 64, 16384, static_cast<const uint16_t *>(a.p.dout.data) + b * a.p.dout.stride_b + h * a.p.dout.stride_h + t0 * a.p.dout.stride_t,
-                 a.p.dout.stride_t, rows);
-    if (upper)
+    };
+    load64(sb + L::KQ, 0, rows_at(a.p.k, b, hk, t0), a.p.k.stride_t);
+    load64(sb + L::KQ, 64, rows_at(a.p.q, b, hk, t0), a.p.q.stride_t);
+    float acc[W];
 #pragma unroll
-      for (int c = 0; c < W / 8; ++c)
-        sts(sb + L::AL + ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c), make_uint4(0, 0, 0, 0));
-    if (tid < 64) gam[tid] = a.w.gam[ch * 64 + tid];
-    const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
-    const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
-    cp_async_wait();
-    publish();
-    mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
-    ph_load ^= 1;
-    __syncwarp();
-    if (warp_leader()) {
-      tc_fence_after();
-      const uint32_t id64 = idesc_f16(128, 64, BF, false, false), id64t = idesc_f16(128, 64, BF, false, true);
-      const uint32_t idD = idesc_f16(128, D, BF, false, true);
-      issue<D / 16>(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, id64, false);
-      const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384};
-      const MNPlain uh{sb + L::U, D}, ul{sb + L::U + D * 128, D};
-      const MNPlain sh{sb + L::S, D}, sl{sb + L::S + D * D * 2, D};
-      issue<D / 16>(tmem + tG2, ah, uh, id64t, false);
-      issue<D / 16>(tmem + tG2, ah, ul, id64t, true);
-      issue<D / 16>(tmem + tG2, al, uh, id64t, true);
-      issue<D / 16>(tmem + tG5, ah, sh, idD, false);
-      issue<D / 16>(tmem + tG5, ah, sl, idD, true);
-      issue<D / 16>(tmem + tG5, al, sh, idD, true);
-      mma_commit(smem_u32(&ctl.mma_bar));
-    }
-    // meanwhile: <S, dS> (same place in both images), and dX . v
-    float dot = 0.f;
-    for (int e = tid; e < D * D / 8; e += kThreads) {
-      const uint32_t off = e * 16;
-      float x[8], y[8], z[8];
-      unpack8<BF>(ld_shared_v4(sb + L::S + off), x);
-      unpack8<BF>(ld_shared_v4(sb + L::S + off + D * D * 2), y);
+    for (int j = 0; j < W; ++j) acc[j] = 0.f;
+
+    for (int hh = 0; hh < G_; ++hh) {
+      const int h = hk * G_ + hh;
+      const size_t ch = (size_t)cidx * a.p.H + h;
+      const char *gD = a.w.dS + ch * (size_t)(D * D * 4);
+      if (tid == 0) {
+        const uint32_t b1 = smem_u32(&ctl.load_bar), b2 = smem_u32(&bar_s);
+        mbar_arrive_expect_tx(b1, NS * 16384 + D * 256);
+        for (int s = 0; s < NS; ++s) {
+          const char *x = a.w.dX + (ch * NS + s) * (size_t)16384;
+          bulk_load(sb + L::AH + s * 16384, x, 8192, b1);
+          bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, b1);
+        }
+        bulk_load(sb + L::U, a.w.U + ch * (size_t)(D * 256), D * 256, b1);
+        mbar_arrive_expect_tx(b2, D * D * 6);
+        bulk_load(sb + L::S, a.w.S + ch * (size_t)(D * D * 4), D * D * 4, b2);
+        bulk_load(sb + L::DH, gD, D * D * 2, b2);
+        prefetch_l2(gD + D * D * 2, D * D * 2);
+        // the next value head's images
+        size_t nx = ch + 1;
+        bool more = hh + 1 < G_;
+        if (!more && u + (int)gridDim.x < a.max_chunks * a.p.Hk) {
+          const int un = u + gridDim.x;
+          nx = (size_t)(un / a.p.Hk) * a.p.H + (size_t)(un % a.p.Hk) * G_;
+          more = true;
+        }
+        if (more) {
+          prefetch_l2(a.w.dX + nx * (size_t)(D * 256), D * 256);
+          prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
+          prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
+          prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
+        }
+      }
+      load64(sb + L::AH, 64, rows_at(a.p.dout, b, h, t0), a.p.dout.stride_t);
+      if (upper)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] += y[j];
-      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off), y);
-      unpack8<BF>(*reinterpret_cast<const uint4 *>(gD + off + D * D * 2), z);
+        for (int c = 0; c < W / 8; ++c)
+          sts(sb + L::AL + ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c), make_uint4(0, 0, 0, 0));
+      if (tid < 64) gam[tid] = a.w.gam[ch * 64 + tid];
+      const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
+      const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
+      uint4 vraw[W / 8];  // this row of V
+      if (!upper)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j] + z[j], dot);
-    }
-    for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    if ((tid & 31) == 0) sm_dot[tid >> 5] = dot;
-    if (!upper) {
+        for (int c = 0; c < W / 8; ++c)
+          vraw[c] = r64 < rows ? *reinterpret_cast<const uint4 *>(rows_at(a.p.v, b, h, t0 + r64) + part * W + 8 * c) : make_uint4(0, 0, 0, 0);
+      cp_async_wait();
+      publish();
+      if (warp_leader()) {
+        mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
+        tc_fence_after();
+        const uint32_t id64 = idesc_f16(128, 64, BF, false, false), id64t = idesc_f16(128, 64, BF, false, true);
+        const uint32_t idD = idesc_f16(128, D, BF, false, true), id6 = idesc_f16(128, D, BF, true, true);
+        issue<D / 16>(tmem + tG1, KMajor{sb + L::KQ, 16384}, KMajor{sb + L::KQ, 16384}, id64, false);
+        const KMajor ah{sb + L::AH, 16384}, al{sb + L::AL, 16384};
+        const MNPlain uh{sb + L::U, D}, ul{sb + L::U + D * 128, D};
+        issue<D / 16>(tmem + tG2, ah, uh, id64t, false);
+        issue<D / 16>(tmem + tG2, ah, ul, id64t, true);
+        issue<D / 16>(tmem + tG2, al, uh, id64t, true);
+        mma_commit(smem_u32(&bar_g2));
+        mbar_wait(smem_u32(&bar_s), ph, a.p.status, &ctl.abort);
+        tc_fence_after();
+        const MNPlain sh{sb + L::S, D}, sl{sb + L::S + D * D * 2, D}, dh{sb + L::DH, D};
+        issue<D / 16>(tmem + tG5, ah, sh, idD, false);
+        issue<D / 16>(tmem + tG5, ah, sl, idD, true);
+        issue<D / 16>(tmem + tG5, al, sh, idD, true);
+        // 64 rows (tokens); the other 64 read bytes behind and are not used
+        issue<D / 16>(tmem + tG6, uh, dh, id6, false);
+        issue<D / 16>(tmem + tG6, ul, dh, id6, true);
+        mma_commit(smem_u32(&ctl.mma_bar));
+      }
+      __syncwarp();
+      // meanwhile dX . v and <S, dS> (same place in both images)
+      mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
       float xv = 0.f;
-      if (r64 < rows) {
-        const uint16_t *vp = static_cast<const uint16_t *>(a.p.v.data) + b * a.p.v.stride_b + h * a.p.v.stride_h + (t0 + r64) * a.p.v.stride_t + half * W;
+      if (!upper) {
 #pragma unroll
         for (int c = 0; c < W / 8; ++c) {
-          const uint32_t at = ((half * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((half * W) >> 3) + c);
+          const uint32_t at = ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c);
           float x[8], y[8], v[8];
           unpack8<BF>(ld_shared_v4(sb + L::AH + at), x);
           unpack8<BF>(ld_shared_v4(sb + L::AL + at), y);
-          unpack8<BF>(*reinterpret_cast<const uint4 *>(vp + 8 * c), v);
+          unpack8<BF>(vraw[c], v);
 #pragma unroll
           for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
         }
       }
-      sm_xv[half][r64] = xv;
-    }
-    wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
-    // M, N over the dX / dO tiles (all their products are done); every thread is past its reads of them
-    float x[32];
-    {
-      float y[32];
-      tmem_ld32(lane_t + tG1 + 32 * half, x);
-      tmem_ld32(lane_t + tG2 + 32 * half, y);
-      float rs = 0.f;
+      mbar_wait(smem_u32(&bar_s), ph, a.p.status, &ctl.abort);
+      float dot = 0.f;
+#pragma unroll 2
+      for (int e = tid; e < D * D / 8; e += kGradThreads) {
+        const uint32_t off = e * 16;
+        float x[8], y[8], z[8];
+        const uint4 lo = *reinterpret_cast<const uint4 *>(gD + off + D * D * 2);
+        unpack8<BF>(ld_shared_v4(sb + L::S + off), x);
+        unpack8<BF>(ld_shared_v4(sb + L::S + off + D * D * 2), y);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const int col = 32 * half + j;
-        const float e = ex2f((gi - gam[col]) * kLog2e);
-        if (!upper) {
-          const float m = col < r64 ? -y[j] * e : 0.f;
-          rs = col < r64 ? fmaf(m, x[j], rs) : rs;
-          x[j] = m * bi;
-        } else {
-          x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
-        }
+        for (int j = 0; j < 8; ++j) x[j] += y[j];
+        unpack8<BF>(ld_shared_v4(sb + L::DH + off), y);
+        unpack8<BF>(lo, z);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j] + z[j], dot);
       }
-      if (!upper) sm_rs[half][r64] = rs;
-    }
-    publish();
-    if (tid == 0) {
-      const uint32_t bar = smem_u32(&ctl.load_bar);
-      mbar_arrive_expect_tx(bar, NS * D * 256);
-      bulk_load(sb + L::S, gD, NS * D * 256, bar);  // the state's products and dot are done
-    }
-    store_split32<BF>(sb + L::MN, sb + L::MN + 16384, row, half, x);
-    publish();
-    if (warp_leader()) {
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if ((tid & 31) == 0) sm_dot[tid >> 5] = dot;
+      // M, N (16 columns)
+      mbar_wait(smem_u32(&bar_g2), 0, a.p.status, &ctl.abort);
+      __syncwarp();
       tc_fence_after();
-      const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
-      const MNMajor kq{sb + L::KQ, 16384};
-      issue<4>(tmem + tG3, KMajor{sb + L::MN, 0}, kq, id3, false);
-      issue<4>(tmem + tG3, KMajor{sb + L::MN + 16384, 0}, kq, id3, true);
-      // 64 rows (k tokens); the other 64 are not used
-      issue<8>(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, id4, false);
-      issue<8>(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, id4, true);
-      mbar_wait(smem_u32(&ctl.load_bar), ph_load, a.p.status, &ctl.abort);
-      const uint32_t id6 = idesc_f16(128, D, BF, true, true);
-      // 64 rows (tokens); the other 64 read bytes behind and are not used
-      const MNPlain uh{sb + L::U, D}, ul{sb + L::U + D * 128, D};
-      const MNPlain dh{sb + L::S, D}, dl{sb + L::S + D * D * 2, D};
-      issue<D / 16>(tmem + tG6, uh, dh, id6, false);
-      issue<D / 16>(tmem + tG6, uh, dl, id6, true);
-      issue<D / 16>(tmem + tG6, ul, dh, id6, true);
-      mma_commit(smem_u32(&ctl.mma_bar));
-    }
-    ph_load ^= 1;
-    // meanwhile the terms through the state
-    float dq_dot = 0.f, t_dot = 0.f, k_dot = 0.f, y_dot = 0.f;
+      uint4 mh[2], ml[2];
+      {
+        float x[16], y[16];
+        tmem_ldn<16>(lane_t + tG1 + 16 * part, x);
+        tmem_ldn<16>(lane_t + tG2 + 16 * part, y);
 #pragma unroll
-    for (int c0 = 0; c0 < W; c0 += 32) {
-      tmem_ld32(lane_t + tG5 + half * W + c0, x);
-      const float f = upper ? a.p.scale * Gi : -Gi * bi;
+        for (int j = 0; j < 16; ++j) {
+          const int col = 16 * part + j;
+          const float e = ex2f((gi - gam[col]) * kLog2e);
+          if (!upper) {
+            const float m = col < r64 ? -y[j] * e : 0.f;
+            xv = col < r64 ? fmaf(m, x[j], xv) : xv;
+            x[j] = m * bi;
+          } else {
+            x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
+          }
+        }
+        split8<BF>(x, mh[0], ml[0]);
+        split8<BF>(x + 8, mh[1], ml[1]);
+      }
+      // over the dX / dO tiles once their products are done and every thread is past its reads of them and of S
+      mbar_wait(smem_u32(&ctl.mma_bar), ph, a.p.status, &ctl.abort);
+      __syncwarp();
+      tc_fence_after();
+      publish();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float k[8];
-        unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+      for (int c = 0; c < 2; ++c) {
+        sts(sb + L::MN + chunk_at(row, 2 * part + c), mh[c]);
+        sts(sb + L::MN + 16384 + chunk_at(row, 2 * part + c), ml[c]);
+      }
+      if (tid == 32) {
+        mbar_arrive_expect_tx(smem_u32(&bar_d), D * D * 2);
+        bulk_load(sb + L::S, gD + D * D * 2, D * D * 2, smem_u32(&bar_d));
+      }
+      publish();
+      if (warp_leader()) {
+        tc_fence_after();
+        const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
+        const MNMajor kq{sb + L::KQ, 16384};
+        issue<4>(tmem + tG3, KMajor{sb + L::MN, 0}, kq, id3, false);
+        issue<4>(tmem + tG3, KMajor{sb + L::MN + 16384, 0}, kq, id3, true);
+        // 64 rows (k tokens); the other 64 are not used
+        issue<8>(tmem + tG4, MNMajor{sb + L::MN, 16384}, kq, id4, false);
+        issue<8>(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, id4, true);
+        mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
+        tc_fence_after();
+        issue<D / 16>(tmem + tG6, MNPlain{sb + L::U, D}, MNPlain{sb + L::S, D}, idesc_f16(128, D, BF, true, true), true);
+        mma_commit(smem_u32(&bar_g2));
+      }
+      __syncwarp();
+      // meanwhile the terms through the state
+      float f_dot = 0.f, t_dot = 0.f, y_dot = 0.f;
+      {
+        float x[W];
+        tmem_ldn<W>(lane_t + tG5 + part * W, x);
+        const float f = upper ? a.p.scale * Gi : -Gi * bi;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float v = f * x[8 * c + j];
-          t_dot = fmaf(k[j], upper ? v : x[8 * c + j], t_dot);
-          acc[c0 + 8 * c + j] += v;
+        for (int c = 0; c < W / 8; ++c) {
+          float k[8];
+          unpack8<BF>(kq_chunk(c), k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            t_dot = fmaf(k[j], x[8 * c + j], t_dot);
+            acc[8 * c + j] = fmaf(f, x[8 * c + j], acc[8 * c + j]);
+          }
+        }
+        f_dot = f * t_dot;
+      }
+      mbar_wait(smem_u32(&bar_g2), 1, a.p.status, &ctl.abort);
+      __syncwarp();
+      tc_fence_after();
+#pragma unroll
+      for (int c0 = 0; c0 < W; c0 += 16) {
+        float x[16], y[16], z[16];
+        tmem_ldn<16>(lane_t + tG3 + part * W + c0, x);
+        if (!upper) {
+          tmem_ldn<16>(lane_t + tG4 + part * W + c0, y);
+          tmem_ldn<16>(lane_t + tG6 + part * W + c0, z);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float k[8];
+          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int i = 8 * c + j;
+            if (upper) {
+              f_dot = fmaf(k[j], x[i], f_dot);
+              acc[c0 + i] += x[i];
+            } else {
+              const float v = wi * z[i];
+              f_dot = fmaf(k[j], x[i] - y[i], f_dot);  // k.(M K) - k.(M^T K + N^T Q)
+              y_dot = fmaf(k[j], v, y_dot);
+              acc[c0 + i] += (x[i] + y[i]) + v;
+            }
+          }
         }
       }
-    }
-    wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
-#pragma unroll
-    for (int c0 = 0; c0 < W; c0 += 32) {
-      tmem_ld32(lane_t + tG3 + half * W + c0, x);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float k[8];
-        unpack8<BF>(kq_chunk(c0 / 8 + c), k);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          dq_dot = fmaf(k[j], x[8 * c + j], dq_dot);
-          acc[c0 + 8 * c + j] += x[8 * c + j];
-        }
-      }
+      if (upper) sm_f[part][r64] = f_dot;
+      __syncthreads();
       if (!upper) {
-        tmem_ld32(lane_t + tG4 + half * W + c0, x);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float k[8];
-          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            k_dot = fmaf(k[j], x[8 * c + j], k_dot);
-            acc[c0 + 8 * c + j] += x[8 * c + j];
-          }
+        sm_f[part][r64] += f_dot;
+        sm_t[part][r64] = t_dot;
+        sm_y[part][r64] = y_dot;
+        sm_d[part][r64] = xv;  // dX.v - sum_j (dX U^T)_ij e_ij k_i.k_j
+      }
+      tc_fence_before();
+      __syncthreads();
+      tc_fence_after();
+      if (tid < 32) {
+        float f[2], y[2];
+        float sd = 0.f;
+        for (int w = 0; w < 16; ++w) sd += sm_dot[w];
+        sd *= exp_fast(gam[63]);
+        auto four = [](const float (&s)[4][64], int i) { return (s[0][i] + s[1][i]) + (s[2][i] + s[3][i]); };
+        for (int j = 0; j < 2; ++j) {
+          const int i = 2 * tid + j;
+          f[j] = four(sm_f, i);
+          y[j] = four(sm_y, i);
+          if (i < rows)
+            store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype, four(sm_d, i) - exp_fast(gam[i]) * four(sm_t, i));
         }
-        tmem_ld32(lane_t + tG6 + half * W + c0, x);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float k[8];
-          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float v = wi * x[8 * c + j];
-            y_dot = fmaf(k[j], v, y_dot);
-            acc[c0 + 8 * c + j] += v;
-          }
+        // suffix sums of f, exclusive prefix sums of y
+        float sf = f[0] + f[1], py = y[0] + y[1];
+        for (int o = 1; o < 32; o <<= 1) {
+          const float un = __shfl_down_sync(0xffffffffu, sf, o), v = __shfl_up_sync(0xffffffffu, py, o);
+          if (tid + o < 32) sf += un;
+          if (tid >= o) py += v;
         }
+        const float next = __shfl_down_sync(0xffffffffu, sf, 1), prev = __shfl_up_sync(0xffffffffu, py, 1);
+        const float s1 = f[1] + (tid < 31 ? next : 0.f), p0 = tid > 0 ? prev : 0.f;
+        if (2 * tid < rows) store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid, a.p.g_dtype, (f[0] + s1) + p0 + sd);
+        if (2 * tid + 1 < rows)
+          store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid + 1, a.p.g_dtype, s1 + (p0 + y[0]) + sd);
       }
+      ph ^= 1;
+      fence_async_smem();  // the next tiles are written over what was read here
+      __syncthreads();
     }
-    if (upper) {
-      sm_q[half][r64] = dq_dot + t_dot;
-    } else {
-      sm_k[half][r64] = dq_dot - k_dot;  // k.(M K) - k.(M^T K + N^T Q)
-      sm_t[half][r64] = t_dot;
-      sm_y[half][r64] = y_dot;
-    }
-    __syncthreads();
-    if (tid < 32) {
-      float f[2], y[2];
-      const float last = exp_fast(gam[63]);
-      float sd = 0.f;
-      for (int w = 0; w < 8; ++w) sd += sm_dot[w];
-      sd *= last;
-      for (int j = 0; j < 2; ++j) {
-        const int i = 2 * tid + j;
-        const float G = exp_fast(gam[i]), be = a.w.beta[ch * 64 + i], t = sm_t[0][i] + sm_t[1][i];
-        f[j] = (sm_q[0][i] + sm_q[1][i]) + (sm_k[0][i] + sm_k[1][i]) - G * be * t;
-        y[j] = sm_y[0][i] + sm_y[1][i];
-        if (i < rows)
-          store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype,
-                     (sm_xv[0][i] + sm_xv[1][i]) - G * t + (sm_rs[0][i] + sm_rs[1][i]));
-      }
-      // suffix sums of f, exclusive prefix sums of y
-      float sf = f[0] + f[1], py = y[0] + y[1];
-      for (int o = 1; o < 32; o <<= 1) {
-        const float u = __shfl_down_sync(0xffffffffu, sf, o), v = __shfl_up_sync(0xffffffffu, py, o);
-        if (tid + o < 32) sf += u;
-        if (tid >= o) py += v;
-      }
-      const float next = __shfl_down_sync(0xffffffffu, sf, 1), prev = __shfl_up_sync(0xffffffffu, py, 1);
-      const float s1 = f[1] + (tid < 31 ? next : 0.f), p0 = tid > 0 ? prev : 0.f;
-      if (2 * tid < rows) store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid, a.p.g_dtype, (f[0] + s1) + p0 + sd);
-      if (2 * tid + 1 < rows)
-        store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid + 1, a.p.g_dtype, s1 + (p0 + y[0]) + sd);
-    }
-    __syncthreads();
-  }
-  if (r64 < rows) {
-    const kda_tensor &o = upper ? a.p.dq : a.p.dk;
-    uint16_t *dst = static_cast<uint16_t *>(o.data) + b * o.stride_b + hk * o.stride_h + (t0 + r64) * o.stride_t + half * W;
+    if (r64 < rows) {
+      uint16_t *dst = rows_at(upper ? a.p.dq : a.p.dk, b, hk, t0 + r64) + part * W;
 #pragma unroll
-    for (int c0 = 0; c0 < W; c0 += 32) {
-      float x[32];
-#pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] = acc[c0 + j];
-      store_row32<BF>(dst + c0, x);
+      for (int c = 0; c < W / 8; ++c)
+        *reinterpret_cast<uint4 *>(dst + 8 * c) =
+            make_uint4(pack2(acc[8 * c], acc[8 * c + 1], BF), pack2(acc[8 * c + 2], acc[8 * c + 3], BF),
+                       pack2(acc[8 * c + 4], acc[8 * c + 5], BF), pack2(acc[8 * c + 6], acc[8 * c + 7], BF));
     }
   }
   cta_end(tmem, 512);
@@ -307,7 +371,11 @@ cudaError_t run_grad(const Args &a, cudaStream_t st) {
   constexpr uint32_t smem = GradSmem<D>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(grad_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  grad_kernel<D, BF><<<dim3((unsigned)a.max_chunks, (unsigned)a.p.Hk), kThreads, smem, st>>>(a);
+  int dev = 0, sms = 0;
+  if ((e = cudaGetDevice(&dev)) != cudaSuccess || (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
+    return e;
+  const int64_t cells = (int64_t)a.max_chunks * a.p.Hk;
+  grad_kernel<D, BF><<<(unsigned)(cells < sms ? cells : sms), kGradThreads, smem, st>>>(a);
   count_launches(1);
   return cudaGetLastError();
 }
@@ -343,7 +411,7 @@ int check_sizes(const kda_delta_params *p) {
   const int64_t nseq = p->cu_seqlens != nullptr ? (int64_t)p->nseq + 1 : p->B;
   if (nseq * p->H * 2 > 0x7fffffff) return KDA_ERR_BAD_SHAPE;
   const int64_t chunks = p->cu_seqlens != nullptr ? (int64_t)p->T / 64 + p->nseq : (int64_t)p->B * (((int64_t)p->T + 63) / 64);
-  if (chunks > 0x7fffffff) return KDA_ERR_BAD_SHAPE;
+  if (chunks * p->H > 0x3fffffff) return KDA_ERR_BAD_SHAPE;
   return KDA_OK;
 }
 
