@@ -85,11 +85,12 @@ constexpr int kLd = 68;  // row stride (floats) of the fp32 64 x 64 matrices: ve
 // One CTA per (chunk, head): T and P T as two-term images, gamma and beta in fp32.
 // The products are k.k, q.k and P T; (I + A)^-1 is by halves in fp32: four 16 x 16 blocks
 // by substitution, a column a thread, then [A 0; B C]^-1 = [a 0; -c B a, c] twice.
+// The q.k rows wait in registers while the inverse is formed, so that the k and q tiles, the
+// fp32 matrices and the two-term tiles can take turns in 34 KB, and four CTAs share an SM:
+// the kernel is a chain of short dependent steps, hidden by other CTAs only.
 template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
-  constexpr uint32_t KQ = 0, kKQ = 128 * D * 2;
-  constexpr uint32_t kMat = 2 * 64 * kLd * 4;
-  constexpr uint32_t TT = ((kKQ > kMat ? kKQ : kMat) + 1023) / 1024 * 1024;  // [T; P] hi, then lo
+__global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
+  constexpr uint32_t KQ = 0, TT = 0;  // [T; P] hi, then lo, over the rest
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
   __shared__ __align__(16) float gam[64], bet[64];
@@ -103,7 +104,7 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
                a.p.k.stride_t, rows);
   load_rows<D>(sb + KQ, 64, 16384, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
                a.p.q.stride_t, rows);
-  const uint32_t tmem = cta_begin(ctl, 128);
+  const uint32_t tmem = cta_begin(ctl, 64);
   const size_t ch = (size_t)blockIdx.x * a.p.H + h;
   if (tid < 32) {
     // running sums in double: rounded once, so that differences of gammas keep fp32's last bits
@@ -137,8 +138,8 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   float *As = reinterpret_cast<float *>(smem + KQ);  // over the k and q tiles: their product is done
   float *Ti = As + 64 * kLd;
+  float x[32];  // 32 columns of a row of A (rows of k) or P (rows of q)
   {
-    float x[32];
     tmem_ld32(tmem + lane_base + 32 * half, x);
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
@@ -153,24 +154,24 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
 #pragma unroll
       for (int j = 0; j < 32; j += 4)
         *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-    } else {
-      store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
     }
   }
+  tc_fence_before();
   __syncthreads();
+  tc_fence_after();
   if (tid < 64) {
     // column j of the inverse of diagonal block blk
     const int blk = tid >> 4, j = tid & 15, o = 16 * blk;
-    float x[16];
+    float y[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s = i == j ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) s = fmaf(-As[(o + i) * kLd + o + m], x[m], s);
-      x[i] = i < j ? 0.f : s;
+      for (int m = 0; m < i; ++m) s = fmaf(-As[(o + i) * kLd + o + m], y[m], s);
+      y[i] = i < j ? 0.f : s;
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i) Ti[(o + i) * kLd + o + j] = x[i];
+    for (int i = 0; i < 16; ++i) Ti[(o + i) * kLd + o + j] = y[i];
   } else {
     // the blocks above the diagonal
     for (int e = tid - 64; e < 4096; e += kThreads - 64) {
@@ -215,7 +216,6 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
     __syncthreads();
   }
   if (row < 64) {
-    float x[32];
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 r = *reinterpret_cast<const float4 *>(Ti + r64 * kLd + 32 * half + j);
@@ -224,8 +224,9 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
       x[j + 2] = r.z;
       x[j + 3] = r.w;
     }
-    store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
   }
+  __syncthreads();
+  store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
   publish();
   if (warp_leader()) {
     tc_fence_after();
@@ -233,19 +234,18 @@ __global__ void __launch_bounds__(kThreads) prep_kernel(const Args a) {
     const uint32_t id = idesc_f16(128, 64, BF, false, true);
     const KMajor ph_{sb + TT, 0}, pl{sb + TT + 16384, 0};
     const MNMajor th{sb + TT, 0}, tl{sb + TT + 16384, 0};
-    issue<4>(tmem + 64, ph_, th, id, false);
-    issue<4>(tmem + 64, ph_, tl, id, true);
-    issue<4>(tmem + 64, pl, th, id, true);
+    issue<4>(tmem, ph_, th, id, false);
+    issue<4>(tmem, ph_, tl, id, true);
+    issue<4>(tmem, pl, th, id, true);
     mma_commit(smem_u32(&ctl.mma_bar));
   }
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   if (row >= 64) {
-    float x[32];
-    tmem_ld32(tmem + lane_base + 64 + 32 * half, x);
+    tmem_ld32(tmem + lane_base + 32 * half, x);
     store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
   }
   fence_async_smem();
-  cta_end(tmem, 128);
+  cta_end(tmem, 64);
   if (tid == 0) {
     bulk_store(a.w.T + ch * kImgT, sb + TT, kImgT);
     tma_store_commit();
@@ -805,8 +805,8 @@ cudaError_t run(K kern, dim3 grid, int threads, uint32_t smem, const Args &a, cu
 
 template <int D>
 constexpr uint32_t prep_smem() {
-  constexpr uint32_t kq = 128 * D * 2, mat = 2 * 64 * kLd * 4;
-  return ((kq > mat ? kq : mat) + 1023) / 1024 * 1024 + kImgT;
+  constexpr uint32_t kq = 128 * D * 2, mat = 2 * 64 * kLd * 4;  // and 32 KB of two-term tiles
+  return kq > mat ? kq : mat;
 }
 
 template <int D, bool BF, int MODE>
