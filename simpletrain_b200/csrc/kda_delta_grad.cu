@@ -34,14 +34,20 @@ struct GradSmem {
   static constexpr uint32_t kTile = 128 * D * 2;
   static constexpr uint32_t KQ = 0, AH = KQ + kTile, AL = AH + kTile;  // [dX; dO] hi, lo (dO's lo rows: zeros)
   static constexpr uint32_t U = AL + kTile, S = U + 256 * D;           // U^T: hi, lo
-  static constexpr uint32_t DH = S + 4 * D * D;                        // S^T hi, lo, then dS^T lo over S^T hi; dS^T hi
-  static constexpr uint32_t RED = D == 128 ? AL : DH + 2 * D * D;      // per-row sums (4 KB): where lo tiles are done with
-  static constexpr uint32_t kBytes = DH + 2 * D * D + (D == 128 ? 0 : 4096);
+  static constexpr uint32_t DH = S + 4 * D * D;                        // S^T hi, lo, then dS^T lo over S^T lo; dS^T hi
+  static constexpr uint32_t kBytes = DH + 2 * D * D;
   static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
 };
 
-__device__ __forceinline__ void prefetch_l2(const void *p, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
+// This thread's 128-byte lines of `bytes` contiguous bytes, into L2.
+__device__ __forceinline__ void prefetch_l2(const char *p, uint32_t bytes) {
+  for (uint32_t o = threadIdx.x * 128; o < bytes; o += kGradThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
+}
+// the same for `rows` (of 64) rows of D 16-bit elements
+template <int D>
+__device__ __forceinline__ void prefetch_l2_rows(const uint16_t *p, int64_t stride, int rows) {
+  const int r = threadIdx.x / (D / 64), c = threadIdx.x % (D / 64);
+  if (r < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + r * stride + c * 64));
 }
 
 // N consecutive fp32 columns of this warp's lanes
@@ -67,12 +73,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   __shared__ Ctl ctl;
   __shared__ uint64_t bar_g2, bar_s, bar_d;
   __shared__ __align__(16) float gam[64];
-  __shared__ float sm_dot[16];
-  typedef float Rows[4][64];  // [quarter][row]
-  Rows &sm_f = *reinterpret_cast<Rows *>(smem + L::RED), &sm_t = (&sm_f)[1], &sm_y = (&sm_f)[2], &sm_d = (&sm_f)[3];
+  __shared__ float sm_dot[16], sm_xv[64];
+  __shared__ float sm_f[2][64], sm_t[2][64], sm_y[2][64], sm_r[2][64];  // [half of the columns][row]
   const int tid = threadIdx.x, row = tid & 127, part = tid >> 7, r64 = row & 63;
   const bool upper = row >= 64;
-  const int G_ = a.p.H / a.p.Hk;
+  const int G_ = a.p.H / a.p.Hk, cells = a.max_chunks * a.p.Hk;
   const uint32_t sb = smem_u32(smem), lane_base = (uint32_t)((tid >> 5) & 3) << 21;
   if (tid == 0) {
     mbar_init(smem_u32(&bar_g2), 1);
@@ -82,76 +87,71 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   const uint32_t tmem = cta_begin(ctl, 512);
   const uint32_t lane_t = tmem + lane_base;
   uint32_t ph = 0;  // every barrier completes once a value head (bar_g2 twice)
-  // this thread's W columns of its row of the [K; Q] tile, eight at a time
-  auto kq_chunk = [&](int c) { return ld_shared_v4(sb + L::KQ + ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c)); };
+  // this thread's W columns of its row of a [128 x D] tile, eight at a time
+  auto own_chunk = [&](int c) { return ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c); };
   auto rows_at = [](const kda_tensor &x, int64_t b, int64_t hd, int64_t t) {
     return static_cast<uint16_t *>(x.data) + b * x.stride_b + hd * x.stride_h + t * x.stride_t;
   };
-
-  for (int u = blockIdx.x; u < a.max_chunks * a.p.Hk; u += gridDim.x) {
-    const int cidx = u / a.p.Hk, hk = u % a.p.Hk;
-    int64_t b, t0;
-    int rows;
-    if (!get_chunk(a, cidx, &b, &t0, &rows)) break;  // the last chunks of the bound do not exist
-    auto load64 = [&](uint32_t tile, int row0, const uint16_t *src, int64_t stride) {
-      constexpr int P = D / 8;
+  auto load64 = [&](uint32_t tile, int row0, const uint16_t *src, int64_t stride, int rows) {
+    constexpr int P = D / 8;
 #pragma unroll
-      for (int i = 0; i < 64 * P / kGradThreads; ++i) {
-        const int p = tid + i * kGradThreads, r = p / P, c = p % P, tr = row0 + r;
-        cp_async16(tile + (c >> 3) * 16384 + chunk_at(tr, c & 7), src + (r < rows ? r * stride : 0) + c * 8, r < rows);
+    for (int i = 0; i < 64 * P / kGradThreads; ++i) {
+      const int p = tid + i * kGradThreads, r = p / P, c = p % P, tr = row0 + r;
+      cp_async16(tile + (c >> 3) * 16384 + chunk_at(tr, c & 7), src + (r < rows ? r * stride : 0) + c * 8, r < rows);
+    }
+  };
+  // the tiles of value head h of chunk cell cidx, all but k and q
+  auto load_head = [&](int cidx, int h, int64_t b, int64_t t0, int rows) {
+    const size_t ch = (size_t)cidx * a.p.H + h;
+    if (tid == 0) {
+      const uint32_t b1 = smem_u32(&ctl.load_bar), b2 = smem_u32(&bar_s);
+      mbar_arrive_expect_tx(b1, NS * 16384 + D * 256);
+      for (int s = 0; s < NS; ++s) {
+        const char *x = a.w.dX + (ch * NS + s) * (size_t)16384;
+        bulk_load(sb + L::AH + s * 16384, x, 8192, b1);
+        bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, b1);
       }
-    };
-    load64(sb + L::KQ, 0, rows_at(a.p.k, b, hk, t0), a.p.k.stride_t);
-    load64(sb + L::KQ, 64, rows_at(a.p.q, b, hk, t0), a.p.q.stride_t);
+      bulk_load(sb + L::U, a.w.U + ch * (size_t)(D * 256), D * 256, b1);
+      mbar_arrive_expect_tx(b2, D * D * 6);
+      bulk_load(sb + L::S, a.w.S + ch * (size_t)(D * D * 4), D * D * 4, b2);
+      bulk_load(sb + L::DH, a.w.dS + ch * (size_t)(D * D * 4), D * D * 2, b2);
+    }
+    load64(sb + L::AH, 64, rows_at(a.p.dout, b, h, t0), a.p.dout.stride_t, rows);
+    if (upper)
+#pragma unroll
+      for (int c = 0; c < W / 8; ++c) sts(sb + L::AL + own_chunk(c), make_uint4(0, 0, 0, 0));
+  };
+
+  int64_t b = 0, t0 = 0;
+  int rows = 0, u = blockIdx.x;
+  bool live = u < cells && get_chunk(a, u / a.p.Hk, &b, &t0, &rows);
+  if (live) load_head(u / a.p.Hk, (u % a.p.Hk) * G_, b, t0, rows);
+  while (live) {
+    const int cidx = u / a.p.Hk, hk = u % a.p.Hk;
+    load64(sb + L::KQ, 0, rows_at(a.p.k, b, hk, t0), a.p.k.stride_t, rows);
+    load64(sb + L::KQ, 64, rows_at(a.p.q, b, hk, t0), a.p.q.stride_t, rows);
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.f;
+    // the cell after this one
+    const int un = u + (int)gridDim.x;
+    int64_t nb = 0, nt = 0;
+    int nrows = 0;
+    const bool more = un < cells && get_chunk(a, un / a.p.Hk, &nb, &nt, &nrows);
 
     for (int hh = 0; hh < G_; ++hh) {
       const int h = hk * G_ + hh;
       const size_t ch = (size_t)cidx * a.p.H + h;
-      const char *gD = a.w.dS + ch * (size_t)(D * D * 4);
-      if (tid == 0) {
-        const uint32_t b1 = smem_u32(&ctl.load_bar), b2 = smem_u32(&bar_s);
-        mbar_arrive_expect_tx(b1, NS * 16384 + D * 256);
-        for (int s = 0; s < NS; ++s) {
-          const char *x = a.w.dX + (ch * NS + s) * (size_t)16384;
-          bulk_load(sb + L::AH + s * 16384, x, 8192, b1);
-          bulk_load(sb + L::AL + s * 16384, x + 8192, 8192, b1);
-        }
-        bulk_load(sb + L::U, a.w.U + ch * (size_t)(D * 256), D * 256, b1);
-        mbar_arrive_expect_tx(b2, D * D * 6);
-        bulk_load(sb + L::S, a.w.S + ch * (size_t)(D * D * 4), D * D * 4, b2);
-        bulk_load(sb + L::DH, gD, D * D * 2, b2);
-        prefetch_l2(gD + D * D * 2, D * D * 2);
-        // the next value head's images
-        size_t nx = ch + 1;
-        bool more = hh + 1 < G_;
-        if (!more && u + (int)gridDim.x < a.max_chunks * a.p.Hk) {
-          const int un = u + gridDim.x;
-          nx = (size_t)(un / a.p.Hk) * a.p.H + (size_t)(un % a.p.Hk) * G_;
-          more = true;
-        }
-        if (more) {
-          prefetch_l2(a.w.dX + nx * (size_t)(D * 256), D * 256);
-          prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
-          prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
-          prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
-        }
-      }
-      load64(sb + L::AH, 64, rows_at(a.p.dout, b, h, t0), a.p.dout.stride_t);
-      if (upper)
-#pragma unroll
-        for (int c = 0; c < W / 8; ++c)
-          sts(sb + L::AL + ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c), make_uint4(0, 0, 0, 0));
+      const bool last = hh + 1 == G_;
       if (tid < 64) gam[tid] = a.w.gam[ch * 64 + tid];
       const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
-      const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
-      uint4 vraw[W / 8];  // this row of V
-      if (!upper)
+      // two 16-byte runs of a row of V, eight threads a row
+      constexpr int VR = D / 64;
+      const int vr = tid >> 3, vc = tid & 7;
+      uint4 vraw[VR];
 #pragma unroll
-        for (int c = 0; c < W / 8; ++c)
-          vraw[c] = r64 < rows ? *reinterpret_cast<const uint4 *>(rows_at(a.p.v, b, h, t0 + r64) + part * W + 8 * c) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < VR; ++c)
+        vraw[c] = vr < rows ? *reinterpret_cast<const uint4 *>(rows_at(a.p.v, b, h, t0 + vr) + 8 * (vc + 8 * c)) : make_uint4(0, 0, 0, 0);
       cp_async_wait();
       publish();
       if (warp_leader()) {
@@ -178,44 +178,61 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         mma_commit(smem_u32(&ctl.mma_bar));
       }
       __syncwarp();
-      // meanwhile dX . v and <S, dS> (same place in both images)
+      // what the next value head loads comes into L2 meanwhile (by the load/store units: bulk prefetches held
+      // up the copies behind them)
+      if (!last || more) {
+        const int nk = last ? un % a.p.Hk : hk, nh = last ? nk * G_ : h + 1;
+        const int64_t pb = last ? nb : b, pt = last ? nt : t0;
+        const int pr = last ? nrows : rows;
+        const size_t nx = (size_t)(last ? un / a.p.Hk : cidx) * a.p.H + nh;
+        if (last) {
+          prefetch_l2_rows<D>(rows_at(a.p.k, pb, nk, pt), a.p.k.stride_t, pr);
+          prefetch_l2_rows<D>(rows_at(a.p.q, pb, nk, pt), a.p.q.stride_t, pr);
+        }
+        prefetch_l2_rows<D>(rows_at(a.p.dout, pb, nh, pt), a.p.dout.stride_t, pr);
+        prefetch_l2_rows<D>(rows_at(a.p.v, pb, nh, pt), a.p.v.stride_t, pr);
+        prefetch_l2(a.w.dX + nx * (size_t)(D * 256), D * 256);
+        prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
+        prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
+        prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
+      }
+      const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
+      // dX . v, and the products of the two images, place by place
       mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
       float xv = 0.f;
-      if (!upper) {
 #pragma unroll
-        for (int c = 0; c < W / 8; ++c) {
-          const uint32_t at = ((part * W + 8 * c) >> 6) * 16384 + chunk_at(row, ((part * W) >> 3) + c);
-          float x[8], y[8], v[8];
-          unpack8<BF>(ld_shared_v4(sb + L::AH + at), x);
-          unpack8<BF>(ld_shared_v4(sb + L::AL + at), y);
-          unpack8<BF>(vraw[c], v);
+      for (int c = 0; c < VR; ++c) {
+        const uint32_t at = c * 16384 + chunk_at(vr, vc);
+        float x[8], y[8], v[8];
+        unpack8<BF>(ld_shared_v4(sb + L::AH + at), x);
+        unpack8<BF>(ld_shared_v4(sb + L::AL + at), y);
+        unpack8<BF>(vraw[c], v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
-        }
+        for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
       }
+      for (int o = 4; o > 0; o >>= 1) xv += __shfl_xor_sync(0xffffffffu, xv, o);
+      if (vc == 0) sm_xv[vr] = xv;
       mbar_wait(smem_u32(&bar_s), ph, a.p.status, &ctl.abort);
+      // <S, dS> = <S, dS hi> now, <S hi, dS lo> when that has come (S lo . dS lo is below fp32's last bits)
       float dot = 0.f;
-#pragma unroll 2
+#pragma unroll
       for (int e = tid; e < D * D / 8; e += kGradThreads) {
         const uint32_t off = e * 16;
-        float x[8], y[8], z[8];
-        const uint4 lo = *reinterpret_cast<const uint4 *>(gD + off + D * D * 2);
+        float x[8], y[8];
         unpack8<BF>(ld_shared_v4(sb + L::S + off), x);
         unpack8<BF>(ld_shared_v4(sb + L::S + off + D * D * 2), y);
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += y[j];
         unpack8<BF>(ld_shared_v4(sb + L::DH + off), y);
-        unpack8<BF>(lo, z);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j] + z[j], dot);
+        for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
       }
-      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if ((tid & 31) == 0) sm_dot[tid >> 5] = dot;
       // M, N (16 columns)
       mbar_wait(smem_u32(&bar_g2), 0, a.p.status, &ctl.abort);
       __syncwarp();
       tc_fence_after();
       uint4 mh[2], ml[2];
+      float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
       {
         float x[16], y[16];
         tmem_ldn<16>(lane_t + tG1 + 16 * part, x);
@@ -226,7 +243,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           const float e = ex2f((gi - gam[col]) * kLog2e);
           if (!upper) {
             const float m = col < r64 ? -y[j] * e : 0.f;
-            xv = col < r64 ? fmaf(m, x[j], xv) : xv;
+            rs = col < r64 ? fmaf(m, x[j], rs) : rs;
             x[j] = m * bi;
           } else {
             x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
@@ -240,14 +257,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       __syncwarp();
       tc_fence_after();
       publish();
+      if (tid == 0) {
+        mbar_arrive_expect_tx(smem_u32(&bar_d), D * D * 2);
+        bulk_load(sb + L::S + D * D * 2, a.w.dS + ch * (size_t)(D * D * 4) + D * D * 2, D * D * 2, smem_u32(&bar_d));
+      }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         sts(sb + L::MN + chunk_at(row, 2 * part + c), mh[c]);
         sts(sb + L::MN + 16384 + chunk_at(row, 2 * part + c), ml[c]);
-      }
-      if (tid == 32) {
-        mbar_arrive_expect_tx(smem_u32(&bar_d), D * D * 2);
-        bulk_load(sb + L::S, gD + D * D * 2, D * D * 2, smem_u32(&bar_d));
       }
       publish();
       if (warp_leader()) {
@@ -261,7 +278,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         issue<8>(tmem + tG4, MNMajor{sb + L::MN + 16384, 16384}, kq, id4, true);
         mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
         tc_fence_after();
-        issue<D / 16>(tmem + tG6, MNPlain{sb + L::U, D}, MNPlain{sb + L::S, D}, idesc_f16(128, D, BF, true, true), true);
+        issue<D / 16>(tmem + tG6, MNPlain{sb + L::U, D}, MNPlain{sb + L::S + D * D * 2, D}, idesc_f16(128, D, BF, true, true), true);
         mma_commit(smem_u32(&bar_g2));
       }
       __syncwarp();
@@ -274,7 +291,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 #pragma unroll
         for (int c = 0; c < W / 8; ++c) {
           float k[8];
-          unpack8<BF>(kq_chunk(c), k);
+          unpack8<BF>(ld_shared_v4(sb + L::KQ + own_chunk(c)), k);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             t_dot = fmaf(k[j], x[8 * c + j], t_dot);
@@ -283,9 +300,26 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         }
         f_dot = f * t_dot;
       }
+      mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
+#pragma unroll
+      for (int e = tid; e < D * D / 8; e += kGradThreads) {
+        float x[8], y[8];
+        unpack8<BF>(ld_shared_v4(sb + L::S + e * 16), x);
+        unpack8<BF>(ld_shared_v4(sb + L::S + D * D * 2 + e * 16), y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dot = fmaf(x[j], y[j], dot);
+      }
+      for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      if ((tid & 31) == 0) sm_dot[tid >> 5] = dot;
       mbar_wait(smem_u32(&bar_g2), 1, a.p.status, &ctl.abort);
       __syncwarp();
       tc_fence_after();
+      publish();
+      // all products and reads of the tiles are done, k and q aside: the next value head's come in
+      if (!last)
+        load_head(cidx, h + 1, b, t0, rows);
+      else if (more)
+        load_head(un / a.p.Hk, (un % a.p.Hk) * G_, nb, nt, nrows);
 #pragma unroll
       for (int c0 = 0; c0 < W; c0 += 16) {
         float x[16], y[16], z[16];
@@ -297,7 +331,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float k[8];
-          unpack8<BF>(kq_chunk(c0 / 8 + c), k);
+          unpack8<BF>(ld_shared_v4(sb + L::KQ + own_chunk(c0 / 8 + c)), k);
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int i = 8 * c + j;
@@ -313,35 +347,42 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           }
         }
       }
-      if (upper) sm_f[part][r64] = f_dot;
-      __syncthreads();
-      if (!upper) {
-        sm_f[part][r64] += f_dot;
-        sm_t[part][r64] = t_dot;
-        sm_y[part][r64] = y_dot;
-        sm_d[part][r64] = xv;  // dX.v - sum_j (dX U^T)_ij e_ij k_i.k_j
+      // the rows' sums, in a fixed order: the quarters of k rows, then those of q rows
+      for (int turn = 0; turn < 2; ++turn) {
+        if (!upper && (part >> 1) == turn) {
+          const int p = part & 1;
+          const float z = 0.f;
+          sm_f[p][r64] = (turn ? sm_f[p][r64] : z) + f_dot;
+          sm_t[p][r64] = (turn ? sm_t[p][r64] : z) + t_dot;
+          sm_y[p][r64] = (turn ? sm_y[p][r64] : z) + y_dot;
+          sm_r[p][r64] = (turn ? sm_r[p][r64] : z) + rs;
+        }
+        __syncthreads();
       }
-      tc_fence_before();
-      __syncthreads();
+      for (int turn = 0; turn < 2; ++turn) {
+        if (upper && (part >> 1) == turn) sm_f[part & 1][r64] += f_dot;
+        if (turn) tc_fence_before();
+        __syncthreads();
+      }
       tc_fence_after();
       if (tid < 32) {
         float f[2], y[2];
         float sd = 0.f;
         for (int w = 0; w < 16; ++w) sd += sm_dot[w];
         sd *= exp_fast(gam[63]);
-        auto four = [](const float (&s)[4][64], int i) { return (s[0][i] + s[1][i]) + (s[2][i] + s[3][i]); };
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * tid + j;
-          f[j] = four(sm_f, i);
-          y[j] = four(sm_y, i);
+          f[j] = sm_f[0][i] + sm_f[1][i];
+          y[j] = sm_y[0][i] + sm_y[1][i];
           if (i < rows)
-            store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype, four(sm_d, i) - exp_fast(gam[i]) * four(sm_t, i));
+            store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype,
+                       sm_xv[i] - exp_fast(gam[i]) * (sm_t[0][i] + sm_t[1][i]) + (sm_r[0][i] + sm_r[1][i]));
         }
         // suffix sums of f, exclusive prefix sums of y
         float sf = f[0] + f[1], py = y[0] + y[1];
         for (int o = 1; o < 32; o <<= 1) {
-          const float un = __shfl_down_sync(0xffffffffu, sf, o), v = __shfl_up_sync(0xffffffffu, py, o);
-          if (tid + o < 32) sf += un;
+          const float un_ = __shfl_down_sync(0xffffffffu, sf, o), v = __shfl_up_sync(0xffffffffu, py, o);
+          if (tid + o < 32) sf += un_;
           if (tid >= o) py += v;
         }
         const float next = __shfl_down_sync(0xffffffffu, sf, 1), prev = __shfl_up_sync(0xffffffffu, py, 1);
@@ -351,17 +392,31 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           store_gate(a.p.dg, (b * a.p.H + h) * a.p.T + t0 + 2 * tid + 1, a.p.g_dtype, s1 + (p0 + y[0]) + sd);
       }
       ph ^= 1;
-      fence_async_smem();  // the next tiles are written over what was read here
-      __syncthreads();
+      if (!last) __syncthreads();
     }
-    if (r64 < rows) {
-      uint16_t *dst = rows_at(upper ? a.p.dq : a.p.dk, b, hk, t0 + r64) + part * W;
+    // dk over k's tile, dq over q's, then out in whole rows
 #pragma unroll
-      for (int c = 0; c < W / 8; ++c)
-        *reinterpret_cast<uint4 *>(dst + 8 * c) =
-            make_uint4(pack2(acc[8 * c], acc[8 * c + 1], BF), pack2(acc[8 * c + 2], acc[8 * c + 3], BF),
-                       pack2(acc[8 * c + 4], acc[8 * c + 5], BF), pack2(acc[8 * c + 6], acc[8 * c + 7], BF));
+    for (int c = 0; c < W / 8; ++c)
+      sts(sb + L::KQ + own_chunk(c), make_uint4(pack2(acc[8 * c], acc[8 * c + 1], BF), pack2(acc[8 * c + 2], acc[8 * c + 3], BF),
+                                                pack2(acc[8 * c + 4], acc[8 * c + 5], BF), pack2(acc[8 * c + 6], acc[8 * c + 7], BF)));
+    __syncthreads();
+    {
+      constexpr int P = D / 8;
+      uint16_t *dk = rows_at(a.p.dk, b, hk, t0), *dq = rows_at(a.p.dq, b, hk, t0);
+#pragma unroll
+      for (int e = tid; e < 128 * P; e += kGradThreads) {
+        const int r = e / P, c = e % P, rr = r & 63;
+        if (rr < rows)
+          *reinterpret_cast<uint4 *>((r < 64 ? dk + rr * a.p.dk.stride_t : dq + rr * a.p.dq.stride_t) + 8 * c) =
+              ld_shared_v4(sb + L::KQ + (c >> 3) * 16384 + chunk_at(r, c & 7));
+      }
     }
+    __syncthreads();
+    u = un;
+    live = more;
+    b = nb;
+    t0 = nt;
+    rows = nrows;
   }
   cta_end(tmem, 512);
 }

@@ -82,6 +82,46 @@ __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
 // -------------------------------------------------------------- preparation --
 constexpr int kLd = 68;  // row stride (floats) of the fp32 64 x 64 matrices: vectors of 8 rows in distinct banks
 
+// Two rows and four columns of sign * L R, with n terms: eight sums a thread on six 16-byte
+// loads every four terms (one row a thread spent its time on the loads).
+template <int n>
+__device__ __forceinline__ void block_product(const float *l, const float *r, float *out, float sign) {
+  float4 s0 = make_float4(0.f, 0.f, 0.f, 0.f), s1 = s0;
+  auto add = [](float4 &s, float f, const float4 &v) {
+    s.x = fmaf(f, v.x, s.x);
+    s.y = fmaf(f, v.y, s.y);
+    s.z = fmaf(f, v.z, s.z);
+    s.w = fmaf(f, v.w, s.w);
+  };
+#pragma unroll 4
+  for (int m = 0; m < n; m += 4) {
+    const float4 l0 = *reinterpret_cast<const float4 *>(l + m), l1 = *reinterpret_cast<const float4 *>(l + kLd + m);
+    const float4 r0 = *reinterpret_cast<const float4 *>(r + m * kLd), r1 = *reinterpret_cast<const float4 *>(r + (m + 1) * kLd);
+    const float4 r2 = *reinterpret_cast<const float4 *>(r + (m + 2) * kLd), r3 = *reinterpret_cast<const float4 *>(r + (m + 3) * kLd);
+    add(s0, l0.x, r0);
+    add(s1, l1.x, r0);
+    add(s0, l0.y, r1);
+    add(s1, l1.y, r1);
+    add(s0, l0.z, r2);
+    add(s1, l1.z, r2);
+    add(s0, l0.w, r3);
+    add(s1, l1.w, r3);
+  }
+  *reinterpret_cast<float4 *>(out) = make_float4(sign * s0.x, sign * s0.y, sign * s0.z, sign * s0.w);
+  *reinterpret_cast<float4 *>(out + kLd) = make_float4(sign * s1.x, sign * s1.y, sign * s1.z, sign * s1.w);
+}
+
+// For each pair of diagonal n-blocks of the inverse, the block below them: -c B a, through the
+// unused block of A above them.
+template <int n>
+__device__ __forceinline__ void inverse_level(float *As, float *Ti) {
+  const int p = threadIdx.x / (n * n / 8), f = threadIdx.x % (n * n / 8), i = f / (n / 4) * 2, j = f % (n / 4) * 4, o = 2 * n * p;
+  if (p < 32 / n) block_product<n>(As + (o + n + i) * kLd + o, Ti + o * kLd + o + j, As + (o + i) * kLd + o + n + j, 1.f);
+  __syncthreads();
+  if (p < 32 / n) block_product<n>(Ti + (o + n + i) * kLd + o + n, As + o * kLd + o + n + j, Ti + (o + n + i) * kLd + o + j, -1.f);
+  __syncthreads();
+}
+
 // One CTA per (chunk, head): T and P T as two-term images, gamma and beta in fp32.
 // The products are k.k, q.k and P T; (I + A)^-1 is by halves in fp32: four 16 x 16 blocks
 // by substitution, a column a thread, then [A 0; B C]^-1 = [a 0; -c B a, c] twice.
@@ -93,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   constexpr uint32_t KQ = 0, TT = 0;  // [T; P] hi, then lo, over the rest
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
-  __shared__ __align__(16) float gam[64], bet[64];
+  __shared__ __align__(16) float gam[64], bet[64], cfac[32];
   int64_t b, t0;
   int rows;
   if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
@@ -121,6 +161,8 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     }
     gam[2 * tid + 1] = (float)c;
     gam[2 * tid] = (float)(c - s[1]);
+    __syncwarp();
+    cfac[tid] = exp_fast(gam[31] - gam[tid]);
   }
   cp_async_wait();
   publish();
@@ -134,27 +176,38 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     a.w.gam[ch * 64 + tid] = gam[tid];
     a.w.beta[ch * 64 + tid] = bet[tid];
   }
-  const float gi = gam[r64] * kLog2e, bi = bet[r64];
+  const float gi = gam[r64] * kLog2e;
+  // The factor e^{gamma_i - gamma_j} of this thread's 32 columns: nothing above the diagonal, a
+  // product of two factors <= 1 that meet at gamma_31 below the diagonal blocks of 32, and an
+  // exponential an element in them (MUFU is what 4 CTAs an SM would otherwise wait for).
+  const int rb = r64 >> 5;  // warp-uniform
+  const float rowf = row < 64 ? bet[r64] : a.p.scale;
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   float *As = reinterpret_cast<float *>(smem + KQ);  // over the k and q tiles: their product is done
   float *Ti = As + 64 * kLd;
   float x[32];  // 32 columns of a row of A (rows of k) or P (rows of q)
-  {
+  if (half > rb) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] = 0.f;
+  } else {
     tmem_ld32(tmem + lane_base + 32 * half, x);
+    if (half < rb) {
+      const float f = rowf * ex2f(gi - gam[31] * kLog2e);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const int col = 32 * half + j;
-      const float d = ex2f(fmaf(-kLog2e, gam[col], gi));
-      if (row < 64)
-        x[j] = col < r64 ? bi * d * x[j] : 0.f;
-      else
-        x[j] = col <= r64 ? a.p.scale * d * x[j] : 0.f;
-    }
-    if (row < 64) {
+      for (int j = 0; j < 32; ++j) x[j] *= f * cfac[j];
+    } else {
 #pragma unroll
-      for (int j = 0; j < 32; j += 4)
-        *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+      for (int j = 0; j < 32; ++j) {
+        const int col = 32 * half + j;
+        const float d = rowf * ex2f(fmaf(-kLog2e, gam[col], gi));
+        x[j] = (row < 64 ? col < r64 : col <= r64) ? d * x[j] : 0.f;
+      }
     }
+  }
+  if (row < 64) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4)
+      *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
   }
   tc_fence_before();
   __syncthreads();
@@ -167,7 +220,13 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     for (int i = 0; i < 16; ++i) {
       float s = i == j ? 1.f : 0.f;
 #pragma unroll
-      for (int m = 0; m < i; ++m) s = fmaf(-As[(o + i) * kLd + o + m], y[m], s);
+      for (int m = 0; m < i; m += 4) {
+        const float4 r = *reinterpret_cast<const float4 *>(As + (o + i) * kLd + o + m);
+        s = fmaf(-r.x, y[m], s);
+        if (m + 1 < i) s = fmaf(-r.y, y[m + 1], s);
+        if (m + 2 < i) s = fmaf(-r.z, y[m + 2], s);
+        if (m + 3 < i) s = fmaf(-r.w, y[m + 3], s);
+      }
       y[i] = i < j ? 0.f : s;
     }
 #pragma unroll
@@ -180,41 +239,8 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int n = 16; n < 64; n *= 2) {
-    // for each pair of diagonal n-blocks: the block below them, -c B a, through the unused block of A above them
-    const int pairs = 32 / n, per = n * n / 4, work = pairs * per;  // float4 outputs
-    for (int e = tid; e < work; e += kThreads) {
-      const int p = e / per, f = e % per, i = f / (n / 4), j = f % (n / 4) * 4, o = 2 * n * p;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < n; ++m) {
-        const float l = As[(o + n + i) * kLd + o + m];
-        const float4 r = *reinterpret_cast<const float4 *>(Ti + (o + m) * kLd + o + j);
-        s.x = fmaf(l, r.x, s.x);
-        s.y = fmaf(l, r.y, s.y);
-        s.z = fmaf(l, r.z, s.z);
-        s.w = fmaf(l, r.w, s.w);
-      }
-      *reinterpret_cast<float4 *>(As + (o + i) * kLd + o + n + j) = s;
-    }
-    __syncthreads();
-    for (int e = tid; e < work; e += kThreads) {
-      const int p = e / per, f = e % per, i = f / (n / 4), j = f % (n / 4) * 4, o = 2 * n * p;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-      for (int m = 0; m < n; ++m) {
-        const float l = Ti[(o + n + i) * kLd + o + n + m];
-        const float4 r = *reinterpret_cast<const float4 *>(As + (o + m) * kLd + o + n + j);
-        s.x = fmaf(-l, r.x, s.x);
-        s.y = fmaf(-l, r.y, s.y);
-        s.z = fmaf(-l, r.z, s.z);
-        s.w = fmaf(-l, r.w, s.w);
-      }
-      *reinterpret_cast<float4 *>(Ti + (o + n + i) * kLd + o + j) = s;
-    }
-    __syncthreads();
-  }
+  inverse_level<16>(As, Ti);
+  inverse_level<32>(As, Ti);
   if (row < 64) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
