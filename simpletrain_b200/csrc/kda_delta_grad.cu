@@ -39,15 +39,8 @@ struct GradSmem {
   static constexpr uint32_t MN = AH;                                   // [M; N] hi, lo (D = 64: runs over AL)
 };
 
-// This thread's 128-byte lines of `bytes` contiguous bytes, into L2.
-__device__ __forceinline__ void prefetch_l2(const char *p, uint32_t bytes) {
-  for (uint32_t o = threadIdx.x * 128; o < bytes; o += kGradThreads * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
-}
-// the same for `rows` (of 64) rows of D 16-bit elements
-template <int D>
-__device__ __forceinline__ void prefetch_l2_rows(const uint16_t *p, int64_t stride, int rows) {
-  const int r = threadIdx.x / (D / 64), c = threadIdx.x % (D / 64);
-  if (r < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + r * stride + c * 64));
+__device__ __forceinline__ void prefetch_l2(const void *p, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(p)), "r"(bytes) : "memory");
 }
 
 // N consecutive fp32 columns of this warp's lanes
@@ -178,24 +171,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         mma_commit(smem_u32(&ctl.mma_bar));
       }
       __syncwarp();
-      // what the next value head loads comes into L2 meanwhile (by the load/store units: bulk prefetches held
-      // up the copies behind them)
-      if (!last || more) {
-        const int nk = last ? un % a.p.Hk : hk, nh = last ? nk * G_ : h + 1;
-        const int64_t pb = last ? nb : b, pt = last ? nt : t0;
-        const int pr = last ? nrows : rows;
-        const size_t nx = (size_t)(last ? un / a.p.Hk : cidx) * a.p.H + nh;
-        if (last) {
-          prefetch_l2_rows<D>(rows_at(a.p.k, pb, nk, pt), a.p.k.stride_t, pr);
-          prefetch_l2_rows<D>(rows_at(a.p.q, pb, nk, pt), a.p.q.stride_t, pr);
-        }
-        prefetch_l2_rows<D>(rows_at(a.p.dout, pb, nh, pt), a.p.dout.stride_t, pr);
-        prefetch_l2_rows<D>(rows_at(a.p.v, pb, nh, pt), a.p.v.stride_t, pr);
-        prefetch_l2(a.w.dX + nx * (size_t)(D * 256), D * 256);
-        prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
-        prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
-        prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
-      }
       const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
       // dX . v, and the products of the two images, place by place
       mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
@@ -260,6 +235,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       if (tid == 0) {
         mbar_arrive_expect_tx(smem_u32(&bar_d), D * D * 2);
         bulk_load(sb + L::S + D * D * 2, a.w.dS + ch * (size_t)(D * D * 4) + D * D * 2, D * D * 2, smem_u32(&bar_d));
+        // what the next value head loads comes into L2 behind that (one bulk request each: line by line through
+        // the load/store units it held up everything else for 5000 cycles)
+        if (!last || more) {
+          const size_t nx = last ? (size_t)(un / a.p.Hk) * a.p.H + (un % a.p.Hk) * G_ : ch + 1;
+          prefetch_l2(a.w.dX + nx * (size_t)(D * 256), D * 256);
+          prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
+          prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
+          prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
+        }
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {

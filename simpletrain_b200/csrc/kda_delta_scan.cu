@@ -232,10 +232,11 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) Ti[(o + i) * kLd + o + j] = y[i];
   } else {
-    // the blocks above the diagonal
-    for (int e = tid - 64; e < 4096; e += kThreads - 64) {
-      const int i = e >> 6, j = e & 63;
-      if ((j >> 4) > (i >> 4)) Ti[i * kLd + j] = 0.f;
+    // the six 16 x 16 blocks above the diagonal blocks
+    for (int e = tid - 64; e < 6 * 64; e += kThreads - 64) {
+      const int q = e >> 6, f = e & 63;
+      const int bi = q < 3 ? 0 : (q < 5 ? 1 : 2), bj = q < 3 ? q + 1 : (q < 5 ? q - 1 : 3);
+      *reinterpret_cast<float4 *>(Ti + (16 * bi + (f >> 2)) * kLd + 16 * bj + (f & 3) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
   }
   __syncthreads();
