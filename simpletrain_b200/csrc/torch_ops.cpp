@@ -10,8 +10,10 @@
 //
 // The schemas and CUDA implementations live here, in C++, so a call costs a
 // dispatcher hop and a few caching-allocator allocations instead of a Python
-// function; fake (meta) implementations and autograd are registered from
-// Python (simpletrain_b200/ops.py).  Outputs and the workspace come from the
+// function; fake (meta) implementations and, but for the delta rule and the
+// token log probabilities, autograd are registered from Python
+// (simpletrain_b200/ops.py).  Those two have their autograd here: behind a
+// Python formula a small training step cost 130 us of host time.  Outputs and the workspace come from the
 // caching allocator and the kernels run on the current stream, so the ops can
 // be captured in CUDA graphs.  Layout rules follow the ABI: a tensor whose
 // innermost stride is not 1, whose other strides are not multiples of 8
@@ -19,6 +21,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <cstdint>
@@ -523,6 +526,93 @@ Tensor token_logprobs_bwd(const Tensor &logits_, const Tensor &tokens_, const Te
   return dlogits;
 }
 
+// ------------------------------------------------------------------ autograd
+using torch::autograd::AutogradContext;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+optional<Tensor> if_defined(const Tensor &t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+struct DeltaFunction : public torch::autograd::Function<DeltaFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                               const Tensor &beta, double scale, const optional<Tensor> &s0, const optional<Tensor> &cu,
+                               bool want_state) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("kda_b200::delta_fwd", "")
+                         .typed<std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                           const Tensor &, double, const optional<Tensor> &,
+                                                           const optional<Tensor> &, bool)>();
+    auto [o, s] = op.call(q, k, v, g, beta, scale, s0, cu, want_state);
+    ctx->save_for_backward({q, k, v, g, beta, s0.has_value() ? *s0 : Tensor(), cu.has_value() ? *cu : Tensor()});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["state"] = want_state;
+    ctx->set_materialize_grads(false);
+    return {o, s};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor &v = t[2];
+    const bool need_ds0 = t[5].defined() && ctx->needs_input_grad(5);  // edges of the tensor arguments: the sixth
+    const Tensor dout = grads[0].defined() ? grads[0] : at::zeros_like(v);
+    const bool state = ctx->saved_data["state"].toBool() && grads[1].defined();
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("kda_b200::delta_bwd", "")
+                         .typed<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>(
+                             const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, double,
+                             const optional<Tensor> &, const optional<Tensor> &, const Tensor &, const optional<Tensor> &,
+                             bool)>();
+    auto [dq, dk, dv, dg, db, ds0] =
+        op.call(t[0], t[1], v, t[3], t[4], ctx->saved_data["scale"].toDouble(), if_defined(t[5]), if_defined(t[6]), dout,
+                state ? optional<Tensor>(grads[1]) : c10::nullopt, need_ds0);
+    return {dq, dk, dv, dg, db, Tensor(), need_ds0 ? ds0 : Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor> delta_fwd_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
+                                              const Tensor &beta, double scale, const optional<Tensor> &s0,
+                                              const optional<Tensor> &cu, bool want_state) {
+  const variable_list r = DeltaFunction::apply(q, k, v, g, beta, scale, s0, cu, want_state);
+  return {r[0], r[1]};
+}
+
+struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &tokens, int64_t top_k,
+                               double temperature, int64_t ignore_index) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("st_b200::token_logprobs", "")
+                         .typed<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, int64_t,
+                                                                                   double, int64_t)>();
+    auto [lp, ent, lse, top, ids] = op.call(logits, tokens, top_k, temperature, ignore_index);
+    ctx->save_for_backward({logits, tokens, ent, lse});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->mark_non_differentiable({lse, top, ids});
+    ctx->set_materialize_grads(false);
+    return {lp, ent, lse, top, ids};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const variable_list t = ctx->get_saved_variables();
+    const Tensor dlp = grads[0].defined() ? grads[0] : at::zeros_like(t[3]);
+    const Tensor dent = grads[1].defined() ? grads[1] : at::zeros_like(t[3]);
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("st_b200::token_logprobs_bwd", "")
+                         .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                       const Tensor &, double, int64_t)>();
+    return {op.call(t[0], t[1], t[2], t[3], dlp, dent, ctx->saved_data["temperature"].toDouble(),
+                    ctx->saved_data["ignore_index"].toInt()),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autograd(const Tensor &logits, const Tensor &tokens,
+                                                                           int64_t top_k, double temperature,
+                                                                           int64_t ignore_index) {
+  const variable_list r = LogprobsFunction::apply(logits, tokens, top_k, temperature, ignore_index);
+  return {r[0], r[1], r[2], r[3], r[4]};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(st_b200, m) {
@@ -580,3 +670,6 @@ TORCH_LIBRARY_IMPL(kda_b200, CUDA, m) {
 }
 
 TORCH_LIBRARY_IMPL(kda_b200, CompositeExplicitAutograd, m) { m.impl("status_word", &status); }
+
+TORCH_LIBRARY_IMPL(kda_b200, Autograd, m) { m.impl("delta_fwd", &delta_fwd_autograd); }
+TORCH_LIBRARY_IMPL(st_b200, Autograd, m) { m.impl("token_logprobs", &token_logprobs_autograd); }

@@ -13,7 +13,7 @@ one token a call on a pool of states (serving); both hold the state in fp32 and
 agree on it to a few parts in 1e6.
 
 ``kda_b200::delta_fwd / delta_bwd / delta_step`` are defined and implemented in
-C++ (``csrc/torch_ops.cpp``) over the C ABI (``include/kda_sm100.h``): they run
+C++, autograd included (``csrc/torch_ops.cpp``), over the C ABI (``include/kda_sm100.h``): they run
 on torch's current stream with workspace from the caching allocator, and can be
 captured in CUDA graphs.  There is no CPU path.
 """
@@ -51,26 +51,6 @@ def _(q, k, v, g, beta, scale, s0, cu_seqlens, dout, ds_T, need_ds0):
 @torch.library.register_fake("kda_b200::delta_step")
 def _(q, k, v, g, beta, state, state_indices, scale):
     return v.new_empty(v.shape)
-
-
-def _setup_context(ctx, inputs, output):
-    q, k, v, g, beta, scale, s0, cu_seqlens, want_state = inputs
-    ctx.save_for_backward(q, k, v, g, beta, s0, cu_seqlens)
-    ctx.scale = scale
-    ctx.want_state = want_state
-
-
-def _backward(ctx, dout, ds_T):
-    q, k, v, g, beta, s0, cu_seqlens = ctx.saved_tensors
-    need_ds0 = bool(ctx.needs_input_grad[6]) and s0 is not None
-    if dout is None:
-        dout = torch.zeros_like(v)
-    dq, dk, dv, dg, dbeta, ds0 = torch.ops.kda_b200.delta_bwd(
-        q, k, v, g, beta, ctx.scale, s0, cu_seqlens, dout, ds_T if ctx.want_state else None, need_ds0)
-    return dq, dk, dv, dg, dbeta, None, ds0 if need_ds0 else None, None, None
-
-
-torch.library.register_autograd("kda_b200::delta_fwd", _backward, setup_context=_setup_context)
 
 
 def _validate(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, names: str):

@@ -188,26 +188,6 @@ def _(logits, tokens, entropy, lse, dlogprob, dentropy, temperature, ignore_inde
     return logits.new_empty(logits.shape)
 
 
-def _lp_setup(ctx, inputs, output):
-    logits, tokens, _, temperature, ignore_index = inputs
-    _, entropy, lse, _, _ = output
-    ctx.save_for_backward(logits, tokens, entropy, lse)
-    ctx.temperature, ctx.ignore_index = temperature, ignore_index
-
-
-def _lp_backward(ctx, dlogprob, dentropy, _dlse, _dtop, _dids):
-    logits, tokens, entropy, lse = ctx.saved_tensors
-    if dlogprob is None:
-        dlogprob = torch.zeros_like(lse)
-    if dentropy is None:
-        dentropy = torch.zeros_like(lse)
-    return torch.ops.st_b200.token_logprobs_bwd(logits, tokens, entropy, lse, dlogprob, dentropy, ctx.temperature,
-                                                ctx.ignore_index), None, None, None, None
-
-
-torch.library.register_autograd("st_b200::token_logprobs", _lp_backward, setup_context=_lp_setup)
-
-
 def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperature: float = 1.0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """Log probabilities of given tokens, entropies and top alternatives of rows of logits.
@@ -240,7 +220,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatur
     _need_cuda(logits, tokens)
     lp, ent, _, top, ids = torch.ops.st_b200.token_logprobs(logits, tokens, int(top_k), float(temperature),
                                                             int(ignore_index))
-    return TokenLogprobs(lp, ent, top.detach(), ids)
+    return TokenLogprobs(lp, ent, top, ids)
 
 
 def _supported_arch() -> bool:
