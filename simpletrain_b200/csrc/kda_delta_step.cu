@@ -60,13 +60,41 @@ __global__ void __launch_bounds__(kBlock) delta_step_kernel(const kda_delta_step
   auto slot_of = [&](int64_t m) {
     return a.slots_int64 ? static_cast<const int64_t *>(a.slots)[m] : (int64_t) static_cast<const int32_t *>(a.slots)[m];
   };
-  if (a.slots != nullptr) {
-    slot = slot_of(n);
-    if (slot < 0 || slot >= a.num_states) {  // a padded row (or an index that names no state)
-      if (slot >= 0 && a.status != nullptr && tid == 0) atomicOr(a.status, KDA_ERR_DEVICE_INDEX);
-      if (rg == 0) store_o(n, make_float4(0.f, 0.f, 0.f, 0.f));
-      return;
+  const int hk = h / (a.H / a.Hk);
+  // a row's inputs; they do not depend on its state, so their latency is the index's and the state's too
+  struct Row {
+    uint32_t k[R / 2], q[R / 2];
+    uint2 v;
+    float alpha, beta;
+  };
+  auto load_row = [&](int64_t m) {
+    Row r;
+    const uint16_t *kp = static_cast<const uint16_t *>(a.k) + m * a.k_stride_n + hk * a.k_stride_h + rg * R;
+    const uint16_t *qp = static_cast<const uint16_t *>(a.q) + m * a.q_stride_n + hk * a.q_stride_h + rg * R;
+    if (R == 8) {
+      *reinterpret_cast<uint4 *>(r.k) = *reinterpret_cast<const uint4 *>(kp);
+      *reinterpret_cast<uint4 *>(r.q) = *reinterpret_cast<const uint4 *>(qp);
+    } else {
+      *reinterpret_cast<uint2 *>(r.k) = *reinterpret_cast<const uint2 *>(kp);
+      *reinterpret_cast<uint2 *>(r.q) = *reinterpret_cast<const uint2 *>(qp);
     }
+    r.v = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.v) + m * a.v_stride_n + h * a.v_stride_h + col);
+    r.alpha = load_gate(a.g, m * a.g_stride_n + h * a.g_stride_h, a.g_dtype);
+    r.beta = load_gate(a.beta, m * a.beta_stride_n + h * a.beta_stride_h, a.beta_dtype);
+    return r;
+  };
+  if (a.slots != nullptr) slot = slot_of(n);
+  Row in = load_row(n);
+  if (a.slots != nullptr && (slot < 0 || slot >= a.num_states)) {  // a padded row (or an index that names no state)
+    if (slot >= 0 && a.status != nullptr && tid == 0) atomicOr(a.status, KDA_ERR_DEVICE_INDEX);
+    if (rg == 0) store_o(n, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  float *S = a.state + slot * a.state_stride_n + h * a.state_stride_h + (int64_t)(rg * R) * D + col;
+  float4 s[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const float4 *>(S + i * D);
+  if (a.slots != nullptr) {  // under the state's loads: which other rows name this state?
     if (tid == 0) sm_next = a.N;
     __syncthreads();
     int dup = 0;
@@ -80,37 +108,18 @@ __global__ void __launch_bounds__(kBlock) delta_step_kernel(const kda_delta_step
     if (__syncthreads_or(dup)) return;  // an earlier row's CTA applies this row
     next = sm_next;
   }
-  float *S = a.state + slot * a.state_stride_n + h * a.state_stride_h + (int64_t)(rg * R) * D + col;
-  float4 s[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const float4 *>(S + i * D);
-  const int hk = h / (a.H / a.Hk);
   while (true) {
     float k[R], q[R];
-    {
-      const uint16_t *kp = static_cast<const uint16_t *>(a.k) + n * a.k_stride_n + hk * a.k_stride_h + rg * R;
-      const uint16_t *qp = static_cast<const uint16_t *>(a.q) + n * a.q_stride_n + hk * a.q_stride_h + rg * R;
-      uint32_t kw[R / 2], qw[R / 2];
-      if (R == 8) {
-        *reinterpret_cast<uint4 *>(kw) = *reinterpret_cast<const uint4 *>(kp);
-        *reinterpret_cast<uint4 *>(qw) = *reinterpret_cast<const uint4 *>(qp);
-      } else {
-        *reinterpret_cast<uint2 *>(kw) = *reinterpret_cast<const uint2 *>(kp);
-        *reinterpret_cast<uint2 *>(qw) = *reinterpret_cast<const uint2 *>(qp);
-      }
 #pragma unroll
-      for (int i = 0; i < R / 2; ++i) {
-        const float2 x = unpack2(kw[i], bf), y = unpack2(qw[i], bf);
-        k[2 * i] = x.x;
-        k[2 * i + 1] = x.y;
-        q[2 * i] = y.x;
-        q[2 * i + 1] = y.y;
-      }
+    for (int i = 0; i < R / 2; ++i) {
+      const float2 x = unpack2(in.k[i], bf), y = unpack2(in.q[i], bf);
+      k[2 * i] = x.x;
+      k[2 * i + 1] = x.y;
+      q[2 * i] = y.x;
+      q[2 * i + 1] = y.y;
     }
-    const uint2 vw = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.v) + n * a.v_stride_n +
-                                                      h * a.v_stride_h + col);
-    const float alpha = expf(load_gate(a.g, n * a.g_stride_n + h * a.g_stride_h, a.g_dtype));
-    const float beta = load_gate(a.beta, n * a.beta_stride_n + h * a.beta_stride_h, a.beta_dtype);
+    const uint2 vw = in.v;
+    const float alpha = expf(in.alpha), beta = in.beta;
     float4 p = make_float4(0.f, 0.f, 0.f, 0.f), r = p;
     float kq = 0.f;
 #pragma unroll
@@ -168,6 +177,7 @@ __global__ void __launch_bounds__(kBlock) delta_step_kernel(const kda_delta_step
     }
     if (next >= a.N) break;
     n = next;  // the next row of the same state
+    in = load_row(n);
     __syncthreads();
     if (tid == 0) sm_next = a.N;
     __syncthreads();

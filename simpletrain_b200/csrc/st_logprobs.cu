@@ -93,6 +93,55 @@ struct Elem {
   }
 };
 
+// Two fp32 lanes at once.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ __forceinline__ float2 get() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// Largest element of a 16-byte vector; NaN if one is NaN.  16-bit types compare in pairs.
+template <int DT>
+__device__ __forceinline__ float vec_max(const uint4 &v) {
+  uint32_t m;
+  if (DT == kF32) {
+    float a, b;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(v.x)), "f"(__uint_as_float(v.y)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
+    return a;
+  } else if (DT == kBF16) {
+    uint32_t a, b;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  } else {
+    uint32_t a, b;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  }
+  const float2 p = unpack2(m, DT == kBF16);
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(p.x), "f"(p.y));
+  return r;
+}
+
 // The part of a row that one CTA of the row's cluster owns: scalar elements
 // [lo, body), 16-byte vectors from element `body`, scalar elements [tail, hi).
 // Rows need only be element-aligned.
@@ -159,50 +208,64 @@ __device__ __forceinline__ void add1(Stat &t, float y) {
   }
 }
 
+// Vectors of a slice that its threads keep in registers, so that the second sweep reads no memory.
+constexpr int kKeep = 8;
+
+// one 16-byte vector into the running triple
 template <int DT>
-__device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c) {
+__device__ __forceinline__ void add_vec(Stat &t, const uint4 &raw, float c) {
+  using E = Elem<DT>;
+  const float mv = vec_max<DT>(raw) * c;
+  if (!(mv <= t.m)) {  // a larger maximum, or a NaN
+    if (mv != mv) {
+      t.s = t.w = NAN;
+      return;
+    }
+    const float d = fmaxf(t.m - mv, kFloor), f = ex2(d);
+    t.w = (t.w + d * t.s) * f;
+    t.s *= f;
+    t.m = mv;
+  }
+  if (t.m == -INFINITY) return;
+  float f[E::kVec];
+  E::unpack(raw, f);
+  const F2 cc(c, c), mm(-t.m, -t.m);
+  F2 s(0.f, 0.f), w(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < E::kVec; k += 2) {
+    const float2 d = fma2(F2(f[k], f[k + 1]), cc, mm).get();
+    const F2 e(ex2(d.x), ex2(d.y));
+    s = add2(s, e);
+    w = fma2(e, F2(fmaxf(d.x, kFloor), fmaxf(d.y, kFloor)), w);
+  }
+  const float2 ss = s.get(), ww = w.get();
+  t.s += ss.x + ss.y;
+  t.w += ww.x + ww.y;
+}
+
+template <int DT>
+__device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c, uint4 (&keep)[kKeep], bool kept) {
   using E = Elem<DT>;
   Stat t{-INFINITY, 0.f, 0.f};
   const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
-  auto vec = [&](const uint4 &raw) {
-    float f[E::kVec];
-    E::unpack(raw, f);
-    float mv = f[0], any = f[0];
+  if (kept) {
 #pragma unroll
-    for (int k = 1; k < E::kVec; ++k) {
-      mv = fmaxf(mv, f[k]);
-      any += f[k];
-    }
-    mv *= c;
-    if (mv > t.m) {
-      const float d = fmaxf(t.m - mv, kFloor), fct = ex2(d);
-      t.w = (t.w + d * t.s) * fct;
-      t.s *= fct;
-      t.m = mv;
-    }
-    if (t.m == -INFINITY) {
-      if (any != any) t.s = t.w = NAN;  // a NaN among -infinities
-      return;
-    }
-    float s = 0.f, w = 0.f;
+    for (int j = 0; j < kKeep; ++j)
+      if (threadIdx.x + j * kBlock < sl.nvec) keep[j] = __ldg(v4 + threadIdx.x + j * kBlock);
 #pragma unroll
-    for (int k = 0; k < E::kVec; ++k) {
-      const float d = fmaf(f[k], c, -t.m), e = ex2(d);
-      s += e;
-      w = fmaf(e, fmaxf(d, kFloor), w);
+    for (int j = 0; j < kKeep; ++j)
+      if (threadIdx.x + j * kBlock < sl.nvec) add_vec<DT>(t, keep[j], c);
+  } else {
+    int64_t i = threadIdx.x;
+    for (; i + 3 * kBlock < sl.nvec; i += 4 * kBlock) {  // four loads in flight a thread
+      uint4 r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = __ldg(v4 + i + j * kBlock);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add_vec<DT>(t, r[j], c);
     }
-    t.s += s;
-    t.w += w;
-  };
-  int64_t i = threadIdx.x;
-  for (; i + 3 * kBlock < sl.nvec; i += 4 * kBlock) {  // four loads in flight a thread
-    uint4 r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = __ldg(v4 + i + j * kBlock);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) vec(r[j]);
+    for (; i < sl.nvec; i += kBlock) add_vec<DT>(t, __ldg(v4 + i), c);
   }
-  for (; i < sl.nvec; i += kBlock) vec(__ldg(v4 + i));
   for (int64_t j = sl.lo + threadIdx.x; j < sl.body; j += kBlock) add1(t, c * E::load(row, j));
   for (int64_t j = sl.tail + threadIdx.x; j < sl.hi; j += kBlock) add1(t, c * E::load(row, j));
   return t;
@@ -212,10 +275,12 @@ __device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c)
 __device__ __forceinline__ bool before(float va, int ia, float vb, int ib) { return va > vb || (va == vb && ia < ib); }
 __device__ __forceinline__ float sort_key(float x) { return x == x ? x : -INFINITY; }
 
+constexpr int kGroups = kBlock / 4;
+
 struct Shared {
   Stat part[kWarps];
   Stat total;         // this CTA's
-  float tmax[kBlock];
+  float gmax[kGroups];
   float bound;
   int count;
   float cand_v[kCand];
@@ -228,23 +293,33 @@ struct Shared {
 
 // This CTA's best k of its slice into sh.top_*, in order; missing places get (-inf, INT_MAX).
 // thread_max is the thread's largest c * logit (c > 0, and rounding keeps the order: a logit
-// at or above the k-th largest has c * logit at or above the bound).
+// at or above the k-th largest has c * logit at or above the bound).  The bound is the k-th
+// largest of the 64 maxima of four threads each: k <= 32 of them leave about 64 ln(64 / (64 -
+// k)) candidates, 24 for k = 20, and ranking them costs a quarter of ranking all threads'.
 template <int DT>
-__device__ void local_top(const char *row, const Slice &sl, float c, float thread_max, int k, Shared &sh) {
+__device__ void local_top(const char *row, const Slice &sl, float c, float thread_max, int k, Shared &sh,
+                          const uint4 (&keep)[kKeep], bool kept) {
+  using E = Elem<DT>;
   const int tid = threadIdx.x;
-  sh.tmax[tid] = thread_max;
+  float gm = fmaxf(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
+  gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 2));
+  if ((tid & 3) == 0) sh.gmax[tid >> 2] = gm;
   if (tid < kTopMax) {
     sh.top_v[tid] = -INFINITY;
     sh.top_i[tid] = 0x7fffffff;
   }
   if (tid == 0) sh.count = 0;
   __syncthreads();
-  int rank = 0;
-  for (int j = 0; j < kBlock; ++j) rank += before(sh.tmax[j], j, thread_max, tid) ? 1 : 0;
-  if (rank == k - 1) sh.bound = thread_max;
+  if (tid < kGroups) {
+    const float mine = sh.gmax[tid];
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < kGroups; ++j) rank += before(sh.gmax[j], j, mine, tid) ? 1 : 0;
+    if (rank == k - 1) sh.bound = mine;
+  }
   __syncthreads();
   const float bound = sh.bound;
-  for_each<DT>(row, sl, [&](int64_t i, float x) {
+  auto offer = [&](int64_t i, float x) {
     x = sort_key(x);
     if (c * x >= bound) {
       const int at = atomicAdd(&sh.count, 1);
@@ -253,7 +328,24 @@ __device__ void local_top(const char *row, const Slice &sl, float c, float threa
         sh.cand_i[at] = (int)i;
       }
     }
-  });
+  };
+  if (kept) {
+#pragma unroll
+    for (int j = 0; j < kKeep; ++j)
+      if (tid + j * kBlock < sl.nvec) {
+        const float mv = vec_max<DT>(keep[j]);
+        if (c * mv >= bound || mv != mv || bound == -INFINITY) {  // few vectors hold a candidate
+          float f[E::kVec];
+          E::unpack(keep[j], f);
+#pragma unroll
+          for (int e = 0; e < E::kVec; ++e) offer(sl.body + (int64_t)(tid + j * kBlock) * E::kVec + e, f[e]);
+        }
+      }
+    for (int64_t i = sl.lo + tid; i < sl.body; i += kBlock) offer(i, E::load(row, i));
+    for (int64_t i = sl.tail + tid; i < sl.hi; i += kBlock) offer(i, E::load(row, i));
+  } else {
+    for_each<DT>(row, sl, offer);
+  }
   __syncthreads();
   const int n = sh.count;
   if (n <= kCand) {
@@ -324,7 +416,7 @@ struct FwdArgs {
   int k;
 };
 
-template <int DT, bool CLUSTER>
+template <int DT, bool CLUSTER, bool TOP>
 __global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x;
@@ -336,9 +428,11 @@ __global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
   const int64_t r = blockIdx.x / parts;
   const char *row = a.logits + r * a.row_bytes;
   const Slice sl = slice_of<DT>(row, a.V, rank, parts);
-  Stat t = sweep<DT>(row, sl, a.c);
-  if (a.k > 0) {
-    local_top<DT>(row, sl, a.c, t.m, a.k, sh);
+  uint4 keep[kKeep];
+  const bool kept = TOP && sl.nvec <= kKeep * kBlock;
+  Stat t = sweep<DT>(row, sl, a.c, keep, kept);
+  if (TOP) {
+    local_top<DT>(row, sl, a.c, t.m, a.k, sh, keep, kept);
   }
   for (int o = 16; o > 0; o >>= 1) {
     const Stat u{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o),
@@ -347,8 +441,12 @@ __global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
   }
   if ((tid & 31) == 0) sh.part[tid >> 5] = t;
   __syncthreads();
-  t = sh.part[0];
-  for (int i = 1; i < kWarps; ++i) t = merge(t, sh.part[i]);
+  t = sh.part[tid & (kWarps - 1)];  // the warps' triples, merged by every warp for itself
+  for (int o = kWarps / 2; o > 0; o >>= 1) {
+    const Stat u{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o),
+                 __shfl_xor_sync(0xffffffffu, t.w, o)};
+    t = merge(t, u);
+  }
   if (CLUSTER) {
     cg::cluster_group cl = cg::this_cluster();
     if (tid == 0) sh.total = t;
@@ -374,7 +472,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
       a.entropy[r] = empty ? 0.f : (l2 - t.w / t.s) * kLn2;
       a.lse[r] = empty ? -INFINITY : (t.m + l2) * kLn2;
     }
-    if (a.k > 0) {
+    if (TOP) {
       // candidates: the CTAs' ordered lists, at most 8 x kTopMax = kBlock of them
       float v = -INFINITY;
       int id = 0x7fffffff;
@@ -457,20 +555,20 @@ int sm_count() {
   return n > 0 ? n : 1;
 }
 
-// CTAs that share a row: enough to give every SM two CTAs, each with at least
-// 4096 elements, up to the portable cluster size.
+// CTAs that share a row: enough to give every SM eight, each with at least 2048 elements, up to
+// the portable cluster size.
 int parts_of(int64_t N, int64_t V) {
-  const int64_t want = 2 * (int64_t)sm_count();
+  const int64_t want = 8 * (int64_t)sm_count();
   int p = 1;
-  while (p < 8 && N * p * 2 <= want && V / (p * 2) >= 4096) p *= 2;
+  while (p < 8 && N * p * 2 <= want && V / (p * 2) >= 2048) p *= 2;
   return p;
 }
 
-template <int DT>
-cudaError_t launch_fwd(const FwdArgs &a, int64_t N, cudaStream_t st) {
+template <int DT, bool TOP>
+cudaError_t launch_fwd_top(const FwdArgs &a, int64_t N, cudaStream_t st) {
   const int parts = parts_of(N, a.V);
   if (parts == 1) {
-    logprobs_fwd_kernel<DT, false><<<(unsigned)N, kBlock, 0, st>>>(a);
+    logprobs_fwd_kernel<DT, false, TOP><<<(unsigned)N, kBlock, 0, st>>>(a);
     return cudaGetLastError();
   }
   cudaLaunchConfig_t cfg = {};
@@ -483,8 +581,13 @@ cudaError_t launch_fwd(const FwdArgs &a, int64_t N, cudaStream_t st) {
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<DT, true>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_fwd_kernel<DT, true, TOP>, a);
   return e != cudaSuccess ? e : cudaGetLastError();
+}
+
+template <int DT>
+cudaError_t launch_fwd(const FwdArgs &a, int64_t N, cudaStream_t st) {
+  return a.k > 0 ? launch_fwd_top<DT, true>(a, N, st) : launch_fwd_top<DT, false>(a, N, st);
 }
 
 template <int DT>

@@ -576,6 +576,22 @@ std::tuple<Tensor, Tensor> delta_fwd_autograd(const Tensor &q, const Tensor &k, 
   return {r[0], r[1]};
 }
 
+Tensor delta_step_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
+                           Tensor &state, const optional<Tensor> &slots, double scale) {
+  if (at::GradMode::is_enabled())
+    for (const Tensor *t : {&q, &k, &v, &g, &beta, const_cast<const Tensor *>(&state)})
+      TORCH_CHECK_NOT_IMPLEMENTED(!t->requires_grad(),
+                                  "gated_delta_step has no gradient: call it under torch.no_grad(), or differentiate "
+                                  "gated_delta_chunk");
+  state.unsafeGetTensorImpl()->bump_version();  // a graph that saved the pool must notice
+  at::AutoDispatchBelowADInplaceOrView below;
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("kda_b200::delta_step", "")
+                       .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, Tensor &,
+                                     const optional<Tensor> &, double)>();
+  return op.call(q, k, v, g, beta, state, slots, scale);
+}
+
 struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
   static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &tokens, int64_t top_k,
                                double temperature, int64_t ignore_index) {
@@ -671,5 +687,8 @@ TORCH_LIBRARY_IMPL(kda_b200, CUDA, m) {
 
 TORCH_LIBRARY_IMPL(kda_b200, CompositeExplicitAutograd, m) { m.impl("status_word", &status); }
 
-TORCH_LIBRARY_IMPL(kda_b200, Autograd, m) { m.impl("delta_fwd", &delta_fwd_autograd); }
+TORCH_LIBRARY_IMPL(kda_b200, Autograd, m) {
+  m.impl("delta_fwd", &delta_fwd_autograd);
+  m.impl("delta_step", &delta_step_autograd);
+}
 TORCH_LIBRARY_IMPL(st_b200, Autograd, m) { m.impl("token_logprobs", &token_logprobs_autograd); }

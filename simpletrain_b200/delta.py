@@ -91,6 +91,25 @@ def _indices(t: Tensor, name: str, device: torch.device):
         raise TypeError(f"{name} must be on q's device")
 
 
+def _check_chunk(q, k, v, g, beta, initial_state, cu_seqlens):
+    _validate(q, k, v, g, beta, "chunk")
+    B, H, T, D = v.shape
+    n = B
+    if cu_seqlens is not None:
+        _indices(cu_seqlens, "cu_seqlens", q.device)
+        if B != 1:
+            raise ValueError(f"cu_seqlens packs sequences into one row: the batch must be 1, got {B}")
+        if cu_seqlens.shape[0] < 1:
+            raise ValueError("cu_seqlens needs at least one offset")
+        n = cu_seqlens.shape[0] - 1
+    if initial_state is not None:
+        if initial_state.shape != (n, H, D, D):
+            raise ValueError(f"initial_state must be [sequences, H, D, D] = {(n, H, D, D)}, got {tuple(initial_state.shape)}")
+        if initial_state.dtype != torch.float32 or initial_state.device != q.device:
+            raise TypeError("initial_state must be float32 on q's device")
+    _need_cuda(q)
+
+
 def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, *, scale: Optional[float] = None,
                       initial_state: Optional[Tensor] = None, cu_seqlens: Optional[Tensor] = None,
                       output_final_state: bool = True) -> Tuple[Tensor, Optional[Tensor]]:
@@ -116,25 +135,30 @@ def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     infinity in a token reaches its own 64-token chunk and what follows in its
     sequence (earlier tokens of the chunk too), and no other sequence.
     """
-    _validate(q, k, v, g, beta, "chunk")
-    B, H, T, D = v.shape
-    n = B
-    if cu_seqlens is not None:
-        _indices(cu_seqlens, "cu_seqlens", q.device)
-        if B != 1:
-            raise ValueError(f"cu_seqlens packs sequences into one row: the batch must be 1, got {B}")
-        if cu_seqlens.shape[0] < 1:
-            raise ValueError("cu_seqlens needs at least one offset")
-        n = cu_seqlens.shape[0] - 1
-    if initial_state is not None:
-        if initial_state.shape != (n, H, D, D):
-            raise ValueError(f"initial_state must be [sequences, H, D, D] = {(n, H, D, D)}, got {tuple(initial_state.shape)}")
-        if initial_state.dtype != torch.float32 or initial_state.device != q.device:
-            raise TypeError("initial_state must be float32 on q's device")
-    _need_cuda(q)
-    o, s = torch.ops.kda_b200.delta_fwd(q, k, v, g, beta, D ** -0.5 if scale is None else float(scale),
-                                        initial_state, cu_seqlens, bool(output_final_state))
+    D = v.shape[-1] if v.dim() else 0
+    try:
+        o, s = torch.ops.kda_b200.delta_fwd(q, k, v, g, beta, float(D or 1) ** -0.5 if scale is None else float(scale),
+                                            initial_state, cu_seqlens, bool(output_final_state))
+    except RuntimeError:  # the op checks its arguments; say what is wrong with them
+        _check_chunk(q, k, v, g, beta, initial_state, cu_seqlens)
+        raise
     return o, (s if output_final_state else None)
+
+
+def _check_step(q, k, v, g, beta, state, state_indices):
+    _validate(q, k, v, g, beta, "step")
+    N, H, D = v.shape
+    if state.dim() != 4 or state.shape[1:] != (H, D, D):
+        raise ValueError(f"state must be [states, H, D, D] with H, D = {H}, {D}, got {tuple(state.shape)}")
+    if state.dtype != torch.float32 or state.device != q.device:
+        raise TypeError("state must be float32 on q's device")
+    if state_indices is not None:
+        _indices(state_indices, "state_indices", q.device)
+        if state_indices.shape[0] != N:
+            raise ValueError(f"state_indices must be [N] = [{N}], got {tuple(state_indices.shape)}")
+    elif N > state.shape[0]:
+        raise ValueError(f"{N} rows need {N} states, got {state.shape[0]}")
+    _need_cuda(q)
 
 
 def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, state: Tensor, *,
@@ -150,21 +174,15 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     bit of ``device_status()``.  Rows that name the same state are applied in row
     order.  The step has no gradient: differentiate ``gated_delta_chunk``.
     """
-    _validate(q, k, v, g, beta, "step")
-    N, H, D = v.shape
-    if state.dim() != 4 or state.shape[1:] != (H, D, D):
-        raise ValueError(f"state must be [states, H, D, D] with H, D = {H}, {D}, got {tuple(state.shape)}")
-    if state.dtype != torch.float32 or state.device != q.device:
-        raise TypeError("state must be float32 on q's device")
-    if state_indices is not None:
-        _indices(state_indices, "state_indices", q.device)
-        if state_indices.shape[0] != N:
-            raise ValueError(f"state_indices must be [N] = [{N}], got {tuple(state_indices.shape)}")
-    elif N > state.shape[0]:
-        raise ValueError(f"{N} rows need {N} states, got {state.shape[0]}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
-        raise NotImplementedError("gated_delta_step has no gradient: call it under torch.no_grad(), "
-                                  "or differentiate gated_delta_chunk")
-    _need_cuda(q)
-    return torch.ops.kda_b200.delta_step(q, k, v, g, beta, state, state_indices,
-                                         D ** -0.5 if scale is None else float(scale))
+    D = v.shape[-1] if v.dim() else 0
+    try:
+        return torch.ops.kda_b200.delta_step(q, k, v, g, beta, state, state_indices,
+                                             float(D or 1) ** -0.5 if scale is None else float(scale))
+    except NotImplementedError:  # gradients asked for, or tensors on the CPU
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, beta, state)):
+            raise
+        _check_step(q, k, v, g, beta, state, state_indices)
+        raise
+    except RuntimeError:
+        _check_step(q, k, v, g, beta, state, state_indices)
+        raise

@@ -188,6 +188,22 @@ def _(logits, tokens, entropy, lse, dlogprob, dentropy, temperature, ignore_inde
     return logits.new_empty(logits.shape)
 
 
+def _check_logprobs(logits, tokens, top_k, temperature):
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [N, V] with V > 0, got {tuple(logits.shape)}")
+    if tokens.shape != logits.shape[:1]:
+        raise ValueError(f"tokens must be [N] = [{logits.shape[0]}], got {tuple(tokens.shape)}")
+    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
+        raise TypeError("tokens must be int32 or int64 on the logits' device")
+    if not 0 <= top_k <= min(32, logits.shape[1]):
+        raise ValueError(f"top_k must be in [0, min(32, V)], got {top_k}")
+    if not 0.0 < temperature < float("inf"):
+        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    _need_cuda(logits, tokens)
+
+
 def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperature: float = 1.0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """Log probabilities of given tokens, entropies and top alternatives of rows of logits.
@@ -205,21 +221,11 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatur
     A row of nothing but -infinity has ``logprob = -inf``, entropy 0 and gradient
     0; a NaN or +infinity makes the row's values NaN.  Sums are fp32.
     """
-    if logits.dim() != 2 or logits.shape[1] == 0:
-        raise ValueError(f"logits must be [N, V] with V > 0, got {tuple(logits.shape)}")
-    if tokens.shape != logits.shape[:1]:
-        raise ValueError(f"tokens must be [N] = [{logits.shape[0]}], got {tuple(tokens.shape)}")
-    if logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise TypeError(f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.device != logits.device:
-        raise TypeError("tokens must be int32 or int64 on the logits' device")
-    if not 0 <= top_k <= min(32, logits.shape[1]):
-        raise ValueError(f"top_k must be in [0, min(32, V)], got {top_k}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
-    _need_cuda(logits, tokens)
-    lp, ent, _, top, ids = torch.ops.st_b200.token_logprobs(logits, tokens, int(top_k), float(temperature),
-                                                            int(ignore_index))
+    try:
+        lp, ent, _, top, ids = torch.ops.st_b200.token_logprobs(logits, tokens, top_k, temperature, ignore_index)
+    except RuntimeError:  # the op checks its arguments; say what is wrong with them
+        _check_logprobs(logits, tokens, top_k, temperature)
+        raise
     return TokenLogprobs(lp, ent, top, ids)
 
 
