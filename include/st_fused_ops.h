@@ -61,14 +61,16 @@ int st_cross_entropy_bwd(const void *logits, const int64_t *labels, const float 
    entropies and top alternatives (additions of this library).  logits: N rows
    of V elements, row_stride elements apart, aligned to their element only;
    dtype KDA_DTYPE_BF16, KDA_DTYPE_F16 or ST_DTYPE_F32.  With x = logits /
-   temperature (temperature > 0) and p = softmax(x):
+   temperature (in [1e-6, 1e6]) and p = softmax(x):
      logprob[n] = x[n, tokens[n]] - lse[n]; 0 where tokens[n] == ignore_index,
                   NaN where it is otherwise outside [0, V)
      entropy[n] = lse[n] - sum_v p_v x_v
      top_logprob, top_id [N, top_k] (top_k <= 32, <= V): the top_k largest
                   logits in order, the lower index first among equals, NaN last
-   A row of nothing but -infinity has lse = logprob = -infinity and entropy 0;
-   a NaN or +infinity makes the row's outputs NaN (its top_id stay in range). */
+   Logits below -1e29 (-infinity, the lowest values of bf16 and f32) are
+   masked: probability 0.  A row of nothing else has lse = logprob = -infinity
+   and entropy 0; a NaN or +infinity makes the row's outputs NaN (its top_id
+   stay in range). */
 enum { ST_DTYPE_F32 = 2 };
 int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprob, float *entropy,
                           float *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
@@ -78,7 +80,7 @@ int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t 
    and the forward's entropy and lse:
      dlogits_v = (dlogprob ([v == token] - p_v) - dentropy p_v (ln p_v + entropy)) / temperature
    A row whose token is ignore_index has no part through dlogprob; a row of
-   nothing but -infinity has gradient 0. */
+   nothing but masked logits has gradient 0. */
 int st_token_logprobs_bwd(const void *logits, int64_t row_stride, const int64_t *tokens, const float *entropy,
                           const float *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
                           int64_t V, float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream);

@@ -44,6 +44,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // y - m below this contributes 2^-300 = 0 in fp32; a floor keeps 0 * (y - m) finite for y = -inf
 constexpr float kFloor = -300.f;
+// Logits below kStart are masked: probability 0 (the lowest values of bf16 and fp32 are).  The running
+// maximum starts there, and masked logits count as kMask, whose distance to it is 2^-huge = 0; the
+// two are far apart so that the rounding of c times them cannot turn that distance positive.
+constexpr float kStart = -1.2345e29f;
+constexpr float kMask = -1e30f;
 
 enum { kBF16 = 0, kF16 = 1, kF32 = 2 };
 
@@ -93,53 +98,59 @@ struct Elem {
   }
 };
 
-// Two fp32 lanes at once.
-struct F2 {
-  uint64_t v;
-  __device__ __forceinline__ F2() {}
-  __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
-  __device__ __forceinline__ float2 get() const {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
+// The largest of each half of a vector of 16-bit pairs (NaN if one is NaN)
+template <int DT>
+__device__ __forceinline__ uint32_t packed_max(const uint4 &v) {
+  uint32_t a, b, m;
+  if (DT == kBF16) {
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
+  } else {
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
   }
-};
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
+  return m;
 }
 
-// Largest element of a 16-byte vector; NaN if one is NaN.  16-bit types compare in pairs.
+// Largest element of a 16-byte vector; NaN if one is NaN.
 template <int DT>
 __device__ __forceinline__ float vec_max(const uint4 &v) {
-  uint32_t m;
   if (DT == kF32) {
     float a, b;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(v.x)), "f"(__uint_as_float(v.y)));
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w)));
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(a), "f"(b));
     return a;
-  } else if (DT == kBF16) {
-    uint32_t a, b;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
-  } else {
-    uint32_t a, b;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(v.x), "r"(v.y));
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(v.z), "r"(v.w));
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(m) : "r"(a), "r"(b));
   }
-  const float2 p = unpack2(m, DT == kBF16);
+  const float2 p = unpack2(packed_max<DT>(v), DT == kBF16);
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(p.x), "f"(p.y));
   return r;
+}
+
+// Elements below kMask raised to it (NaN stays NaN): what a mask leaves (-inf, a type's lowest
+// value) has probability 0, and 0 * (y - m) must be 0 and not NaN.  bf16 does that in pairs; fp16
+// ends at -65504, which is a value like others, so it is done after the conversion.
+__device__ __forceinline__ float floor1(float x) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(kMask));
+  return r;
+}
+template <int DT, int N>
+__device__ __forceinline__ void unpack_floored(uint4 v, float (&f)[N]) {
+  if (DT == kBF16) {
+    auto pair = [](uint32_t &x) { asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(x) : "r"(x), "r"(0xF149F149u)); };
+    pair(v.x);
+    pair(v.y);
+    pair(v.z);
+    pair(v.w);
+  }
+  Elem<DT>::unpack(v, f);
+  if (DT != kBF16)
+#pragma unroll
+    for (int k = 0; k < N; ++k) f[k] = floor1(f[k]);
 }
 
 // The part of a row that one CTA of the row's cluster owns: scalar elements
@@ -181,72 +192,97 @@ __device__ __forceinline__ void for_each(const char *row, const Slice &sl, F fn)
   for (int64_t i = sl.tail + threadIdx.x; i < sl.hi; i += kBlock) fn(i, E::load(row, i));
 }
 
-// running (m, s, w); m = -inf means "nothing but -inf yet" (s = w = 0)
+// running (m, s, w), m = c * (largest logit, kStart at least).  A row whose m never leaves c * kStart
+// is empty.
 struct Stat {
   float m, s, w;
 };
 
 __device__ __forceinline__ Stat merge(const Stat &a, const Stat &b) {
-  const float M = fmaxf(a.m, b.m);
-  if (M == -INFINITY) return {M, a.s + b.s, a.w + b.w};  // sums are 0, or NaN from a NaN logit
-  const float da = fmaxf(a.m - M, kFloor), db = fmaxf(b.m - M, kFloor);
+  const float M = fmaxf(a.m, b.m), da = fmaxf(a.m - M, kFloor), db = fmaxf(b.m - M, kFloor);
   const float fa = ex2(da), fb = ex2(db);
   return {M, a.s * fa + b.s * fb, (a.w + da * a.s) * fa + (b.w + db * b.s) * fb};
 }
 
-__device__ __forceinline__ void add1(Stat &t, float y) {
-  if (y > t.m) {
-    const float d = fmaxf(t.m - y, kFloor), f = ex2(d);
-    t.w = (t.w + d * t.s) * f;
-    t.s *= f;
-    t.m = y;
-  }
-  if (t.m != -INFINITY || y != y) {
-    const float d = y - t.m, e = ex2(d);
-    t.s += e;
-    t.w = fmaf(e, fmaxf(d, kFloor), t.w);
-  }
+__device__ __forceinline__ void raise(Stat &t, float m) {
+  const float d = fmaxf(t.m - m, kFloor), f = ex2(d);
+  t.w = (t.w + d * t.s) * f;
+  t.s *= f;
+  t.m = m;
 }
+
+__device__ __forceinline__ void add1(Stat &t, float x, float c) {
+  const float y = c * floor1(x);
+  if (y > t.m) raise(t, y);
+  const float d = y - t.m, e = ex2(d);
+  t.s += e;
+  t.w = fmaf(e, fmaxf(d, kFloor), t.w);
+}
+
+// The largest logit so far in the logits' own type, both halves alike where two share a register:
+// whether a vector holds a larger one (or a NaN) takes three packed maxima and a packed comparison.
+template <int DT>
+struct RawMax {
+  uint32_t m = DT == kF32 ? 0xFF800000u : (DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u);  // -inf
+  // true if `v` is to raise it, which it then does; *top: the vector's largest, or NaN
+  __device__ __forceinline__ bool raised(const uint4 &v, float *top) {
+    if (DT == kF32) {
+      *top = vec_max<DT>(v);
+      if (*top <= __uint_as_float(m)) return false;
+      if (*top == *top) m = __float_as_uint(*top);
+      return true;
+    }
+    const uint32_t x = packed_max<DT>(v);
+    uint32_t le;
+    if (DT == kBF16)
+      asm("{\n\t.reg .pred p, q;\n\tsetp.le.bf16x2 p|q, %1, %2;\n\tand.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(le) : "r"(x), "r"(m));
+    else
+      asm("{\n\t.reg .pred p, q;\n\tsetp.le.f16x2 p|q, %1, %2;\n\tand.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(le) : "r"(x), "r"(m));
+    if (le) return false;
+    const float2 p = unpack2(x, DT == kBF16);
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(*top) : "f"(p.x), "f"(p.y));
+    if (*top == *top) m = pack2(*top, *top, DT == kBF16);
+    return true;
+  }
+};
 
 // Vectors of a slice that its threads keep in registers, so that the second sweep reads no memory.
 constexpr int kKeep = 8;
 
 // one 16-byte vector into the running triple
 template <int DT>
-__device__ __forceinline__ void add_vec(Stat &t, const uint4 &raw, float c) {
+__device__ __forceinline__ void add_vec(Stat &t, RawMax<DT> &mx, const uint4 &raw, float c) {
   using E = Elem<DT>;
-  const float mv = vec_max<DT>(raw) * c;
-  if (!(mv <= t.m)) {  // a larger maximum, or a NaN
-    if (mv != mv) {
+  float top;
+  if (mx.raised(raw, &top)) {
+    if (top != top) {
       t.s = t.w = NAN;
       return;
     }
-    const float d = fmaxf(t.m - mv, kFloor), f = ex2(d);
-    t.w = (t.w + d * t.s) * f;
-    t.s *= f;
-    t.m = mv;
+    const float y = c * floor1(top);
+    if (y > t.m) raise(t, y);
   }
-  if (t.m == -INFINITY) return;
   float f[E::kVec];
-  E::unpack(raw, f);
-  const F2 cc(c, c), mm(-t.m, -t.m);
-  F2 s(0.f, 0.f), w(0.f, 0.f);
+  unpack_floored<DT>(raw, f);
+  float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
   for (int k = 0; k < E::kVec; k += 2) {
-    const float2 d = fma2(F2(f[k], f[k + 1]), cc, mm).get();
-    const F2 e(ex2(d.x), ex2(d.y));
-    s = add2(s, e);
-    w = fma2(e, F2(fmaxf(d.x, kFloor), fmaxf(d.y, kFloor)), w);
+    const float d0 = fmaf(f[k], c, -t.m), d1 = fmaf(f[k + 1], c, -t.m);
+    const float e0 = ex2(d0), e1 = ex2(d1);
+    s0 += e0;
+    s1 += e1;
+    w0 = fmaf(e0, d0, w0);
+    w1 = fmaf(e1, d1, w1);
   }
-  const float2 ss = s.get(), ww = w.get();
-  t.s += ss.x + ss.y;
-  t.w += ww.x + ww.y;
+  t.s += s0 + s1;
+  t.w += w0 + w1;
 }
 
 template <int DT>
 __device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c, uint4 (&keep)[kKeep], bool kept) {
   using E = Elem<DT>;
-  Stat t{-INFINITY, 0.f, 0.f};
+  Stat t{c * kStart, 0.f, 0.f};
+  RawMax<DT> mx;
   const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
   if (kept) {
 #pragma unroll
@@ -254,20 +290,21 @@ __device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c,
       if (threadIdx.x + j * kBlock < sl.nvec) keep[j] = __ldg(v4 + threadIdx.x + j * kBlock);
 #pragma unroll
     for (int j = 0; j < kKeep; ++j)
-      if (threadIdx.x + j * kBlock < sl.nvec) add_vec<DT>(t, keep[j], c);
+      if (threadIdx.x + j * kBlock < sl.nvec) add_vec<DT>(t, mx, keep[j], c);
   } else {
-    int64_t i = threadIdx.x;
-    for (; i + 3 * kBlock < sl.nvec; i += 4 * kBlock) {  // four loads in flight a thread
-      uint4 r[4];
+    constexpr int F = 4;  // loads in flight a thread
+    for (int64_t i = threadIdx.x; i < sl.nvec; i += F * kBlock) {
+      uint4 r[F];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = __ldg(v4 + i + j * kBlock);
+      for (int j = 0; j < F; ++j)
+        if (i + j * kBlock < sl.nvec) r[j] = __ldg(v4 + i + j * kBlock);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) add_vec<DT>(t, r[j], c);
+      for (int j = 0; j < F; ++j)
+        if (i + j * kBlock < sl.nvec) add_vec<DT>(t, mx, r[j], c);
     }
-    for (; i < sl.nvec; i += kBlock) add_vec<DT>(t, __ldg(v4 + i), c);
   }
-  for (int64_t j = sl.lo + threadIdx.x; j < sl.body; j += kBlock) add1(t, c * E::load(row, j));
-  for (int64_t j = sl.tail + threadIdx.x; j < sl.hi; j += kBlock) add1(t, c * E::load(row, j));
+  for (int64_t j = sl.lo + threadIdx.x; j < sl.body; j += kBlock) add1(t, E::load(row, j), c);
+  for (int64_t j = sl.tail + threadIdx.x; j < sl.hi; j += kBlock) add1(t, E::load(row, j), c);
   return t;
 }
 
@@ -318,10 +355,10 @@ __device__ void local_top(const char *row, const Slice &sl, float c, float threa
     if (rank == k - 1) sh.bound = mine;
   }
   __syncthreads();
-  const float bound = sh.bound;
+  const float bound = sh.bound > c * kStart ? sh.bound : -INFINITY;  // fewer than k logits that are not masked
   auto offer = [&](int64_t i, float x) {
     x = sort_key(x);
-    if (c * x >= bound) {
+    if (c * floor1(x) >= bound) {
       const int at = atomicAdd(&sh.count, 1);
       if (at < kCand) {
         sh.cand_v[at] = x;
@@ -329,23 +366,34 @@ __device__ void local_top(const char *row, const Slice &sl, float c, float threa
       }
     }
   };
+  auto offer_vec = [&](int64_t i, const uint4 &raw) {
+    const float mv = vec_max<DT>(raw);
+    if (c * floor1(mv) >= bound || mv != mv) {  // few vectors hold a candidate
+      float f[E::kVec];
+      E::unpack(raw, f);
+#pragma unroll
+      for (int e = 0; e < E::kVec; ++e) offer(sl.body + i * E::kVec + e, f[e]);
+    }
+  };
   if (kept) {
 #pragma unroll
     for (int j = 0; j < kKeep; ++j)
-      if (tid + j * kBlock < sl.nvec) {
-        const float mv = vec_max<DT>(keep[j]);
-        if (c * mv >= bound || mv != mv || bound == -INFINITY) {  // few vectors hold a candidate
-          float f[E::kVec];
-          E::unpack(keep[j], f);
-#pragma unroll
-          for (int e = 0; e < E::kVec; ++e) offer(sl.body + (int64_t)(tid + j * kBlock) * E::kVec + e, f[e]);
-        }
-      }
-    for (int64_t i = sl.lo + tid; i < sl.body; i += kBlock) offer(i, E::load(row, i));
-    for (int64_t i = sl.tail + tid; i < sl.hi; i += kBlock) offer(i, E::load(row, i));
+      if (tid + j * kBlock < sl.nvec) offer_vec(tid + j * kBlock, keep[j]);
   } else {
-    for_each<DT>(row, sl, offer);
+    const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
+    constexpr int F = 8;  // loads in flight a thread
+    for (int64_t i = tid; i < sl.nvec; i += F * kBlock) {
+      uint4 r[F];
+#pragma unroll
+      for (int j = 0; j < F; ++j)
+        if (i + j * kBlock < sl.nvec) r[j] = __ldg(v4 + i + j * kBlock);
+#pragma unroll
+      for (int j = 0; j < F; ++j)
+        if (i + j * kBlock < sl.nvec) offer_vec(i + j * kBlock, r[j]);
+    }
   }
+  for (int64_t i = sl.lo + tid; i < sl.body; i += kBlock) offer(i, E::load(row, i));
+  for (int64_t i = sl.tail + tid; i < sl.hi; i += kBlock) offer(i, E::load(row, i));
   __syncthreads();
   const int n = sh.count;
   if (n <= kCand) {
@@ -417,7 +465,7 @@ struct FwdArgs {
 };
 
 template <int DT, bool CLUSTER, bool TOP>
-__global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
+__global__ void __launch_bounds__(kBlock, TOP ? 4 : 6) logprobs_fwd_kernel(const FwdArgs a) {
   __shared__ Shared sh;
   const int tid = threadIdx.x;
   int rank = 0, parts = 1;
@@ -456,7 +504,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_fwd_kernel(const FwdArgs a) {
   }
   if (rank == 0) {
     const float l2 = log2f(t.s);
-    const bool empty = t.m == -INFINITY && t.s == 0.f;  // no finite logit in the row
+    const bool empty = t.m <= a.c * kStart && t.s == t.s;  // only masked logits in the row
     if (tid == 0) {
       const int64_t tok = a.tokens[r];
       float lp;
@@ -524,8 +572,8 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r], l2 = lse * kLog2e;
   const float base = -a - b * H, slope = -b * kLn2;
   auto grad = [&](int64_t i, float x) {
-    const float d = fmaf(x, g.c, -l2), p = ex2(d);
-    float v = p * fmaf(slope, fmaxf(d, kFloor), base);
+    const float d = fmaf(floor1(x), g.c, -l2), p = ex2(d);
+    float v = p * fmaf(slope, d, base);
     if (i == tok) v += a;
     return empty ? 0.f : v;
   };
@@ -555,10 +603,10 @@ int sm_count() {
   return n > 0 ? n : 1;
 }
 
-// CTAs that share a row: enough to give every SM eight, each with at least 2048 elements, up to
+// CTAs that share a row: enough to give every SM two, each with at least 2048 elements, up to
 // the portable cluster size.
 int parts_of(int64_t N, int64_t V) {
-  const int64_t want = 8 * (int64_t)sm_count();
+  const int64_t want = 2 * (int64_t)sm_count();
   int p = 1;
   while (p < 8 && N * p * 2 <= want && V / (p * 2) >= 2048) p *= 2;
   return p;
@@ -603,7 +651,7 @@ cudaError_t launch_bwd(const BwdArgs &a, int64_t N, cudaStream_t st) {
 
 int check(int64_t N, int64_t V, int64_t stride, float temperature, int32_t dtype) {
   if (N < 0 || V <= 0 || N > 0x7fffffff / 8 || V > 0x7ffffffe || (N > 1 && stride < V)) return KDA_ERR_BAD_SHAPE;
-  if (!(temperature > 0.f) || temperature > 3.4e38f) return KDA_ERR_UNSUPPORTED;
+  if (!(temperature >= 1e-6f) || temperature > 1e6f) return KDA_ERR_UNSUPPORTED;  // c * kMask is finite
   if (dtype != kBF16 && dtype != kF16 && dtype != kF32) return KDA_ERR_UNSUPPORTED;
   return KDA_OK;
 }

@@ -199,8 +199,8 @@ def _check_logprobs(logits, tokens, top_k, temperature):
         raise TypeError("tokens must be int32 or int64 on the logits' device")
     if not 0 <= top_k <= min(32, logits.shape[1]):
         raise ValueError(f"top_k must be in [0, min(32, V)], got {top_k}")
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"temperature must be in [1e-6, 1e6], got {temperature}")
     _need_cuda(logits, tokens)
 
 
@@ -218,8 +218,10 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatur
     * ``top_logprobs, top_ids [N, top_k]`` (top_k <= 32): the largest logits in
       order, the lower index first among equal ones; plain tensors without gradient.
 
-    A row of nothing but -infinity has ``logprob = -inf``, entropy 0 and gradient
-    0; a NaN or +infinity makes the row's values NaN.  Sums are fp32.
+    Logits below -1e29 (-infinity, the lowest values of bf16 and fp32) are
+    masked, with probability 0.  A row of nothing else has ``logprob = -inf``,
+    entropy 0 and gradient 0; a NaN or +infinity makes the row's values NaN.  Sums
+    are fp32.
     """
     try:
         lp, ent, _, top, ids = torch.ops.st_b200.token_logprobs(logits, tokens, top_k, temperature, ignore_index)

@@ -103,6 +103,34 @@ def test_masked_logits_rows_and_padding():
     assert torch.isnan(r.logprob[5]) and torch.isfinite(r.entropy[5])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_lowest_values_as_masks(dtype):
+    """A mask may be the type's lowest value; in fp16 that is a logit like others."""
+    from simpletrain_b200.fused_ops import token_logprobs
+    low = torch.finfo(dtype).min
+    x, tok, a, b = make(4, 3001, dtype)
+    x[0, 7:] = low
+    x[1] = low
+    x[2, ::2] = low
+    x[2, 1::4] = -torch.inf
+    x[3] = low
+    x[3, 11] = -3.0
+    tok = torch.tensor([3, 3, 3, 11], device=DEV)
+    leaf = x.requires_grad_(True)
+    r = token_logprobs(leaf, tok, top_k=2)
+    (dx,) = torch.autograd.grad((r.logprob, r.entropy), leaf, (a, b))
+    ref = x.detach().double()
+    lp, H = logprobs(ref, tok)
+    for n in (0, 2, 3):
+        assert abs(r.logprob[n].item() - lp[n].item()) <= ABS and abs(r.entropy[n].item() - H[n].item()) <= ABS
+    if dtype == torch.float16:
+        assert abs(r.logprob[1].item() - lp[1].item()) <= ABS and abs(r.entropy[1].item() - H[1].item()) <= ABS
+    else:
+        assert r.logprob[1].item() == -torch.inf and r.entropy[1].item() == 0 and (dx[1] == 0).all()
+    assert torch.isfinite(dx).all() and (dx[0, 7:] == 0).all() and (dx[2, ::2] == 0).all()
+    assert r.top_ids[1].tolist() == [0, 1] and r.top_ids[3].tolist() == [11, 0]
+
+
 def test_non_finite_logits_spoil_their_row_only():
     from simpletrain_b200.fused_ops import token_logprobs
     x, tok, _, _ = make(4, 20000, torch.bfloat16)
