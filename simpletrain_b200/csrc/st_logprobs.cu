@@ -219,60 +219,61 @@ __device__ __forceinline__ void add1(Stat &t, float x, float c) {
   t.w = fmaf(e, fmaxf(d, kFloor), t.w);
 }
 
-// The largest logit so far in the logits' own type, both halves alike where two share a register:
-// whether a vector holds a larger one (or a NaN) takes three packed maxima and a packed comparison.
-template <int DT>
-struct RawMax {
-  uint32_t m = DT == kF32 ? 0xFF800000u : (DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u);  // -inf
-  // true if `v` is to raise it, which it then does; *top: the vector's largest, or NaN
-  __device__ __forceinline__ bool raised(const uint4 &v, float *top) {
-    if (DT == kF32) {
-      *top = vec_max<DT>(v);
-      if (*top <= __uint_as_float(m)) return false;
-      if (*top == *top) m = __float_as_uint(*top);
-      return true;
-    }
-    const uint32_t x = packed_max<DT>(v);
-    uint32_t le;
-    if (DT == kBF16)
-      asm("{\n\t.reg .pred p, q;\n\tsetp.le.bf16x2 p|q, %1, %2;\n\tand.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(le) : "r"(x), "r"(m));
-    else
-      asm("{\n\t.reg .pred p, q;\n\tsetp.le.f16x2 p|q, %1, %2;\n\tand.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(le) : "r"(x), "r"(m));
-    if (le) return false;
-    const float2 p = unpack2(x, DT == kBF16);
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(*top) : "f"(p.x), "f"(p.y));
-    if (*top == *top) m = pack2(*top, *top, DT == kBF16);
-    return true;
-  }
-};
-
 // Vectors of a slice that its threads keep in registers, so that the second sweep reads no memory.
 constexpr int kKeep = 8;
 
-// one 16-byte vector into the running triple
+// -infinity in every element
 template <int DT>
-__device__ __forceinline__ void add_vec(Stat &t, RawMax<DT> &mx, const uint4 &raw, float c) {
+__device__ __forceinline__ uint4 vec_nothing() {
+  const uint32_t x = DT == kF32 ? 0xFF800000u : (DT == kBF16 ? 0xFF80FF80u : 0xFC00FC00u);
+  return make_uint4(x, x, x, x);
+}
+
+template <int DT>
+__device__ __forceinline__ uint4 vec_max2(const uint4 &a, const uint4 &b) {
+  auto f = [](uint32_t x, uint32_t y) {
+    uint32_t r;
+    if (DT == kBF16)
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    else if (DT == kF16)
+      asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    else
+      asm("max.NaN.f32 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(y));
+    return r;
+  };
+  return make_uint4(f(a.x, b.x), f(a.y, b.y), f(a.z, b.z), f(a.w, b.w));
+}
+
+// F vectors into the running triple.  The maximum is looked after once for all of them: some lane of
+// a warp raises it nearly every time, and the whole warp then pays for the rescaling.
+template <int DT, int F, int N>
+__device__ __forceinline__ void add_batch(Stat &t, const uint4 (&raw)[N], int first, float c) {
   using E = Elem<DT>;
-  float top;
-  if (mx.raised(raw, &top)) {
-    if (top != top) {
+  uint4 mv = raw[first];
+#pragma unroll
+  for (int j = 1; j < F; ++j) mv = vec_max2<DT>(mv, raw[first + j]);
+  const float top = vec_max<DT>(mv), y = c * floor1(top);
+  if (!(y <= t.m)) {  // a larger maximum, or a NaN
+    if (y != y) {
       t.s = t.w = NAN;
       return;
     }
-    const float y = c * floor1(top);
-    if (y > t.m) raise(t, y);
+    raise(t, y);
   }
-  float f[E::kVec];
-  unpack_floored<DT>(raw, f);
   float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
 #pragma unroll
-  for (int k = 0; k < E::kVec; k += 2) {
-    const float d0 = fmaf(f[k], c, -t.m), d1 = fmaf(f[k + 1], c, -t.m);
-    const float e0 = ex2(d0), e1 = ex2(d1);
-    s0 += e0;
-    s1 += e1;
-    w0 = fmaf(e0, d0, w0);
-    w1 = fmaf(e1, d1, w1);
+  for (int j = 0; j < F; ++j) {
+    float f[E::kVec];
+    unpack_floored<DT>(raw[first + j], f);
+#pragma unroll
+    for (int k = 0; k < E::kVec; k += 2) {
+      const float d0 = fmaf(f[k], c, -t.m), d1 = fmaf(f[k + 1], c, -t.m);
+      const float e0 = ex2(d0), e1 = ex2(d1);
+      s0 += e0;
+      s1 += e1;
+      w0 = fmaf(e0, d0, w0);
+      w1 = fmaf(e1, d1, w1);
+    }
   }
   t.s += s0 + s1;
   t.w += w0 + w1;
@@ -282,25 +283,21 @@ template <int DT>
 __device__ __forceinline__ Stat sweep(const char *row, const Slice &sl, float c, uint4 (&keep)[kKeep], bool kept) {
   using E = Elem<DT>;
   Stat t{c * kStart, 0.f, 0.f};
-  RawMax<DT> mx;
   const uint4 *v4 = reinterpret_cast<const uint4 *>(row + sl.body * E::kBytes);
+  const int n = (int)sl.nvec, tid = threadIdx.x;
+  constexpr int F = 4;  // loads in flight a thread
   if (kept) {
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j)
-      if (threadIdx.x + j * kBlock < sl.nvec) keep[j] = __ldg(v4 + threadIdx.x + j * kBlock);
+    for (int j = 0; j < kKeep; ++j) keep[j] = tid + j * kBlock < n ? __ldg(v4 + tid + j * kBlock) : vec_nothing<DT>();
 #pragma unroll
-    for (int j = 0; j < kKeep; ++j)
-      if (threadIdx.x + j * kBlock < sl.nvec) add_vec<DT>(t, mx, keep[j], c);
+    for (int j = 0; j < kKeep; j += F)
+      if (j * kBlock < n) add_batch<DT, F>(t, keep, j, c);
   } else {
-    constexpr int F = 4;  // loads in flight a thread
-    for (int64_t i = threadIdx.x; i < sl.nvec; i += F * kBlock) {
+    for (int i = tid; i < n; i += F * kBlock) {
       uint4 r[F];
 #pragma unroll
-      for (int j = 0; j < F; ++j)
-        if (i + j * kBlock < sl.nvec) r[j] = __ldg(v4 + i + j * kBlock);
-#pragma unroll
-      for (int j = 0; j < F; ++j)
-        if (i + j * kBlock < sl.nvec) add_vec<DT>(t, mx, r[j], c);
+      for (int j = 0; j < F; ++j) r[j] = i + j * kBlock < n ? __ldg(v4 + i + j * kBlock) : vec_nothing<DT>();
+      add_batch<DT, F>(t, r, 0, c);
     }
   }
   for (int64_t j = sl.lo + threadIdx.x; j < sl.body; j += kBlock) add1(t, E::load(row, j), c);
