@@ -21,6 +21,8 @@
 // depend on the launch.  The tiles of one value head fill an SM's shared memory, so the
 // next head's are brought into L2 meanwhile; 16 warps, a token row and a quarter of the
 // columns a thread, work off the products.
+#include <atomic>
+
 #include "kda_delta_tc.cuh"
 
 namespace kda {
@@ -456,6 +458,21 @@ int check_sizes(const kda_delta_params *p) {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
+// CTAs of a scan: one an SM, and no more than there are streams (sequence, head).
+int scan_ranges(int64_t nseq, int64_t H) {
+  static std::atomic<int> cache[64];  // by device; 0 = not asked yet
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
+    sms = cache[dev].load(std::memory_order_relaxed);
+    if (sms == 0) {
+      if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+      cache[dev].store(sms, std::memory_order_relaxed);
+    }
+  }
+  const int64_t n = nseq * H;
+  return (int)(n < 1 ? 1 : (n < sms ? n : sms));
+}
+
 // Sizes and workspace regions; returns the bytes needed (p->workspace may be NULL).
 size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->p = *p;
@@ -476,6 +493,9 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
     a->w.bound = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
     a->w.first = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
   }
+  a->ranges = scan_ranges(a->nseq, p->H);
+  a->w.queue = reinterpret_cast<int *>(take(sizeof(int) * 2 * ((size_t)a->ranges + 2)));
+  a->w.slots = reinterpret_cast<float *>(take(((size_t)a->ranges + 1) * p->D * p->D * 4));
   a->w.gam = reinterpret_cast<float *>(take(cells * 256));
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
   a->w.T = take(cells * kda::delta::kImgT);

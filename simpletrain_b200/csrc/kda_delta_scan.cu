@@ -136,6 +136,8 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   __shared__ __align__(16) float gam[64], bet[64], cfac[32];
   int64_t b, t0;
   int rows;
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < 2 * (a.ranges + 2); i += kThreads) a.w.queue[i] = 0;
   if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
   const int h = blockIdx.y, hk = h / (a.p.H / a.p.Hk), tid = threadIdx.x;
   const int row = tid & 127, half = tid >> 7, r64 = row & 63;
@@ -286,7 +288,7 @@ __device__ void zero_outside(const Args &a, const kda_tensor &o, int h, int col0
   const int lo = a.w.bound[0], hi = a.w.bound[a.nseq];
   const int64_t rows = (int64_t)lo + (a.p.T - hi);
   uint16_t *base = static_cast<uint16_t *>(o.data) + h * o.stride_h + col0;
-  for (int64_t e = threadIdx.x; e < rows * 8; e += kThreads) {
+  for (int64_t e = threadIdx.x; e < rows * 8; e += blockDim.x) {
     const int64_t r = e >> 3, t = r < lo ? r : r - lo + hi;
     *reinterpret_cast<uint4 *>(base + t * o.stride_t + (e & 7) * 8) = make_uint4(0, 0, 0, 0);
   }
@@ -294,12 +296,12 @@ __device__ void zero_outside(const Args &a, const kda_tensor &o, int h, int col0
 __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
   const int lo = a.w.bound[0], hi = a.w.bound[a.nseq];
   const int64_t rows = (int64_t)lo + (a.p.T - hi);
-  for (int64_t r = threadIdx.x; r < rows; r += kThreads)
+  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x)
     store_gate(p, (int64_t)h * a.p.T + (r < lo ? r : r - lo + hi), dtype, 0.f);
 }
 
 // ------------------------------------------------------------------ the scans --
-// One CTA per (sequence, head) and direction, with the state transposed in tensor memory:
+// The state is transposed in tensor memory:
 // lanes are the value channels, columns the key channels, so that the operand that changes
 // from step to step (the state, X, U) is always the first one and goes from registers
 // straight back into tensor memory, split in two terms, without touching shared memory:
@@ -308,6 +310,13 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // (U' = e^{gamma_63 - gamma} U, dY = -G beta dX, Q' = scale G Q).  A first version with the
 // state as the second operand in shared memory spent 880 of 6750 cycles a chunk and half
 // state on the first product alone: its operands, not its arithmetic, set the time.
+//
+// Scheduling.  The chunks of all streams (sequence, head), stream after stream, are cut into as
+// many equal ranges as there are CTAs (one an SM), so that 160 streams on 148 SMs take 35 chunks'
+// time and not 64.  The state crosses a cut through a slot in global memory.  A CTA first runs the
+// piece that ends its range, which begins a stream and waits for nobody, and publishes its state;
+// the piece that begins its range, whose first state is the one that the range before published
+// first of all, comes last.  Ranges go by tickets, so a CTA only waits for one that is running.
 //
 // Warps: 8 walk the dependent chain (a value channel a thread, half the columns each), 4
 // turn finished tiles into output or workspace rows, one starts the loads, one issues the
@@ -333,7 +342,99 @@ struct ScanSmem {
 
 struct ScanBars {
   uint64_t full[2], empty[2];
-  uint64_t tail, s_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
+  uint64_t tail[2], s_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
+};
+
+// Wait (bounded, like mbar_wait) for a range's entry state.
+__device__ __forceinline__ void wait_flag(const int *flag, int32_t *status, volatile int *abort_flag) {
+  if ((threadIdx.x & 31) == 0) {
+    const long long t0 = clock64();
+    int v = 0;
+    while (!*abort_flag) {
+      asm volatile("ld.acquire.gpu.global.b32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
+      if (v != 0) break;
+      if (clock64() - t0 > kWaitCycles) {
+        if (status) atomicOr(status, KDA_ERR_DEVICE_TIMEOUT);
+        *abort_flag = 1;
+      }
+    }
+    __threadfence();
+  }
+  __syncwarp();
+}
+
+// A part of a stream: positions [p0, p1) of its nc chunks (position 0 is the last chunk in reverse).
+struct Piece {
+  int n, h, p0, p1, nc;
+};
+// The pieces of chunks [lo, hi), in the order in which a CTA runs them: the last stream's, the
+// streams between, the first stream's.
+struct Pieces {
+  int n0, h0, c0, nc0, n1, h1, c1;  // streams and positions of the first and the last chunk
+  int turn, n, h;
+  static __device__ __forceinline__ int chunks(const Args &a, int i) {
+    return a.p.cu_seqlens == nullptr ? a.per_seq : a.w.first[i + 1] - a.w.first[i];
+  }
+  static __device__ __forceinline__ void locate(const Args &a, int x, int *sn, int *sh, int *sc) {
+    if (a.p.cu_seqlens == nullptr) {
+      const int s = x / a.per_seq;
+      *sn = s / a.p.H;
+      *sh = s % a.p.H;
+      *sc = x % a.per_seq;
+      return;
+    }
+    int l = 0, r = a.nseq;  // H first[l] <= x < H first[r]
+    while (r - l > 1) {
+      const int mid = (l + r) >> 1;
+      if ((int64_t)a.w.first[mid] * a.p.H <= x) l = mid; else r = mid;
+    }
+    const int nc = chunks(a, l), rem = x - a.w.first[l] * a.p.H;
+    *sn = l;
+    *sh = rem / nc;
+    *sc = rem % nc;
+  }
+  __device__ __forceinline__ void begin(const Args &a, int lo, int hi) {
+    turn = lo < hi ? 0 : 3;
+    if (turn == 3) return;
+    locate(a, lo, &n0, &h0, &c0);
+    locate(a, hi - 1, &n1, &h1, &c1);
+    nc0 = chunks(a, n0);
+  }
+  __device__ __forceinline__ bool next(const Args &a, Piece *p) {
+    if (turn == 0) {
+      const bool one = n0 == n1 && h0 == h1;
+      *p = {n1, h1, one ? c0 : 0, c1 + 1, chunks(a, n1)};
+      turn = one ? 3 : 1;
+      n = n0;
+      h = h0;
+      return true;
+    }
+    if (turn == 1) {  // the next stream that has chunks; the range's last one is not behind us
+      if (++h == a.p.H) {
+        h = 0;
+        do ++n; while (chunks(a, n) == 0);
+      }
+      if (n != n1 || h != h1) {
+        const int nc = chunks(a, n);
+        *p = {n, h, 0, nc, nc};
+        return true;
+      }
+      turn = 2;
+    }
+    if (turn == 2) {
+      *p = {n0, h0, c0, nc0, nc0};
+      turn = 3;
+      return true;
+    }
+    return false;
+  }
+};
+// Each warp keeps its place in shared memory: as registers of every thread it made the chain spill.
+struct WarpPlace {
+  Pieces pieces;
+  Piece pc;
+  Seq s;
+  int more;
 };
 
 // tensor-memory columns
@@ -379,39 +480,51 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   __shared__ __align__(16) Factors fac[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
+  __shared__ WarpPlace places[kScanThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int h = blockIdx.x % a.p.H, n = blockIdx.x / a.p.H, G_ = a.p.H / a.p.Hk, hk = h / G_;
-  if (n == a.nseq) {  // packed sequences: the rows outside them
-    for (int c = 0; c < D; c += 64) {
-      if (MODE == kOut) zero_outside(a, a.p.o, h, c);
-      if (REV) {
-        zero_outside(a, a.p.dv, h, c);
-        if (h % G_ == 0) {
-          zero_outside(a, a.p.dq, hk, c);
-          zero_outside(a, a.p.dk, hk, c);
+  const int G_ = a.p.H / a.p.Hk;
+  if (MODE != kStore) {
+    if (a.p.cu_seqlens != nullptr)  // the rows outside all sequences
+      for (int h = blockIdx.x; h < a.p.H; h += gridDim.x) {
+        for (int c = 0; c < D; c += 64) {
+          if (MODE == kOut) zero_outside(a, a.p.o, h, c);
+          if (REV) {
+            zero_outside(a, a.p.dv, h, c);
+            if (h % G_ == 0) {
+              zero_outside(a, a.p.dq, h / G_, c);
+              zero_outside(a, a.p.dk, h / G_, c);
+            }
+          }
+        }
+        if (REV) {
+          zero_outside(a, a.p.dg, a.p.g_dtype, h);
+          zero_outside(a, a.p.dbeta, a.p.beta_dtype, h);
         }
       }
-    }
-    if (REV) {
-      zero_outside(a, a.p.dg, a.p.g_dtype, h);
-      zero_outside(a, a.p.dbeta, a.p.beta_dtype, h);
-    }
-    return;
+    const float *src = REV ? a.p.dstate_out : a.p.state_in;
+    float *dst = REV ? a.p.dstate_in : a.p.state_out;
+    if (dst != nullptr)  // sequences without tokens hand their state on
+      for (int i = blockIdx.x; i < a.nseq * a.p.H; i += gridDim.x)
+        if (get_seq(a, i / a.p.H).len == 0)
+          for (int e = tid; e < D * D; e += kScanThreads) dst[(size_t)i * D * D + e] = src != nullptr ? src[(size_t)i * D * D + e] : 0.f;
   }
+  __shared__ int range_slot;
+  int *queue = a.w.queue + (MODE == kRev ? a.ranges + 2 : 0);
   const uint32_t sb = smem_u32(smem);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&bars.full[i]), 32);
       mbar_init(smem_u32(&bars.empty[i]), MODE == kStore ? 1 : 1 + Q);
       mbar_init(smem_u32(&bars.s_ready[i]), 2 * Q);
+      mbar_init(smem_u32(&bars.tail[i]), 32);
     }
     for (uint64_t *b : {&bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
     for (uint64_t *b : {&bars.ks_done, &bars.u_done, &bars.s_done, &bars.o_done}) mbar_init(smem_u32(b), 1);
     mbar_init(smem_u32(&bars.out_free), Q);
     mbar_init(smem_u32(&bars.qs_ready), Q);
-    mbar_init(smem_u32(&bars.tail), 32);
     mbar_fence_init();
     abort_flag = 0;
+    range_slot = a.max_chunks > 0 ? atomicAdd(queue, 1) : 0;
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -431,15 +544,41 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     if (lane == 0) mbar_arrive(smem_u32(&b));
   };
 
-  const Seq s = get_seq(a, n);
-  const int nc = (s.len + kChunk - 1) / kChunk;
-  auto chunk_of = [&](int it) { return REV ? nc - 1 - it : it; };
-  auto cell = [&](int it) { return (size_t)(s.chunk0 + chunk_of(it)) * a.p.H + h; };
-  auto rows_of = [&](int it) { return min(kChunk, s.len - chunk_of(it) * kChunk); };
+  const int range = *reinterpret_cast<volatile int *>(&range_slot);
+  const int64_t total = a.max_chunks == 0 ? 0 : (int64_t)a.p.H * (a.p.cu_seqlens == nullptr ? a.max_chunks : a.w.first[a.nseq]);
+  const int lo = range < a.ranges ? (int)(total * range / a.ranges) : 0, hi = range < a.ranges ? (int)(total * (range + 1) / a.ranges) : 0;
+  WarpPlace &place = places[warp];
+  if (lane == 0) place.pieces.begin(a, lo, hi);
+  const Piece &pc = place.pc;
+  const Seq &s = place.s;
+  auto step_piece = [&]() {  // one lane
+    place.more = place.pieces.next(a, &place.pc);
+    if (place.more) place.s = get_seq(a, place.pc.n);
+  };
+  auto next_piece = [&]() {
+    __syncwarp();
+    if (lane == 0) step_piece();
+    __syncwarp();
+    return *reinterpret_cast<volatile int *>(&place.more) != 0;
+  };
+  // of position `pos` of the current piece's stream
+  auto chunk_of = [&](int pos) { return REV ? pc.nc - 1 - pos : pos; };
+  auto cell = [&](int pos) { return (size_t)(s.chunk0 + chunk_of(pos)) * a.p.H + pc.h; };
+  auto rows_of = [&](int pos) { return min(kChunk, s.len - chunk_of(pos) * kChunk); };
+  // Every role counts the chunks that it has begun, over all pieces (it: stages and barrier phases), and
+  // keeps the phases of the stages' tail barriers, which ragged chunks alone complete (bits of tails).
+  int it = 0, tails = 0;
+  auto wait_tail = [&](int st) {
+    mbar_wait(smem_u32(&bars.tail[st]), (tails >> st) & 1, a.p.status, &abort_flag);
+    tails ^= 1 << st;
+  };
   // a stage's tiles have landed (and, in a sequence's ragged chunk, the rows behind its end are zeros)
-  auto wait_full = [&](int it) {
+  auto wait_full = [&](int pos) {
     wait(bars.full[it & 1], (it >> 1) & 1);
-    if (rows_of(it) < kChunk) wait(bars.tail, 0);
+    if (rows_of(pos) < kChunk) {
+      wait_tail(it & 1);
+      __syncwarp();
+    }
   };
 
   if (warp < kOutWarp) {
@@ -449,15 +588,23 @@ __global__ void __launch_bounds__(kScanThreads, 1)
       const uint32_t tl = tmem + ((uint32_t)quad << 21);
       const int dv = 32 * quad + lane;
       constexpr int W = D / 2;  // key channels of this thread
-      const float *src = REV ? a.p.dstate_out : a.p.state_in;
-      const size_t st_off = (((size_t)n * a.p.H + h) * D + half * W) * D + dv;
+      const size_t own = (size_t)(half * W) * D + dv;  // this thread's first element of a [D][D] state
       // byte offsets of column dv in rows t = 0..7 of a swizzled tile
       uint32_t vcol[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) vcol[i] = (uint32_t)((dv >> 6) * 8192 + i * 128 + ((((dv >> 3) ^ i) & 7) << 4) + (dv & 7) * 2);
-      for (int it = 0; it < nc; ++it) {
+      while (next_piece()) {
+        const size_t state = ((size_t)pc.n * a.p.H + pc.h) * D * D;
+        // the piece's first state: the caller's, or the one that the range before published
+        const float *src = REV ? a.p.dstate_out : a.p.state_in;
+        if (src != nullptr) src += state;
+        if (pc.p0 > 0) {
+          wait_flag(queue + 1 + range, a.p.status, &abort_flag);
+          src = a.w.slots + (size_t)range * D * D;
+        }
+      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
         const int st = it & 1;
-        wait_full(it);
+        wait_full(pos);
         const float last = fac[st].last[0];
         if (it > 0) {
           if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
@@ -467,11 +614,11 @@ __global__ void __launch_bounds__(kScanThreads, 1)
 #pragma unroll
         for (int c0 = 0; c0 < W; c0 += 32) {
           float x[32];
-          if (it > 0) {
+          if (pos > pc.p0) {
             tmem_ld32(tl + cS + half * W + c0, x);
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? src[st_off + (size_t)(c0 + j) * D] : 0.f;
+            for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
           }
           tmem_split32<BF>(tl + cSH + (half * W + c0) / 2, tl + cSL + (half * W + c0) / 2, x);
           uint32_t r[32];
@@ -516,17 +663,28 @@ __global__ void __launch_bounds__(kScanThreads, 1)
           arrive_warp(bars.up_ready);
         }
       }
-      float *dst = REV ? a.p.dstate_in : (MODE == kOut ? a.p.state_out : nullptr);
-      if (dst != nullptr) {
-        if (nc > 0) wait(bars.s_done, (nc - 1) & 1);
-        tc_fence_after();
+        // where the state goes from here: to the next range, or to the caller
+        float *dst = pc.p1 < pc.nc ? a.w.slots + (size_t)(range + 1) * D * D
+                                   : (REV ? a.p.dstate_in : (MODE == kOut ? a.p.state_out : nullptr));
+        if (dst != nullptr) {
+          if (pc.p1 == pc.nc) dst += state;
+          wait(bars.s_done, (it - 1) & 1);
+          tc_fence_after();
 #pragma unroll
-        for (int c0 = 0; c0 < W; c0 += 32) {
-          float x[32];
-          if (nc > 0) tmem_ld32(tl + cS + half * W + c0, x);
+          for (int c0 = 0; c0 < W; c0 += 32) {
+            float x[32];
+            tmem_ld32(tl + cS + half * W + c0, x);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            dst[st_off + (size_t)(c0 + j) * D] = nc > 0 ? x[j] : (src != nullptr ? src[st_off + (size_t)(c0 + j) * D] : 0.f);
+            for (int j = 0; j < 32; ++j) __stcg(dst + own + (size_t)(c0 + j) * D, x[j]);
+          }
+          if (pc.p1 < pc.nc) {
+            __threadfence();
+            named_bar_sync(2, 2 * Q * 32);
+            if (warp == 0 && lane == 0) {
+              __threadfence();
+              atomicExch(queue + 2 + range, 1);
+            }
+          }
         }
       }
     }
@@ -541,15 +699,15 @@ __global__ void __launch_bounds__(kScanThreads, 1)
       const kda_tensor &ot = REV ? a.p.dv : a.p.o;
       // a [64 x D] tile of o or dV from shared memory, once all warps have written it (store_tile ends the wait
       // for its reads; the caller's next tile starts with tile_free)
-      auto store_tile = [&](uint32_t at, int it) {
-        const int c = chunk_of(it), rows = rows_of(it);
+      auto store_tile = [&](uint32_t at, int pos) {
+        const int c = chunk_of(pos), rows = rows_of(pos);
         fence_async_smem();
         named_bar_sync(1, 32 * Q);
         if (rows == kChunk) {
           if (t == 0)
-            for (int b = 0; b < NB; ++b) tma_store_4d(&mo, at + 8192 * b, 64 * b, (int)(s.t0 + (int64_t)c * kChunk), h, (int)s.b);
+            for (int b = 0; b < NB; ++b) tma_store_4d(&mo, at + 8192 * b, 64 * b, (int)(s.t0 + (int64_t)c * kChunk), pc.h, (int)s.b);
         } else {  // what lies behind a packed sequence is another's
-          uint16_t *ob = static_cast<uint16_t *>(ot.data) + s.b * ot.stride_b + h * ot.stride_h + (s.t0 + (int64_t)c * kChunk) * ot.stride_t;
+          uint16_t *ob = static_cast<uint16_t *>(ot.data) + s.b * ot.stride_b + pc.h * ot.stride_h + (s.t0 + (int64_t)c * kChunk) * ot.stride_t;
           for (int e = t; e < rows * (D / 8); e += 32 * Q) {
             const int r = e / (D / 8), g = e % (D / 8);
             *reinterpret_cast<uint4 *>(ob + r * ot.stride_t + 8 * g) = ld_shared_v4(at + (g >> 3) * 8192 + chunk_at(r, g & 7));
@@ -560,10 +718,11 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         if (t == 0) tma_store_wait_read0();
         named_bar_sync(1, 32 * Q);
       };
-      for (int it = 0; it < nc; ++it) {
+      while (next_piece()) {
+      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
         const int st = it & 1;
         if (MODE == kOut) {
-          wait_full(it);
+          wait_full(pos);
           wait(bars.o_done, it & 1);
           tc_fence_after();
           uint32_t pk[2][16];  // [16-lane half][column block j, row half]
@@ -589,11 +748,11 @@ __global__ void __launch_bounds__(kScanThreads, 1)
 #pragma unroll
             for (int j = 0; j < 8; j += 2)
               tile.put(sb + L::OUT, hh, j, pk[hh][2 * j], pk[hh][2 * j + 1], pk[hh][2 * j + 2], pk[hh][2 * j + 3]);
-          store_tile(sb + L::OUT, it);
+          store_tile(sb + L::OUT, pos);
           if (t == 0) tma_store_commit();
         } else {
           if (REV) {  // Q' product's first operand: scale e^gamma dO, transposed, in two terms
-            wait_full(it);
+            wait_full(pos);
             if (it > 0) wait(bars.s_done, (it - 1) & 1);  // the last one is used
             const uint32_t vt = sb + st * L::kStage + L::V + (row >> 6) * 8192 + (row & 7) * 2;
 #pragma unroll
@@ -611,7 +770,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
             arrive_warp(bars.qs_ready);
           }
           // the state (reverse: its gradient) as the chain split it
-          char *img = (REV ? a.w.dS : a.w.S) + cell(it) * (size_t)(D * D * 4) + row * 16;
+          char *img = (REV ? a.w.dS : a.w.S) + cell(pos) * (size_t)(D * D * 4) + row * 16;
 #pragma unroll
           for (int b = 0; b < NB; ++b) wait(bars.s_ready[b], it & 1);
           tc_fence_after();
@@ -629,7 +788,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
           wait(bars.u_done, it & 1);
           tc_fence_after();
           if (MODE == kStore) {  // U^T
-            char *ui = a.w.U + cell(it) * (size_t)(D * 256) + row * 16;
+            char *ui = a.w.U + cell(pos) * (size_t)(D * 256) + row * 16;
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
               float x[32];
@@ -670,9 +829,9 @@ __global__ void __launch_bounds__(kScanThreads, 1)
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
-            store_tile(sb + L::OUT + 2 * L::kTile, it);
+            store_tile(sb + L::OUT + 2 * L::kTile, pos);
             if (t == 0) {  // the dX tiles are the images
-              char *xi = a.w.dX + cell(it) * (size_t)(D * 256);
+              char *xi = a.w.dX + cell(pos) * (size_t)(D * 256);
               for (int b = 0; b < NB; ++b) {
                 bulk_store(xi + b * 16384, sb + L::OUT + b * 8192, 8192);
                 bulk_store(xi + b * 16384 + 8192, sb + L::OUT + L::kTile + b * 8192, 8192);
@@ -682,24 +841,25 @@ __global__ void __launch_bounds__(kScanThreads, 1)
           }
         }
       }
+      }
       if (t == 0) tma_store_wait_all();
     }
   } else if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ loads --
     constexpr uint32_t kBytes = (MODE == kStore ? 2 : 3) * L::kTile + (MODE == kStore ? 16384 : kImgT);
-    auto load = [&](int it) {
+    auto load = [&](int pos) {
       const int st = it & 1;
       const uint32_t base = sb + st * L::kStage, bar = smem_u32(&bars.full[st]);
       if (it >= 2) wait(bars.empty[st], ((it >> 1) - 1) & 1);
       if (lane == 0) {
-        const int t0 = (int)(s.t0 + (int64_t)chunk_of(it) * kChunk), b = (int)s.b;
+        const int t0 = (int)(s.t0 + (int64_t)chunk_of(pos) * kChunk), b = (int)s.b;
         mbar_expect_tx(bar, kBytes);
         for (int i = 0; i < NB; ++i) {
-          tma_load_4d(base + L::K + 8192 * i, &mk, bar, 64 * i, t0, hk, b);
-          if (MODE != kStore) tma_load_4d(base + L::Q + 8192 * i, &mq, bar, 64 * i, t0, hk, b);
-          tma_load_4d(base + L::V + 8192 * i, &mv, bar, 64 * i, t0, h, b);
+          tma_load_4d(base + L::K + 8192 * i, &mk, bar, 64 * i, t0, pc.h / G_, b);
+          if (MODE != kStore) tma_load_4d(base + L::Q + 8192 * i, &mq, bar, 64 * i, t0, pc.h / G_, b);
+          tma_load_4d(base + L::V + 8192 * i, &mv, bar, 64 * i, t0, pc.h, b);
         }
-        const char *img = a.w.T + cell(it) * kImgT;
+        const char *img = a.w.T + cell(pos) * kImgT;
         if (MODE == kStore) {  // T alone
           bulk_load(base + L::T, img, 8192, bar);
           bulk_load(base + L::T + 16384, img + 16384, 8192, bar);
@@ -707,7 +867,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
           bulk_load(base + L::T, img, kImgT, bar);
         }
       }
-      const size_t at = cell(it) * 64;
+      const size_t at = cell(pos) * 64;
       const float gl = a.w.gam[at + 63];
 #pragma unroll
       for (int i = lane; i < 64; i += 32) {
@@ -721,37 +881,43 @@ __global__ void __launch_bounds__(kScanThreads, 1)
       mbar_arrive(bar);
       __syncwarp();
     };
-    for (int it = 0; it < nc + 1; ++it) {
-      if (it < nc) load(it);
-      // a ragged chunk has landed: zeros behind its end
-      if (it > 0 && rows_of(it - 1) < kChunk) {
-        const int st = (it - 1) & 1, rows = rows_of(it - 1);
-        wait(bars.full[st], ((it - 1) >> 1) & 1);
-        for (int tl = 0; tl < 3; ++tl) {
-          if (MODE == kStore && tl == 1) continue;
-          const uint32_t base = sb + st * L::kStage + tl * L::kTile;
-          for (int e = lane; e < (kChunk - rows) * (D / 8); e += 32) {
-            const int r = rows + e / (D / 8), g = e % (D / 8);
-            sts(base + (g >> 3) * 8192 + chunk_at(r, g & 7), make_uint4(0, 0, 0, 0));
-          }
+    // a ragged chunk once it has landed: zeros behind its end
+    auto zero_tail = [&](int st, int phase, int rows) {
+      wait(bars.full[st], phase);
+      for (int tl = 0; tl < 3; ++tl) {
+        if (MODE == kStore && tl == 1) continue;
+        const uint32_t base = sb + st * L::kStage + tl * L::kTile;
+        for (int e = lane; e < (kChunk - rows) * (D / 8); e += 32) {
+          const int r = rows + e / (D / 8), g = e % (D / 8);
+          sts(base + (g >> 3) * 8192 + chunk_at(r, g & 7), make_uint4(0, 0, 0, 0));
         }
-        fence_async_smem();
-        mbar_arrive(smem_u32(&bars.tail));
+      }
+      fence_async_smem();
+      mbar_arrive(smem_u32(&bars.tail[st]));
+    };
+    int ragged = kChunk;  // rows of the chunk before
+    while (next_piece()) {
+      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
+        load(pos);
+        if (ragged < kChunk) zero_tail((it - 1) & 1, ((it - 1) >> 1) & 1, ragged);
+        ragged = rows_of(pos);
       }
     }
-  } else if (elect_one()) {
+    if (ragged < kChunk) zero_tail((it - 1) & 1, ((it - 1) >> 1) & 1, ragged);
+  } else if (__syncwarp(), elect_one()) {
     // ---------------------------------------------------------------- products --
     auto wait = [&](uint64_t &b, uint32_t parity) { mbar_wait(smem_u32(&b), parity, a.p.status, &abort_flag); };
     const uint32_t id_k = idesc_f16(128, 64, BF, false, false), id_mn = idesc_f16(128, 64, BF, false, true);
     const uint32_t id_u = idesc_f16(128, D, BF, false, true);   // update: N = key channels
     const uint32_t id_a64 = idesc_f16(128, 64, BF, true, true);  // dO^T from shared memory
-    for (int it = 0; it < nc; ++it) {
+    while (step_piece(), place.more) {
+    for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
       const int st = it & 1;
       const uint32_t base = sb + st * L::kStage;
       const KMajor k_rows(base + L::K, 8192), q_rows(base + L::Q, 8192);
       const MNMajor k_cols(base + L::K, 8192), q_cols(base + L::Q, 8192);
       wait(bars.full[st], (it >> 1) & 1);
-      if (rows_of(it) < kChunk) wait(bars.tail, 0);
+      if (rows_of(pos) < kChunk) wait_tail(st);
       // key channels in the order in which the chain hands them over: quarters 0 and 2, then 1 and 3
       wait(bars.s_ready[0], it & 1);
       tc_fence_after();
@@ -814,6 +980,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
       mma_commit(smem_u32(&bars.s_done));
       mma_commit(smem_u32(&bars.empty[st]));
     }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -850,9 +1017,7 @@ cudaError_t run_scan_mode(const Args &a, cudaStream_t st) {
   constexpr uint32_t smem = ScanSmem<D, MODE>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(scan_kernel<D, BF, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)((a.nseq + (p.cu_seqlens != nullptr ? 1 : 0)) * p.H));
-  if (grid.x == 0) return cudaSuccess;
-  scan_kernel<D, BF, MODE><<<grid, kScanThreads, smem, st>>>(a, m[0], m[1], m[2], m[3]);
+  scan_kernel<D, BF, MODE><<<(unsigned)a.ranges, kScanThreads, smem, st>>>(a, m[0], m[1], m[2], m[3]);
   count_launches(1);
   return cudaGetLastError();
 }

@@ -36,6 +36,8 @@ constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
 
 // Workspace regions (device pointers) of one call.
 struct Work {
+  int *queue;      // [2 scans][2 + ranges]: ticket, then a flag a range whose entry state is published; cleared by the preparation
+  float *slots;    // [ranges + 1][D][D] states at the ranges' boundaries
   int *bound;      // [nseq + 1] sequence offsets, clamped into order and range (packed sequences only)
   int *first;      // [nseq + 1] first chunk of each sequence
   float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
@@ -53,6 +55,7 @@ struct Args {
   int nseq;       // sequences (batch rows, or those of cu_seqlens)
   int per_seq;    // chunks of a batch row (without cu_seqlens)
   int max_chunks; // upper bound of the chunks over all sequences
+  int ranges;     // CTAs of a scan
 };
 
 struct Seq {

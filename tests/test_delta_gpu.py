@@ -101,6 +101,9 @@ CASES = [
     (1, 4, 2, 200, 128, torch.float16, torch.float16, True),
     (2, 6, 2, 257, 64, torch.float16, torch.float32, True),
     (1, 2, 1, 320, 128, torch.bfloat16, torch.float32, True),
+    # more streams than SMs: work ranges that cut streams, their states handed from CTA to CTA
+    (5, 40, 20, 190, 64, torch.bfloat16, torch.float32, True),
+    (10, 18, 18, 300, 128, torch.bfloat16, torch.bfloat16, True),
 ]
 
 
@@ -123,6 +126,7 @@ def packed(lens, lead=0, tail=0, dtype=torch.int32):
     ([1] * 40 + [0] * 3, 0, 70, 2, 1, 64, torch.float16, torch.int32),
     ([0], 0, 17, 1, 1, 128, torch.bfloat16, torch.int32),
     ([128], 0, 0, 2, 1, 128, torch.float16, torch.int32),
+    ([7] * 50 + [900, 0, 64, 130] + [65] * 20, 3, 0, 4, 2, 64, torch.bfloat16, torch.int32),  # one stream over several ranges
 ])
 def test_packed_sequences(lens, lead, tail, H, Hk, D, dtype, index):
     cu, bounds, T = packed(lens, lead, tail, index)
