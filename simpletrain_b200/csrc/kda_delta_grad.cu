@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       for (int c = 0; c < W / 8; ++c) sts(sb + L::AL + own_chunk(c), make_uint4(0, 0, 0, 0));
   };
 
+  pdl_wait();
   int64_t b = 0, t0 = 0;
   int rows = 0, u = blockIdx.x;
   bool live = u < cells && get_chunk(a, u / a.p.Hk, &b, &t0, &rows);
@@ -416,9 +417,9 @@ cudaError_t run_grad(const Args &a, cudaStream_t st) {
   if ((e = cudaGetDevice(&dev)) != cudaSuccess || (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
     return e;
   const int64_t cells = (int64_t)a.max_chunks * a.p.Hk;
-  grad_kernel<D, BF><<<(unsigned)(cells < sms ? cells : sms), kGradThreads, smem, st>>>(a);
+  e = launch_kernel(grad_kernel<D, BF>, dim3((unsigned)(cells < sms ? cells : sms)), dim3(kGradThreads), smem, st, true, a);
   count_launches(1);
-  return cudaGetLastError();
+  return e;
 }
 
 }  // namespace

@@ -27,6 +27,7 @@ namespace {
 // bound[i] = cu_seqlens[i] clamped into [0, T] and to no less than its predecessors;
 // first[i] = chunks before sequence i.
 __global__ void __launch_bounds__(1024) plan_kernel(const Args a) {
+  pdl_launch_dependents();
   __shared__ int sm_max[32], sm_sum[32];
   __shared__ int carry_max, carry_sum;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = a.nseq;
@@ -136,6 +137,8 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   __shared__ __align__(16) float gam[64], bet[64], cfac[32];
   int64_t b, t0;
   int rows;
+  if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
+  pdl_launch_dependents();
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int i = threadIdx.x; i < 2 * (a.ranges + 2); i += kThreads) a.w.queue[i] = 0;
   if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
@@ -483,6 +486,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   __shared__ WarpPlace places[kScanThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G_ = a.p.H / a.p.Hk;
+  pdl_wait();
   if (MODE != kStore) {
     if (a.p.cu_seqlens != nullptr)  // the rows outside all sequences
       for (int h = blockIdx.x; h < a.p.H; h += gridDim.x) {
@@ -524,7 +528,8 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     mbar_init(smem_u32(&bars.qs_ready), Q);
     mbar_fence_init();
     abort_flag = 0;
-    range_slot = a.max_chunks > 0 ? atomicAdd(queue, 1) : 0;
+    // ranges that are whole streams need no order
+    range_slot = a.p.cu_seqlens == nullptr && a.ranges == a.nseq * a.p.H ? (int)blockIdx.x : (a.max_chunks > 0 ? atomicAdd(queue, 1) : 0);
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -544,6 +549,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     if (lane == 0) mbar_arrive(smem_u32(&b));
   };
 
+  pdl_launch_dependents();
   const int range = *reinterpret_cast<volatile int *>(&range_slot);
   const int64_t total = a.max_chunks == 0 ? 0 : (int64_t)a.p.H * (a.p.cu_seqlens == nullptr ? a.max_chunks : a.w.first[a.nseq]);
   const int lo = range < a.ranges ? (int)(total * range / a.ranges) : 0, hi = range < a.ranges ? (int)(total * (range + 1) / a.ranges) : 0;
@@ -555,11 +561,19 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     place.more = place.pieces.next(a, &place.pc);
     if (place.more) place.s = get_seq(a, place.pc.n);
   };
+  int p0 = 0, p1 = 0, rp = -1;  // the piece's positions, and that of its stream's ragged chunk
+  auto take_piece = [&]() {
+    if (*reinterpret_cast<volatile int *>(&place.more) == 0) return false;
+    p0 = pc.p0;
+    p1 = pc.p1;
+    rp = s.len % kChunk == 0 ? -1 : (REV ? 0 : pc.nc - 1);
+    return true;
+  };
   auto next_piece = [&]() {
     __syncwarp();
     if (lane == 0) step_piece();
     __syncwarp();
-    return *reinterpret_cast<volatile int *>(&place.more) != 0;
+    return take_piece();
   };
   // of position `pos` of the current piece's stream
   auto chunk_of = [&](int pos) { return REV ? pc.nc - 1 - pos : pos; };
@@ -575,7 +589,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   // a stage's tiles have landed (and, in a sequence's ragged chunk, the rows behind its end are zeros)
   auto wait_full = [&](int pos) {
     wait(bars.full[it & 1], (it >> 1) & 1);
-    if (rows_of(pos) < kChunk) {
+    if (pos == rp) {
       wait_tail(it & 1);
       __syncwarp();
     }
@@ -602,7 +616,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
           wait_flag(queue + 1 + range, a.p.status, &abort_flag);
           src = a.w.slots + (size_t)range * D * D;
         }
-      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
+      for (int pos = p0; pos < p1; ++pos, ++it) {
         const int st = it & 1;
         wait_full(pos);
         const float last = fac[st].last[0];
@@ -614,7 +628,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
 #pragma unroll
         for (int c0 = 0; c0 < W; c0 += 32) {
           float x[32];
-          if (pos > pc.p0) {
+          if (pos > p0) {
             tmem_ld32(tl + cS + half * W + c0, x);
           } else {
 #pragma unroll
@@ -719,7 +733,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         named_bar_sync(1, 32 * Q);
       };
       while (next_piece()) {
-      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
+      for (int pos = p0; pos < p1; ++pos, ++it) {
         const int st = it & 1;
         if (MODE == kOut) {
           wait_full(pos);
@@ -897,7 +911,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     };
     int ragged = kChunk;  // rows of the chunk before
     while (next_piece()) {
-      for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
+      for (int pos = p0; pos < p1; ++pos, ++it) {
         load(pos);
         if (ragged < kChunk) zero_tail((it - 1) & 1, ((it - 1) >> 1) & 1, ragged);
         ragged = rows_of(pos);
@@ -910,14 +924,14 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     const uint32_t id_k = idesc_f16(128, 64, BF, false, false), id_mn = idesc_f16(128, 64, BF, false, true);
     const uint32_t id_u = idesc_f16(128, D, BF, false, true);   // update: N = key channels
     const uint32_t id_a64 = idesc_f16(128, 64, BF, true, true);  // dO^T from shared memory
-    while (step_piece(), place.more) {
-    for (int pos = pc.p0; pos < pc.p1; ++pos, ++it) {
+    while (step_piece(), take_piece()) {
+    for (int pos = p0; pos < p1; ++pos, ++it) {
       const int st = it & 1;
       const uint32_t base = sb + st * L::kStage;
       const KMajor k_rows(base + L::K, 8192), q_rows(base + L::Q, 8192);
       const MNMajor k_cols(base + L::K, 8192), q_cols(base + L::Q, 8192);
       wait(bars.full[st], (it >> 1) & 1);
-      if (rows_of(pos) < kChunk) wait_tail(st);
+      if (pos == rp) wait_tail(st);
       // key channels in the order in which the chain hands them over: quarters 0 and 2, then 1 and 3
       wait(bars.s_ready[0], it & 1);
       tc_fence_after();
@@ -992,9 +1006,9 @@ template <typename K>
 cudaError_t run(K kern, dim3 grid, int threads, uint32_t smem, const Args &a, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  kern<<<grid, threads, smem, st>>>(a);
+  e = launch_kernel(kern, grid, dim3(threads), smem, st, a.p.cu_seqlens != nullptr, a);
   count_launches(1);
-  return cudaGetLastError();
+  return e;
 }
 
 template <int D>
@@ -1017,9 +1031,9 @@ cudaError_t run_scan_mode(const Args &a, cudaStream_t st) {
   constexpr uint32_t smem = ScanSmem<D, MODE>::kBytes;
   cudaError_t e = cudaFuncSetAttribute(scan_kernel<D, BF, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  scan_kernel<D, BF, MODE><<<(unsigned)a.ranges, kScanThreads, smem, st>>>(a, m[0], m[1], m[2], m[3]);
+  e = launch_kernel(scan_kernel<D, BF, MODE>, dim3((unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m[0], m[1], m[2], m[3]);
   count_launches(1);
-  return cudaGetLastError();
+  return e;
 }
 
 template <int D, bool BF>
