@@ -126,7 +126,7 @@ __device__ __forceinline__ void inverse_level(float *As, float *Ti) {
 // One CTA per (chunk, head): T and P T as two-term images, gamma and beta in fp32.
 // The products are k.k, q.k and P T; (I + A)^-1 is by halves in fp32: four 16 x 16 blocks
 // by substitution, a column a thread, then [A 0; B C]^-1 = [a 0; -c B a, c] twice.
-// The q.k rows wait in registers while the inverse is formed, so that the k and q tiles, the
+// The q.k rows wait in tensor memory while the inverse is formed, so that the k and q tiles, the
 // fp32 matrices and the two-term tiles can take turns in 34 KB, and four CTAs share an SM:
 // the kernel is a chain of short dependent steps, hidden by other CTAs only.
 template <int D, bool BF>
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   constexpr uint32_t KQ = 0, TT = 0;  // [T; P] hi, then lo, over the rest
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
-  __shared__ __align__(16) float gam[64], bet[64], cfac[32];
+  __shared__ __align__(16) float gam[64], bet[64];
   int64_t b, t0;
   int rows;
   if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
@@ -166,8 +166,6 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     }
     gam[2 * tid + 1] = (float)c;
     gam[2 * tid] = (float)(c - s[1]);
-    __syncwarp();
-    cfac[tid] = exp_fast(gam[31] - gam[tid]);
   }
   cp_async_wait();
   publish();
@@ -182,37 +180,34 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     a.w.beta[ch * 64 + tid] = bet[tid];
   }
   const float gi = gam[r64] * kLog2e;
-  // The factor e^{gamma_i - gamma_j} of this thread's 32 columns: nothing above the diagonal, a
-  // product of two factors <= 1 that meet at gamma_31 below the diagonal blocks of 32, and an
-  // exponential an element in them (MUFU is what 4 CTAs an SM would otherwise wait for).
-  const int rb = r64 >> 5;  // warp-uniform
   const float rowf = row < 64 ? bet[r64] : a.p.scale;
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   float *As = reinterpret_cast<float *>(smem + KQ);  // over the k and q tiles: their product is done
   float *Ti = As + 64 * kLd;
-  float x[32];  // 32 columns of a row of A (rows of k) or P (rows of q)
-  if (half > rb) {
+  const uint32_t taddr = tmem + lane_base + 32 * half;
+  // 16 columns at a time of a row of A (rows of k) or P (rows of q)
+  const int last = r64 - (row < 64 ? 1 : 0) - 32 * half;  // last column that counts
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = 0.f;
-  } else {
-    tmem_ld32(tmem + lane_base + 32 * half, x);
-    if (half < rb) {
-      const float f = rowf * ex2f(gi - gam[31] * kLog2e);
+  for (int c0 = 0; c0 < 32; c0 += 16) {
+    float x[16];
+    tmem_ld16(taddr + c0, x);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) x[j] *= f * cfac[j];
-    } else {
+    for (int j = 0; j < 16; j += 4) {
+      const float4 c = *reinterpret_cast<const float4 *>(gam + 32 * half + c0 + j);
+      const float d[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-      for (int j = 0; j < 32; ++j) {
-        const int col = 32 * half + j;
-        const float d = rowf * ex2f(fmaf(-kLog2e, gam[col], gi));
-        x[j] = (row < 64 ? col < r64 : col <= r64) ? d * x[j] : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        const float f = rowf * ex2f(fmaf(-kLog2e, d[e], gi));
+        x[j + e] = c0 + j + e <= last ? f * x[j + e] : 0.f;
       }
     }
-  }
-  if (row < 64) {
+    if (row < 64) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 4)
-      *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + c0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    } else {
+      tmem_st16(taddr + c0, x);  // P waits there for the inverse
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -247,18 +242,35 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   __syncthreads();
   inverse_level<16>(As, Ti);
   inverse_level<32>(As, Ti);
-  if (row < 64) {
+  {
+    // T and P as two-term tiles over the matrices: read, then (every thread being past its reads) written
+    uint4 h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 32; j += 4) {
-      const float4 r = *reinterpret_cast<const float4 *>(Ti + r64 * kLd + 32 * half + j);
-      x[j] = r.x;
-      x[j + 1] = r.y;
-      x[j + 2] = r.z;
-      x[j + 3] = r.w;
+    for (int c0 = 0; c0 < 2; ++c0) {
+      float x[16];
+      if (row < 64) {
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 r = *reinterpret_cast<const float4 *>(Ti + r64 * kLd + 32 * half + 16 * c0 + j);
+          x[j] = r.x;
+          x[j + 1] = r.y;
+          x[j + 2] = r.z;
+          x[j + 3] = r.w;
+        }
+      } else {
+        tmem_ld16(taddr + 16 * c0, x);
+      }
+      split8<BF>(x, h[2 * c0], l[2 * c0]);
+      split8<BF>(x + 8, h[2 * c0 + 1], l[2 * c0 + 1]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t at = chunk_at(row, 4 * half + c);
+      sts(sb + TT + at, h[c]);
+      sts(sb + TT + 16384 + at, l[c]);
     }
   }
-  __syncthreads();
-  store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
   publish();
   if (warp_leader()) {
     tc_fence_after();
@@ -273,8 +285,12 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   }
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   if (row >= 64) {
-    tmem_ld32(tmem + lane_base + 32 * half, x);
-    store_split32<BF>(sb + TT, sb + TT + 16384, row, half, x);
+#pragma unroll
+    for (int c0 = 0; c0 < 2; ++c0) {
+      float x[16];
+      tmem_ld16(taddr + 16 * c0, x);
+      store_split16<BF>(sb + TT, sb + TT + 16384, row, 4 * half + 2 * c0, x);
+    }
   }
   fence_async_smem();
   cta_end(tmem, 64);

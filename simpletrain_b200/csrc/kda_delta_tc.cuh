@@ -187,6 +187,18 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int c16) {
 }
 __device__ __forceinline__ void sts(uint32_t addr, const uint4 &v) { st_shared_v4(addr, v.x, v.y, v.z, v.w); }
 
+// 16 columns (chunks c16 and c16 + 1) of a row into the hi and lo tiles
+template <bool BF>
+__device__ __forceinline__ void store_split16(uint32_t hi_tile, uint32_t lo_tile, int row, int c16, const float (&x)[16]) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint4 h, l;
+    split8<BF>(x + 8 * c, h, l);
+    const uint32_t at = chunk_at(row, c16 + c);
+    sts(hi_tile + at, h);
+    sts(lo_tile + at, l);
+  }
+}
 // 32 columns (chunks 4*half ..) of a row into the hi and lo tiles
 template <bool BF>
 __device__ __forceinline__ void store_split32(uint32_t hi_tile, uint32_t lo_tile, int row, int half, const float (&x)[32]) {
@@ -233,6 +245,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&x)[32]) {
   tmem_ld_32x32b_x32(taddr, r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&x)[16]) {
+  uint32_t r[16];
+  tmem_ld_32x32b_x16(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&x)[16]) {
+  uint32_t r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(x[i]);
+  tmem_st_32x32b_x16(taddr, r);
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&x)[32]) {
   uint32_t r[32];
