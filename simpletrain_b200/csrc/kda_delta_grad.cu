@@ -30,6 +30,8 @@ namespace delta {
 namespace {
 
 constexpr int kGradThreads = 512;
+// Products and copies are issued by warps whose threads own q rows: they have less to do with the results.
+constexpr int kMmaWarp = 2, kCopyThread = 96;
 
 template <int D>
 struct GradSmem {
@@ -95,10 +97,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       cp_async16(tile + (c >> 3) * 16384 + chunk_at(tr, c & 7), src + (r < rows ? r * stride : 0) + c * 8, r < rows);
     }
   };
+  auto mma_leader = [&]() { return (tid >> 5) == kMmaWarp && elect_one(); };
   // the tiles of value head h of chunk cell cidx, all but k and q
   auto load_head = [&](int cidx, int h, int64_t b, int64_t t0, int rows) {
     const size_t ch = (size_t)cidx * a.p.H + h;
-    if (tid == 0) {
+    if (tid == kCopyThread) {
       const uint32_t b1 = smem_u32(&ctl.load_bar), b2 = smem_u32(&bar_s);
       mbar_arrive_expect_tx(b1, NS * 16384 + D * 256);
       for (int s = 0; s < NS; ++s) {
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         vraw[c] = vr < rows ? *reinterpret_cast<const uint4 *>(rows_at(a.p.v, b, h, t0 + vr) + 8 * (vc + 8 * c)) : make_uint4(0, 0, 0, 0);
       cp_async_wait();
       publish();
-      if (warp_leader()) {
+      if (mma_leader()) {
         mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
         tc_fence_after();
         const uint32_t id64 = idesc_f16(128, 64, BF, false, false), id64t = idesc_f16(128, 64, BF, false, true);
@@ -174,6 +177,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         mma_commit(smem_u32(&ctl.mma_bar));
       }
       __syncwarp();
+      {  // rows that come next, a 128-byte line a thread: k, q, dout, v
+        const int64_t pb = last ? nb : b, pt = last ? nt : t0;
+        const int nk = last ? un % a.p.Hk : hk, nh = last ? nk * G_ : h + 1, pr = last ? (more ? nrows : 0) : rows;
+        const kda_tensor &x = part == 0 ? a.p.k : (part == 1 ? a.p.q : (part == 2 ? a.p.dout : a.p.v));
+        const int r = row / (D / 64), c = row % (D / 64);
+        if (r < pr && (last || part > 1))
+          asm volatile("prefetch.global.L2 [%0];" ::"l"(rows_at(x, pb, part < 2 ? nk : nh, pt + r) + c * 64));
+      }
       const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
       // dX . v, and the products of the two images, place by place
       mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
@@ -235,7 +246,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       __syncwarp();
       tc_fence_after();
       publish();
-      if (tid == 0) {
+      if (tid == kCopyThread) {
         mbar_arrive_expect_tx(smem_u32(&bar_d), D * D * 2);
         bulk_load(sb + L::S + D * D * 2, a.w.dS + ch * (size_t)(D * D * 4) + D * D * 2, D * D * 2, smem_u32(&bar_d));
         // what the next value head loads comes into L2 behind that (one bulk request each: line by line through
@@ -254,7 +265,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         sts(sb + L::MN + 16384 + chunk_at(row, 2 * part + c), ml[c]);
       }
       publish();
-      if (warp_leader()) {
+      if (mma_leader()) {
         tc_fence_after();
         const uint32_t id3 = idesc_f16(128, D, BF, false, true), id4 = idesc_f16(128, D, BF, true, true);
         const MNMajor kq{sb + L::KQ, 16384};
