@@ -21,8 +21,6 @@
 // depend on the launch.  The tiles of one value head fill an SM's shared memory, so the
 // next head's are brought into L2 meanwhile; 16 warps, a token row and a quarter of the
 // columns a thread, work off the products.
-#include <atomic>
-
 #include "kda_delta_tc.cuh"
 
 namespace kda {
@@ -422,11 +420,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 template <int D, bool BF>
 cudaError_t run_grad(const Args &a, cudaStream_t st) {
   constexpr uint32_t smem = GradSmem<D>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(grad_kernel<D, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(grad_kernel<D, BF>, smem, done);
   if (e != cudaSuccess) return e;
-  int dev = 0, sms = 0;
-  if ((e = cudaGetDevice(&dev)) != cudaSuccess || (e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess)
-    return e;
+  const int sms = a.sms;
   const int64_t cells = (int64_t)a.max_chunks * a.p.Hk;
   e = launch_kernel(grad_kernel<D, BF>, dim3((unsigned)(cells < sms ? cells : sms)), dim3(kGradThreads), smem, st, true, a);
   count_launches(1);
@@ -470,17 +467,19 @@ int check_sizes(const kda_delta_params *p) {
 
 size_t align256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-// CTAs of a scan: one an SM, and no more than there are streams (sequence, head).
-int scan_ranges(int64_t nseq, int64_t H) {
+int sm_count() {
   static std::atomic<int> cache[64];  // by device; 0 = not asked yet
   int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
-    sms = cache[dev].load(std::memory_order_relaxed);
-    if (sms == 0) {
-      if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
-      cache[dev].store(sms, std::memory_order_relaxed);
-    }
-  }
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms;
+  const int known = cache[dev].load(std::memory_order_relaxed);
+  if (known > 0) return known;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+  cache[dev].store(sms, std::memory_order_relaxed);
+  return sms;
+}
+
+// CTAs of a scan: one an SM, and no more than there are streams (sequence, head).
+int scan_ranges(int64_t nseq, int64_t H, int sms) {
   const int64_t n = nseq * H;
   return (int)(n < 1 ? 1 : (n < sms ? n : sms));
 }
@@ -505,9 +504,10 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
     a->w.bound = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
     a->w.first = reinterpret_cast<int *>(take(4 * ((size_t)p->nseq + 1)));
   }
-  a->ranges = scan_ranges(a->nseq, p->H);
+  a->sms = sm_count();
+  a->ranges = scan_ranges(a->nseq, p->H, a->sms);
   a->w.queue = reinterpret_cast<int *>(take(sizeof(int) * 2 * ((size_t)a->ranges + 2)));
-  a->w.slots = reinterpret_cast<float *>(take(((size_t)a->ranges + 1) * p->D * p->D * 4));
+  a->w.slots = reinterpret_cast<float *>(take((backward ? 2 : 1) * ((size_t)a->ranges + 1) * p->D * p->D * 4));
   a->w.gam = reinterpret_cast<float *>(take(cells * 256));
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
   a->w.T = take(cells * kda::delta::kImgT);
@@ -573,7 +573,7 @@ int kda_delta_fwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = p->cu_seqlens != nullptr ? kda::delta::launch_plan(a, st) : cudaSuccess;
   if (e == cudaSuccess) e = kda::delta::launch_prep(a, st);
-  if (e == cudaSuccess) e = kda::delta::launch_scan(a, false, st);
+  if (e == cudaSuccess) e = kda::delta::launch_scan(a, st);
   return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
 }
 
@@ -598,8 +598,7 @@ int kda_delta_bwd_sm100(const kda_delta_params *p, kda_stream_t stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e = p->cu_seqlens != nullptr ? kda::delta::launch_plan(a, st) : cudaSuccess;
   if (e == cudaSuccess) e = kda::delta::launch_prep(a, st);
-  if (e == cudaSuccess) e = kda::delta::launch_scan(a, true, st);
-  if (e == cudaSuccess) e = kda::delta::launch_rev(a, st);
+  if (e == cudaSuccess) e = kda::delta::launch_backward_scans(a, st);
   if (e == cudaSuccess) e = kda::delta::launch_grad(a, st);
   return e == cudaSuccess ? KDA_OK : KDA_ERR_CUDA;
 }

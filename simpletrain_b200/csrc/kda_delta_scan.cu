@@ -486,10 +486,14 @@ struct TileOut {
   }
 };
 
+// TMA maps of a scan: k, q, v (reverse: dout), o (reverse: dv)
+struct Maps {
+  CUtensorMap k, q, v, o;
+};
+
+// `block`: this CTA's number among the scan's
 template <int D, bool BF, int MODE>
-__global__ void __launch_bounds__(kScanThreads, 1)
-    scan_kernel(const Args a, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mq,
-                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo) {
+__device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int block) {
   using L = ScanSmem<D, MODE>;
   constexpr int Q = D / 32;  // warps that own live tensor-memory lanes, of four
   constexpr int NB = D / 64;
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   pdl_wait();
   if (MODE != kStore) {
     if (a.p.cu_seqlens != nullptr)  // the rows outside all sequences
-      for (int h = blockIdx.x; h < a.p.H; h += gridDim.x) {
+      for (int h = block; h < a.p.H; h += a.ranges) {
         for (int c = 0; c < D; c += 64) {
           if (MODE == kOut) zero_outside(a, a.p.o, h, c);
           if (REV) {
@@ -524,12 +528,13 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     const float *src = REV ? a.p.dstate_out : a.p.state_in;
     float *dst = REV ? a.p.dstate_in : a.p.state_out;
     if (dst != nullptr)  // sequences without tokens hand their state on
-      for (int i = blockIdx.x; i < a.nseq * a.p.H; i += gridDim.x)
+      for (int i = block; i < a.nseq * a.p.H; i += a.ranges)
         if (get_seq(a, i / a.p.H).len == 0)
           for (int e = tid; e < D * D; e += kScanThreads) dst[(size_t)i * D * D + e] = src != nullptr ? src[(size_t)i * D * D + e] : 0.f;
   }
   __shared__ int range_slot;
-  int *queue = a.w.queue + (MODE == kRev ? a.ranges + 2 : 0);
+  int *queue = a.w.queue + (REV ? a.ranges + 2 : 0);
+  float *slots = a.w.slots + (REV ? (size_t)(a.ranges + 1) * D * D : 0);
   const uint32_t sb = smem_u32(smem);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -545,7 +550,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
     mbar_fence_init();
     abort_flag = 0;
     // ranges that are whole streams need no order
-    range_slot = a.p.cu_seqlens == nullptr && a.ranges == a.nseq * a.p.H ? (int)blockIdx.x : (a.max_chunks > 0 ? atomicAdd(queue, 1) : 0);
+    range_slot = a.p.cu_seqlens == nullptr && a.ranges == a.nseq * a.p.H ? block : (a.max_chunks > 0 ? atomicAdd(queue, 1) : 0);
   }
   if (warp == kMmaWarp) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
@@ -630,7 +635,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         if (src != nullptr) src += state;
         if (pc.p0 > 0) {
           wait_flag(queue + 1 + range, a.p.status, &abort_flag);
-          src = a.w.slots + (size_t)range * D * D;
+          src = slots + (size_t)range * D * D;
         }
       for (int pos = p0; pos < p1; ++pos, ++it) {
         const int st = it & 1;
@@ -694,7 +699,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         }
       }
         // where the state goes from here: to the next range, or to the caller
-        float *dst = pc.p1 < pc.nc ? a.w.slots + (size_t)(range + 1) * D * D
+        float *dst = pc.p1 < pc.nc ? slots + (size_t)(range + 1) * D * D
                                    : (REV ? a.p.dstate_in : (MODE == kOut ? a.p.state_out : nullptr));
         if (dst != nullptr) {
           if (pc.p1 == pc.nc) dst += state;
@@ -735,7 +740,7 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         named_bar_sync(1, 32 * Q);
         if (rows == kChunk) {
           if (t == 0)
-            for (int b = 0; b < NB; ++b) tma_store_4d(&mo, at + 8192 * b, 64 * b, (int)(s.t0 + (int64_t)c * kChunk), pc.h, (int)s.b);
+            for (int b = 0; b < NB; ++b) tma_store_4d(&maps.o, at + 8192 * b, 64 * b, (int)(s.t0 + (int64_t)c * kChunk), pc.h, (int)s.b);
         } else {  // what lies behind a packed sequence is another's
           uint16_t *ob = static_cast<uint16_t *>(ot.data) + s.b * ot.stride_b + pc.h * ot.stride_h + (s.t0 + (int64_t)c * kChunk) * ot.stride_t;
           for (int e = t; e < rows * (D / 8); e += 32 * Q) {
@@ -885,9 +890,9 @@ __global__ void __launch_bounds__(kScanThreads, 1)
         const int t0 = (int)(s.t0 + (int64_t)chunk_of(pos) * kChunk), b = (int)s.b;
         mbar_expect_tx(bar, kBytes);
         for (int i = 0; i < NB; ++i) {
-          tma_load_4d(base + L::K + 8192 * i, &mk, bar, 64 * i, t0, pc.h / G_, b);
-          if (MODE != kStore) tma_load_4d(base + L::Q + 8192 * i, &mq, bar, 64 * i, t0, pc.h / G_, b);
-          tma_load_4d(base + L::V + 8192 * i, &mv, bar, 64 * i, t0, pc.h, b);
+          tma_load_4d(base + L::K + 8192 * i, &maps.k, bar, 64 * i, t0, pc.h / G_, b);
+          if (MODE != kStore) tma_load_4d(base + L::Q + 8192 * i, &maps.q, bar, 64 * i, t0, pc.h / G_, b);
+          tma_load_4d(base + L::V + 8192 * i, &maps.v, bar, 64 * i, t0, pc.h, b);
         }
         const char *img = a.w.T + cell(pos) * kImgT;
         if (MODE == kStore) {  // T alone
@@ -1018,14 +1023,21 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   if (warp == kMmaWarp) tmem_dealloc(tmem, 512);
 }
 
-template <typename K>
-cudaError_t run(K kern, dim3 grid, int threads, uint32_t smem, const Args &a, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
-  e = launch_kernel(kern, grid, dim3(threads), smem, st, a.p.cu_seqlens != nullptr, a);
-  count_launches(1);
-  return e;
+template <int D, bool BF, int MODE>
+__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+  scan_cta<D, BF, MODE>(a, maps, blockIdx.x);
 }
+
+// The backward's two scans side by side, where there are SMs for both: neither needs the other.
+template <int D, bool BF>
+__global__ void __launch_bounds__(kScanThreads, 1)
+    scan_pair_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps store, const __grid_constant__ Maps rev) {
+  if (blockIdx.x < a.ranges)
+    scan_cta<D, BF, kRev>(a, rev, blockIdx.x);
+  else
+    scan_cta<D, BF, kStore>(a, store, blockIdx.x - a.ranges);
+}
+
 
 template <int D>
 constexpr uint32_t prep_smem() {
@@ -1033,36 +1045,57 @@ constexpr uint32_t prep_smem() {
   return kq > mat ? kq : mat;
 }
 
-template <int D, bool BF, int MODE>
-cudaError_t run_scan_mode(const Args &a, cudaStream_t st) {
+template <int D, bool BF>
+bool make_maps(const Args &a, int mode, Maps *m) {
   const kda_delta_params &p = a.p;
-  CUtensorMap m[4] = {};
-  if (a.max_chunks > 0 && p.T > 0) {
-    auto view = [](const kda_tensor &t) { return View{t.data, t.stride_b, t.stride_h, t.stride_t, t.stride_d}; };
-    const kda_tensor &v = MODE == kRev ? p.dout : p.v, &o = MODE == kRev ? p.dv : (MODE == kOut ? p.o : p.v);
-    if (!make_tmap_bhtd(&m[0], view(p.k), p.B, p.Hk, p.T, D, BF) || !make_tmap_bhtd(&m[1], view(p.q), p.B, p.Hk, p.T, D, BF) ||
-        !make_tmap_bhtd(&m[2], view(v), p.B, p.H, p.T, D, BF) || !make_tmap_bhtd(&m[3], view(o), p.B, p.H, p.T, D, BF))
-      return cudaErrorInvalidValue;
-  }
+  *m = {};
+  if (a.max_chunks == 0 || p.T == 0) return true;
+  auto view = [](const kda_tensor &t) { return View{t.data, t.stride_b, t.stride_h, t.stride_t, t.stride_d}; };
+  const kda_tensor &v = mode == kRev ? p.dout : p.v, &o = mode == kRev ? p.dv : (mode == kOut ? p.o : p.v);
+  return make_tmap_bhtd(&m->k, view(p.k), p.B, p.Hk, p.T, D, BF) && make_tmap_bhtd(&m->q, view(p.q), p.B, p.Hk, p.T, D, BF) &&
+         make_tmap_bhtd(&m->v, view(v), p.B, p.H, p.T, D, BF) && make_tmap_bhtd(&m->o, view(o), p.B, p.H, p.T, D, BF);
+}
+
+template <int D, bool BF, int MODE>
+cudaError_t run_scan(const Args &a, cudaStream_t st) {
+  Maps m;
+  if (!make_maps<D, BF>(a, MODE, &m)) return cudaErrorInvalidValue;
   constexpr uint32_t smem = ScanSmem<D, MODE>::kBytes;
-  cudaError_t e = cudaFuncSetAttribute(scan_kernel<D, BF, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(scan_kernel<D, BF, MODE>, smem, done);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(scan_kernel<D, BF, MODE>, dim3((unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m[0], m[1], m[2], m[3]);
+  e = launch_kernel(scan_kernel<D, BF, MODE>, dim3((unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m);
   count_launches(1);
   return e;
 }
 
 template <int D, bool BF>
-cudaError_t run_scan(const Args &a, int mode, cudaStream_t st) {
-  if (mode == kOut) return run_scan_mode<D, BF, kOut>(a, st);
-  if (mode == kStore) return run_scan_mode<D, BF, kStore>(a, st);
-  return run_scan_mode<D, BF, kRev>(a, st);
+cudaError_t run_backward(const Args &a, cudaStream_t st) {
+  if (2 * a.ranges > a.sms) {
+    const cudaError_t e = run_scan<D, BF, kStore>(a, st);
+    return e == cudaSuccess ? run_scan<D, BF, kRev>(a, st) : e;
+  }
+  Maps m1, m2;
+  if (!make_maps<D, BF>(a, kStore, &m1) || !make_maps<D, BF>(a, kRev, &m2)) return cudaErrorInvalidValue;
+  constexpr uint32_t smem = ScanSmem<D, kRev>::kBytes;
+  static_assert(smem >= ScanSmem<D, kStore>::kBytes, "");
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(scan_pair_kernel<D, BF>, smem, done);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(scan_pair_kernel<D, BF>, dim3(2 * (unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m1, m2);
+  count_launches(1);
+  return e;
 }
 
-cudaError_t scan(const Args &a, int mode, cudaStream_t st) {
-  const bool bf = a.p.dtype == KDA_DTYPE_BF16;
-  if (a.p.D == 64) return bf ? run_scan<64, true>(a, mode, st) : run_scan<64, false>(a, mode, st);
-  return bf ? run_scan<128, true>(a, mode, st) : run_scan<128, false>(a, mode, st);
+template <int D, bool BF>
+cudaError_t run_prep(const Args &a, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(prep_kernel<D, BF>, prep_smem<D>(), done);
+  if (e != cudaSuccess) return e;
+  e = launch_kernel(prep_kernel<D, BF>, dim3((unsigned)a.max_chunks, (unsigned)a.p.H), dim3(kThreads), prep_smem<D>(), st,
+                    a.p.cu_seqlens != nullptr, a);
+  count_launches(1);
+  return e;
 }
 
 }  // namespace
@@ -1073,18 +1106,13 @@ cudaError_t launch_plan(const Args &a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_prep(const Args &a, cudaStream_t st) {
-  if (a.max_chunks == 0) return cudaSuccess;
-  const dim3 grid((unsigned)a.max_chunks, (unsigned)a.p.H);
-  const bool bf = a.p.dtype == KDA_DTYPE_BF16;
-  if (a.p.D == 64) return bf ? run(prep_kernel<64, true>, grid, kThreads, prep_smem<64>(), a, st)
-                             : run(prep_kernel<64, false>, grid, kThreads, prep_smem<64>(), a, st);
-  return bf ? run(prep_kernel<128, true>, grid, kThreads, prep_smem<128>(), a, st)
-            : run(prep_kernel<128, false>, grid, kThreads, prep_smem<128>(), a, st);
-}
+#define KDA_DELTA_PICK(FN, ...)                                                                     \
+  (a.p.dtype == KDA_DTYPE_BF16 ? (a.p.D == 64 ? FN<64, true __VA_ARGS__>(a, st) : FN<128, true __VA_ARGS__>(a, st)) \
+                               : (a.p.D == 64 ? FN<64, false __VA_ARGS__>(a, st) : FN<128, false __VA_ARGS__>(a, st)))
 
-cudaError_t launch_scan(const Args &a, bool store, cudaStream_t st) { return scan(a, store ? kStore : kOut, st); }
-cudaError_t launch_rev(const Args &a, cudaStream_t st) { return scan(a, kRev, st); }
+cudaError_t launch_prep(const Args &a, cudaStream_t st) { return a.max_chunks == 0 ? cudaSuccess : KDA_DELTA_PICK(run_prep); }
+cudaError_t launch_scan(const Args &a, cudaStream_t st) { return KDA_DELTA_PICK(run_scan, , kOut); }
+cudaError_t launch_backward_scans(const Args &a, cudaStream_t st) { return KDA_DELTA_PICK(run_backward); }
 
 }  // namespace delta
 }  // namespace kda

@@ -19,6 +19,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/kda_sm100.h"
 #include "kda_internal.h"
 #include "tc_common.cuh"
@@ -37,7 +39,7 @@ constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
 // Workspace regions (device pointers) of one call.
 struct Work {
   int *queue;      // [2 scans][2 + ranges]: ticket, then a flag a range whose entry state is published; cleared by the preparation
-  float *slots;    // [ranges + 1][D][D] states at the ranges' boundaries
+  float *slots;    // [scan][ranges + 1][D][D] states at the ranges' boundaries
   int *bound;      // [nseq + 1] sequence offsets, clamped into order and range (packed sequences only)
   int *first;      // [nseq + 1] first chunk of each sequence
   float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
@@ -56,6 +58,7 @@ struct Args {
   int per_seq;    // chunks of a batch row (without cu_seqlens)
   int max_chunks; // upper bound of the chunks over all sequences
   int ranges;     // CTAs of a scan
+  int sms;        // of the device
 };
 
 struct Seq {
@@ -370,11 +373,25 @@ __device__ __forceinline__ void wait_bar(uint64_t &bar, uint32_t &phase, Ctl &ct
   tc_fence_after();
 }
 
+// Allow `kern` `smem` bytes of dynamic shared memory on the current device, once a device (`done`: a
+// bit for each, kept by the caller).
+template <typename K>
+cudaError_t allow_smem(K kern, uint32_t smem, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 // launchers (kda_delta_scan.cu, kda_delta_grad.cu)
 cudaError_t launch_plan(const Args &a, cudaStream_t st);
 cudaError_t launch_prep(const Args &a, cudaStream_t st);
-cudaError_t launch_scan(const Args &a, bool store, cudaStream_t st);
-cudaError_t launch_rev(const Args &a, cudaStream_t st);
+cudaError_t launch_scan(const Args &a, cudaStream_t st);           // outputs
+cudaError_t launch_backward_scans(const Args &a, cudaStream_t st);  // states and u rows, then the reverse scan
 cudaError_t launch_grad(const Args &a, cudaStream_t st);
 
 }  // namespace delta
