@@ -531,19 +531,32 @@ using torch::autograd::AutogradContext;
 using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
+// Whether a call has to be recorded; without that it goes straight to the kernels (an autograd node
+// costs a call 5 us of host time).
+bool recorded(std::initializer_list<const Tensor *> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor *t : ts)
+    if (t != nullptr && t->requires_grad()) return true;
+  return false;
+}
+
 optional<Tensor> if_defined(const Tensor &t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
+
+const auto &delta_fwd_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("kda_b200::delta_fwd", "")
+                             .typed<std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                                               const Tensor &, double, const optional<Tensor> &,
+                                                               const optional<Tensor> &, bool)>();
+  return op;
+}
 
 struct DeltaFunction : public torch::autograd::Function<DeltaFunction> {
   static variable_list forward(AutogradContext *ctx, const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
                                const Tensor &beta, double scale, const optional<Tensor> &s0, const optional<Tensor> &cu,
                                bool want_state) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("kda_b200::delta_fwd", "")
-                         .typed<std::tuple<Tensor, Tensor>(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                                                           const Tensor &, double, const optional<Tensor> &,
-                                                           const optional<Tensor> &, bool)>();
-    auto [o, s] = op.call(q, k, v, g, beta, scale, s0, cu, want_state);
+    auto [o, s] = delta_fwd_op().call(q, k, v, g, beta, scale, s0, cu, want_state);
     ctx->save_for_backward({q, k, v, g, beta, s0.has_value() ? *s0 : Tensor(), cu.has_value() ? *cu : Tensor()});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["state"] = want_state;
@@ -572,6 +585,10 @@ struct DeltaFunction : public torch::autograd::Function<DeltaFunction> {
 std::tuple<Tensor, Tensor> delta_fwd_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g,
                                               const Tensor &beta, double scale, const optional<Tensor> &s0,
                                               const optional<Tensor> &cu, bool want_state) {
+  if (!recorded({&q, &k, &v, &g, &beta, s0.has_value() ? &*s0 : nullptr})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return delta_fwd_op().call(q, k, v, g, beta, scale, s0, cu, want_state);
+  }
   const variable_list r = DeltaFunction::apply(q, k, v, g, beta, scale, s0, cu, want_state);
   return {r[0], r[1]};
 }
@@ -592,15 +609,19 @@ Tensor delta_step_autograd(const Tensor &q, const Tensor &k, const Tensor &v, co
   return op.call(q, k, v, g, beta, state, slots, scale);
 }
 
+const auto &token_logprobs_op() {
+  static const auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("st_b200::token_logprobs", "")
+                             .typed<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, int64_t,
+                                                                                       double, int64_t)>();
+  return op;
+}
+
 struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
   static variable_list forward(AutogradContext *ctx, const Tensor &logits, const Tensor &tokens, int64_t top_k,
                                double temperature, int64_t ignore_index) {
     at::AutoDispatchBelowADInplaceOrView below;
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("st_b200::token_logprobs", "")
-                         .typed<std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor>(const Tensor &, const Tensor &, int64_t,
-                                                                                   double, int64_t)>();
-    auto [lp, ent, lse, top, ids] = op.call(logits, tokens, top_k, temperature, ignore_index);
+    auto [lp, ent, lse, top, ids] = token_logprobs_op().call(logits, tokens, top_k, temperature, ignore_index);
     ctx->save_for_backward({logits, tokens, ent, lse});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -625,6 +646,10 @@ struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs_autograd(const Tensor &logits, const Tensor &tokens,
                                                                            int64_t top_k, double temperature,
                                                                            int64_t ignore_index) {
+  if (!recorded({&logits})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return token_logprobs_op().call(logits, tokens, top_k, temperature, ignore_index);
+  }
   const variable_list r = LogprobsFunction::apply(logits, tokens, top_k, temperature, ignore_index);
   return {r[0], r[1], r[2], r[3], r[4]};
 }
