@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
   __shared__ uint64_t bar_g2, bar_s, bar_d;
-  __shared__ __align__(16) float gam[64];
+  __shared__ __align__(16) float gam[128];  // hi, then lo
   __shared__ float sm_dot[16], sm_xv[64];
   __shared__ float sm_f[2][64], sm_t[2][64], sm_y[2][64], sm_r[2][64];  // [half of the columns][row]
   const int tid = threadIdx.x, row = tid & 127, part = tid >> 7, r64 = row & 63;
@@ -140,8 +140,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       const int h = hk * G_ + hh;
       const size_t ch = (size_t)cidx * a.p.H + h;
       const bool last = hh + 1 == G_;
-      if (tid < 64) gam[tid] = a.w.gam[ch * 64 + tid];
-      const float gi = a.w.gam[ch * 64 + r64], gl = a.w.gam[ch * 64 + 63], bi = a.w.beta[ch * 64 + r64];
+      const float *gsrc = a.w.gam + ch * 128;
+      if (tid < 128) gam[tid] = gsrc[tid];
+      const float bi = a.w.beta[ch * 64 + r64];
       // two 16-byte runs of a row of V, eight threads a row
       constexpr int VR = D / 64;
       const int vr = tid >> 3, vc = tid & 7;
@@ -183,7 +184,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         if (r < pr && (last || part > 1))
           asm volatile("prefetch.global.L2 [%0];" ::"l"(rows_at(x, pb, part < 2 ? nk : nh, pt + r) + c * 64));
       }
-      const float Gi = exp_fast(gi), wi = exp_fast(gl - gi);
       // dX . v, and the products of the two images, place by place
       mbar_wait(smem_u32(&ctl.load_bar), ph, a.p.status, &ctl.abort);
       float xv = 0.f;
@@ -221,19 +221,26 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       uint4 mh[2], ml[2];
       float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
       {
+        const float gh = gam[r64], gl = gam[64 + r64];
         float x[16], y[16];
         tmem_ldn<16>(lane_t + tG1 + 16 * part, x);
         tmem_ldn<16>(lane_t + tG2 + 16 * part, y);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int col = 16 * part + j;
-          const float e = ex2f((gi - gam[col]) * kLog2e);
-          if (!upper) {
-            const float m = col < r64 ? -y[j] * e : 0.f;
-            rs = col < r64 ? fmaf(m, x[j], rs) : rs;
-            x[j] = m * bi;
-          } else {
-            x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
+        for (int j4 = 0; j4 < 16; j4 += 4) {
+          const float4 ch4 = *reinterpret_cast<const float4 *>(gam + 16 * part + j4);
+          const float4 cl4 = *reinterpret_cast<const float4 *>(gam + 64 + 16 * part + j4);
+          const float hi[4] = {ch4.x, ch4.y, ch4.z, ch4.w}, lo[4] = {cl4.x, cl4.y, cl4.z, cl4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int j = j4 + i, col = 16 * part + j;
+            const float e = decay(gh, gl, hi[i], lo[i]);
+            if (!upper) {
+              const float m = col < r64 ? -y[j] * e : 0.f;
+              rs = col < r64 ? fmaf(m, x[j], rs) : rs;
+              x[j] = m * bi;
+            } else {
+              x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
+            }
           }
         }
         split8<BF>(x, mh[0], ml[0]);
@@ -283,7 +290,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       {
         float x[W];
         tmem_ldn<W>(lane_t + tG5 + part * W, x);
-        const float f = upper ? a.p.scale * Gi : -Gi * bi;
+        const float f = ex2f(gam[r64]) * (upper ? a.p.scale : -bi);
 #pragma unroll
         for (int c = 0; c < W / 8; ++c) {
           float k[8];
@@ -316,6 +323,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         load_head(cidx, h + 1, b, t0, rows);
       else if (more)
         load_head(un / a.p.Hk, (un % a.p.Hk) * G_, nb, nt, nrows);
+      const float wi = decay(gam[63], gam[127], gam[r64], gam[64 + r64]);
 #pragma unroll
       for (int c0 = 0; c0 < W; c0 += 16) {
         float x[16], y[16], z[16];
@@ -365,14 +373,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         float f[2], y[2];
         float sd = 0.f;
         for (int w = 0; w < 16; ++w) sd += sm_dot[w];
-        sd *= exp_fast(gam[63]);
+        sd *= ex2f(gam[63]);
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * tid + j;
           f[j] = sm_f[0][i] + sm_f[1][i];
           y[j] = sm_y[0][i] + sm_y[1][i];
           if (i < rows)
             store_gate(a.p.dbeta, (b * a.p.H + h) * a.p.T + t0 + i, a.p.beta_dtype,
-                       sm_xv[i] - exp_fast(gam[i]) * (sm_t[0][i] + sm_t[1][i]) + (sm_r[0][i] + sm_r[1][i]));
+                       sm_xv[i] - ex2f(gam[i]) * (sm_t[0][i] + sm_t[1][i]) + (sm_r[0][i] + sm_r[1][i]));
         }
         // suffix sums of f, exclusive prefix sums of y
         float sf = f[0] + f[1], py = y[0] + y[1];
@@ -508,7 +516,7 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->ranges = scan_ranges(a->nseq, p->H, a->sms);
   a->w.queue = reinterpret_cast<int *>(take(sizeof(int) * 2 * ((size_t)a->ranges + 2)));
   a->w.slots = reinterpret_cast<float *>(take((backward ? 2 : 1) * ((size_t)a->ranges + 1) * p->D * p->D * 4));
-  a->w.gam = reinterpret_cast<float *>(take(cells * 256));
+  a->w.gam = reinterpret_cast<float *>(take(cells * 512));
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
   a->w.T = take(cells * kda::delta::kImgT);
   if (backward) {

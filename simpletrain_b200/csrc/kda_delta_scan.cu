@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   constexpr uint32_t KQ = 0, TT = 0;  // [T; P] hi, then lo, over the rest
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
-  __shared__ __align__(16) float gam[64], bet[64];
+  __shared__ __align__(16) float gam[2][64], bet[64];
   int64_t b, t0;
   int rows;
   if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   const uint32_t tmem = cta_begin(ctl, 64);
   const size_t ch = (size_t)blockIdx.x * a.p.H + h;
   if (tid < 32) {
-    // running sums in double: rounded once, so that differences of gammas keep fp32's last bits
+    // running sums in double, then in two fp32 terms
     double s[2];
     for (int j = 0; j < 2; ++j) {
       const int i = 2 * tid + j;
@@ -164,8 +164,12 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
       const double y = __shfl_up_sync(0xffffffffu, c, o);
       if (tid >= o) c += y;
     }
-    gam[2 * tid + 1] = (float)c;
-    gam[2 * tid] = (float)(c - s[1]);
+    for (int j = 0; j < 2; ++j) {
+      const double x = kLog2e * (j ? c : c - s[1]);
+      const float hi = (float)x;
+      gam[0][2 * tid + j] = hi;
+      gam[1][2 * tid + j] = (float)(x - (double)hi);
+    }
   }
   cp_async_wait();
   publish();
@@ -175,11 +179,9 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     issue<D / 16>(tmem, KMajor{sb + KQ, 16384}, KMajor{sb + KQ, 16384}, idesc_f16(128, 64, BF, false, false), false);
     mma_commit(smem_u32(&ctl.mma_bar));
   }
-  if (tid < 64) {
-    a.w.gam[ch * 64 + tid] = gam[tid];
-    a.w.beta[ch * 64 + tid] = bet[tid];
-  }
-  const float gi = gam[r64] * kLog2e;
+  if (tid < 128) a.w.gam[ch * 128 + tid] = gam[tid >> 6][tid & 63];
+  if (tid < 64) a.w.beta[ch * 64 + tid] = bet[tid];
+  const float gh = gam[0][r64], gl = gam[1][r64];
   const float rowf = row < 64 ? bet[r64] : a.p.scale;
   wait_bar(ctl.mma_bar, ph, ctl, a.p.status);
   float *As = reinterpret_cast<float *>(smem + KQ);  // over the k and q tiles: their product is done
@@ -193,11 +195,12 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     tmem_ld16(taddr + c0, x);
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
-      const float4 c = *reinterpret_cast<const float4 *>(gam + 32 * half + c0 + j);
-      const float d[4] = {c.x, c.y, c.z, c.w};
+      const float4 c = *reinterpret_cast<const float4 *>(gam[0] + 32 * half + c0 + j);
+      const float4 l = *reinterpret_cast<const float4 *>(gam[1] + 32 * half + c0 + j);
+      const float d[4] = {c.x, c.y, c.z, c.w}, dl[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float f = rowf * ex2f(fmaf(-kLog2e, d[e], gi));
+        const float f = rowf * decay(gh, gl, d[e], dl[e]);
         x[j + e] = c0 + j + e <= last ? f * x[j + e] : 0.f;
       }
     }
@@ -903,16 +906,17 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         }
       }
       const size_t at = cell(pos) * 64;
-      const float gl = a.w.gam[at + 63];
+      const float *gam = a.w.gam + 2 * at;
+      const float lh = gam[63], ll = gam[127];
 #pragma unroll
       for (int i = lane; i < 64; i += 32) {
-        const float gi = a.w.gam[at + i], be = a.w.beta[at + i], G = exp_fast(gi);
+        const float gh = gam[i], gl = gam[64 + i], be = a.w.beta[at + i], G = ex2f(gh);
         fac[st].beta[i] = be;
         fac[st].bg[i] = -be * G;
-        fac[st].w[i] = exp_fast(gl - gi);
+        fac[st].w[i] = decay(lh, ll, gh, gl);
         fac[st].sg[i] = a.p.scale * G;
       }
-      if (lane == 0) fac[st].last[0] = exp_fast(gl);
+      if (lane == 0) fac[st].last[0] = ex2f(lh);
       mbar_arrive(bar);
       __syncwarp();
     };

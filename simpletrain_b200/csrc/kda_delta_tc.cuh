@@ -33,7 +33,7 @@ using namespace kda::tc;
 constexpr int kChunk = 64;
 constexpr int kThreads = 256;
 constexpr int kImgT = 32768;  // T / PT image of a (chunk, head): [128 x 64] hi, then lo
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
 
 // Workspace regions (device pointers) of one call.
@@ -42,7 +42,9 @@ struct Work {
   float *slots;    // [scan][ranges + 1][D][D] states at the ranges' boundaries
   int *bound;      // [nseq + 1] sequence offsets, clamped into order and range (packed sequences only)
   int *first;      // [nseq + 1] first chunk of each sequence
-  float *gam;      // [chunk][H][64] running sums of the log decay inside the chunk
+  float *gam;      // [chunk][H][2][64] running sums of the log decay inside the chunk, in units of log 2 and in two
+                   // terms: their differences decide the factors, and after a few strong decays (-110 each) one
+                   // fp32 term is 1e-4 from the sum (the state was 2e-4 from the recurrence's)
   float *beta;     // [chunk][H][64]
   char *T;         // [chunk][H] images of T over P T
   char *S, *dS;    // [chunk][H] images of the state before / the state gradient after the chunk, transposed: hi,
@@ -99,7 +101,8 @@ __device__ __forceinline__ float ex2f(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ float exp_fast(float x) { return ex2f(x * kLog2e); }
+// e^{gamma_i - gamma_j} from two-term gammas
+__device__ __forceinline__ float decay(float hi_i, float lo_i, float hi_j, float lo_j) { return ex2f((hi_i - hi_j) + (lo_i - lo_j)); }
 
 __device__ __forceinline__ float load_gate(const void *p, int64_t i, int dtype) {
   if (dtype == KDA_DTYPE_F32) return static_cast<const float *>(p)[i];

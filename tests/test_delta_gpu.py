@@ -228,6 +228,21 @@ def test_strong_and_absent_decay():
     compare(got, exp)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("case", ["every other", "runs", "every third"])
+def test_many_resets_in_a_chunk(case, D):
+    """The running sum of the decay gets long; the factors between tokens after the resets keep their last bits."""
+    x = make(1, 4, 2, 250, D, torch.float16, torch.float32, seed=3, state=True)
+    if case == "every other":
+        x["g"][..., ::2] = -110.0
+    elif case == "runs":
+        for i in range(4):
+            x["g"][..., 64 * i:64 * i + 40] = -110.0
+    else:
+        x["g"][..., ::3] = -60.0
+    compare(*run_both(x, D))
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the library's own forward, through the fp32 state."""
     from simpletrain_b200 import gated_delta_chunk
