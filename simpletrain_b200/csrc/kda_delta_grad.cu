@@ -222,29 +222,33 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
       {
         const float gh = gam[r64], gl = gam[64 + r64];
-        float x[16], y[16];
-        tmem_ldn<16>(lane_t + tG1 + 16 * part, x);
-        tmem_ldn<16>(lane_t + tG2 + 16 * part, y);
 #pragma unroll
-        for (int j4 = 0; j4 < 16; j4 += 4) {
-          const float4 ch4 = *reinterpret_cast<const float4 *>(gam + 16 * part + j4);
-          const float4 cl4 = *reinterpret_cast<const float4 *>(gam + 64 + 16 * part + j4);
-          const float hi[4] = {ch4.x, ch4.y, ch4.z, ch4.w}, lo[4] = {cl4.x, cl4.y, cl4.z, cl4.w};
+        for (int c = 0; c < 2; ++c) {
+          uint32_t xr[8], yr[8];
+          tmem_ld_32x32b_x8_nowait(lane_t + tG1 + 16 * part + 8 * c, xr);
+          tmem_ld_32x32b_x8_nowait(lane_t + tG2 + 16 * part + 8 * c, yr);
+          tmem_wait_ld_bind(xr, yr);
+          float m8[8];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int j = j4 + i, col = 16 * part + j;
-            const float e = decay(gh, gl, hi[i], lo[i]);
-            if (!upper) {
-              const float m = col < r64 ? -y[j] * e : 0.f;
-              rs = col < r64 ? fmaf(m, x[j], rs) : rs;
-              x[j] = m * bi;
-            } else {
-              x[j] = col <= r64 ? a.p.scale * y[j] * e : 0.f;
+          for (int j4 = 0; j4 < 8; j4 += 4) {
+            const float4 ch4 = *reinterpret_cast<const float4 *>(gam + 16 * part + 8 * c + j4);
+            const float4 cl4 = *reinterpret_cast<const float4 *>(gam + 64 + 16 * part + 8 * c + j4);
+            const float hi[4] = {ch4.x, ch4.y, ch4.z, ch4.w}, lo[4] = {cl4.x, cl4.y, cl4.z, cl4.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = j4 + i, col = 16 * part + 8 * c + j;
+              const float e = decay(gh, gl, hi[i], lo[i]), y = __uint_as_float(yr[j]);
+              if (!upper) {
+                const float m = col < r64 ? -y * e : 0.f;
+                rs = col < r64 ? fmaf(m, __uint_as_float(xr[j]), rs) : rs;
+                m8[j] = m * bi;
+              } else {
+                m8[j] = col <= r64 ? a.p.scale * y * e : 0.f;
+              }
             }
           }
+          split8<BF>(m8, mh[c], ml[c]);
         }
-        split8<BF>(x, mh[0], ml[0]);
-        split8<BF>(x + 8, mh[1], ml[1]);
       }
       // over the dX / dO tiles once their products are done and every thread is past its reads of them and of S
       mbar_wait(smem_u32(&ctl.mma_bar), ph, a.p.status, &ctl.abort);
