@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     double s[2];
     for (int j = 0; j < 2; ++j) {
       const int i = 2 * tid + j;
-      s[j] = i < rows ? (double)fmaxf(load_gate(a.p.g, b * a.p.g_stride_b + h * a.p.g_stride_h + (t0 + i) * a.p.g_stride_t, a.p.g_dtype), kMinGate) : 0.0;
+      const float gate = i < rows ? load_gate(a.p.g, b * a.p.g_stride_b + h * a.p.g_stride_h + (t0 + i) * a.p.g_stride_t, a.p.g_dtype) : 0.f;
+      s[j] = gate < kMinGate ? kMinGate : gate;  // a NaN stays one
       bet[i] = i < rows ? load_gate(a.p.beta, b * a.p.beta_stride_b + h * a.p.beta_stride_h + (t0 + i) * a.p.beta_stride_t, a.p.beta_dtype) : 0.f;
     }
     double c = s[0] + s[1];

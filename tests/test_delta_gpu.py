@@ -162,6 +162,21 @@ def test_packed_rows_equal_their_own_calls():
     assert torch.isnan(o[:, :, 100:164]).any()
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_nan_is_not_swallowed(name):
+    """A NaN of any input reaches the outputs from its token on, the state and the gradients."""
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(1, 1, 1, 200, 64, torch.bfloat16, torch.float32)
+    x[name][0, 0, 70] = torch.nan
+    leaf = [x[n].detach().requires_grad_(True) for n in NAMES]
+    o, s = gated_delta_chunk(*leaf)
+    assert torch.isfinite(o[:, :, :64]).all() and torch.isnan(o[0, 0, 70]).all()
+    if name != "q":
+        assert torch.isnan(o[0, 0, 71:]).any(-1).all() and torch.isnan(s).any()
+    grads = torch.autograd.grad(o, leaf, x["do"])
+    assert any(torch.isnan(g).any() for g in grads)
+
+
 @pytest.mark.parametrize("raw", [[0, 90, 40, 130], [-5, 20, 130, 131], [0, 10 ** 12, 60, 130], [200, 300, 400, 500]])
 def test_bad_offsets_are_clamped_and_reported(raw):
     from simpletrain_b200 import _ffi, device_status, gated_delta_chunk
