@@ -217,7 +217,7 @@ int kda_fwd_sm100_noalloc(const kda_fwd_params *p, kda_stream_t stream);
  * counts as -110 (exp is 0 in fp32 either way).
  *
  * Sequences: with cu_seqlens == NULL each of the B batch rows is one sequence
- * of T tokens.  With cu_seqlens (device [nseq + 1], B == 1) sequence i is
+ * of T tokens.  With cu_seqlens (device [nseq + 1], B == 1, T <= 2^24) sequence i is
  * tokens [cu_seqlens[i], cu_seqlens[i + 1]); it may be empty.  Offsets are not
  * trusted: out-of-order or out-of-range ones are clamped into order and range
  * and set KDA_ERR_DEVICE_INDEX in *status.  Tokens outside every sequence get

@@ -87,14 +87,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   auto rows_at = [](const kda_tensor &x, int64_t b, int64_t hd, int64_t t) {
     return static_cast<uint16_t *>(x.data) + b * x.stride_b + hd * x.stride_h + t * x.stride_t;
   };
-  auto load64 = [&](uint32_t tile, int row0, const uint16_t *src, int64_t stride, int rows) {
-    constexpr int P = D / 8;
-#pragma unroll
-    for (int i = 0; i < 64 * P / kGradThreads; ++i) {
-      const int p = tid + i * kGradThreads, r = p / P, c = p % P, tr = row0 + r;
-      cp_async16(tile + (c >> 3) * 16384 + chunk_at(tr, c & 7), src + (r < rows ? r * stride : 0) + c * 8, r < rows);
-    }
-  };
   auto mma_leader = [&]() { return (tid >> 5) == kMmaWarp && elect_one(); };
   // the tiles of value head h of chunk cell cidx, all but k and q
   auto load_head = [&](int cidx, int h, int64_t b, int64_t t0, int rows) {
@@ -112,7 +104,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       bulk_load(sb + L::S, a.w.S + ch * (size_t)(D * D * 4), D * D * 4, b2);
       bulk_load(sb + L::DH, a.w.dS + ch * (size_t)(D * D * 4), D * D * 2, b2);
     }
-    load64(sb + L::AH, 64, rows_at(a.p.dout, b, h, t0), a.p.dout.stride_t, rows);
+    load_rows<D, kGradThreads>(sb + L::AH, 64, rows_at(a.p.dout, b, h, t0), a.p.dout.stride_t, rows);
     if (upper)
 #pragma unroll
       for (int c = 0; c < W / 8; ++c) sts(sb + L::AL + own_chunk(c), make_uint4(0, 0, 0, 0));
@@ -125,8 +117,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   if (live) load_head(u / a.p.Hk, (u % a.p.Hk) * G_, b, t0, rows);
   while (live) {
     const int cidx = u / a.p.Hk, hk = u % a.p.Hk;
-    load64(sb + L::KQ, 0, rows_at(a.p.k, b, hk, t0), a.p.k.stride_t, rows);
-    load64(sb + L::KQ, 64, rows_at(a.p.q, b, hk, t0), a.p.q.stride_t, rows);
+    load_rows<D, kGradThreads>(sb + L::KQ, 0, rows_at(a.p.k, b, hk, t0), a.p.k.stride_t, rows);
+    load_rows<D, kGradThreads>(sb + L::KQ, 64, rows_at(a.p.q, b, hk, t0), a.p.q.stride_t, rows);
     float acc[W];
 #pragma unroll
     for (int j = 0; j < W; ++j) acc[j] = 0.f;
@@ -469,6 +461,8 @@ int check_sizes(const kda_delta_params *p) {
   if (!gate_ok(p->g_dtype) || !gate_ok(p->beta_dtype)) return KDA_ERR_UNSUPPORTED;
   if (p->B > 0 && p->H > 0 && (p->Hk == 0 || p->H % p->Hk)) return KDA_ERR_BAD_SHAPE;
   if (p->cu_seqlens != nullptr && (p->B != 1 || p->nseq < 0)) return KDA_ERR_BAD_SHAPE;
+  // a work range waits for a long sequence's state, and waits are bounded: 2^18 chunks are 0.6 s of 2
+  if (p->cu_seqlens != nullptr && p->T > 1 << 24) return KDA_ERR_BAD_SHAPE;
   if (p->H > 65535) return KDA_ERR_BAD_SHAPE;  // a grid dimension
   const int64_t nseq = p->cu_seqlens != nullptr ? (int64_t)p->nseq + 1 : p->B;
   if (nseq * p->H * 2 > 0x7fffffff) return KDA_ERR_BAD_SHAPE;

@@ -128,9 +128,13 @@ __device__ __forceinline__ void inverse_level(float *As, float *Ti) {
 // by substitution, a column a thread, then [A 0; B C]^-1 = [a 0; -c B a, c] twice.
 // The q.k rows wait in tensor memory while the inverse is formed, so that the k and q tiles, the
 // fp32 matrices and the two-term tiles can take turns in 34 KB, and four CTAs share an SM:
-// the kernel is a chain of short dependent steps, hidden by other CTAs only.
+// the kernel is a chain of short dependent steps, hidden by other CTAs only.  Measured:
+// 107 us for the 8192 (chunk, head) cells of 8 x 8192 tokens, 8 heads of 128 (64 KB of k, q and images a
+// cell: 5.0 TB/s); 128 threads a CTA and six CTAs an SM came to the same.
+constexpr int kPrepThreads = 256;
+
 template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
+__global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   constexpr uint32_t KQ = 0, TT = 0;  // [T; P] hi, then lo, over the rest
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
@@ -140,14 +144,14 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
   if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
   pdl_launch_dependents();
   if (blockIdx.x == 0 && blockIdx.y == 0)
-    for (int i = threadIdx.x; i < 2 * (a.ranges + 2); i += kThreads) a.w.queue[i] = 0;
+    for (int i = threadIdx.x; i < 2 * (a.ranges + 2); i += kPrepThreads) a.w.queue[i] = 0;
   if (!get_chunk(a, blockIdx.x, &b, &t0, &rows)) return;
   const int h = blockIdx.y, hk = h / (a.p.H / a.p.Hk), tid = threadIdx.x;
   const int row = tid & 127, half = tid >> 7, r64 = row & 63;
   const uint32_t sb = smem_u32(smem), lane_base = (uint32_t)((tid >> 5) & 3) << 21;
-  load_rows<D>(sb + KQ, 0, 16384, static_cast<const uint16_t *>(a.p.k.data) + b * a.p.k.stride_b + hk * a.p.k.stride_h + t0 * a.p.k.stride_t,
+  load_rows<D, kPrepThreads>(sb + KQ, 0, static_cast<const uint16_t *>(a.p.k.data) + b * a.p.k.stride_b + hk * a.p.k.stride_h + t0 * a.p.k.stride_t,
                a.p.k.stride_t, rows);
-  load_rows<D>(sb + KQ, 64, 16384, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
+  load_rows<D, kPrepThreads>(sb + KQ, 64, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
                a.p.q.stride_t, rows);
   const uint32_t tmem = cta_begin(ctl, 64);
   const size_t ch = (size_t)blockIdx.x * a.p.H + h;
@@ -237,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 4) prep_kernel(const Args a) {
     for (int i = 0; i < 16; ++i) Ti[(o + i) * kLd + o + j] = y[i];
   } else {
     // the six 16 x 16 blocks above the diagonal blocks
-    for (int e = tid - 64; e < 6 * 64; e += kThreads - 64) {
+    for (int e = tid - 64; e < 6 * 64; e += kPrepThreads - 64) {
       const int q = e >> 6, f = e & 63;
       const int bi = q < 3 ? 0 : (q < 5 ? 1 : 2), bj = q < 3 ? q + 1 : (q < 5 ? q - 1 : 3);
       *reinterpret_cast<float4 *>(Ti + (16 * bi + (f >> 2)) * kLd + 16 * bj + (f & 3) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -641,67 +645,67 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           wait_flag(queue + 1 + range, a.p.status, &abort_flag);
           src = slots + (size_t)range * D * D;
         }
-      for (int pos = p0; pos < p1; ++pos, ++it) {
-        const int st = it & 1;
-        wait_full(pos);
-        const float last = fac[st].last[0];
-        if (it > 0) {
-          if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
-          wait(bars.s_done, (it - 1) & 1);
-        }
-        tc_fence_after();
-#pragma unroll
-        for (int c0 = 0; c0 < W; c0 += 32) {
-          float x[32];
-          if (pos > p0) {
-            tmem_ld32(tl + cS + half * W + c0, x);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
+        for (int pos = p0; pos < p1; ++pos, ++it) {
+          const int st = it & 1;
+          wait_full(pos);
+          const float last = fac[st].last[0];
+          if (it > 0) {
+            if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
+            wait(bars.s_done, (it - 1) & 1);
           }
-          tmem_split32<BF>(tl + cSH + (half * W + c0) / 2, tl + cSL + (half * W + c0) / 2, x);
-          uint32_t r[32];
+          tc_fence_after();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(x[j] * last);
-          tmem_st_32x32b_x32_nowait(tl + cS + half * W + c0, r);
-          tmem_wait_st();
-          arrive_warp(bars.s_ready[c0 / 32]);
-        }
-        float v[32];
-        if (!REV) {  // V^T: this value channel of 32 tokens
-          const uint32_t vt = sb + st * L::kStage + L::V + half * 4096;
+          for (int c0 = 0; c0 < W; c0 += 32) {
+            float x[32];
+            if (pos > p0) {
+              tmem_ld32(tl + cS + half * W + c0, x);
+            } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            uint16_t u;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + vcol[j & 7] + (j >> 3) * 1024));
-            v[j] = unpack2((uint32_t)u, BF).x * fac[st].beta[32 * half + j];
+              for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
+            }
+            tmem_split32<BF>(tl + cSH + (half * W + c0) / 2, tl + cSL + (half * W + c0) / 2, x);
+            uint32_t r[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(x[j] * last);
+            tmem_st_32x32b_x32_nowait(tl + cS + half * W + c0, r);
+            tmem_wait_st();
+            arrive_warp(bars.s_ready[c0 / 32]);
+          }
+          float v[32];
+          if (!REV) {  // V^T: this value channel of 32 tokens
+            const uint32_t vt = sb + st * L::kStage + L::V + half * 4096;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              uint16_t u;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + vcol[j & 7] + (j >> 3) * 1024));
+              v[j] = unpack2((uint32_t)u, BF).x * fac[st].beta[32 * half + j];
+            }
+          }
+          wait(bars.ks_done, it & 1);
+          tc_fence_after();
+          {
+            float x[32];
+            tmem_ld32(tl + cR1 + 32 * half, x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] = REV ? fac[st].w[32 * half + j] * x[j] : fmaf(fac[st].bg[32 * half + j], x[j], v[j]);
+            tmem_split32<BF>(tl + cXH + 16 * half, tl + cXL + 16 * half, x);
+            tmem_wait_st();
+            arrive_warp(bars.x_ready);
+          }
+          wait(bars.u_done, it & 1);
+          tc_fence_after();
+          {
+            float x[32];
+            tmem_ld32(tl + (REV ? cR2 : cR1) + 32 * half, x);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) x[j] *= REV ? fac[st].bg[32 * half + j] : fac[st].w[32 * half + j];
+            // over an operand whose products are done: S^T's (outputs: X^T may still be in use), else X^T's
+            const uint32_t at = MODE == kOut ? cSH : cXH;
+            tmem_split32<BF>(tl + at + 16 * half, tl + at + 32 + 16 * half, x);
+            tmem_wait_st();
+            arrive_warp(bars.up_ready);
           }
         }
-        wait(bars.ks_done, it & 1);
-        tc_fence_after();
-        {
-          float x[32];
-          tmem_ld32(tl + cR1 + 32 * half, x);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] = REV ? fac[st].w[32 * half + j] * x[j] : fmaf(fac[st].bg[32 * half + j], x[j], v[j]);
-          tmem_split32<BF>(tl + cXH + 16 * half, tl + cXL + 16 * half, x);
-          tmem_wait_st();
-          arrive_warp(bars.x_ready);
-        }
-        wait(bars.u_done, it & 1);
-        tc_fence_after();
-        {
-          float x[32];
-          tmem_ld32(tl + (REV ? cR2 : cR1) + 32 * half, x);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) x[j] *= REV ? fac[st].bg[32 * half + j] : fac[st].w[32 * half + j];
-          // over an operand whose products are done: S^T's (outputs: X^T may still be in use), else X^T's
-          const uint32_t at = MODE == kOut ? cSH : cXH;
-          tmem_split32<BF>(tl + at + 16 * half, tl + at + 32 + 16 * half, x);
-          tmem_wait_st();
-          arrive_warp(bars.up_ready);
-        }
-      }
         // where the state goes from here: to the next range, or to the caller
         float *dst = pc.p1 < pc.nc ? slots + (size_t)(range + 1) * D * D
                                    : (REV ? a.p.dstate_in : (MODE == kOut ? a.p.state_out : nullptr));
@@ -758,128 +762,128 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         named_bar_sync(1, 32 * Q);
       };
       while (next_piece()) {
-      for (int pos = p0; pos < p1; ++pos, ++it) {
-        const int st = it & 1;
-        if (MODE == kOut) {
-          wait_full(pos);
-          wait(bars.o_done, it & 1);
-          tc_fence_after();
-          uint32_t pk[2][16];  // [16-lane half][column block j, row half]
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh) {
-            uint32_t qs[32], o[32];
-            tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, qs);
-            tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR3, o);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float f0 = fac[st].sg[8 * j + q2], f1 = fac[st].sg[8 * j + q2 + 1];
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                pk[hh][2 * j + e] = pack2(fmaf(f0, __uint_as_float(qs[4 * j + 2 * e]), __uint_as_float(o[4 * j + 2 * e])),
-                                          fmaf(f1, __uint_as_float(qs[4 * j + 2 * e + 1]), __uint_as_float(o[4 * j + 2 * e + 1])), BF);
-            }
-          }
-          arrive_warp(bars.out_free);
-          if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
-          tile_free();
-#pragma unroll
-          for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-            for (int j = 0; j < 8; j += 2)
-              tile.put(sb + L::OUT, hh, j, pk[hh][2 * j], pk[hh][2 * j + 1], pk[hh][2 * j + 2], pk[hh][2 * j + 3]);
-          store_tile(sb + L::OUT, pos);
-          if (t == 0) tma_store_commit();
-        } else {
-          if (REV) {  // Q' product's first operand: scale e^gamma dO, transposed, in two terms
+        for (int pos = p0; pos < p1; ++pos, ++it) {
+          const int st = it & 1;
+          if (MODE == kOut) {
             wait_full(pos);
-            if (it > 0) wait(bars.s_done, (it - 1) & 1);  // the last one is used
-            const uint32_t vt = sb + st * L::kStage + L::V + (row >> 6) * 8192 + (row & 7) * 2;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              float x[32];
-#pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                uint16_t u;
-                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + (32 * b + j) * 128 + ((((row >> 3) ^ j) & 7) << 4)));
-                x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * b + j];
-              }
-              tmem_split32<BF>(tl + cR3 + 16 * b, tl + cR3 + 32 + 16 * b, x);
-            }
-            tmem_wait_st();
-            arrive_warp(bars.qs_ready);
-          }
-          // the state (reverse: its gradient) as the chain split it
-          char *img = (REV ? a.w.dS : a.w.S) + cell(pos) * (size_t)(D * D * 4) + row * 16;
-#pragma unroll
-          for (int b = 0; b < NB; ++b) wait(bars.s_ready[b], it & 1);
-          tc_fence_after();
-#pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-              uint32_t r[32];
-              tmem_ld_32x32b_x32(tl + (part ? cSL : cSH) + 32 * b, r);
-#pragma unroll
-              for (int g = 0; g < 8; ++g)
-                *reinterpret_cast<uint4 *>(img + part * (D * D * 2) + (8 * b + g) * (D * 16)) =
-                    make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
-            }
-          wait(bars.u_done, it & 1);
-          tc_fence_after();
-          if (MODE == kStore) {  // U^T
-            char *ui = a.w.U + cell(pos) * (size_t)(D * 256) + row * 16;
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              float x[32];
-              tmem_ld32(tl + cR1 + 32 * b, x);
-              if (b == 1) arrive_warp(bars.out_free);
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                uint4 hi, lo;
-                split8<BF>(x + 8 * g, hi, lo);
-                *reinterpret_cast<uint4 *>(ui + (4 * b + g) * (D * 16)) = hi;
-                *reinterpret_cast<uint4 *>(ui + D * 128 + (4 * b + g) * (D * 16)) = lo;
-              }
-            }
-          } else {  // dX, and dV = beta dX
-            tile_free();
+            wait(bars.o_done, it & 1);
+            tc_fence_after();
+            uint32_t pk[2][16];  // [16-lane half][column block j, row half]
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-              uint32_t x[32], hi[16], lo[16];
-              tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, x);
-              if (hh == 1) arrive_warp(bars.out_free);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) split2<BF>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), hi[i], lo[i]);
-#pragma unroll
-              for (int j = 0; j < 8; j += 2) {
-                tile.put(sb + L::OUT, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
-                tile.put(sb + L::OUT + L::kTile, hh, j, lo[2 * j], lo[2 * j + 1], lo[2 * j + 2], lo[2 * j + 3]);
-              }
+              uint32_t qs[32], o[32];
+              tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, qs);
+              tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR3, o);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const float f0 = fac[st].beta[8 * j + q2], f1 = fac[st].beta[8 * j + q2 + 1];
+                const float f0 = fac[st].sg[8 * j + q2], f1 = fac[st].sg[8 * j + q2 + 1];
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
-                  hi[2 * j + e] = pack2(f0 * __uint_as_float(x[4 * j + 2 * e]), f1 * __uint_as_float(x[4 * j + 2 * e + 1]), BF);
+                  pk[hh][2 * j + e] = pack2(fmaf(f0, __uint_as_float(qs[4 * j + 2 * e]), __uint_as_float(o[4 * j + 2 * e])),
+                                            fmaf(f1, __uint_as_float(qs[4 * j + 2 * e + 1]), __uint_as_float(o[4 * j + 2 * e + 1])), BF);
               }
+            }
+            arrive_warp(bars.out_free);
+            if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
+            tile_free();
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
               for (int j = 0; j < 8; j += 2)
-                tile.put(sb + L::OUT + 2 * L::kTile, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
-            store_tile(sb + L::OUT + 2 * L::kTile, pos);
-            if (t == 0) {  // the dX tiles are the images
-              char *xi = a.w.dX + cell(pos) * (size_t)(D * 256);
-              for (int b = 0; b < NB; ++b) {
-                bulk_store(xi + b * 16384, sb + L::OUT + b * 8192, 8192);
-                bulk_store(xi + b * 16384 + 8192, sb + L::OUT + L::kTile + b * 8192, 8192);
+                tile.put(sb + L::OUT, hh, j, pk[hh][2 * j], pk[hh][2 * j + 1], pk[hh][2 * j + 2], pk[hh][2 * j + 3]);
+            store_tile(sb + L::OUT, pos);
+            if (t == 0) tma_store_commit();
+          } else {
+            if (REV) {  // Q' product's first operand: scale e^gamma dO, transposed, in two terms
+              wait_full(pos);
+              if (it > 0) wait(bars.s_done, (it - 1) & 1);  // the last one is used
+              const uint32_t vt = sb + st * L::kStage + L::V + (row >> 6) * 8192 + (row & 7) * 2;
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                float x[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  uint16_t u;
+                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + (32 * b + j) * 128 + ((((row >> 3) ^ j) & 7) << 4)));
+                  x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * b + j];
+                }
+                tmem_split32<BF>(tl + cR3 + 16 * b, tl + cR3 + 32 + 16 * b, x);
               }
-              tma_store_commit();
+              tmem_wait_st();
+              arrive_warp(bars.qs_ready);
+            }
+            // the state (reverse: its gradient) as the chain split it
+            char *img = (REV ? a.w.dS : a.w.S) + cell(pos) * (size_t)(D * D * 4) + row * 16;
+#pragma unroll
+            for (int b = 0; b < NB; ++b) wait(bars.s_ready[b], it & 1);
+            tc_fence_after();
+#pragma unroll
+            for (int part = 0; part < 2; ++part)
+#pragma unroll
+              for (int b = 0; b < NB; ++b) {
+                uint32_t r[32];
+                tmem_ld_32x32b_x32(tl + (part ? cSL : cSH) + 32 * b, r);
+#pragma unroll
+                for (int g = 0; g < 8; ++g)
+                  *reinterpret_cast<uint4 *>(img + part * (D * D * 2) + (8 * b + g) * (D * 16)) =
+                      make_uint4(r[4 * g], r[4 * g + 1], r[4 * g + 2], r[4 * g + 3]);
+              }
+            wait(bars.u_done, it & 1);
+            tc_fence_after();
+            if (MODE == kStore) {  // U^T
+              char *ui = a.w.U + cell(pos) * (size_t)(D * 256) + row * 16;
+#pragma unroll
+              for (int b = 0; b < 2; ++b) {
+                float x[32];
+                tmem_ld32(tl + cR1 + 32 * b, x);
+                if (b == 1) arrive_warp(bars.out_free);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                  uint4 hi, lo;
+                  split8<BF>(x + 8 * g, hi, lo);
+                  *reinterpret_cast<uint4 *>(ui + (4 * b + g) * (D * 16)) = hi;
+                  *reinterpret_cast<uint4 *>(ui + D * 128 + (4 * b + g) * (D * 16)) = lo;
+                }
+              }
+            } else {  // dX, and dV = beta dX
+              tile_free();
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                uint32_t x[32], hi[16], lo[16];
+                tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, x);
+                if (hh == 1) arrive_warp(bars.out_free);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) split2<BF>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), hi[i], lo[i]);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                  tile.put(sb + L::OUT, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
+                  tile.put(sb + L::OUT + L::kTile, hh, j, lo[2 * j], lo[2 * j + 1], lo[2 * j + 2], lo[2 * j + 3]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                  const float f0 = fac[st].beta[8 * j + q2], f1 = fac[st].beta[8 * j + q2 + 1];
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    hi[2 * j + e] = pack2(f0 * __uint_as_float(x[4 * j + 2 * e]), f1 * __uint_as_float(x[4 * j + 2 * e + 1]), BF);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                  tile.put(sb + L::OUT + 2 * L::kTile, hh, j, hi[2 * j], hi[2 * j + 1], hi[2 * j + 2], hi[2 * j + 3]);
+              }
+              __syncwarp();
+              if (lane == 0) mbar_arrive(smem_u32(&bars.empty[st]));
+              store_tile(sb + L::OUT + 2 * L::kTile, pos);
+              if (t == 0) {  // the dX tiles are the images
+                char *xi = a.w.dX + cell(pos) * (size_t)(D * 256);
+                for (int b = 0; b < NB; ++b) {
+                  bulk_store(xi + b * 16384, sb + L::OUT + b * 8192, 8192);
+                  bulk_store(xi + b * 16384 + 8192, sb + L::OUT + L::kTile + b * 8192, 8192);
+                }
+                tma_store_commit();
+              }
             }
           }
         }
-      }
       }
       if (t == 0) tma_store_wait_all();
     }
@@ -951,75 +955,75 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
     const uint32_t id_u = idesc_f16(128, D, BF, false, true);   // update: N = key channels
     const uint32_t id_a64 = idesc_f16(128, 64, BF, true, true);  // dO^T from shared memory
     while (step_piece(), take_piece()) {
-    for (int pos = p0; pos < p1; ++pos, ++it) {
-      const int st = it & 1;
-      const uint32_t base = sb + st * L::kStage;
-      const KMajor k_rows(base + L::K, 8192), q_rows(base + L::Q, 8192);
-      const MNMajor k_cols(base + L::K, 8192), q_cols(base + L::Q, 8192);
-      wait(bars.full[st], (it >> 1) & 1);
-      if (pos == rp) wait_tail(st);
-      // key channels in the order in which the chain hands them over: quarters 0 and 2, then 1 and 3
-      wait(bars.s_ready[0], it & 1);
-      tc_fence_after();
-      constexpr int H4 = D / 32;  // steps of half the key channels
-      issue_ts<0, 2>(tmem + cR1, tmem + cSH, k_rows, id_k, false);
-      issue_ts<0, 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
-      issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
-      issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
-      if (D == 128) {
-        wait(bars.s_ready[1], it & 1);
+      for (int pos = p0; pos < p1; ++pos, ++it) {
+        const int st = it & 1;
+        const uint32_t base = sb + st * L::kStage;
+        const KMajor k_rows(base + L::K, 8192), q_rows(base + L::Q, 8192);
+        const MNMajor k_cols(base + L::K, 8192), q_cols(base + L::Q, 8192);
+        wait(bars.full[st], (it >> 1) & 1);
+        if (pos == rp) wait_tail(st);
+        // key channels in the order in which the chain hands them over: quarters 0 and 2, then 1 and 3
+        wait(bars.s_ready[0], it & 1);
         tc_fence_after();
-        issue_ts<2, 4>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
-        issue_ts<2, 4>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
-        issue_ts<6, 8>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
-        issue_ts<6, 8>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
-      }
-      mma_commit(smem_u32(&bars.ks_done));
-      if (MODE == kOut) {
-        if (it > 0) wait(bars.out_free, (it - 1) & 1);
+        constexpr int H4 = D / 32;  // steps of half the key channels
+        issue_ts<0, 2>(tmem + cR1, tmem + cSH, k_rows, id_k, false);
+        issue_ts<0, 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+        issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+        issue_ts<H4, H4 + 2>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+        if (D == 128) {
+          wait(bars.s_ready[1], it & 1);
+          tc_fence_after();
+          issue_ts<2, 4>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+          issue_ts<2, 4>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+          issue_ts<6, 8>(tmem + cR1, tmem + cSH, k_rows, id_k, true);
+          issue_ts<6, 8>(tmem + cR1, tmem + cSL, k_rows, id_k, true);
+        }
+        mma_commit(smem_u32(&bars.ks_done));
+        if (MODE == kOut) {
+          if (it > 0) wait(bars.out_free, (it - 1) & 1);
+          tc_fence_after();
+          issue_ts<0, D / 16>(tmem + cR2, tmem + cSH, q_rows, id_k, false);
+          issue_ts<0, D / 16>(tmem + cR2, tmem + cSL, q_rows, id_k, true);
+        }
+        if (REV) {  // dO^T P T
+          const MNMajor dO(base + L::V, 8192);
+          issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 8192, 0), id_a64, false);
+          issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 16384 + 8192, 0), id_a64, true);
+        }
+        wait(bars.x_ready, it & 1);
         tc_fence_after();
-        issue_ts<0, D / 16>(tmem + cR2, tmem + cSH, q_rows, id_k, false);
-        issue_ts<0, D / 16>(tmem + cR2, tmem + cSL, q_rows, id_k, true);
-      }
-      if (REV) {  // dO^T P T
-        const MNMajor dO(base + L::V, 8192);
-        issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 8192, 0), id_a64, false);
-        issue_ss<0, 4>(tmem + cR2, dO, MNMajor(base + L::T + 16384 + 8192, 0), id_a64, true);
-      }
-      wait(bars.x_ready, it & 1);
-      tc_fence_after();
-      if (REV) {
-        const MNMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
-        issue_ts<0, 4>(tmem + cR2, tmem + cXH, th, id_mn, true);
-        issue_ts<0, 4>(tmem + cR2, tmem + cXH, tl, id_mn, true);
-        issue_ts<0, 4>(tmem + cR2, tmem + cXL, th, id_mn, true);
-        mma_commit(smem_u32(&bars.u_done));
-        wait(bars.qs_ready, it & 1);
+        if (REV) {
+          const MNMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
+          issue_ts<0, 4>(tmem + cR2, tmem + cXH, th, id_mn, true);
+          issue_ts<0, 4>(tmem + cR2, tmem + cXH, tl, id_mn, true);
+          issue_ts<0, 4>(tmem + cR2, tmem + cXL, th, id_mn, true);
+          mma_commit(smem_u32(&bars.u_done));
+          wait(bars.qs_ready, it & 1);
+          tc_fence_after();
+          issue_ts<0, 4>(tmem + cS, tmem + cR3, q_cols, id_u, true);
+          issue_ts<0, 4>(tmem + cS, tmem + cR3 + 32, q_cols, id_u, true);
+        } else {
+          const KMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
+          issue_ts<0, 4>(tmem + cR1, tmem + cXH, th, id_k, false);
+          issue_ts<0, 4>(tmem + cR1, tmem + cXH, tl, id_k, true);
+          issue_ts<0, 4>(tmem + cR1, tmem + cXL, th, id_k, true);
+          mma_commit(smem_u32(&bars.u_done));
+        }
+        if (MODE == kOut) {
+          const KMajor ph(base + L::T + 8192, 0), pl(base + L::T + 16384 + 8192, 0);
+          issue_ts<0, 4>(tmem + cR3, tmem + cXH, ph, id_k, false);
+          issue_ts<0, 4>(tmem + cR3, tmem + cXH, pl, id_k, true);
+          issue_ts<0, 4>(tmem + cR3, tmem + cXL, ph, id_k, true);
+          mma_commit(smem_u32(&bars.o_done));
+        }
+        wait(bars.up_ready, it & 1);
         tc_fence_after();
-        issue_ts<0, 4>(tmem + cS, tmem + cR3, q_cols, id_u, true);
-        issue_ts<0, 4>(tmem + cS, tmem + cR3 + 32, q_cols, id_u, true);
-      } else {
-        const KMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
-        issue_ts<0, 4>(tmem + cR1, tmem + cXH, th, id_k, false);
-        issue_ts<0, 4>(tmem + cR1, tmem + cXH, tl, id_k, true);
-        issue_ts<0, 4>(tmem + cR1, tmem + cXL, th, id_k, true);
-        mma_commit(smem_u32(&bars.u_done));
+        const uint32_t up = tmem + (MODE == kOut ? cSH : cXH);
+        issue_ts<0, 4>(tmem + cS, up, k_cols, id_u, true);
+        issue_ts<0, 4>(tmem + cS, up + 32, k_cols, id_u, true);
+        mma_commit(smem_u32(&bars.s_done));
+        mma_commit(smem_u32(&bars.empty[st]));
       }
-      if (MODE == kOut) {
-        const KMajor ph(base + L::T + 8192, 0), pl(base + L::T + 16384 + 8192, 0);
-        issue_ts<0, 4>(tmem + cR3, tmem + cXH, ph, id_k, false);
-        issue_ts<0, 4>(tmem + cR3, tmem + cXH, pl, id_k, true);
-        issue_ts<0, 4>(tmem + cR3, tmem + cXL, ph, id_k, true);
-        mma_commit(smem_u32(&bars.o_done));
-      }
-      wait(bars.up_ready, it & 1);
-      tc_fence_after();
-      const uint32_t up = tmem + (MODE == kOut ? cSH : cXH);
-      issue_ts<0, 4>(tmem + cS, up, k_cols, id_u, true);
-      issue_ts<0, 4>(tmem + cS, up + 32, k_cols, id_u, true);
-      mma_commit(smem_u32(&bars.s_done));
-      mma_commit(smem_u32(&bars.empty[st]));
-    }
     }
   }
   tc_fence_before();
@@ -1042,7 +1046,6 @@ __global__ void __launch_bounds__(kScanThreads, 1)
   else
     scan_cta<D, BF, kStore>(a, store, blockIdx.x - a.ranges);
 }
-
 
 template <int D>
 constexpr uint32_t prep_smem() {
@@ -1097,7 +1100,7 @@ cudaError_t run_prep(const Args &a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(prep_kernel<D, BF>, prep_smem<D>(), done);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(prep_kernel<D, BF>, dim3((unsigned)a.max_chunks, (unsigned)a.p.H), dim3(kThreads), prep_smem<D>(), st,
+  e = launch_kernel(prep_kernel<D, BF>, dim3((unsigned)a.max_chunks, (unsigned)a.p.H), dim3(kPrepThreads), prep_smem<D>(), st,
                     a.p.cu_seqlens != nullptr, a);
   count_launches(1);
   return e;

@@ -1,13 +1,6 @@
 // Pieces shared by the gated delta rule's kernels: arguments, sequence and chunk
 // bookkeeping, tile loads, the two-term operand split, and MMA issue.
 //
-// Every kernel is one CTA of 256 threads that alternates between tcgen05 products
-// issued by one thread and epilogues by all: thread t owns tensor-memory lane t % 128
-// (an output row) and one half (t / 128) of the columns, so per-token factors are
-// per-thread scalars.  Products have M = 128: the 64 rows of a chunk's k tile are
-// stacked on the 64 of its q tile (and T on P T, dX on dO), or, for the state, rows
-// are the key channels.
-//
 // Two-term operands.  A value x that is not an input is handed to the tensor cores as
 // hi + lo, hi = round16(x), lo = round16(x - hi): 16 bits of mantissa in bf16, 22 in
 // fp16, against 8 and 11 in one term.  A product of two such values is issued as
@@ -31,7 +24,6 @@ namespace delta {
 using namespace kda::tc;
 
 constexpr int kChunk = 64;
-constexpr int kThreads = 256;
 constexpr int kImgT = 32768;  // T / PT image of a (chunk, head): [128 x 64] hi, then lo
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
@@ -122,27 +114,17 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool l
 }
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// `rows` live rows (of 64) of a [T, D] view at `base` into tile rows [row0, row0 + 64)
-// of D/64 swizzled [128 x 64] blocks `block` bytes apart; rows past `rows` become zeros.
-template <int D>
-__device__ __forceinline__ void load_rows(uint32_t tile, int row0, uint32_t block, const uint16_t *base, int64_t stride_t,
-                                          int rows) {
+// `rows` live rows (of 64) of a [T, D] view at `base` into rows [row0, row0 + 64) of D/64
+// swizzled [128 x 64] blocks, by THREADS threads; rows past `rows` become zeros.
+template <int D, int THREADS>
+__device__ __forceinline__ void load_rows(uint32_t tile, int row0, const uint16_t *base, int64_t stride_t, int rows) {
   constexpr int P = D / 8;
 #pragma unroll
-  for (int i = 0; i < 64 * P / kThreads; ++i) {
-    const int p = threadIdx.x + i * kThreads, r = p / P, c = p % P, tr = row0 + r;
+  for (int i = 0; i < 64 * P / THREADS; ++i) {
+    const int p = threadIdx.x + i * THREADS, r = p / P, c = p % P, tr = row0 + r;
     const bool live = r < rows;
-    cp_async16(tile + (c >> 3) * block + tr * 128 + (((c & 7) ^ (tr & 7)) << 4), base + (live ? r * stride_t : 0) + c * 8,
-               live);
+    cp_async16(tile + (c >> 3) * 16384 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4), base + (live ? r * stride_t : 0) + c * 8, live);
   }
-}
-
-// Bring the 128-byte lines of `rows` rows of a [T, D] view into L2 ahead of their loads.
-template <int D>
-__device__ __forceinline__ void prefetch_rows(const uint16_t *base, int64_t stride_t, int rows) {
-  constexpr int LINES = D / 64;
-  const int r = threadIdx.x / LINES, c = threadIdx.x % LINES;
-  if (r < rows) asm volatile("prefetch.global.L2 [%0];" ::"l"(base + r * stride_t + c * 64));
 }
 
 // Announce bytes to an mbarrier's phase without arriving on it.
@@ -205,30 +187,6 @@ __device__ __forceinline__ void store_split16(uint32_t hi_tile, uint32_t lo_tile
     sts(lo_tile + at, l);
   }
 }
-// 32 columns (chunks 4*half ..) of a row into the hi and lo tiles
-template <bool BF>
-__device__ __forceinline__ void store_split32(uint32_t hi_tile, uint32_t lo_tile, int row, int half, const float (&x)[32]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint4 h, l;
-    split8<BF>(x + 8 * c, h, l);
-    const uint32_t at = chunk_at(row, 4 * half + c);
-    sts(hi_tile + at, h);
-    sts(lo_tile + at, l);
-  }
-}
-// the same into an image in global memory
-template <bool BF>
-__device__ __forceinline__ void store_split32(char *hi_tile, char *lo_tile, int row, int half, const float (&x)[32]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint4 h, l;
-    split8<BF>(x + 8 * c, h, l);
-    const uint32_t at = chunk_at(row, 4 * half + c);
-    *reinterpret_cast<uint4 *>(hi_tile + at) = h;
-    *reinterpret_cast<uint4 *>(lo_tile + at) = l;
-  }
-}
 template <bool BF>
 __device__ __forceinline__ void unpack8(const uint4 &v, float *f) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -238,13 +196,6 @@ __device__ __forceinline__ void unpack8(const uint4 &v, float *f) {
     f[2 * i] = p.x;
     f[2 * i + 1] = p.y;
   }
-}
-template <bool BF>
-__device__ __forceinline__ void store_row32(uint16_t *dst, const float (&x)[32]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    reinterpret_cast<uint4 *>(dst)[c] = make_uint4(pack2(x[8 * c], x[8 * c + 1], BF), pack2(x[8 * c + 2], x[8 * c + 3], BF),
-                                                   pack2(x[8 * c + 4], x[8 * c + 5], BF), pack2(x[8 * c + 6], x[8 * c + 7], BF));
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&x)[32]) {
   uint32_t r[32];
@@ -264,13 +215,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&x)[16]) 
   for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(x[i]);
   tmem_st_32x32b_x16(taddr, r);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&x)[32]) {
-  uint32_t r[32];
-#pragma unroll
-  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(x[i]);
-  tmem_st_32x32b_x32(taddr, r);
-}
-
 // -------------------------------------------------------------- MMA issue --
 // Operand views of a swizzled tile: K-major (rows are M or N, 64-column blocks `block`
 // bytes apart along K) or MN-major (rows are K, 64-column blocks `block` bytes apart
@@ -363,7 +307,7 @@ __device__ __forceinline__ void cta_end(uint32_t tmem, uint32_t cols) {
   if (threadIdx.x < 32) tmem_dealloc(tmem, cols);
 }
 // Writes of this thread to shared and tensor memory before the barrier are seen by the
-// products that thread 0 issues after it.
+// products issued after it.
 __device__ __forceinline__ void publish() {
   fence_async_smem();
   tc_fence_before();

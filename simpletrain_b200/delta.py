@@ -101,6 +101,8 @@ def _check_chunk(q, k, v, g, beta, initial_state, cu_seqlens):
             raise ValueError(f"cu_seqlens packs sequences into one row: the batch must be 1, got {B}")
         if cu_seqlens.shape[0] < 1:
             raise ValueError("cu_seqlens needs at least one offset")
+        if T > 1 << 24:
+            raise ValueError(f"a packed row holds at most 2^24 tokens, got {T}")
         n = cu_seqlens.shape[0] - 1
     if initial_state is not None:
         if initial_state.shape != (n, H, D, D):
@@ -123,7 +125,7 @@ def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     the decay is 0 in fp32 already).  ``scale`` defaults to ``D ** -0.5``.
 
     ``cu_seqlens`` (int32 or int64, ``[n + 1]``, on the device, with B == 1) packs
-    n sequences into the row: sequence i is tokens ``cu_seqlens[i]`` to
+    n sequences into the row (of at most 2^24 tokens): sequence i is tokens ``cu_seqlens[i]`` to
     ``cu_seqlens[i + 1]`` and starts from ``initial_state[i]``.  Sequences may be
     empty; tokens outside all of them get zero outputs and zero gradients.
     Offsets out of order or range are clamped and set a bit of

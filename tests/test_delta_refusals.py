@@ -41,6 +41,9 @@ def test_chunk_refusals_of_packed_sequences():
     a = chunk_args(B=1)
     with pytest.raises(ValueError):
         gated_delta_chunk(**a, cu_seqlens=torch.zeros(0, dtype=torch.int32))
+    long = {n: t[:, :, :1].expand(t.shape[0], t.shape[1], 2 ** 24 + 1, *t.shape[3:]) for n, t in a.items()}
+    with pytest.raises(ValueError, match="2.24"):
+        gated_delta_chunk(**long, cu_seqlens=torch.tensor([0, 5]))
     with pytest.raises(ValueError):  # three sequences, one state
         gated_delta_chunk(**a, cu_seqlens=torch.tensor([0, 1, 2, 5]), initial_state=torch.zeros(1, 4, 64, 64))
 
@@ -119,6 +122,7 @@ def delta_params(**kw):
     (dict(H=70000, Hk=70000), _ffi.KDA_ERR_BAD_SHAPE),
     (dict(B=2, cu_seqlens=0x10000, nseq=1), _ffi.KDA_ERR_BAD_SHAPE),
     (dict(cu_seqlens=0x10000, nseq=-1), _ffi.KDA_ERR_BAD_SHAPE),
+    (dict(T=2 ** 24 + 1, cu_seqlens=0x10000, nseq=1), _ffi.KDA_ERR_BAD_SHAPE),
     (dict(q=_ffi.KdaTensor(0x10008, 64, 64, 64, 1)), _ffi.KDA_ERR_BAD_LAYOUT),
     (dict(v=_ffi.KdaTensor(0x10000, 64, 64, 60, 1)), _ffi.KDA_ERR_BAD_LAYOUT),
     (dict(k=_ffi.KdaTensor(None, 64, 64, 64, 1)), _ffi.KDA_ERR_NULL_ARGUMENT),
@@ -143,8 +147,9 @@ def test_delta_workspace_sizes():
     one = delta_params()
     f, b = lib.kda_delta_fwd_workspace_bytes(ctypes.byref(one)), lib.kda_delta_bwd_workspace_bytes(ctypes.byref(one))
     assert 0 < f < b
-    packed = delta_params(cu_seqlens=0x10000, nseq=7)  # 64 tokens in 7 sequences: at most 8 chunks
-    assert lib.kda_delta_fwd_workspace_bytes(ctypes.byref(packed)) >= 8 * (f - 512)
+    # 64 tokens in n sequences are at most 1 + n chunks, each with 32 KB of T and P T
+    few, many = (lib.kda_delta_fwd_workspace_bytes(ctypes.byref(delta_params(cu_seqlens=0x10000, nseq=n))) for n in (7, 15))
+    assert few >= 8 * 32768 and many - few >= 8 * 32768
     assert lib.kda_delta_fwd_workspace_bytes(ctypes.byref(delta_params(D=96))) == 0
 
 
