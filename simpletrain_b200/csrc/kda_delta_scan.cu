@@ -127,10 +127,13 @@ __device__ __forceinline__ void inverse_level(float *As, float *Ti) {
 // The products are k.k, q.k and P T; (I + A)^-1 is by halves in fp32: four 16 x 16 blocks
 // by substitution, a column a thread, then [A 0; B C]^-1 = [a 0; -c B a, c] twice.
 // The q.k rows wait in tensor memory while the inverse is formed, so that the k and q tiles, the
-// fp32 matrices and the two-term tiles can take turns in 34 KB, and four CTAs share an SM:
-// the kernel is a chain of short dependent steps, hidden by other CTAs only.  Measured:
-// 107 us for the 8192 (chunk, head) cells of 8 x 8192 tokens, 8 heads of 128 (64 KB of k, q and images a
-// cell: 5.0 TB/s); 128 threads a CTA and six CTAs an SM came to the same.
+// fp32 matrices and the two-term tiles can take turns in 34 KB, and four CTAs share an SM: a cell is a
+// chain of short dependent steps, hidden by other CTAs only.
+//
+// Measured: 110 us for 16 x 2048 tokens, 10 heads of 128 (5120 cells, 64 KB of k, q and images each:
+// 3.1 TB/s).  The shared-memory pipe sets that (77% of its cycles taken, the tensor pipe 13%): 128 threads a
+// CTA and six CTAs an SM, persistent CTAs that load the next cell under this one, and half the loads
+// in the inverse's upper level all came to the same time.
 constexpr int kPrepThreads = 256;
 
 template <int D, bool BF>
