@@ -133,9 +133,9 @@ __device__ __forceinline__ float vec_max(const uint4 &v) {
 // Elements below kMask raised to it (NaN stays NaN): what a mask leaves (-inf, a type's lowest
 // value) has probability 0, and 0 * (y - m) must be 0 and not NaN.  bf16 does that in pairs; fp16
 // ends at -65504, which is a value like others, so it is done after the conversion.
-__device__ __forceinline__ float floor1(float x) {
+__device__ __forceinline__ float floor1(float x, float low = kMask) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(kMask));
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(low));
   return r;
 }
 template <int DT, int N>
@@ -568,8 +568,9 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   const float a = !counted ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
   const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r], l2 = lse * kLog2e;
   const float base = -a - b * H, slope = -b * kLn2;
+  const float low = (l2 + kFloor) / g.c;  // p is 0 from here down, where slope * d might overflow
   auto grad = [&](int64_t i, float x) {
-    const float d = fmaf(floor1(x), g.c, -l2), p = ex2(d);
+    const float d = fmaf(floor1(x, low), g.c, -l2), p = ex2(d);
     float v = p * fmaf(slope, d, base);
     if (i == tok) v += a;
     return empty ? 0.f : v;

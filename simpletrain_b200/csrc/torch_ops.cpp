@@ -21,6 +21,7 @@
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -352,6 +353,8 @@ Tensor delta_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Te
   TORCH_CHECK(state.numel() == 0 ||
                   (state.stride(3) == 1 && state.stride(2) == D && state.stride(0) % 4 == 0 && state.stride(1) % 4 == 0 &&
                    (state.size(0) == 1 || state.stride(0) >= D * D) && (H == 1 || state.stride(1) >= D * D) &&
+                   (state.size(0) == 1 || H == 1 || state.stride(0) >= H * state.stride(1) ||
+                    state.stride(1) >= state.size(0) * state.stride(0)) &&
                    reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0),
               "state is updated in place: each [D, D] must be contiguous, 16-byte aligned and apart from the others");
   c10::cuda::CUDAGuard guard(q_.device());
@@ -540,6 +543,21 @@ bool recorded(std::initializer_list<const Tensor *> ts) {
   return false;
 }
 
+// Gradients that cannot be differentiated again: under create_graph they carry an error for whoever tries.
+variable_list once(variable_list grads, const char *what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list live;
+  for (Tensor &g : grads)
+    if (g.defined()) live.push_back(g.detach().set_requires_grad(true));
+  const auto error = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " can be differentiated once only", (int64_t)live.size());
+  live = (*error)(std::move(live));
+  size_t i = 0;
+  for (Tensor &g : grads)
+    if (g.defined()) g = live[i++];
+  return grads;
+}
+
 optional<Tensor> if_defined(const Tensor &t) { return t.defined() ? optional<Tensor>(t) : c10::nullopt; }
 
 const auto &delta_fwd_op() {
@@ -575,10 +593,11 @@ struct DeltaFunction : public torch::autograd::Function<DeltaFunction> {
                              const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &, double,
                              const optional<Tensor> &, const optional<Tensor> &, const Tensor &, const optional<Tensor> &,
                              bool)>();
+    at::AutoDispatchBelowADInplaceOrView below;
     auto [dq, dk, dv, dg, db, ds0] =
         op.call(t[0], t[1], v, t[3], t[4], ctx->saved_data["scale"].toDouble(), if_defined(t[5]), if_defined(t[6]), dout,
                 state ? optional<Tensor>(grads[1]) : c10::nullopt, need_ds0);
-    return {dq, dk, dv, dg, db, Tensor(), need_ds0 ? ds0 : Tensor(), Tensor(), Tensor()};
+    return once({dq, dk, dv, dg, db, Tensor(), need_ds0 ? ds0 : Tensor(), Tensor(), Tensor()}, "gated_delta_chunk");
   }
 };
 
@@ -637,9 +656,11 @@ struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
                          .findSchemaOrThrow("st_b200::token_logprobs_bwd", "")
                          .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
                                        const Tensor &, double, int64_t)>();
-    return {op.call(t[0], t[1], t[2], t[3], dlp, dent, ctx->saved_data["temperature"].toDouble(),
-                    ctx->saved_data["ignore_index"].toInt()),
-            Tensor(), Tensor(), Tensor(), Tensor()};
+    at::AutoDispatchBelowADInplaceOrView below;
+    return once({op.call(t[0], t[1], t[2], t[3], dlp, dent, ctx->saved_data["temperature"].toDouble(),
+                         ctx->saved_data["ignore_index"].toInt()),
+                 Tensor(), Tensor(), Tensor(), Tensor()},
+                "token_logprobs");
   }
 };
 

@@ -285,6 +285,23 @@ def test_gradients_against_differences():
         assert (diff - (grad.double() * d.double()).sum()).abs() <= allowed, name
 
 
+def test_second_derivatives_are_refused():
+    from simpletrain_b200 import gated_delta_chunk
+    from simpletrain_b200.fused_ops import token_logprobs
+    x = make(1, 2, 1, 70, 64, torch.bfloat16, torch.float32, state=True)
+    leaf = [x[n].requires_grad_(True) for n in NAMES]
+    logits = torch.randn(3, 50, device=DEV, requires_grad=True)
+    for out, wrt in ((gated_delta_chunk(*leaf, initial_state=x["s0"])[0].float().square().sum(), leaf),
+                     (token_logprobs(logits, torch.zeros(3, dtype=torch.long, device=DEV)).logprob.square().sum(), [logits])):
+        plain = torch.autograd.grad(out, wrt, retain_graph=True)
+        again = torch.autograd.grad(out, wrt, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, again))
+        with pytest.raises(RuntimeError):  # the gradient is no function of the inputs
+            torch.autograd.grad(again[0].float().sum(), wrt[0], retain_graph=True)
+        with pytest.raises(RuntimeError, match="once"):
+            again[0].float().sum().backward()
+
+
 @pytest.mark.parametrize("T,B", [(0, 2), (5, 0)])
 def test_empty(T, B):
     from simpletrain_b200 import gated_delta_chunk
@@ -414,6 +431,11 @@ def test_step_on_a_strided_pool_and_bad_indices():
     assert (o[1] == 0).all() and (o[3] == 0).all()
     with pytest.raises(RuntimeError):  # one state for all rows cannot be updated in place
         gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], layers[:1, 0].expand(4, 2, 64, 64))
+    flat = torch.zeros(9 * 64 * 64, device=DEV)
+    with pytest.raises(RuntimeError, match="apart"):  # head 1 of a state is head 0 of the next
+        gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], flat.as_strided((6, 2, 64, 64), (4096, 4096, 64, 1)))
+    by_head = flat[:2 * 4 * 4096].view(2, 4, 64, 64).transpose(0, 1)  # [heads, states] memory
+    assert gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], by_head).shape == (4, 2, 64)
 
 
 def test_prefill_steps_and_scores_agree():

@@ -103,6 +103,16 @@ def test_masked_logits_rows_and_padding():
     assert torch.isnan(r.logprob[5]) and torch.isfinite(r.entropy[5])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masks_at_a_low_temperature(dtype):
+    """A masked logit's gradient is 0 whatever 1 / temperature and the upstream gradient are."""
+    x, tok, a, b = make(4, 3001, dtype, seed=5)
+    x = (x.float() * 1e-4).to(dtype)
+    x[:, 100:] = -torch.inf
+    x[1, 100:] = torch.finfo(dtype).min
+    check(x, tok % 100, a, 1e6 * b, 1e-4)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_lowest_values_as_masks(dtype):
     """A mask may be the type's lowest value; in fp16 that is a logit like others."""
