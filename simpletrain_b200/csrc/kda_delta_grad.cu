@@ -21,6 +21,11 @@
 // depend on the launch.  The tiles of one value head fill an SM's shared memory, so the
 // next head's are brought into L2 meanwhile; 16 warps, a token row and a quarter of the
 // columns a thread, work off the products.
+//
+// Measured: 450 us for 16 x 2048 tokens, 10 heads of 128 (5120 cells of 288 KB: 3.4 TB/s, 25,000
+// cycles a cell).  One value head's tiles are all that fit, so copies, products and what the threads make of them
+// follow one another; what can overlap does (prefetch into L2, terms through the state under
+// the second products).  Holding k and q rows in registers to free room for the next tiles spilled (514 us).
 #include "kda_delta_tc.cuh"
 
 namespace kda {

@@ -351,6 +351,12 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // Warps: 8 walk the dependent chain (a value channel a thread, half the columns each), 4
 // turn finished tiles into output or workspace rows, one starts the loads, one issues the
 // products.  TMA brings the tiles two chunks ahead.
+//
+// Measured at D = 128: 2.5 us a chunk (4600 cycles) with outputs, whatever the number of streams up
+// to one an SM (28 streams of 32768 tokens: 1.29 ms).  It is latency: three dependent products with a
+// tensor-memory round trip, a conversion to two terms and two barriers each (state conversion 970 cycles, K S 820,
+// X 540, T X 610, U 620, update 650).  16 x 2048 tokens of 10 heads (160 streams on 148 SMs): outputs 118 us
+// (503 MB, 4.3 TB/s), states and u rows 148 us (755 MB, 5.1 TB/s), reverse 206 us (983 MB, 4.8 TB/s).
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
 constexpr int kScanThreads = 448;
