@@ -563,7 +563,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
     for (uint64_t *b : {&bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
     for (uint64_t *b : {&bars.ks_done, &bars.u_done, &bars.s_done, &bars.o_done}) mbar_init(smem_u32(b), 1);
     mbar_init(smem_u32(&bars.out_free), Q);
-    mbar_init(smem_u32(&bars.qs_ready), Q);
+    mbar_init(smem_u32(&bars.qs_ready), 2 * Q);
     mbar_fence_init();
     abort_flag = 0;
     // ranges that are whole streams need no order
@@ -701,6 +701,19 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             tmem_wait_st();
             arrive_warp(bars.x_ready);
           }
+          if (REV) {  // Q' product's first operand, scale e^gamma dO transposed, under the product with T
+            const uint32_t vt = sb + st * L::kStage + L::V + half * 4096;
+            float x[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              uint16_t u;
+              asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + vcol[j & 7] + (j >> 3) * 1024));
+              x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * half + j];
+            }
+            tmem_split32<BF>(tl + cR3 + 16 * half, tl + cR3 + 32 + 16 * half, x);
+            tmem_wait_st();
+            arrive_warp(bars.qs_ready);
+          }
           wait(bars.u_done, it & 1);
           tc_fence_after();
           {
@@ -803,25 +816,8 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             store_tile(sb + L::OUT, pos);
             if (t == 0) tma_store_commit();
           } else {
-            if (REV) {  // Q' product's first operand: scale e^gamma dO, transposed, in two terms
-              wait_full(pos);
-              if (it > 0) wait(bars.s_done, (it - 1) & 1);  // the last one is used
-              const uint32_t vt = sb + st * L::kStage + L::V + (row >> 6) * 8192 + (row & 7) * 2;
-#pragma unroll
-              for (int b = 0; b < 2; ++b) {
-                float x[32];
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  uint16_t u;
-                  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + (32 * b + j) * 128 + ((((row >> 3) ^ j) & 7) << 4)));
-                  x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * b + j];
-                }
-                tmem_split32<BF>(tl + cR3 + 16 * b, tl + cR3 + 32 + 16 * b, x);
-              }
-              tmem_wait_st();
-              arrive_warp(bars.qs_ready);
-            }
-            // the state (reverse: its gradient) as the chain split it
+            if (REV) wait_full(pos);  // for the factors
+          // the state (reverse: its gradient) as the chain split it
             char *img = (REV ? a.w.dS : a.w.S) + cell(pos) * (size_t)(D * D * 4) + row * 16;
 #pragma unroll
             for (int b = 0; b < NB; ++b) wait(bars.s_ready[b], it & 1);
