@@ -356,7 +356,9 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // to one an SM (28 streams of 32768 tokens: 1.29 ms).  It is latency: three dependent products with a
 // tensor-memory round trip, a conversion to two terms and two barriers each (state conversion 970 cycles, K S 820,
 // X 540, T X 610, U 620, update 650).  16 x 2048 tokens of 10 heads (160 streams on 148 SMs): outputs 118 us
-// (503 MB, 4.3 TB/s), states and u rows 148 us (755 MB, 5.1 TB/s), reverse 206 us (983 MB, 4.8 TB/s).
+// (503 MB, 4.3 TB/s), states and u rows 148 us (755 MB, 5.1 TB/s), reverse 199 us (983 MB, 4.9 TB/s; its start
+// under the end of the one before is in that).  dO becomes an operand in the chain's wait for its
+// product with T: in the output warps that took 2000 to 3000 cycles a chunk and made them the slowest.
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
 constexpr int kScanThreads = 448;
@@ -1042,7 +1044,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_cons
   scan_cta<D, BF, MODE>(a, maps, blockIdx.x);
 }
 
-// The backward's two scans side by side, where there are SMs for both: neither needs the other.
+// The backward's two scans side by side, where there are SMs for both: neither needs the other.  (On
+// half of the SMs each where there are not, they took longer: 1210 against 1170 us for 16 x 2048 tokens' step.)
 template <int D, bool BF>
 __global__ void __launch_bounds__(kScanThreads, 1)
     scan_pair_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps store, const __grid_constant__ Maps rev) {

