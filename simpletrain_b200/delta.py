@@ -132,7 +132,7 @@ def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     ``device_status()``.  ``initial_state``: float32 ``[n or B, H, D, D]`` or None
     (zeros); ``final_state`` has that shape.
 
-    Differentiable in q, k, v, g, beta and initial_state, through o and
+    Differentiable (once) in q, k, v, g, beta and initial_state, through o and
     final_state; gradients of shared heads are summed in a fixed order.  A NaN or
     infinity in a token reaches its own 64-token chunk and what follows in its
     sequence (earlier tokens of the chunk too), and no other sequence.

@@ -414,6 +414,24 @@ def test_step(N, H, Hk, D, states, dtype, gate, slots, index):
         assert torch.equal(a["state"][s], before[s])
 
 
+def test_inference_mode_and_in_place_counting():
+    """Inference tensors are taken; an ordinary pool's version moves with every step, so a graph that saved it notices."""
+    from simpletrain_b200 import gated_delta_chunk, gated_delta_step
+    a = step_inputs(3, 2, 1, 64, 4, torch.bfloat16)
+    want = a["state"].clone()
+    o = gated_delta_step(*(a[n] for n in NAMES), want)
+    with torch.inference_mode():
+        b = {n: t.clone() for n, t in a.items()}
+        assert torch.equal(gated_delta_step(*(b[n] for n in NAMES), b["state"]), o) and torch.equal(b["state"], want)
+        x = [b[n].transpose(0, 1)[None] for n in NAMES]
+        assert gated_delta_chunk(*x)[0].shape == (1, 2, 3, 64)
+    w = torch.ones(4, 2, 64, 64, device=DEV, requires_grad=True)
+    loss = (w * a["state"]).sum()
+    gated_delta_step(*(a[n] for n in NAMES), a["state"])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_step_on_a_strided_pool_and_bad_indices():
     from simpletrain_b200 import _ffi, device_status, gated_delta_step
     a = step_inputs(4, 2, 2, 64, 6, torch.bfloat16)
