@@ -16,6 +16,7 @@
 // and the scans, which are sequential in the chunks, are left with three dependent
 // products a chunk: with the state, with T (or its transpose), and the state update, which
 // accumulates on the state in tensor memory.
+#include "kda_delta_ranges.h"
 #include "kda_delta_tc.cuh"
 #include "tmap.h"
 
@@ -401,72 +402,9 @@ __device__ __forceinline__ void wait_flag(const int *flag, int32_t *status, vola
   __syncwarp();
 }
 
-// A part of a stream: positions [p0, p1) of its nc chunks (position 0 is the last chunk in reverse).
-struct Piece {
-  int n, h, p0, p1, nc;
-};
-// The pieces of chunks [lo, hi), in the order in which a CTA runs them: the last stream's, the
-// streams between, the first stream's.
-struct Pieces {
-  int n0, h0, c0, nc0, n1, h1, c1;  // streams and positions of the first and the last chunk
-  int turn, n, h;
-  static __device__ __forceinline__ int chunks(const Args &a, int i) {
-    return a.p.cu_seqlens == nullptr ? a.per_seq : a.w.first[i + 1] - a.w.first[i];
-  }
-  static __device__ __forceinline__ void locate(const Args &a, int x, int *sn, int *sh, int *sc) {
-    if (a.p.cu_seqlens == nullptr) {
-      const int s = x / a.per_seq;
-      *sn = s / a.p.H;
-      *sh = s % a.p.H;
-      *sc = x % a.per_seq;
-      return;
-    }
-    int l = 0, r = a.nseq;  // H first[l] <= x < H first[r]
-    while (r - l > 1) {
-      const int mid = (l + r) >> 1;
-      if ((int64_t)a.w.first[mid] * a.p.H <= x) l = mid; else r = mid;
-    }
-    const int nc = chunks(a, l), rem = x - a.w.first[l] * a.p.H;
-    *sn = l;
-    *sh = rem / nc;
-    *sc = rem % nc;
-  }
-  __device__ __forceinline__ void begin(const Args &a, int lo, int hi) {
-    turn = lo < hi ? 0 : 3;
-    if (turn == 3) return;
-    locate(a, lo, &n0, &h0, &c0);
-    locate(a, hi - 1, &n1, &h1, &c1);
-    nc0 = chunks(a, n0);
-  }
-  __device__ __forceinline__ bool next(const Args &a, Piece *p) {
-    if (turn == 0) {
-      const bool one = n0 == n1 && h0 == h1;
-      *p = {n1, h1, one ? c0 : 0, c1 + 1, chunks(a, n1)};
-      turn = one ? 3 : 1;
-      n = n0;
-      h = h0;
-      return true;
-    }
-    if (turn == 1) {  // the next stream that has chunks; the range's last one is not behind us
-      if (++h == a.p.H) {
-        h = 0;
-        do ++n; while (chunks(a, n) == 0);
-      }
-      if (n != n1 || h != h1) {
-        const int nc = chunks(a, n);
-        *p = {n, h, 0, nc, nc};
-        return true;
-      }
-      turn = 2;
-    }
-    if (turn == 2) {
-      *p = {n0, h0, c0, nc0, nc0};
-      turn = 3;
-      return true;
-    }
-    return false;
-  }
-};
+__device__ __forceinline__ Streams streams_of(const Args &a) {
+  return {a.p.cu_seqlens == nullptr ? nullptr : a.w.first, a.per_seq, a.nseq, a.p.H};
+}
 // Each warp keeps its place in shared memory: as registers of every thread it made the chain spill.
 struct WarpPlace {
   Pieces pieces;
@@ -591,14 +529,14 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
 
   pdl_launch_dependents();
   const int range = *reinterpret_cast<volatile int *>(&range_slot);
-  const int64_t total = a.max_chunks == 0 ? 0 : (int64_t)a.p.H * (a.p.cu_seqlens == nullptr ? a.max_chunks : a.w.first[a.nseq]);
-  const int lo = range < a.ranges ? (int)(total * range / a.ranges) : 0, hi = range < a.ranges ? (int)(total * (range + 1) / a.ranges) : 0;
+  int lo, hi;
+  range_of(a.max_chunks == 0 ? 0 : streams_of(a).total(), a.ranges, range, &lo, &hi);
   WarpPlace &place = places[warp];
-  if (lane == 0) place.pieces.begin(a, lo, hi);
+  if (lane == 0) place.pieces.begin(streams_of(a), lo, hi);
   const Piece &pc = place.pc;
   const Seq &s = place.s;
   auto step_piece = [&]() {  // one lane
-    place.more = place.pieces.next(a, &place.pc);
+    place.more = place.pieces.next(streams_of(a), &place.pc);
     if (place.more) place.s = get_seq(a, place.pc.n);
   };
   int p0 = 0, p1 = 0, rp = -1;  // the piece's positions, and that of its stream's ragged chunk

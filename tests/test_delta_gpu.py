@@ -148,6 +148,17 @@ def test_packed_sequences(lens, lead, tail, H, Hk, D, dtype, index):
     compare(got, exp)
 
 
+@pytest.mark.parametrize("lens,H,Hk,D,dtype", [
+    ([128] + [0] * 31, 8, 8, 64, torch.bfloat16),  # offsets padded with empty sequences, as a captured graph has them
+    ([0] * 15 + [200], 10, 5, 128, torch.float16),
+    ([0] * 9 + [129, 0, 0, 70] + [0] * 30, 6, 3, 64, torch.bfloat16),
+])
+def test_packed_with_fewer_chunks_than_ranges(lens, H, Hk, D, dtype):
+    cu, bounds, T = packed(lens)
+    x = make(1, H, Hk, T, D, dtype, torch.float32, seed=13, state=True, n=len(lens))
+    compare(*run_both(x, D, cu, bounds))
+
+
 def test_packed_rows_equal_their_own_calls():
     """A sequence's results do not depend on what it is packed with."""
     from simpletrain_b200 import gated_delta_chunk
