@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define KDA_ABI_VERSION 3
+#define KDA_ABI_VERSION 4
 
 typedef struct CUstream_st *kda_stream_t; /* identical to cudaStream_t */
 

@@ -68,12 +68,13 @@ int st_cross_entropy_bwd(const void *logits, const int64_t *labels, const float 
      top_logprob, top_id [N, top_k] (top_k <= 32, <= V): the top_k largest
                   logits in order, the lower index first among equals, NaN last
    Logits below -1e29 (-infinity, the lowest values of bf16 and f32) are
-   masked: probability 0.  A row of nothing else has lse = logprob = -infinity
+   masked: probability 0.  lse [N] is in double (since ABI version 4): the gradient
+   takes differences with it.  A row of nothing else has lse = logprob = -infinity
    and entropy 0; a NaN or +infinity makes the row's outputs NaN (its top_id
    stay in range). */
 enum { ST_DTYPE_F32 = 2 };
 int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprob, float *entropy,
-                          float *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
+                          double *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
                           float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream);
 
 /* dlogits [N, V] (contiguous, the logits' dtype) from dlogprob and dentropy [N]
@@ -82,7 +83,7 @@ int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t 
    A row whose token is ignore_index has no part through dlogprob; a row of
    nothing but masked logits has gradient 0. */
 int st_token_logprobs_bwd(const void *logits, int64_t row_stride, const int64_t *tokens, const float *entropy,
-                          const float *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
+                          const double *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
                           int64_t V, float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream);
 
 #ifdef __cplusplus

@@ -10,7 +10,7 @@ import ctypes
 import os
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 # KDA_B200_LIB_DIR selects another build of both libraries (default: in-tree _lib/)
 LIB_DIR = os.environ.get("KDA_B200_LIB_DIR") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libkda_sm100.so")

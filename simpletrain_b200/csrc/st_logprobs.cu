@@ -3,7 +3,7 @@
 //
 // Mathematics, in base 2 so that each element costs one ex2: y = c * logit with
 // c = log2(e) / temperature, m = max y, s = sum 2^(y-m), w = sum 2^(y-m) (y-m):
-//   lse = ln2 (m + log2 s)      logprob = ln2 (y_token - m - log2 s)
+//   lse = ln2 (m + log2 s), kept in double for the gradient      logprob = ln2 (y_token - m - log2 s)
 //   entropy = ln2 (log2 s - w / s)
 //   dlogit_v = (a ([v = token] - p_v) - b p_v (ln p_v + entropy)) / temperature
 // One pass over the row keeps a running (m, s, w) per thread, rescaled when a
@@ -45,6 +45,7 @@ constexpr int kTopMax = 32;
 constexpr int kCand = 1024;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr double kLog2eD = 1.4426950408889634, kLn2D = 0.6931471805599453;
 // y - m below this contributes 2^-300 = 0 in fp32; a floor keeps 0 * (y - m) finite for y = -inf
 constexpr float kFloor = -300.f;
 // Logits below kStart are masked: probability 0 (the lowest values of bf16 and fp32 are).  The running
@@ -459,7 +460,8 @@ struct FwdArgs {
   const int64_t *tokens;
   int64_t ignore_index;
   float c;  // log2(e) / temperature
-  float *logprob, *entropy, *lse, *top_logprob;
+  float *logprob, *entropy, *top_logprob;
+  double *lse;
   int64_t *top_id;
   int k;
 };
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 4 : 6) logprobs_fwd_kernel(const
         lp = (fmaf(Elem<DT>::load(row, tok), a.c, -t.m) - l2) * kLn2;
       a.logprob[r] = lp;
       a.entropy[r] = empty ? 0.f : (l2 - t.w / t.s) * kLn2;
-      a.lse[r] = empty ? -INFINITY : (t.m + l2) * kLn2;
+      a.lse[r] = empty ? -INFINITY : ((double)t.m + (double)l2) * kLn2D;
     }
     if (TOP) {
       // candidates: the CTAs' ordered lists, at most 8 x kTopMax = kBlock of them
@@ -553,7 +555,8 @@ struct BwdArgs {
   const int64_t *tokens;
   int64_t ignore_index;
   float c, inv_t;
-  const float *entropy, *lse, *dlogprob, *dentropy;
+  const float *entropy, *dlogprob, *dentropy;
+  const double *lse;
   char *dlogits;  // [N, V] contiguous
 };
 
@@ -565,15 +568,18 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   char *out = g.dlogits + r * g.V * E::kBytes;
   const int64_t tok = g.tokens[r];
   const bool counted = tok != g.ignore_index;
-  const float lse = g.lse[r];
+  // lse in two fp32 terms: p's error is that of the exponent, and one term is off by 2^-24 of lse, which
+  // over a low temperature or with a common offset of the logits is far more than the exponents that count
+  const double lse = g.lse[r] * kLog2eD;
   const bool empty = lse == -INFINITY;
+  const float l2 = (float)lse, l2_low = empty ? 0.f : (float)(lse - (double)l2);
   // a token outside [0, V): its log probability is NaN, and so is the row's gradient through it
   const float a = !counted ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
-  const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r], l2 = lse * kLog2e;
+  const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r];
   const float base = -a - b * H, slope = -b * kLn2;
   const float low = (l2 + kFloor) / g.c;  // p is 0 from here down, where slope * d might overflow
   auto grad = [&](int64_t i, float x) {
-    const float d = fmaf(floor1(x, low), g.c, -l2), p = ex2(d);
+    const float d = fmaf(floor1(x, low), g.c, -l2) - l2_low, p = ex2(d);
     float v = p * fmaf(slope, d, base);
     if (i == tok) v += a;
     return empty ? 0.f : v;
@@ -666,7 +672,7 @@ bool element_aligned(const void *p, int32_t dtype) {
 extern "C" {
 
 int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t *tokens, float *logprob, float *entropy,
-                          float *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
+                          double *lse, float *top_logprob, int64_t *top_id, int32_t top_k, int64_t N, int64_t V,
                           float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream) {
   int rc = check(N, V, row_stride, temperature, dtype);
   if (rc != KDA_OK) return rc;
@@ -698,7 +704,7 @@ int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t 
 }
 
 int st_token_logprobs_bwd(const void *logits, int64_t row_stride, const int64_t *tokens, const float *entropy,
-                          const float *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
+                          const double *lse, const float *dlogprob, const float *dentropy, void *dlogits, int64_t N,
                           int64_t V, float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream) {
   int rc = check(N, V, row_stride, temperature, dtype);
   if (rc != KDA_OK) return rc;

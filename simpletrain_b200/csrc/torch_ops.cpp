@@ -505,10 +505,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &
   c10::cuda::CUDAGuard guard(logits_.device());
   const Tensor logits = logit_rows(logits_), tokens = tokens_.contiguous().to(at::kLong);
   const auto f32 = logits.options().dtype(at::kFloat);
-  Tensor lp = at::empty({N}, f32), ent = at::empty({N}, f32), lse = at::empty({N}, f32);
+  Tensor lp = at::empty({N}, f32), ent = at::empty({N}, f32), lse = at::empty({N}, logits.options().dtype(at::kDouble));
   Tensor top = at::empty({N, top_k}, f32), ids = at::empty({N, top_k}, tokens.options());
   check(st_token_logprobs_fwd(logits.data_ptr(), row_stride(logits), tokens.data_ptr<int64_t>(), lp.data_ptr<float>(),
-                              ent.data_ptr<float>(), lse.data_ptr<float>(), static_cast<float *>(ptr(&top)),
+                              ent.data_ptr<float>(), lse.data_ptr<double>(), static_cast<float *>(ptr(&top)),
                               static_cast<int64_t *>(ptr(&ids)), (int32_t)top_k, N, V, (float)temperature, ignore_index,
                               dt, stream_of(logits)),
         "st_token_logprobs_fwd");
@@ -523,7 +523,7 @@ Tensor token_logprobs_bwd(const Tensor &logits_, const Tensor &tokens_, const Te
                lse = lse_.contiguous(), dlp = dlp_.contiguous().to(at::kFloat), dent = dent_.contiguous().to(at::kFloat);
   Tensor dlogits = at::empty({N, V}, logits.options());
   check(st_token_logprobs_bwd(logits.data_ptr(), row_stride(logits), tokens.data_ptr<int64_t>(), ent.data_ptr<float>(),
-                              lse.data_ptr<float>(), dlp.data_ptr<float>(), dent.data_ptr<float>(), dlogits.data_ptr(), N,
+                              lse.data_ptr<double>(), dlp.data_ptr<float>(), dent.data_ptr<float>(), dlogits.data_ptr(), N,
                               V, (float)temperature, ignore_index, logit_code(logits), stream_of(logits)),
         "st_token_logprobs_bwd");
   return dlogits;
@@ -650,8 +650,8 @@ struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const variable_list t = ctx->get_saved_variables();
-    const Tensor dlp = grads[0].defined() ? grads[0] : at::zeros_like(t[3]);
-    const Tensor dent = grads[1].defined() ? grads[1] : at::zeros_like(t[3]);
+    const Tensor dlp = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
+    const Tensor dent = grads[1].defined() ? grads[1] : at::zeros_like(t[2]);
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("st_b200::token_logprobs_bwd", "")
                          .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,

@@ -179,7 +179,7 @@ class TokenLogprobs(NamedTuple):
 def _(logits, tokens, top_k, temperature, ignore_index):
     N = logits.shape[0]
     f32 = torch.float32
-    return (logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=f32),
+    return (logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=f32), logits.new_empty((N,), dtype=torch.float64),
             logits.new_empty((N, top_k), dtype=f32), logits.new_empty((N, top_k), dtype=torch.int64))
 
 

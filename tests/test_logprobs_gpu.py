@@ -113,6 +113,21 @@ def test_masks_at_a_low_temperature(dtype):
     check(x, tok % 100, a, 1e6 * b, 1e-4)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,offset", [(1e-2, 0.0), (1e-3, 0.0), (1.0, 1e4), (1.0, -1e4), (1e-3, 300.0)])
+def test_gradients_where_the_rows_sum_is_large(dtype, t, offset):
+    """The probabilities keep their last bits when lse is large: logits over a low temperature, logits with a
+    common offset.  A log probability's gradient sums to a (1 - sum p) / t over the row, at most 2^-15 |a| / t."""
+    from simpletrain_b200.fused_ops import token_logprobs
+    x, tok, a, b = make(6, 5003, dtype, seed=7)
+    x = (x.float() + offset).to(dtype)
+    tok[:3] = x[:3].argmax(-1)
+    check(x, tok, a, b, t)
+    leaf = x.float().requires_grad_(True)
+    (dx,) = torch.autograd.grad(token_logprobs(leaf, tok, temperature=t).logprob, leaf, a)
+    assert (dx.double().sum(-1).abs() <= 2.0 ** -15 * a.abs().double() / t).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_lowest_values_as_masks(dtype):
     """A mask may be the type's lowest value; in fp16 that is a logit like others."""
