@@ -68,7 +68,7 @@ int st_cross_entropy_bwd(const void *logits, const int64_t *labels, const float 
      top_logprob, top_id [N, top_k] (top_k <= 32, <= V): the top_k largest
                   logits in order, the lower index first among equals, NaN last
    Logits below -1e29 (-infinity, the lowest values of bf16 and f32) are
-   masked: probability 0.  lse [N] is in double (since ABI version 4): the gradient
+   masked: probability 0, log probability -infinity.  lse [N] is in double (since ABI version 4): the gradient
    takes differences with it.  A row of nothing else has lse = logprob = -infinity
    and entropy 0; a NaN or +infinity makes the row's outputs NaN (its top_id
    stay in range). */

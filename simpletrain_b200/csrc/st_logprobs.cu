@@ -507,6 +507,10 @@ __global__ void __launch_bounds__(kBlock, TOP ? 4 : 6) logprobs_fwd_kernel(const
   if (rank == 0) {
     const float l2 = log2f(t.s);
     const bool empty = t.m <= a.c * kStart && t.s == t.s;  // only masked logits in the row
+    // masked logits have probability 0 at any temperature; the row's NaN comes first
+    auto log_p = [&](float x) {
+      return empty || (x < kStart && l2 == l2) ? -INFINITY : (fmaf(x, a.c, -t.m) - l2) * kLn2;
+    };
     if (tid == 0) {
       const int64_t tok = a.tokens[r];
       float lp;
@@ -514,10 +518,8 @@ __global__ void __launch_bounds__(kBlock, TOP ? 4 : 6) logprobs_fwd_kernel(const
         lp = 0.f;
       else if (tok < 0 || tok >= a.V)
         lp = NAN;
-      else if (empty)
-        lp = -INFINITY;
       else
-        lp = (fmaf(Elem<DT>::load(row, tok), a.c, -t.m) - l2) * kLn2;
+        lp = log_p(Elem<DT>::load(row, tok));
       a.logprob[r] = lp;
       a.entropy[r] = empty ? 0.f : (l2 - t.w / t.s) * kLn2;
       a.lse[r] = empty ? -INFINITY : ((double)t.m + (double)l2) * kLn2D;
@@ -540,7 +542,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 4 : 6) logprobs_fwd_kernel(const
         int pos = 0;
         for (int j = 0; j < n; ++j) pos += before(sh.cand_v[j], sh.cand_i[j], v, id) ? 1 : 0;
         if (pos < a.k && id != 0x7fffffff) {
-          a.top_logprob[r * a.k + pos] = empty ? -INFINITY : (fmaf(v, a.c, -t.m) - l2) * kLn2;
+          a.top_logprob[r * a.k + pos] = log_p(v);
           a.top_id[r * a.k + pos] = id;
         }
       }

@@ -219,7 +219,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, *, top_k: int = 0, temperatur
       order, the lower index first among equal ones; plain tensors without gradient.
 
     Logits below -1e29 (-infinity, the lowest values of bf16 and fp32) are
-    masked, with probability 0.  A row of nothing else has ``logprob = -inf``,
+    masked, with probability 0 and log probability -inf.  A row of nothing else has
     entropy 0 and gradient 0; a NaN or +infinity makes the row's values NaN.  Sums
     are fp32.
     """

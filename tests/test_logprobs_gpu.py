@@ -128,6 +128,20 @@ def test_gradients_where_the_rows_sum_is_large(dtype, t, offset):
     assert (dx.double().sum(-1).abs() <= 2.0 ** -15 * a.abs().double() / t).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t", [0.5, 1.0, 2.0, 100.0])
+def test_a_masked_logit_has_probability_0_at_every_temperature(dtype, t):
+    from simpletrain_b200.fused_ops import token_logprobs
+    x, tok, _, _ = make(3, 2500, dtype, seed=8)
+    x[0, 2:] = torch.finfo(dtype).min
+    x[1, 2:] = -2e29
+    x[2, 2:] = -torch.inf
+    tok[:] = 2
+    r = token_logprobs(x, tok, temperature=t, top_k=4)
+    assert (r.logprob == -torch.inf).all() and (r.top_logprobs[:, 2:] == -torch.inf).all()
+    assert torch.isfinite(r.top_logprobs[:, :2]).all() and torch.isfinite(r.entropy).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_lowest_values_as_masks(dtype):
     """A mask may be the type's lowest value; in fp16 that is a logit like others."""
