@@ -78,7 +78,7 @@ int st_token_logprobs_fwd(const void *logits, int64_t row_stride, const int64_t 
                           float temperature, int64_t ignore_index, int32_t dtype, kda_stream_t stream);
 
 /* dlogits [N, V] (contiguous, the logits' dtype) from dlogprob and dentropy [N]
-   and the forward's entropy and lse:
+   (NULL: zero) and the forward's entropy and lse:
      dlogits_v = (dlogprob ([v == token] - p_v) - dentropy p_v (ln p_v + entropy)) / temperature
    A row whose token is ignore_index has no part through dlogprob; a row of
    nothing but masked logits has gradient 0. */

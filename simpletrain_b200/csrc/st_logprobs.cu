@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   const char *row = g.logits + r * g.row_bytes;
   char *out = g.dlogits + r * g.V * E::kBytes;
   const int64_t tok = g.tokens[r];
-  const bool counted = tok != g.ignore_index;
+  const bool counted = g.dlogprob != nullptr && tok != g.ignore_index;
   // lse in two fp32 terms: p's error is that of the exponent, and one term is off by 2^-24 of lse, which
   // over a low temperature or with a common offset of the logits is far more than the exponents that count
   const double lse = g.lse[r] * kLog2eD;
@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   const float l2 = (float)lse, l2_low = empty ? 0.f : (float)(lse - (double)l2);
   // a token outside [0, V): its log probability is NaN, and so is the row's gradient through it
   const float a = !counted ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
-  const float b = g.dentropy[r] * g.inv_t, H = g.entropy[r];
+  const float b = g.dentropy != nullptr ? g.dentropy[r] * g.inv_t : 0.f, H = g.entropy[r];
   const float base = -a - b * H, slope = -b * kLn2;
   const float low = (l2 + kFloor) / g.c;  // p is 0 from here down, where slope * d might overflow
   auto grad = [&](int64_t i, float x) {
@@ -711,7 +711,7 @@ int st_token_logprobs_bwd(const void *logits, int64_t row_stride, const int64_t 
   int rc = check(N, V, row_stride, temperature, dtype);
   if (rc != KDA_OK) return rc;
   if (N == 0) return KDA_OK;
-  if (!logits || !tokens || !entropy || !lse || !dlogprob || !dentropy || !dlogits) return KDA_ERR_NULL_ARGUMENT;
+  if (!logits || !tokens || !entropy || !lse || !dlogits) return KDA_ERR_NULL_ARGUMENT;
   if (!element_aligned(logits, dtype) || !element_aligned(dlogits, dtype)) return KDA_ERR_BAD_LAYOUT;
   BwdArgs a{};
   a.logits = static_cast<const char *>(logits);

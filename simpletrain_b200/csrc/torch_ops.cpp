@@ -516,15 +516,19 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> token_logprobs(const Tensor &
 }
 
 Tensor token_logprobs_bwd(const Tensor &logits_, const Tensor &tokens_, const Tensor &ent_, const Tensor &lse_,
-                          const Tensor &dlp_, const Tensor &dent_, double temperature, int64_t ignore_index) {
+                          const optional<Tensor> &dlp_, const optional<Tensor> &dent_, double temperature,
+                          int64_t ignore_index) {
   c10::cuda::CUDAGuard guard(logits_.device());
   const int64_t N = logits_.size(0), V = logits_.size(1);
   const Tensor logits = logit_rows(logits_), tokens = tokens_.contiguous().to(at::kLong), ent = ent_.contiguous(),
-               lse = lse_.contiguous(), dlp = dlp_.contiguous().to(at::kFloat), dent = dent_.contiguous().to(at::kFloat);
+               lse = lse_.contiguous();
+  auto upstream = [](const optional<Tensor> &t) { return t.has_value() ? t->contiguous().to(at::kFloat) : Tensor(); };
+  const Tensor dlp = upstream(dlp_), dent = upstream(dent_);
   Tensor dlogits = at::empty({N, V}, logits.options());
   check(st_token_logprobs_bwd(logits.data_ptr(), row_stride(logits), tokens.data_ptr<int64_t>(), ent.data_ptr<float>(),
-                              lse.data_ptr<double>(), dlp.data_ptr<float>(), dent.data_ptr<float>(), dlogits.data_ptr(), N,
-                              V, (float)temperature, ignore_index, logit_code(logits), stream_of(logits)),
+                              lse.data_ptr<double>(), dlp.defined() ? dlp.data_ptr<float>() : nullptr,
+                              dent.defined() ? dent.data_ptr<float>() : nullptr, dlogits.data_ptr(), N, V,
+                              (float)temperature, ignore_index, logit_code(logits), stream_of(logits)),
         "st_token_logprobs_bwd");
   return dlogits;
 }
@@ -650,15 +654,13 @@ struct LogprobsFunction : public torch::autograd::Function<LogprobsFunction> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const variable_list t = ctx->get_saved_variables();
-    const Tensor dlp = grads[0].defined() ? grads[0] : at::zeros_like(t[2]);
-    const Tensor dent = grads[1].defined() ? grads[1] : at::zeros_like(t[2]);
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("st_b200::token_logprobs_bwd", "")
-                         .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &, const Tensor &,
-                                       const Tensor &, double, int64_t)>();
+                         .typed<Tensor(const Tensor &, const Tensor &, const Tensor &, const Tensor &,
+                                       const optional<Tensor> &, const optional<Tensor> &, double, int64_t)>();
     at::AutoDispatchBelowADInplaceOrView below;
-    return once({op.call(t[0], t[1], t[2], t[3], dlp, dent, ctx->saved_data["temperature"].toDouble(),
-                         ctx->saved_data["ignore_index"].toInt()),
+    return once({op.call(t[0], t[1], t[2], t[3], if_defined(grads[0]), if_defined(grads[1]),
+                         ctx->saved_data["temperature"].toDouble(), ctx->saved_data["ignore_index"].toInt()),
                  Tensor(), Tensor(), Tensor(), Tensor()},
                 "token_logprobs");
   }
@@ -688,7 +690,7 @@ TORCH_LIBRARY(st_b200, m) {
       "token_logprobs(Tensor logits, Tensor tokens, int top_k, float temperature, int ignore_index) "
       "-> (Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def(
-      "token_logprobs_bwd(Tensor logits, Tensor tokens, Tensor entropy, Tensor lse, Tensor dlogprob, Tensor dentropy, "
+      "token_logprobs_bwd(Tensor logits, Tensor tokens, Tensor entropy, Tensor lse, Tensor? dlogprob, Tensor? dentropy, "
       "float temperature, int ignore_index) -> Tensor");
 }
 

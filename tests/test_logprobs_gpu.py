@@ -142,6 +142,22 @@ def test_a_masked_logit_has_probability_0_at_every_temperature(dtype, t):
     assert torch.isfinite(r.top_logprobs[:, :2]).all() and torch.isfinite(r.entropy).all()
 
 
+def test_the_entropy_does_not_depend_on_the_token():
+    """A token that names nothing makes its log probability NaN; the entropy alone and its gradient stay what they are."""
+    from simpletrain_b200.fused_ops import token_logprobs
+    x, tok, _, b = make(4, 1500, torch.float32, seed=9)
+    bad = tok.clone()
+    bad[1], bad[2] = -7, 1500
+    got = []
+    for t in (tok, bad):
+        leaf = x.detach().requires_grad_(True)
+        got.append(torch.autograd.grad(token_logprobs(leaf, t).entropy, leaf, b)[0])
+    assert torch.equal(*got)
+    leaf = x.detach().requires_grad_(True)
+    (dx,) = torch.autograd.grad(token_logprobs(leaf, bad).logprob, leaf, b)
+    assert torch.isnan(dx[1:3]).all() and torch.isfinite(dx[0]).all() and torch.isfinite(dx[3]).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_lowest_values_as_masks(dtype):
     """A mask may be the type's lowest value; in fp16 that is a logit like others."""
