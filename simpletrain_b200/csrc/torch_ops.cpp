@@ -539,11 +539,13 @@ using torch::autograd::Variable;
 using torch::autograd::variable_list;
 
 // Whether a call has to be recorded; without that it goes straight to the kernels (an autograd node
-// costs a call 5 us of host time).
+// costs a call 5 us of host time).  A forward-mode tangent counts whatever the gradient mode: the
+// node refuses it, where the kernels would leave it out.
+bool has_tangent(const Tensor &t) { return t._fw_grad(/*level=*/0).defined(); }
 bool recorded(std::initializer_list<const Tensor *> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grad = at::GradMode::is_enabled();
   for (const Tensor *t : ts)
-    if (t != nullptr && t->requires_grad()) return true;
+    if (t != nullptr && ((grad && t->requires_grad()) || has_tangent(*t))) return true;
   return false;
 }
 
@@ -618,11 +620,9 @@ std::tuple<Tensor, Tensor> delta_fwd_autograd(const Tensor &q, const Tensor &k, 
 
 Tensor delta_step_autograd(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &g, const Tensor &beta,
                            Tensor &state, const optional<Tensor> &slots, double scale) {
-  if (at::GradMode::is_enabled())
-    for (const Tensor *t : {&q, &k, &v, &g, &beta, const_cast<const Tensor *>(&state)})
-      TORCH_CHECK_NOT_IMPLEMENTED(!t->requires_grad(),
-                                  "gated_delta_step has no gradient: call it under torch.no_grad(), or differentiate "
-                                  "gated_delta_chunk");
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded({&q, &k, &v, &g, &beta, const_cast<const Tensor *>(&state)}),
+                              "gated_delta_step has no gradient: call it under torch.no_grad(), or differentiate "
+                              "gated_delta_chunk");
   state.unsafeGetTensorImpl()->bump_version();  // a graph that saved the pool must notice
   at::AutoDispatchBelowADInplaceOrView below;
   static auto op = c10::Dispatcher::singleton()

@@ -98,6 +98,31 @@ def test_logprob_refusals(kw, error):
         token_logprobs(a.pop("logits"), a.pop("tokens"), **a)
 
 
+def test_forward_mode_derivatives_are_refused():
+    """No tangent is computed, so none is left out silently (meta tensors: no kernel runs)."""
+    import torch.autograd.forward_ad as fw
+    bf = dict(dtype=torch.bfloat16, device="meta")
+
+    def chunk(v):
+        return gated_delta_chunk(torch.zeros(1, 2, 5, 64, **bf), torch.zeros(1, 2, 5, 64, **bf), v,
+                                 torch.zeros(1, 2, 5, device="meta"), torch.zeros(1, 2, 5, device="meta"))[0]
+
+    def step(v):
+        return gated_delta_step(torch.zeros(3, 2, 64, **bf), torch.zeros(3, 2, 64, **bf), v, torch.zeros(3, 2, device="meta"),
+                                torch.zeros(3, 2, device="meta"), torch.zeros(3, 2, 64, 64, device="meta"))
+
+    def score(x):
+        return token_logprobs(x, torch.zeros(3, dtype=torch.long, device="meta")).logprob
+
+    for fn, x in ((chunk, torch.zeros(1, 2, 5, 64, **bf)), (step, torch.zeros(3, 2, 64, **bf)), (score, torch.zeros(3, 9, device="meta"))):
+        assert fn(x).device.type == "meta"
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+                fn(fw.make_dual(x, torch.ones_like(x)))
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(fn, (x,), (torch.ones_like(x),))
+
+
 # ------------------------------------------------------------------ C ABI --
 TENSOR = _ffi.KdaTensor(0x10000, 64 * 64, 64 * 64, 64, 1)
 
