@@ -350,12 +350,14 @@ Tensor delta_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Te
   const int64_t N = v_.size(0), H = v_.size(1), D = v_.size(2);
   TORCH_CHECK(state.dim() == 4 && state.scalar_type() == at::kFloat && state.size(1) == H && state.size(2) == D &&
                   state.size(3) == D, "state must be float32 [states, H, D, D]");
-  TORCH_CHECK(state.numel() == 0 ||
-                  (state.stride(3) == 1 && state.stride(2) == D && state.stride(0) % 4 == 0 && state.stride(1) % 4 == 0 &&
-                   (state.size(0) == 1 || state.stride(0) >= D * D) && (H == 1 || state.stride(1) >= D * D) &&
-                   (state.size(0) == 1 || H == 1 || state.stride(0) >= H * state.stride(1) ||
-                    state.stride(1) >= state.size(0) * state.stride(0)) &&
-                   reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0),
+  // a dimension of one element is never stepped over, whatever stride it reports
+  auto st = [](const Tensor &t, int i) { return t.size(i) == 1 ? (int64_t)0 : t.stride(i); };
+  // one of the two dimensions steps over all that the other spans
+  const int64_t states = state.size(0), sn = st(state, 0), sh = st(state, 1);
+  const bool apart = (states == 1 || sn >= D * D) && (H == 1 || sh >= D * D) &&
+                     (states == 1 || H == 1 || sn >= (H - 1) * sh + D * D || sh >= (states - 1) * sn + D * D);
+  TORCH_CHECK(state.numel() == 0 || (state.stride(3) == 1 && state.stride(2) == D && sn % 4 == 0 && sh % 4 == 0 && apart &&
+                                     reinterpret_cast<uintptr_t>(state.data_ptr()) % 16 == 0),
               "state is updated in place: each [D, D] must be contiguous, 16-byte aligned and apart from the others");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = prep(q_), k = prep(k_), v = prep(v_);
@@ -367,8 +369,6 @@ Tensor delta_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Te
   p.beta_dtype = gate_code(beta, "beta");
   p.scale = (float)scale;
   p.q = ptr(&q); p.k = ptr(&k); p.v = ptr(&v); p.o = ptr(&o); p.g = ptr(&g); p.beta = ptr(&beta);
-  // a dimension of one element is never stepped over, whatever stride it reports
-  auto st = [](const Tensor &t, int i) { return t.size(i) == 1 ? (int64_t)0 : t.stride(i); };
   p.q_stride_n = st(q, 0); p.q_stride_h = st(q, 1);
   p.k_stride_n = st(k, 0); p.k_stride_h = st(k, 1);
   p.v_stride_n = st(v, 0); p.v_stride_h = st(v, 1);
@@ -376,8 +376,8 @@ Tensor delta_step(const Tensor &q_, const Tensor &k_, const Tensor &v_, const Te
   p.g_stride_n = g.stride(0); p.g_stride_h = g.stride(1);
   p.beta_stride_n = beta.stride(0); p.beta_stride_h = beta.stride(1);
   p.state = static_cast<float *>(ptr(&state));
-  p.state_stride_n = st(state, 0);
-  p.state_stride_h = st(state, 1);
+  p.state_stride_n = sn;
+  p.state_stride_h = sh;
   Tensor idx;
   if (slots.has_value()) {
     p.slots_int64 = index64(*slots, "state_indices", q.device()) ? 1 : 0;

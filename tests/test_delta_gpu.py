@@ -467,6 +467,21 @@ def test_step_on_a_strided_pool_and_bad_indices():
     assert gated_delta_step(a["q"], a["k"], a["v"], a["g"], a["beta"], by_head).shape == (4, 2, 64)
 
 
+def test_step_on_every_third_head_of_a_pool():
+    """States need only be apart: a slice of another model's heads is taken as it is."""
+    from simpletrain_b200 import gated_delta_step
+    a = step_inputs(3, 4, 2, 64, 5, torch.bfloat16)
+    wide = torch.randn(5, 10, 64, 64, generator=torch.Generator().manual_seed(2)).to(DEV)
+    keep = wide.clone()
+    a["state"] = wide[:, ::3]
+    o_ref, s_ref = step_ref(a, [4, 1, 0], 64 ** -0.5)
+    o = gated_delta_step(*(a[n] for n in NAMES), wide[:, ::3], state_indices=torch.tensor([4, 1, 0], device=DEV))
+    check("o", o, as_result(o_ref, o))
+    check("state", wide[:, ::3], as_result(s_ref, wide))
+    for h in (1, 2, 4, 5, 7, 8):
+        assert torch.equal(wide[:, h], keep[:, h])
+
+
 def test_prefill_steps_and_scores_agree():
     """Prefill, single steps with the tokens' log probabilities, and the chunked form over the whole
     sequence with its gradient: the three operators as a serving and a training loop use them."""
