@@ -31,12 +31,26 @@ _HALF = (torch.bfloat16, torch.float16)
 _GATE = (torch.float32, torch.bfloat16, torch.float16)
 
 
+def _empty_in_order_of(like: Tensor) -> Tensor:
+    """The ops' rule for their [B, H, T, D] outputs: the input's strides where they are dense,
+    [B, T, H, D] memory where it is time-major, else contiguous."""
+    step, dense = 1, True
+    for i in sorted((i for i in range(4) if like.shape[i] != 1), key=like.stride):
+        dense = dense and like.stride(i) == step
+        step = step * like.shape[i]
+    if dense:
+        return torch.empty_like(like)
+    if like.stride(1) < like.stride(2):
+        return like.new_empty(like.shape[0], like.shape[2], like.shape[1], like.shape[3]).transpose(1, 2)
+    return like.new_empty(like.shape)
+
+
 @torch.library.register_fake("kda_b200::delta_fwd")
 def _(q, k, v, g, beta, scale, s0, cu_seqlens, want_state):
     n = v.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
     D = v.shape[3]
     shape = (n, v.shape[1], D, D) if want_state else (0,)
-    return torch.empty_like(v), q.new_empty(shape, dtype=torch.float32)
+    return _empty_in_order_of(v), q.new_empty(shape, dtype=torch.float32)
 
 
 @torch.library.register_fake("kda_b200::delta_bwd")
@@ -44,7 +58,7 @@ def _(q, k, v, g, beta, scale, s0, cu_seqlens, dout, ds_T, need_ds0):
     n = v.shape[0] if cu_seqlens is None else cu_seqlens.shape[0] - 1
     D = v.shape[3]
     ds0 = q.new_empty((n, v.shape[1], D, D) if need_ds0 else (0,), dtype=torch.float32)
-    return (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v),
+    return (_empty_in_order_of(q), _empty_in_order_of(k), _empty_in_order_of(v),
             g.new_empty(g.shape), beta.new_empty(beta.shape), ds0)
 
 

@@ -482,6 +482,41 @@ def test_step_on_every_third_head_of_a_pool():
         assert torch.equal(wide[:, h], keep[:, h])
 
 
+@pytest.mark.parametrize("layout", ["heads first", "tokens first", "fused", "broadcast"])
+def test_fake_implementations_tell_the_truth(layout):
+    """Shapes, strides and types of the ops under fake tensors are those of the real ones (what a compiler builds on)."""
+    from simpletrain_b200 import delta, fused_ops  # noqa: F401  (register them)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    B, H, T, D = 2, 4, 70, 64
+    x = make(B, H, H, T, D, torch.bfloat16, torch.float32, state=True)
+    a = {n: x[n].contiguous() if layout == "heads first" else x[n] for n in (*NAMES, "do")}
+    if layout == "fused":
+        proj = torch.stack([x[n].transpose(1, 2) for n in "qkv"], 2)
+        a.update(zip("qkv", (t.transpose(1, 2) for t in proj.unbind(2))))
+    if layout == "broadcast":
+        a["k"] = a["k"][:, :1].expand(B, H, T, D)
+        a["v"] = a["v"][:1].expand(B, H, T, D)
+    logits = torch.randn(5, 40, device=DEV)[:, :33]
+    row = torch.zeros(5, device=DEV)
+    st = {n: a[n][:, :, 0] for n in NAMES}
+    ops = torch.ops.kda_b200
+    calls = [
+        lambda t: ops.delta_fwd(*(t[n] for n in NAMES), 0.1, t["s0"], None, True),
+        lambda t: ops.delta_fwd(*(t[n] for n in NAMES), 0.1, None, None, False),
+        lambda t: ops.delta_bwd(*(t[n] for n in NAMES), 0.1, t["s0"], None, t["do"], None, True),
+        lambda t: (ops.delta_step(*(t["st_" + n] for n in NAMES), t["s0"], None, 0.1),),
+        lambda t: torch.ops.st_b200.token_logprobs(t["logits"], t["tok"], 3, 1.0, -100),
+    ]
+    real = {**a, "s0": x["s0"], "logits": logits, "tok": row.long(), **{"st_" + n: t for n, t in st.items()}}
+    with FakeTensorMode() as mode:
+        fake = {n: mode.from_tensor(t) for n, t in real.items()}
+        told = [call(fake) for call in calls]
+    for call, said in zip(calls, told):
+        for r, f in zip(call(real), said):
+            assert r.shape == f.shape and r.dtype == f.dtype and r.device == f.device
+            assert r.numel() == 0 or [s for s, n in zip(r.stride(), r.shape) if n > 1] == [s for s, n in zip(f.stride(), f.shape) if n > 1]
+
+
 def test_prefill_steps_and_scores_agree():
     """Prefill, single steps with the tokens' log probabilities, and the chunked form over the whole
     sequence with its gradient: the three operators as a serving and a training loop use them."""
