@@ -214,7 +214,9 @@ int kda_fwd_sm100_noalloc(const kda_fwd_params *p, kda_stream_t stream);
  *
  * H value heads share Hk query/key heads in groups of H / Hk (value head h uses
  * query/key head h / (H / Hk)).  g and beta may be bf16, f16 or f32; g below -110
- * counts as -110 (exp is 0 in fp32 either way).
+ * counts as -110 (exp is 0 in fp32 either way).  With f16 inputs, too, states and
+ * gradients have fp32's range: the products' operands are carried relative to the
+ * largest state, value and gradient of a chunk and head.
  *
  * Sequences: with cu_seqlens == NULL each of the B batch rows is one sequence
  * of T tokens.  With cu_seqlens (device [nseq + 1], B == 1, T <= 2^24) sequence i is

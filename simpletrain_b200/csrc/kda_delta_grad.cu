@@ -74,6 +74,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   __shared__ uint64_t bar_g2, bar_s, bar_d;
   __shared__ __align__(16) float gam[128];  // hi, then lo
   __shared__ float sm_dot[16], sm_xv[64];
+  __shared__ uint32_t sm_size[16];
   __shared__ float sm_f[2][64], sm_t[2][64], sm_y[2][64], sm_r[2][64];  // [half of the columns][row]
   const int tid = threadIdx.x, row = tid & 127, part = tid >> 7, r64 = row & 63;
   const bool upper = row >= 64;
@@ -140,6 +141,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       const float *gsrc = a.w.gam + ch * 128;
       if (tid < 128) gam[tid] = gsrc[tid];
       const float bi = a.w.beta[ch * 64 + r64];
+      // what a unit of the S and U images, of the dS and dX images, and of this row's products with the former is worth
+      const float iF = BF ? 1.f : a.w.unit[ch * kUnits + kUnitF], iR = BF ? 1.f : a.w.unit[ch * kUnits + kUnitR];
+      const float iRow = BF ? 1.f : (upper ? iF : iF * iR);
       // two 16-byte runs of a row of V, eight threads a row
       constexpr int VR = D / 64;
       const int vr = tid >> 3, vc = tid & 7;
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
       }
       for (int o = 4; o > 0; o >>= 1) xv += __shfl_xor_sync(0xffffffffu, xv, o);
-      if (vc == 0) sm_xv[vr] = xv;
+      if (vc == 0) sm_xv[vr] = BF ? xv : xv * iR;
       mbar_wait(smem_u32(&bar_s), ph, a.p.status, &ctl.abort);
       // <S, dS> = <S, dS hi> now, <S hi, dS lo> when that has come (S lo . dS lo is below fp32's last bits)
       float dot = 0.f;
@@ -216,6 +220,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       __syncwarp();
       tc_fence_after();
       uint4 mh[2], ml[2];
+      float mn[BF ? 1 : 2][8];  // fp16: M, N until their unit is known
+      uint32_t size = 0;
       float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
       {
         const float gh = gam[r64], gl = gam[64 + r64];
@@ -234,7 +240,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int j = j4 + i, col = 16 * part + 8 * c + j;
-              const float e = decay(gh, gl, hi[i], lo[i]), y = __uint_as_float(yr[j]);
+              const float e = decay(gh, gl, hi[i], lo[i]), y = BF ? __uint_as_float(yr[j]) : __uint_as_float(yr[j]) * iRow;
               if (!upper) {
                 const float m = col < r64 ? -y * e : 0.f;
                 rs = col < r64 ? fmaf(m, __uint_as_float(xr[j]), rs) : rs;
@@ -244,7 +250,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
               }
             }
           }
-          split8<BF>(m8, mh[c], ml[c]);
+          if constexpr (BF) {
+            split8<BF>(m8, mh[c], ml[c]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              mn[c][j] = m8[j];
+              size = max(size, abs_bits(m8[j]));
+            }
+          }
+        }
+        if constexpr (!BF) {
+          size = __reduce_max_sync(0xffffffffu, size);
+          if ((tid & 31) == 0) sm_size[tid >> 5] = size;
         }
       }
       // over the dX / dO tiles once their products are done and every thread is past its reads of them and of S
@@ -263,6 +281,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           prefetch_l2(a.w.U + nx * (size_t)(D * 256), D * 256);
           prefetch_l2(a.w.S + nx * (size_t)(D * D * 4), D * D * 4);
           prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
+        }
+      }
+      float iMN = 1.f;
+      if constexpr (!BF) {
+        size = 0;
+        for (int w = 0; w < 16; ++w) size = max(size, sm_size[w]);
+        const float sMN = unit_of(size, &iMN);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mn[c][j] *= sMN;
+          split8<BF>(mn[c], mh[c], ml[c]);
         }
       }
 #pragma unroll
@@ -291,7 +321,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       {
         float x[W];
         tmem_ldn<W>(lane_t + tG5 + part * W, x);
-        const float f = ex2f(gam[r64]) * (upper ? a.p.scale : -bi);
+        float f = ex2f(gam[r64]) * (upper ? a.p.scale : -bi);
+        if constexpr (!BF) f *= iRow;
 #pragma unroll
         for (int c = 0; c < W / 8; ++c) {
           float k[8];
@@ -303,6 +334,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           }
         }
         f_dot = f * t_dot;
+        if constexpr (!BF) t_dot *= iRow;
       }
       mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
 #pragma unroll
@@ -332,6 +364,16 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         if (!upper) {
           tmem_ldn<16>(lane_t + tG4 + part * W + c0, y);
           tmem_ldn<16>(lane_t + tG6 + part * W + c0, z);
+        }
+        if constexpr (!BF) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            x[i] *= iMN;
+            if (!upper) {
+              y[i] *= iMN;
+              z[i] *= iF * iR;
+            }
+          }
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -375,6 +417,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         float sd = 0.f;
         for (int w = 0; w < 16; ++w) sd += sm_dot[w];
         sd *= ex2f(gam[63]);
+        if constexpr (!BF) sd *= iF * iR;
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * tid + j;
           f[j] = sm_f[0][i] + sm_f[1][i];
@@ -499,6 +542,7 @@ int scan_ranges(int64_t nseq, int64_t H, int sms) {
 size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->p = *p;
   const bool packed = p->cu_seqlens != nullptr;
+  a->backward = backward ? 1 : 0;
   a->nseq = packed ? p->nseq : p->B;
   a->per_seq = packed ? 0 : (int)(((int64_t)p->T + 63) / 64);
   a->max_chunks = packed ? p->T / 64 + p->nseq : p->B * a->per_seq;
@@ -521,6 +565,7 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->w.slots = reinterpret_cast<float *>(take((backward ? 2 : 1) * ((size_t)a->ranges + 1) * p->D * p->D * 4));
   a->w.gam = reinterpret_cast<float *>(take(cells * 512));
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
+  if (p->dtype == KDA_DTYPE_F16) a->w.unit = reinterpret_cast<float *>(take(cells * kda::delta::kUnits * 4));
   a->w.T = take(cells * kda::delta::kImgT);
   if (backward) {
     a->w.S = take(cells * p->D * p->D * 4);

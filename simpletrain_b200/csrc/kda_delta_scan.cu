@@ -143,6 +143,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
   __shared__ __align__(16) float gam[2][64], bet[64];
+  __shared__ uint32_t size[4];  // fp16: the largest |V|, |dO|, |beta|, |P|, as bits
   int64_t b, t0;
   int rows;
   if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
@@ -157,8 +158,26 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
                a.p.k.stride_t, rows);
   load_rows<D, kPrepThreads>(sb + KQ, 64, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
                a.p.q.stride_t, rows);
+  if (!BF && tid < 4) size[tid] = 0;
   const uint32_t tmem = cta_begin(ctl, 64);
   const size_t ch = (size_t)blockIdx.x * a.p.H + h;
+  if constexpr (!BF) {
+    auto rows_size = [&](const kda_tensor &x) {
+      const uint16_t *base = static_cast<const uint16_t *>(x.data) + b * x.stride_b + h * x.stride_h + t0 * x.stride_t;
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < 64 * (D / 8) / kPrepThreads; ++i) {
+        const int p = tid + i * kPrepThreads, r = p / (D / 8), c = p % (D / 8);
+        if (r < rows) m = max(m, half_size(*reinterpret_cast<const uint4 *>(base + r * x.stride_t + 8 * c)));
+      }
+      return __reduce_max_sync(0xffffffffu, m);
+    };
+    const uint32_t mv = rows_size(a.p.v), mo = a.backward ? rows_size(a.p.dout) : 0;
+    if ((tid & 31) == 0) {
+      atomicMax(&size[0], mv);
+      atomicMax(&size[1], mo);
+    }
+  }
   if (tid < 32) {
     // running sums in double, then in two fp32 terms
     double s[2];
@@ -167,6 +186,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
       const float gate = i < rows ? load_gate(a.p.g, b * a.p.g_stride_b + h * a.p.g_stride_h + (t0 + i) * a.p.g_stride_t, a.p.g_dtype) : 0.f;
       s[j] = gate < kMinGate ? kMinGate : gate;  // a NaN stays one
       bet[i] = i < rows ? load_gate(a.p.beta, b * a.p.beta_stride_b + h * a.p.beta_stride_h + (t0 + i) * a.p.beta_stride_t, a.p.beta_dtype) : 0.f;
+      if constexpr (!BF) atomicMax(&size[2], abs_bits(bet[i]));
     }
     double c = s[0] + s[1];
     for (int o = 1; o < 32; o <<= 1) {
@@ -198,6 +218,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   const uint32_t taddr = tmem + lane_base + 32 * half;
   // 16 columns at a time of a row of A (rows of k) or P (rows of q)
   const int last = r64 - (row < 64 ? 1 : 0) - 32 * half;  // last column that counts
+  uint32_t mp = 0;
 #pragma unroll
   for (int c0 = 0; c0 < 32; c0 += 16) {
     float x[16];
@@ -219,7 +240,14 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
         *reinterpret_cast<float4 *>(As + r64 * kLd + 32 * half + c0 + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
     } else {
       tmem_st16(taddr + c0, x);  // P waits there for the inverse
+      if constexpr (!BF)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) mp = max(mp, abs_bits(x[j]));
     }
+  }
+  if constexpr (!BF) {
+    mp = __reduce_max_sync(0xffffffffu, mp);
+    if ((tid & 31) == 0) atomicMax(&size[3], mp);
   }
   tc_fence_before();
   __syncthreads();
@@ -254,6 +282,19 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   __syncthreads();
   inverse_level<16>(As, Ti);
   inverse_level<32>(As, Ti);
+  float sP = 1.f;
+  if constexpr (!BF) {
+    float inv;
+    sP = unit_of(size[3], &inv);
+    if (tid == 0) {
+      auto half = [](uint32_t x) { return unpack2(x, false).x; };
+      const float be = fmaxf(1.f, __uint_as_float(size[2]));
+      float *u = a.w.unit + ch * kUnits;
+      u[kUnitP] = inv;
+      u[kSizeV] = half(size[0]) * be;
+      u[kSizeDO] = half(size[1]) * fmaxf(fabsf(a.p.scale), __uint_as_float(size[3])) * be;
+    }
+  }
   {
     // T and P as two-term tiles over the matrices: read, then (every thread being past its reads) written
     uint4 h[4], l[4];
@@ -271,6 +312,9 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
         }
       } else {
         tmem_ld16(taddr + 16 * c0, x);
+        if constexpr (!BF)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) x[j] *= sP;
       }
       split8<BF>(x, h[2 * c0], l[2 * c0]);
       split8<BF>(x + 8, h[2 * c0 + 1], l[2 * c0 + 1]);
@@ -368,7 +412,7 @@ constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 13;  // the chain: warps 
 // Per-token factors of a chunk, one array a factor: beta, -beta e^gamma, e^{gamma_63 - gamma}, scale e^gamma.
 struct Factors {
   float beta[64], bg[64], w[64], sg[64];
-  float last[4];  // e^{gamma_63}
+  float last[4];  // e^{gamma_63}; fp16: the inputs' size, 1 / unit of P T
 };
 
 template <int D, int MODE>
@@ -381,7 +425,7 @@ struct ScanSmem {
 
 struct ScanBars {
   uint64_t full[2], empty[2];
-  uint64_t tail[2], s_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
+  uint64_t tail[2], s_ready[2], unit_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
 };
 
 // Wait (bounded, like mbar_wait) for a range's entry state.
@@ -490,6 +534,8 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           for (int e = tid; e < D * D; e += kScanThreads) dst[(size_t)i * D * D + e] = src != nullptr ? src[(size_t)i * D * D + e] : 0.f;
   }
   __shared__ int range_slot;
+  __shared__ uint32_t sizes[2][8];  // fp16: the chain's warps' largest state elements, by chunk parity
+  __shared__ float units[2][2];     // fp16: a chunk's unit and its inverse
   int *queue = a.w.queue + (REV ? a.ranges + 2 : 0);
   float *slots = a.w.slots + (REV ? (size_t)(a.ranges + 1) * D * D : 0);
   const uint32_t sb = smem_u32(smem);
@@ -499,6 +545,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       mbar_init(smem_u32(&bars.empty[i]), MODE == kStore ? 1 : 1 + Q);
       mbar_init(smem_u32(&bars.s_ready[i]), 2 * Q);
       mbar_init(smem_u32(&bars.tail[i]), 32);
+      mbar_init(smem_u32(&bars.unit_ready[i]), 1);
     }
     for (uint64_t *b : {&bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
     for (uint64_t *b : {&bars.ks_done, &bars.u_done, &bars.s_done, &bars.o_done}) mbar_init(smem_u32(b), 1);
@@ -594,6 +641,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           wait_flag(queue + 1 + range, a.p.status, &abort_flag);
           src = slots + (size_t)range * D * D;
         }
+        float unit = 1.f, worth = 1.f;  // fp16: of the state in tensor memory (a first state comes as it is)
         for (int pos = p0; pos < p1; ++pos, ++it) {
           const int st = it & 1;
           wait_full(pos);
@@ -603,6 +651,34 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             wait(bars.s_done, (it - 1) & 1);
           }
           tc_fence_after();
+          float held = worth;
+          if constexpr (!BF) {  // the unit of this chunk: from the state's largest element and the inputs'
+            uint32_t m = 0;
+#pragma unroll
+            for (int c0 = 0; c0 < W; c0 += 32) {
+              float x[32];
+              if (pos > p0) {
+                tmem_ld32(tl + cS + half * W + c0, x);
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) m = max(m, abs_bits(x[j]));
+            }
+            m = abs_bits(__uint_as_float(__reduce_max_sync(0xffffffffu, m)) * held);
+            if (lane == 0) sizes[it & 1][half * Q + quad] = m;
+            named_bar_sync(3, 2 * Q * 32);
+            m = abs_bits(fac[st].last[1]);
+#pragma unroll
+            for (int w = 0; w < 2 * Q; ++w) m = max(m, sizes[it & 1][w]);
+            unit = unit_of(m, &worth);
+            if (warp == 0 && lane == 0) {
+              units[it & 1][0] = unit;
+              units[it & 1][1] = worth;
+              mbar_arrive(smem_u32(&bars.unit_ready[it & 1]));
+            }
+          }
 #pragma unroll
           for (int c0 = 0; c0 < W; c0 += 32) {
             float x[32];
@@ -612,6 +688,9 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
             }
+            if constexpr (!BF)
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = (x[j] * held) * unit;
             tmem_split32<BF>(tl + cSH + (half * W + c0) / 2, tl + cSL + (half * W + c0) / 2, x);
             uint32_t r[32];
 #pragma unroll
@@ -628,6 +707,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
               uint16_t u;
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + vcol[j & 7] + (j >> 3) * 1024));
               v[j] = unpack2((uint32_t)u, BF).x * fac[st].beta[32 * half + j];
+              if constexpr (!BF) v[j] *= unit;
             }
           }
           wait(bars.ks_done, it & 1);
@@ -649,6 +729,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
               uint16_t u;
               asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(vt + vcol[j & 7] + (j >> 3) * 1024));
               x[j] = unpack2((uint32_t)u, BF).x * fac[st].sg[32 * half + j];
+              if constexpr (!BF) x[j] *= unit;
             }
             tmem_split32<BF>(tl + cR3 + 16 * half, tl + cR3 + 32 + 16 * half, x);
             tmem_wait_st();
@@ -658,7 +739,14 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           tc_fence_after();
           {
             float x[32];
-            tmem_ld32(tl + (REV ? cR2 : cR1) + 32 * half, x);
+            tmem_ld32(tl + (REV && BF ? cR2 : cR1) + 32 * half, x);
+            if constexpr (REV && !BF) {  // fp16: dO's part is in P T's unit
+              float y[32];
+              tmem_ld32(tl + cR2 + 32 * half, y);
+              const float f = fac[st].last[2] * unit;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) x[j] = fmaf(f, y[j], x[j]);
+            }
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] *= REV ? fac[st].bg[32 * half + j] : fac[st].w[32 * half + j];
             // over an operand whose products are done: S^T's (outputs: X^T may still be in use), else X^T's
@@ -680,7 +768,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             float x[32];
             tmem_ld32(tl + cS + half * W + c0, x);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) __stcg(dst + own + (size_t)(c0 + j) * D, x[j]);
+            for (int j = 0; j < 32; ++j) __stcg(dst + own + (size_t)(c0 + j) * D, BF ? x[j] : x[j] * worth);
           }
           if (pc.p1 < pc.nc) {
             __threadfence();
@@ -723,13 +811,23 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         if (t == 0) tma_store_wait_read0();
         named_bar_sync(1, 32 * Q);
       };
+      // fp16: the chunk's unit and its inverse
+      auto unit_at = [&](float *worth) {
+        if (BF) return *worth = 1.f;
+        wait(bars.unit_ready[it & 1], (it >> 1) & 1);
+        *worth = units[it & 1][1];
+        return units[it & 1][0];
+      };
       while (next_piece()) {
         for (int pos = p0; pos < p1; ++pos, ++it) {
           const int st = it & 1;
+          float worth;
+          const float unit = unit_at(&worth);
           if (MODE == kOut) {
             wait_full(pos);
             wait(bars.o_done, it & 1);
             tc_fence_after();
+            const float of = BF ? 1.f : fac[st].last[2] * worth;
             uint32_t pk[2][16];  // [16-lane half][column block j, row half]
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -738,7 +836,13 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
               tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR3, o);
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                const float f0 = fac[st].sg[8 * j + q2], f1 = fac[st].sg[8 * j + q2 + 1];
+                float f0 = fac[st].sg[8 * j + q2], f1 = fac[st].sg[8 * j + q2 + 1];
+                if constexpr (!BF) {
+                  f0 *= worth;
+                  f1 *= worth;
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[4 * j + e] = __float_as_uint(__uint_as_float(o[4 * j + e]) * of);
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
                   pk[hh][2 * j + e] = pack2(fmaf(f0, __uint_as_float(qs[4 * j + 2 * e]), __uint_as_float(o[4 * j + 2 * e])),
@@ -757,6 +861,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             if (t == 0) tma_store_commit();
           } else {
             if (REV) wait_full(pos);  // for the factors
+            if (!BF && t == 0) a.w.unit[cell(pos) * kUnits + (REV ? kUnitR : kUnitF)] = worth;
           // the state (reverse: its gradient) as the chain split it
             char *img = (REV ? a.w.dS : a.w.S) + cell(pos) * (size_t)(D * D * 4) + row * 16;
 #pragma unroll
@@ -796,6 +901,13 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
               for (int hh = 0; hh < 2; ++hh) {
                 uint32_t x[32], hi[16], lo[16];
                 tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR2, x);
+                if constexpr (!BF) {
+                  uint32_t z[32];
+                  tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR1, z);
+                  const float f = fac[st].last[2] * unit;
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(fmaf(f, __uint_as_float(x[i]), __uint_as_float(z[i])));
+                }
                 if (hh == 1) arrive_warp(bars.out_free);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) split2<BF>(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]), hi[i], lo[i]);
@@ -806,7 +918,11 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                  const float f0 = fac[st].beta[8 * j + q2], f1 = fac[st].beta[8 * j + q2 + 1];
+                  float f0 = fac[st].beta[8 * j + q2], f1 = fac[st].beta[8 * j + q2 + 1];
+                  if constexpr (!BF) {
+                    f0 *= worth;
+                    f1 *= worth;
+                  }
 #pragma unroll
                   for (int e = 0; e < 2; ++e)
                     hi[2 * j + e] = pack2(f0 * __uint_as_float(x[4 * j + 2 * e]), f1 * __uint_as_float(x[4 * j + 2 * e + 1]), BF);
@@ -866,7 +982,14 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         fac[st].w[i] = decay(lh, ll, gh, gl);
         fac[st].sg[i] = a.p.scale * G;
       }
-      if (lane == 0) fac[st].last[0] = ex2f(lh);
+      if (lane == 0) {
+        fac[st].last[0] = ex2f(lh);
+        if constexpr (!BF) {
+          const float *u = a.w.unit + cell(pos) * kUnits;
+          fac[st].last[1] = u[REV ? kSizeDO : kSizeV];
+          fac[st].last[2] = u[kUnitP];
+        }
+      }
       mbar_arrive(bar);
       __syncwarp();
     };
@@ -939,9 +1062,10 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         tc_fence_after();
         if (REV) {
           const MNMajor th(base + L::T, 0), tl(base + L::T + 16384, 0);
-          issue_ts<0, 4>(tmem + cR2, tmem + cXH, th, id_mn, true);
-          issue_ts<0, 4>(tmem + cR2, tmem + cXH, tl, id_mn, true);
-          issue_ts<0, 4>(tmem + cR2, tmem + cXL, th, id_mn, true);
+          constexpr uint32_t at = BF ? cR2 : cR1;  // fp16: apart from dO's part, which is in another unit
+          issue_ts<0, 4>(tmem + at, tmem + cXH, th, id_mn, BF);
+          issue_ts<0, 4>(tmem + at, tmem + cXH, tl, id_mn, true);
+          issue_ts<0, 4>(tmem + at, tmem + cXL, th, id_mn, true);
           mma_commit(smem_u32(&bars.u_done));
           wait(bars.qs_ready, it & 1);
           tc_fence_after();

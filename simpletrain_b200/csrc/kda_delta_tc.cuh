@@ -3,10 +3,17 @@
 //
 // Two-term operands.  A value x that is not an input is handed to the tensor cores as
 // hi + lo, hi = round16(x), lo = round16(x - hi): 16 bits of mantissa in bf16, 22 in
-// fp16, against 8 and 11 in one term.  A product of two such values is issued as
+// fp16 (whose exponents need the units below for that), against 8 and 11 in one term.  A product of two such values is issued as
 // hi*hi + hi*lo + lo*hi into one fp32 accumulator.  With single terms the state,
 // which feeds on itself chunk after chunk, was 2.5e-3 from the 64-bit recurrence;
 // with two it is 4e-6, and the tensor pipe is not what bounds these kernels.
+//
+// Units (fp16 only).  fp16 ends at 65504, and its two terms have their 22 bits from about 2^-3 up: a
+// gradient of 1e-5, as a loss's mean gives, was 7% off, and a state past 65504 became infinite.  The
+// recurrence is linear in (S, V) and its reverse in (dS, dO), so within a chunk everything that is
+// split is carried times a power of two, chosen from the largest elements of both so that they lie at
+// 2^6 to 2^7: 2^9 of room above for what a chunk's products make of them, 2^9 below before a
+// bit is lost.  Products and sums are scaled back in fp32, which is exact.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -38,12 +45,17 @@ struct Work {
                    // terms: their differences decide the factors, and after a few strong decays (-110 each) one
                    // fp32 term is 1e-4 from the sum (the state was 2e-4 from the recurrence's)
   float *beta;     // [chunk][H][64]
+  float *unit;     // fp16: [chunk][H][kUnits], see below
   char *T;         // [chunk][H] images of T over P T
   char *S, *dS;    // [chunk][H] images of the state before / the state gradient after the chunk, transposed: hi,
                    // then lo, each D / 8 runs of [D value rows x 8 key channels]
   char *U;         // [chunk][H] images of the chunk's u rows, transposed: hi, then lo, each 8 runs of [D value rows x 8 tokens]
   char *dX;        // [chunk][H][D / 64] images of the gradient of X: [64 tokens x 64] hi, then lo
 };
+
+// Of a (chunk, head): 1 / unit of P T; the largest element of beta V; what bounds the gradient that dO
+// brings in; 1 / unit of the S and U images, and of the dS and dX images.
+enum { kUnitP = 0, kSizeV = 1, kSizeDO = 2, kUnitF = 3, kUnitR = 4, kUnits = 8 };
 
 struct Args {
   kda_delta_params p;
@@ -53,6 +65,7 @@ struct Args {
   int max_chunks; // upper bound of the chunks over all sequences
   int ranges;     // CTAs of a scan
   int sms;        // of the device
+  int backward;
 };
 
 struct Seq {
@@ -105,6 +118,20 @@ __device__ __forceinline__ void store_gate(void *p, int64_t i, int dtype, float 
     static_cast<float *>(p)[i] = v;
   else
     static_cast<uint16_t *>(p)[i] = (uint16_t)(pack2(v, 0.f, dtype == KDA_DTYPE_BF16) & 0xffffu);
+}
+
+// The unit of numbers up to m (the bits of a value >= 0) and its inverse.  NaN and infinity: 1, they pass through.
+__device__ __forceinline__ float unit_of(uint32_t m, float *inverse) {
+  int e = (int)(m >> 23) - 127;
+  e = m >= 0x7f800000u ? 6 : min(max(e, -60), 80);
+  *inverse = __uint_as_float((uint32_t)(127 - 6 + e) << 23);
+  return __uint_as_float((uint32_t)(127 + 6 - e) << 23);
+}
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+// the larger one of both halves of eight fp16 values, as bits of |x|
+__device__ __forceinline__ uint32_t half_size(const uint4 &v) {
+  const uint32_t m = 0x7fff7fffu, x = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return max(x & 0xffffu, x >> 16);
 }
 
 // ------------------------------------------------------------- tile loads --

@@ -150,6 +150,10 @@ def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
     final_state; gradients of shared heads are summed in a fixed order.  A NaN or
     infinity in a token reaches its own 64-token chunk and what follows in its
     sequence (earlier tokens of the chunk too), and no other sequence.
+
+    States and gradients are fp32 whatever the inputs' type, of any size: in fp16 what a chunk
+    computes is carried relative to the largest state, value and gradient of that chunk and head, with
+    room for 2^9 times as much inside the chunk (a rule with ``beta |k|^2 <= 2`` stays far below).
     """
     D = v.shape[-1] if v.dim() else 0
     try:

@@ -269,6 +269,99 @@ def test_many_resets_in_a_chunk(case, D):
     compare(*run_both(x, D))
 
 
+def sized(x, **by):
+    """Inputs of `make` times a power of ten each, in their own types."""
+    return {n: (t.double() * by[n]).to(t.dtype) if n in by and t is not None else t for n, t in x.items()}
+
+
+def compare_sized(got, exp):
+    """As compare(); fp16 steps by 2^-24 below 2^-14, so each element of a small result is off by up to 2^-25 more."""
+    for name, a, b in zip(("o", "state", "dq", "dk", "dv", "dg", "dbeta", "ds0"), got, exp):
+        dtype_of = a.dtype
+        a, b = a.detach().double(), b.detach()
+        if half := dtype_of == torch.float16:  # from 65520 on the nearest value of the type is infinity
+            far = b.abs() >= 65520 * (1 + F32_TOL)
+            assert (a[far] == b[far].sign() * torch.inf).all(), name
+            fine = b.abs() <= 65520 * (1 - F32_TOL)
+            a, b = a[fine], b[fine]
+        assert torch.isfinite(a).all(), name
+        err, norm = (a - b).norm().item(), b.norm().item()
+        least = 2.0 ** -25 * a.numel() ** 0.5 if half else 0.0
+        assert err <= tol(dtype_of) * norm + least, f"{name}: {err / max(norm, 1e-300):.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("by", [
+    dict(do=1e-2, dsT=1e-2), dict(do=1e-4, dsT=1e-4), dict(do=1e-5, dsT=1e-5),  # a loss's mean without a loss scale
+    dict(do=1e-5, dsT=1.0), dict(do=0.0, dsT=1e-8), dict(do=1e3, dsT=1e5, q=0.01),
+    dict(v=1e-4, s0=1e-4), dict(v=1e-3, s0=1e-7), dict(s0=1e5, do=1e-3, dsT=1e-3), dict(v=300.0, do=1e-5, dsT=1e-5),
+    dict(q=1e-2), dict(q=30.0, do=1e-2), dict(k=0.1), dict(k=0.1, beta=50.0), dict(k=1.4, do=1e-3, dsT=1e-3),
+], ids=lambda by: " ".join(f"{n}={x:g}" for n, x in by.items()))
+def test_sizes_of_the_inputs(by, dtype):
+    """What the products' operands are rounded to does not depend on how large the inputs and the gradients are.
+    fp16 carries them in units of a power of two a chunk, so that its range does not bound states and gradients."""
+    x = sized(make(1, 2, 1, 300, 128, dtype, torch.float32, seed=14, state=True), **by)
+    compare_sized(*run_both(x, 128))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sizes_that_change_along_a_sequence(dtype):
+    """Values of very different size in different chunks and sequences."""
+    lens = [200, 64, 130, 70]
+    cu, bounds, T = packed(lens)
+    x = make(1, 4, 2, T, 64, dtype, torch.float32, seed=15, state=True, n=len(lens))
+    x["v"][:, :, :64] *= 1e-3
+    x["v"][:, :, 128:150] *= 1e3
+    x["do"][:, :, :128] *= 1e-4
+    x["g"][:, 1, 160] = -200.0
+    x["s0"][1] *= 1e6
+    x["s0"][2] = 0
+    x["v"][:, :, 264:394] *= 1e-4
+    x["do"][:, :, 264:394] *= 1e-4
+    x["dsT"][3] *= 1e-6
+    x["q"][:, :, 200:264] *= 1e-2
+    got, exp = run_both(x, 64, cu, bounds)
+    for i, (lo, hi) in enumerate(bounds):  # each sequence by itself: a large one does not hide a small one
+        part = lambda r: [r[0][:, :, lo:hi], r[1][i], *(t[:, :, lo:hi] for t in r[2:7]), r[7][i]]
+        compare_sized(part(got), part(exp))
+
+
+def test_a_scale_far_from_the_default():
+    for scale in (1e-4, 50.0):
+        x = make(1, 2, 2, 150, 64, torch.float16, torch.float32, seed=16, state=True)
+        x = sized(x, do=1e-2 / scale if scale > 1 else 1.0)
+        compare_sized(*run_both(x, 64, scale=scale))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("beta", [1.0, 1.9])
+@pytest.mark.parametrize("case", ["one key", "two keys", "near"])
+def test_repeated_and_correlated_keys(case, beta, dtype):
+    """(I + A)^-1 is largest where keys repeat.  For one key and no decay its rows are 1, -beta, -beta (1 - beta),
+    -beta (1 - beta)^2 ...: an operand's error comes out of U = T X up to 1 + beta / (1 - |1 - beta|) times as large,
+    2 for beta 1 and 20 for 1.9, and the fp32 part of the tolerance is that many times the others'."""
+    x = make(1, 2, 1, 200, 64, dtype, torch.float32, seed=17, state=True, decay=8.0)
+    k = x["k"].clone()
+    if case == "one key":
+        k[:] = k[:, :, :1]
+    elif case == "two keys":
+        k[:, :, ::2], k[:, :, 1::2] = k[:, :, :1], -k[:, :, 1:2]
+    else:
+        k = (k.float() * 0.05 + k[:, :, :1].float())
+        k = (k / k.norm(dim=-1, keepdim=True)).to(dtype)
+    x["k"] = k
+    x["beta"][:] = beta
+    grown = 1 + beta / (1 - abs(1 - beta))
+    for name, a, b in zip(("o", "state", "dq", "dk", "dv", "dg", "dbeta", "ds0"), *run_both(x, 64)):
+        err, norm = (a.detach().double() - b.detach()).norm().item(), b.detach().norm().item()
+        assert err <= (tol(a.dtype) + (grown - 1) * F32_TOL) * norm, f"{name}: {err / norm:.3e}"
+
+
+def test_long_training_sequence_of_wide_heads():
+    x = make(1, 2, 1, 1700, 128, torch.bfloat16, torch.bfloat16, seed=18, state=True, decay=6.0)
+    compare(*run_both(x, 128))
+
+
 def test_gradients_against_differences():
     """Directional derivatives of the library's own forward, through the fp32 state."""
     from simpletrain_b200 import gated_delta_chunk
