@@ -74,7 +74,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
   __shared__ uint64_t bar_g2, bar_s, bar_d;
   __shared__ __align__(16) float gam[128];  // hi, then lo
   __shared__ float sm_dot[16], sm_xv[64];
-  __shared__ uint32_t sm_size[16];
+  __shared__ __align__(16) uint32_t sm_size[16];
+  __shared__ volatile float sm_unit[2];
   __shared__ float sm_f[2][64], sm_t[2][64], sm_y[2][64], sm_r[2][64];  // [half of the columns][row]
   const int tid = threadIdx.x, row = tid & 127, part = tid >> 7, r64 = row & 63;
   const bool upper = row >= 64;
@@ -141,9 +142,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       const float *gsrc = a.w.gam + ch * 128;
       if (tid < 128) gam[tid] = gsrc[tid];
       const float bi = a.w.beta[ch * 64 + r64];
-      // what a unit of the S and U images, of the dS and dX images, and of this row's products with the former is worth
-      const float iF = BF ? 1.f : a.w.unit[ch * kUnits + kUnitF], iR = BF ? 1.f : a.w.unit[ch * kUnits + kUnitR];
-      const float iRow = BF ? 1.f : (upper ? iF : iF * iR);
+      // fp16: what a unit of the S and U images (F), of the dS and dX images (R), and of this row's products with the
+      // former is worth; read again where they are used, registers being what this kernel has least of
+      if (!BF && tid < 2) sm_unit[tid] = a.w.unit[ch * kUnits + kUnitF + tid];
+      auto worth_F = [&]() { return sm_unit[0]; };
+      auto worth_R = [&]() { return sm_unit[1]; };
+      auto worth_row = [&]() { return upper ? sm_unit[0] : sm_unit[0] * sm_unit[1]; };
       // two 16-byte runs of a row of V, eight threads a row
       constexpr int VR = D / 64;
       const int vr = tid >> 3, vc = tid & 7;
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         for (int j = 0; j < 8; ++j) xv = fmaf(x[j] + y[j], v[j], xv);
       }
       for (int o = 4; o > 0; o >>= 1) xv += __shfl_xor_sync(0xffffffffu, xv, o);
-      if (vc == 0) sm_xv[vr] = BF ? xv : xv * iR;
+      if (vc == 0) sm_xv[vr] = BF ? xv : xv * worth_R();
       mbar_wait(smem_u32(&bar_s), ph, a.p.status, &ctl.abort);
       // <S, dS> = <S, dS hi> now, <S hi, dS lo> when that has come (S lo . dS lo is below fp32's last bits)
       float dot = 0.f;
@@ -222,6 +226,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       uint4 mh[2], ml[2];
       float mn[BF ? 1 : 2][8];  // fp16: M, N until their unit is known
       uint32_t size = 0;
+      const float y_unit = BF ? 1.f : worth_row();
       float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
       {
         const float gh = gam[r64], gl = gam[64 + r64];
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const int j = j4 + i, col = 16 * part + 8 * c + j;
-              const float e = decay(gh, gl, hi[i], lo[i]), y = BF ? __uint_as_float(yr[j]) : __uint_as_float(yr[j]) * iRow;
+              const float e = decay(gh, gl, hi[i], lo[i]), y = BF ? __uint_as_float(yr[j]) : __uint_as_float(yr[j]) * y_unit;
               if (!upper) {
                 const float m = col < r64 ? -y * e : 0.f;
                 rs = col < r64 ? fmaf(m, __uint_as_float(xr[j]), rs) : rs;
@@ -286,7 +291,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       float iMN = 1.f;
       if constexpr (!BF) {
         size = 0;
-        for (int w = 0; w < 16; ++w) size = max(size, sm_size[w]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint4 z = *reinterpret_cast<const uint4 *>(sm_size + 4 * w);
+          size = max(size, max(max(z.x, z.y), max(z.z, z.w)));
+        }
         const float sMN = unit_of(size, &iMN);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -322,7 +331,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         float x[W];
         tmem_ldn<W>(lane_t + tG5 + part * W, x);
         float f = ex2f(gam[r64]) * (upper ? a.p.scale : -bi);
-        if constexpr (!BF) f *= iRow;
+        if constexpr (!BF) f *= worth_row();
 #pragma unroll
         for (int c = 0; c < W / 8; ++c) {
           float k[8];
@@ -334,7 +343,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           }
         }
         f_dot = f * t_dot;
-        if constexpr (!BF) t_dot *= iRow;
+        if constexpr (!BF) t_dot *= worth_row();
       }
       mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
 #pragma unroll
@@ -356,7 +365,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         load_head(cidx, h + 1, b, t0, rows);
       else if (more)
         load_head(un / a.p.Hk, (un % a.p.Hk) * G_, nb, nt, nrows);
-      const float wi = decay(gam[63], gam[127], gam[r64], gam[64 + r64]);
+      float wi = decay(gam[63], gam[127], gam[r64], gam[64 + r64]), c_dot = 0.f;
+      if constexpr (!BF) wi *= worth_F() * worth_R();
 #pragma unroll
       for (int c0 = 0; c0 < W; c0 += 16) {
         float x[16], y[16], z[16];
@@ -365,16 +375,6 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           tmem_ldn<16>(lane_t + tG4 + part * W + c0, y);
           tmem_ldn<16>(lane_t + tG6 + part * W + c0, z);
         }
-        if constexpr (!BF) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            x[i] *= iMN;
-            if (!upper) {
-              y[i] *= iMN;
-              z[i] *= iF * iR;
-            }
-          }
-        }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float k[8];
@@ -382,7 +382,12 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int i = 8 * c + j;
-            if (upper) {
+            if constexpr (!BF) {
+              const float s = upper ? x[i] : x[i] + y[i], d = upper ? x[i] : x[i] - y[i], v = upper ? 0.f : wi * z[i];
+              c_dot = fmaf(k[j], d, c_dot);
+              y_dot = fmaf(k[j], v, y_dot);
+              acc[c0 + i] += fmaf(iMN, s, v);
+            } else if (upper) {
               f_dot = fmaf(k[j], x[i], f_dot);
               acc[c0 + i] += x[i];
             } else {
@@ -394,6 +399,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           }
         }
       }
+      if constexpr (!BF) f_dot = fmaf(iMN, c_dot, f_dot);
       // the rows' sums, in a fixed order: the quarters of k rows, then those of q rows
       for (int turn = 0; turn < 2; ++turn) {
         if (!upper && (part >> 1) == turn) {
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         float sd = 0.f;
         for (int w = 0; w < 16; ++w) sd += sm_dot[w];
         sd *= ex2f(gam[63]);
-        if constexpr (!BF) sd *= iF * iR;
+        if constexpr (!BF) sd *= worth_F() * worth_R();
         for (int j = 0; j < 2; ++j) {
           const int i = 2 * tid + j;
           f[j] = sm_f[0][i] + sm_f[1][i];
@@ -542,7 +548,6 @@ int scan_ranges(int64_t nseq, int64_t H, int sms) {
 size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->p = *p;
   const bool packed = p->cu_seqlens != nullptr;
-  a->backward = backward ? 1 : 0;
   a->nseq = packed ? p->nseq : p->B;
   a->per_seq = packed ? 0 : (int)(((int64_t)p->T + 63) / 64);
   a->max_chunks = packed ? p->T / 64 + p->nseq : p->B * a->per_seq;

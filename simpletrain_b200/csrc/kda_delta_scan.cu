@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   extern __shared__ __align__(1024) char smem[];
   __shared__ Ctl ctl;
   __shared__ __align__(16) float gam[2][64], bet[64];
-  __shared__ uint32_t size[4];  // fp16: the largest |V|, |dO|, |beta|, |P|, as bits
+  __shared__ uint32_t size[3];  // fp16: the largest |beta|, |P| and k_t.k_t, as bits
   int64_t b, t0;
   int rows;
   if (a.p.cu_seqlens != nullptr) pdl_wait();  // for the plan
@@ -158,26 +158,9 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
                a.p.k.stride_t, rows);
   load_rows<D, kPrepThreads>(sb + KQ, 64, static_cast<const uint16_t *>(a.p.q.data) + b * a.p.q.stride_b + hk * a.p.q.stride_h + t0 * a.p.q.stride_t,
                a.p.q.stride_t, rows);
-  if (!BF && tid < 4) size[tid] = 0;
+  if (!BF && tid < 3) size[tid] = 0;
   const uint32_t tmem = cta_begin(ctl, 64);
   const size_t ch = (size_t)blockIdx.x * a.p.H + h;
-  if constexpr (!BF) {
-    auto rows_size = [&](const kda_tensor &x) {
-      const uint16_t *base = static_cast<const uint16_t *>(x.data) + b * x.stride_b + h * x.stride_h + t0 * x.stride_t;
-      uint32_t m = 0;
-#pragma unroll
-      for (int i = 0; i < 64 * (D / 8) / kPrepThreads; ++i) {
-        const int p = tid + i * kPrepThreads, r = p / (D / 8), c = p % (D / 8);
-        if (r < rows) m = max(m, half_size(*reinterpret_cast<const uint4 *>(base + r * x.stride_t + 8 * c)));
-      }
-      return __reduce_max_sync(0xffffffffu, m);
-    };
-    const uint32_t mv = rows_size(a.p.v), mo = a.backward ? rows_size(a.p.dout) : 0;
-    if ((tid & 31) == 0) {
-      atomicMax(&size[0], mv);
-      atomicMax(&size[1], mo);
-    }
-  }
   if (tid < 32) {
     // running sums in double, then in two fp32 terms
     double s[2];
@@ -186,7 +169,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
       const float gate = i < rows ? load_gate(a.p.g, b * a.p.g_stride_b + h * a.p.g_stride_h + (t0 + i) * a.p.g_stride_t, a.p.g_dtype) : 0.f;
       s[j] = gate < kMinGate ? kMinGate : gate;  // a NaN stays one
       bet[i] = i < rows ? load_gate(a.p.beta, b * a.p.beta_stride_b + h * a.p.beta_stride_h + (t0 + i) * a.p.beta_stride_t, a.p.beta_dtype) : 0.f;
-      if constexpr (!BF) atomicMax(&size[2], abs_bits(bet[i]));
+      if constexpr (!BF) atomicMax(&size[0], abs_bits(bet[i]));
     }
     double c = s[0] + s[1];
     for (int o = 1; o < 32; o <<= 1) {
@@ -223,6 +206,15 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   for (int c0 = 0; c0 < 32; c0 += 16) {
     float x[16];
     tmem_ld16(taddr + c0, x);
+    if constexpr (!BF) {
+      const int own = r64 - 32 * half - c0;  // k_t.k_t
+      if (row < 64 && own >= 0 && own < 16) {
+        float kk = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) kk = j == own ? x[j] : kk;
+        atomicMax(&size[2], abs_bits(kk));
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
       const float4 c = *reinterpret_cast<const float4 *>(gam[0] + 32 * half + c0 + j);
@@ -247,7 +239,7 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   }
   if constexpr (!BF) {
     mp = __reduce_max_sync(0xffffffffu, mp);
-    if ((tid & 31) == 0) atomicMax(&size[3], mp);
+    if ((tid & 31) == 0) atomicMax(&size[1], mp);
   }
   tc_fence_before();
   __syncthreads();
@@ -285,15 +277,11 @@ __global__ void __launch_bounds__(kPrepThreads, 4) prep_kernel(const Args a) {
   float sP = 1.f;
   if constexpr (!BF) {
     float inv;
-    sP = unit_of(size[3], &inv);
-    if (tid == 0) {
-      auto half = [](uint32_t x) { return unpack2(x, false).x; };
-      const float be = fmaxf(1.f, __uint_as_float(size[2]));
-      float *u = a.w.unit + ch * kUnits;
-      u[kUnitP] = inv;
-      u[kSizeV] = half(size[0]) * be;
-      u[kSizeDO] = half(size[1]) * fmaxf(fabsf(a.p.scale), __uint_as_float(size[3])) * be;
-    }
+    sP = unit_of(size[1], &inv);
+    if (tid == 0)
+      *reinterpret_cast<float4 *>(a.w.unit + ch * kUnits) =
+          make_float4(inv, fmaxf(1.f, __uint_as_float(size[0])), fmaxf(fabsf(a.p.scale), __uint_as_float(size[1])),
+                      sqrtf(__uint_as_float(size[2])));
   }
   {
     // T and P as two-term tiles over the matrices: read, then (every thread being past its reads) written
@@ -406,13 +394,15 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // product with T: in the output warps that took 2000 to 3000 cycles a chunk and made them the slowest.
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
-constexpr int kScanThreads = 448;
-constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 13;  // the chain: warps 0 .. 7
+template <bool BF>
+constexpr int kScanThreads = BF ? 448 : 512;
+constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 13, kSizeWarp = 14;  // the chain: warps 0 .. 7; fp16: two size warps
 
 // Per-token factors of a chunk, one array a factor: beta, -beta e^gamma, e^{gamma_63 - gamma}, scale e^gamma.
 struct Factors {
   float beta[64], bg[64], w[64], sg[64];
-  float last[4];  // e^{gamma_63}; fp16: the inputs' size, 1 / unit of P T
+  float last[4];  // e^{gamma_63}
+  float4 unit;    // fp16: the preparation's four sizes
 };
 
 template <int D, int MODE>
@@ -425,7 +415,7 @@ struct ScanSmem {
 
 struct ScanBars {
   uint64_t full[2], empty[2];
-  uint64_t tail[2], s_ready[2], unit_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
+  uint64_t tail[2], s_ready[2], inputs_sized[2], state_sized[2], unit_ready[2], ks_done, x_ready, u_done, up_ready, s_done, o_done, out_free, qs_ready;
 };
 
 // Wait (bounded, like mbar_wait) for a range's entry state.
@@ -504,7 +494,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
   __shared__ __align__(16) Factors fac[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  __shared__ WarpPlace places[kScanThreads / 32];
+  __shared__ WarpPlace places[kScanThreads<BF> / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int G_ = a.p.H / a.p.Hk;
   pdl_wait();
@@ -531,10 +521,13 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
     if (dst != nullptr)  // sequences without tokens hand their state on
       for (int i = block; i < a.nseq * a.p.H; i += a.ranges)
         if (get_seq(a, i / a.p.H).len == 0)
-          for (int e = tid; e < D * D; e += kScanThreads) dst[(size_t)i * D * D + e] = src != nullptr ? src[(size_t)i * D * D + e] : 0.f;
+          for (int e = tid; e < D * D; e += kScanThreads<BF>) dst[(size_t)i * D * D + e] = src != nullptr ? src[(size_t)i * D * D + e] : 0.f;
   }
   __shared__ int range_slot;
-  __shared__ uint32_t sizes[2][8];  // fp16: the chain's warps' largest state elements, by chunk parity
+  // fp16, by chunk parity: a warp of the chain each, the largest element that is left of the state before the chunk
+  // and of what half the tokens added to it; the second sizing warp's part of the inputs' sizes
+  __shared__ float2 sizes[2][8];
+  __shared__ uint2 part_size[2];
   __shared__ float units[2][2];     // fp16: a chunk's unit and its inverse
   int *queue = a.w.queue + (REV ? a.ranges + 2 : 0);
   float *slots = a.w.slots + (REV ? (size_t)(a.ranges + 1) * D * D : 0);
@@ -545,6 +538,8 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       mbar_init(smem_u32(&bars.empty[i]), MODE == kStore ? 1 : 1 + Q);
       mbar_init(smem_u32(&bars.s_ready[i]), 2 * Q);
       mbar_init(smem_u32(&bars.tail[i]), 32);
+      mbar_init(smem_u32(&bars.inputs_sized[i]), 1);
+      mbar_init(smem_u32(&bars.state_sized[i]), 2 * Q);
       mbar_init(smem_u32(&bars.unit_ready[i]), 1);
     }
     for (uint64_t *b : {&bars.x_ready, &bars.up_ready}) mbar_init(smem_u32(b), 2 * Q);
@@ -632,6 +627,13 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       uint32_t vcol[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) vcol[i] = (uint32_t)((dv >> 6) * 8192 + i * 128 + ((((dv >> 3) ^ i) & 7) << 4) + (dv & 7) * 2);
+      // what chunk i's unit goes by: what is left of the state before the chunk, what half of its tokens added
+      auto tell_size = [&](int i, float left, float grown) {
+        if (lane == 0) {
+          sizes[i & 1][half * Q + quad] = make_float2(left, grown);
+          mbar_arrive(smem_u32(&bars.state_sized[i & 1]));
+        }
+      };
       while (next_piece()) {
         const size_t state = ((size_t)pc.n * a.p.H + pc.h) * D * D;
         // the piece's first state: the caller's, or the one that the range before published
@@ -646,38 +648,24 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           const int st = it & 1;
           wait_full(pos);
           const float last = fac[st].last[0];
+          if (!BF && pos == p0) {  // fp16: how large a piece's first state is
+            uint32_t m = 0;
+            if (src != nullptr)
+#pragma unroll 8
+              for (int j = 0; j < W; ++j) m = max(m, abs_bits(__ldcg(src + own + (size_t)j * D)));
+            tell_size(it, __uint_as_float(__reduce_max_sync(0xffffffffu, m)), 0.f);
+          }
           if (it > 0) {
             if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
             wait(bars.s_done, (it - 1) & 1);
           }
           tc_fence_after();
-          float held = worth;
-          if constexpr (!BF) {  // the unit of this chunk: from the state's largest element and the inputs'
-            uint32_t m = 0;
-#pragma unroll
-            for (int c0 = 0; c0 < W; c0 += 32) {
-              float x[32];
-              if (pos > p0) {
-                tmem_ld32(tl + cS + half * W + c0, x);
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
-              }
-#pragma unroll
-              for (int j = 0; j < 32; ++j) m = max(m, abs_bits(x[j]));
-            }
-            m = abs_bits(__uint_as_float(__reduce_max_sync(0xffffffffu, m)) * held);
-            if (lane == 0) sizes[it & 1][half * Q + quad] = m;
-            named_bar_sync(3, 2 * Q * 32);
-            m = abs_bits(fac[st].last[1]);
-#pragma unroll
-            for (int w = 0; w < 2 * Q; ++w) m = max(m, sizes[it & 1][w]);
-            unit = unit_of(m, &worth);
-            if (warp == 0 && lane == 0) {
-              units[it & 1][0] = unit;
-              units[it & 1][1] = worth;
-              mbar_arrive(smem_u32(&bars.unit_ready[it & 1]));
-            }
+          float held = 1.f, large = 0.f;  // fp16: new units of an old one; of the state that the chunk begins with, in its units
+          if constexpr (!BF) {
+            wait(bars.unit_ready[st], (it >> 1) & 1);
+            unit = units[st][0];
+            held = fminf(worth * unit, 0x1p126f);  // beyond that nothing is left of what is held
+            worth = units[st][1];
           }
 #pragma unroll
           for (int c0 = 0; c0 < W; c0 += 32) {
@@ -688,9 +676,15 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = src != nullptr ? __ldcg(src + own + (size_t)(c0 + j) * D) : 0.f;
             }
-            if constexpr (!BF)
+            if constexpr (!BF) {
+              if (held != 1.f)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = (x[j] * held) * unit;
+                for (int j = 0; j < 32; ++j) x[j] *= held;
+              float m[4] = {large, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 32; ++j) m[j & 3] = fmaxf(m[j & 3], fabsf(x[j]));
+              large = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            }
             tmem_split32<BF>(tl + cSH + (half * W + c0) / 2, tl + cSL + (half * W + c0) / 2, x);
             uint32_t r[32];
 #pragma unroll
@@ -743,7 +737,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             if constexpr (REV && !BF) {  // fp16: dO's part is in P T's unit
               float y[32];
               tmem_ld32(tl + cR2 + 32 * half, y);
-              const float f = fac[st].last[2] * unit;
+              const float f = fac[st].unit.x * unit;
 #pragma unroll
               for (int j = 0; j < 32; ++j) x[j] = fmaf(f, y[j], x[j]);
             }
@@ -753,7 +747,17 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             const uint32_t at = MODE == kOut ? cSH : cXH;
             tmem_split32<BF>(tl + at + 16 * half, tl + at + 32 + 16 * half, x);
             tmem_wait_st();
+            const float kn = BF ? 0.f : fac[st].unit.w;
             arrive_warp(bars.up_ready);
+            if constexpr (!BF) {  // under the update: |sum_t k_t u'_t| <= max |k_t| sum_t |u'_t|
+              float g4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 32; ++j) g4[j & 3] += fabsf(x[j]);
+              const float g = (g4[0] + g4[1]) + (g4[2] + g4[3]);
+              if (pos + 1 < p1)
+                tell_size(it + 1, __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(large))) * last * worth,
+                          __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(g))) * kn * worth);
+            }
           }
         }
         // where the state goes from here: to the next range, or to the caller
@@ -827,7 +831,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             wait_full(pos);
             wait(bars.o_done, it & 1);
             tc_fence_after();
-            const float of = BF ? 1.f : fac[st].last[2] * worth;
+            const float of = BF ? 1.f : fac[st].unit.x * worth;
             uint32_t pk[2][16];  // [16-lane half][column block j, row half]
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -904,7 +908,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
                 if constexpr (!BF) {
                   uint32_t z[32];
                   tmem_ld_16x256b_x8(tl + ((uint32_t)(16 * hh) << 16) + cR1, z);
-                  const float f = fac[st].last[2] * unit;
+                  const float f = fac[st].unit.x * unit;
 #pragma unroll
                   for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(fmaf(f, __uint_as_float(x[i]), __uint_as_float(z[i])));
                 }
@@ -954,6 +958,24 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
     auto load = [&](int pos) {
       const int st = it & 1;
       const uint32_t base = sb + st * L::kStage, bar = smem_u32(&bars.full[st]);
+      const size_t at = cell(pos) * 64;
+      const float *gam = a.w.gam + 2 * at;
+      float4 unit;
+      float lh, ll, gh[2], gl[2], be[2];
+      auto fetch = [&]() {
+        lh = gam[63];
+        ll = gam[127];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          gh[i] = gam[lane + 32 * i];
+          gl[i] = gam[64 + lane + 32 * i];
+          be[i] = a.w.beta[at + lane + 32 * i];
+        }
+      };
+      if constexpr (!BF) {  // (the sizes of the chunk need the time behind the tiles)
+        unit = *reinterpret_cast<const float4 *>(a.w.unit + cell(pos) * kUnits);
+        fetch();
+      }
       if (it >= 2) wait(bars.empty[st], ((it >> 1) - 1) & 1);
       if (lane == 0) {
         const int t0 = (int)(s.t0 + (int64_t)chunk_of(pos) * kChunk), b = (int)s.b;
@@ -971,24 +993,18 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           bulk_load(base + L::T, img, kImgT, bar);
         }
       }
-      const size_t at = cell(pos) * 64;
-      const float *gam = a.w.gam + 2 * at;
-      const float lh = gam[63], ll = gam[127];
+      if constexpr (BF) fetch();
 #pragma unroll
-      for (int i = lane; i < 64; i += 32) {
-        const float gh = gam[i], gl = gam[64 + i], be = a.w.beta[at + i], G = ex2f(gh);
-        fac[st].beta[i] = be;
-        fac[st].bg[i] = -be * G;
-        fac[st].w[i] = decay(lh, ll, gh, gl);
-        fac[st].sg[i] = a.p.scale * G;
+      for (int i = 0; i < 2; ++i) {
+        const float G = ex2f(gh[i]);
+        fac[st].beta[lane + 32 * i] = be[i];
+        fac[st].bg[lane + 32 * i] = -be[i] * G;
+        fac[st].w[lane + 32 * i] = decay(lh, ll, gh[i], gl[i]);
+        fac[st].sg[lane + 32 * i] = a.p.scale * G;
       }
       if (lane == 0) {
         fac[st].last[0] = ex2f(lh);
-        if constexpr (!BF) {
-          const float *u = a.w.unit + cell(pos) * kUnits;
-          fac[st].last[1] = u[REV ? kSizeDO : kSizeV];
-          fac[st].last[2] = u[kUnitP];
-        }
+        if constexpr (!BF) fac[st].unit = unit;
       }
       mbar_arrive(bar);
       __syncwarp();
@@ -1016,7 +1032,67 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       }
     }
     if (ragged < kChunk) zero_tail((it - 1) & 1, ((it - 1) >> 1) & 1, ragged);
-  } else if (__syncwarp(), elect_one()) {
+  } else if (!BF && warp >= kSizeWarp) {
+    // -------------------------------------------------------- fp16: the chunks' units --
+    // From the inputs' largest elements and a bound of the state's: |S + sum_t k_t u'_t| <= |S| + max |k_t| sum_t |u'_t|
+    // (exact for a piece's first state).  The chain gives its part before the update is done, and this is done before
+    // it has to wait.  Two warps, eight rows of the tiles in turn, in a loop of few instructions: unrolled,
+    // code that a warp runs once a chunk waits thousands of cycles to be fetched.
+    constexpr int P = D / 8, RW = 32 / P, NL = 8 / RW;  // 16-byte pieces a row, rows a load, loads for eight rows
+    const int second = warp - kSizeWarp;
+    uint32_t off[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r = lane / P + RW * i, g = lane % P;
+      off[i] = (g >> 3) * 8192 + chunk_at(r, g & 7) + 1024 * second;
+    }
+    while (next_piece()) {
+      float added = 0.f;  // to dS by the dO of the chunk before, at most
+      for (int pos = p0; pos < p1; ++pos, ++it) {
+        const int st = it & 1, rows = rows_of(pos);  // what lies behind a sequence's end is another's
+        wait(bars.full[st], (it >> 1) & 1);
+        uint32_t m[2] = {0, 0};
+#pragma unroll
+        for (int tl = 0; tl < (REV ? 2 : 1); ++tl) {
+          const char *base = smem + st * L::kStage + (tl == 0 ? L::V : L::Q);
+#pragma unroll 1
+          for (int r0 = lane / P + 8 * second; r0 < rows; r0 += 16, base += 2048) {
+            uint4 x[NL];
+#pragma unroll
+            for (int i = 0; i < NL; ++i) x[i] = *reinterpret_cast<const uint4 *>(base + off[i]);
+#pragma unroll
+            for (int i = 0; i < NL; ++i) m[tl] = max(m[tl], r0 + RW * i < rows ? half_size(x[i]) : 0u);
+          }
+          __syncwarp();
+          m[tl] = __reduce_max_sync(0xffffffffu, m[tl]);
+        }
+        if (second) {
+          if (lane == 0) {
+            part_size[st] = make_uint2(m[0], m[1]);
+            mbar_arrive(smem_u32(&bars.inputs_sized[st]));
+          }
+          __syncwarp();
+          continue;
+        }
+        wait(bars.inputs_sized[st], (it >> 1) & 1);
+        const uint2 other = part_size[st];
+        const float x = unpack2(max(m[0], other.x), false).x, q = unpack2(max(m[1], other.y), false).x;
+        const float inputs = x * fac[st].unit.y * (REV ? fac[st].unit.z : 1.f);
+        wait(bars.state_sized[st], (it >> 1) & 1);
+        const float2 z = sizes[st][lane & (2 * Q - 1)];
+        const uint32_t left = __reduce_max_sync(0xffffffffu, abs_bits(z.x)), grown = __reduce_max_sync(0xffffffffu, abs_bits(z.y));
+        if (lane == 0) {
+          float worth;
+          const float bound = __uint_as_float(left) + 2.f * __uint_as_float(grown) + added;
+          units[st][0] = unit_of(max(abs_bits(bound), abs_bits(inputs)), &worth);
+          units[st][1] = worth;
+          mbar_arrive(smem_u32(&bars.unit_ready[st]));
+        }
+        if (REV) added = 64.f * fabsf(a.p.scale) * x * q;
+        __syncwarp();
+      }
+    }
+  } else if (warp == kMmaWarp && (__syncwarp(), elect_one())) {
     // ---------------------------------------------------------------- products --
     auto wait = [&](uint64_t &b, uint32_t parity) { mbar_wait(smem_u32(&b), parity, a.p.status, &abort_flag); };
     const uint32_t id_k = idesc_f16(128, 64, BF, false, false), id_mn = idesc_f16(128, 64, BF, false, true);
@@ -1102,14 +1178,14 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
 }
 
 template <int D, bool BF, int MODE>
-__global__ void __launch_bounds__(kScanThreads, 1) scan_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(kScanThreads<BF>, 1) scan_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps maps) {
   scan_cta<D, BF, MODE>(a, maps, blockIdx.x);
 }
 
 // The backward's two scans side by side, where there are SMs for both: neither needs the other.  (On
 // half of the SMs each where there are not, they took longer: 1210 against 1170 us for 16 x 2048 tokens' step.)
 template <int D, bool BF>
-__global__ void __launch_bounds__(kScanThreads, 1)
+__global__ void __launch_bounds__(kScanThreads<BF>, 1)
     scan_pair_kernel(const __grid_constant__ Args a, const __grid_constant__ Maps store, const __grid_constant__ Maps rev) {
   if (blockIdx.x < a.ranges)
     scan_cta<D, BF, kRev>(a, rev, blockIdx.x);
@@ -1142,7 +1218,7 @@ cudaError_t run_scan(const Args &a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(scan_kernel<D, BF, MODE>, smem, done);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(scan_kernel<D, BF, MODE>, dim3((unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m);
+  e = launch_kernel(scan_kernel<D, BF, MODE>, dim3((unsigned)a.ranges), dim3(kScanThreads<BF>), smem, st, true, a, m);
   count_launches(1);
   return e;
 }
@@ -1160,7 +1236,7 @@ cudaError_t run_backward(const Args &a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(scan_pair_kernel<D, BF>, smem, done);
   if (e != cudaSuccess) return e;
-  e = launch_kernel(scan_pair_kernel<D, BF>, dim3(2 * (unsigned)a.ranges), dim3(kScanThreads), smem, st, true, a, m1, m2);
+  e = launch_kernel(scan_pair_kernel<D, BF>, dim3(2 * (unsigned)a.ranges), dim3(kScanThreads<BF>), smem, st, true, a, m1, m2);
   count_launches(1);
   return e;
 }

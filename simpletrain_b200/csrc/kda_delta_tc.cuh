@@ -53,9 +53,9 @@ struct Work {
   char *dX;        // [chunk][H][D / 64] images of the gradient of X: [64 tokens x 64] hi, then lo
 };
 
-// Of a (chunk, head): 1 / unit of P T; the largest element of beta V; what bounds the gradient that dO
-// brings in; 1 / unit of the S and U images, and of the dS and dX images.
-enum { kUnitP = 0, kSizeV = 1, kSizeDO = 2, kUnitF = 3, kUnitR = 4, kUnits = 8 };
+// Of a (chunk, head), from the preparation: 1 / unit of P T, and the largest of 1 and |beta|, of |scale| and |P|,
+// of |k_t|; from the scans: 1 / unit of the S and U images, and of the dS and dX images.
+enum { kUnitP = 0, kSizeB = 1, kSizeP = 2, kSizeK = 3, kUnitF = 4, kUnitR = 5, kUnits = 8 };
 
 struct Args {
   kda_delta_params p;
@@ -65,7 +65,6 @@ struct Args {
   int max_chunks; // upper bound of the chunks over all sequences
   int ranges;     // CTAs of a scan
   int sms;        // of the device
-  int backward;
 };
 
 struct Seq {
