@@ -574,17 +574,17 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const BwdArgs g) {
   // over a low temperature or with a common offset of the logits is far more than the exponents that count
   const double lse = g.lse[r] * kLog2eD;
   const bool empty = lse == -INFINITY;
-  const float l2 = (float)lse, l2_low = empty ? 0.f : (float)(lse - (double)l2);
+  const float l2 = empty ? 0.f : (float)lse, l2_low = empty ? 0.f : (float)(lse - (double)l2);
   // a token outside [0, V): its log probability is NaN, and so is the row's gradient through it
-  const float a = !counted ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
-  const float b = g.dentropy != nullptr ? g.dentropy[r] * g.inv_t : 0.f, H = g.entropy[r];
+  const float a = !counted || empty ? 0.f : (tok < 0 || tok >= g.V) ? NAN : g.dlogprob[r] * g.inv_t;
+  const float b = g.dentropy != nullptr && !empty ? g.dentropy[r] * g.inv_t : 0.f, H = g.entropy[r];
   const float base = -a - b * H, slope = -b * kLn2;
   const float low = (l2 + kFloor) / g.c;  // p is 0 from here down, where slope * d might overflow
   auto grad = [&](int64_t i, float x) {
     const float d = fmaf(floor1(x, low), g.c, -l2) - l2_low, p = ex2(d);
     float v = p * fmaf(slope, d, base);
     if (i == tok) v += a;
-    return empty ? 0.f : v;
+    return v;  // of an empty row: p = 0 everywhere, a = b = 0
   };
   const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   if (!same) {
