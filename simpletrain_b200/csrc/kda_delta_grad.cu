@@ -568,6 +568,7 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   a->ranges = scan_ranges(a->nseq, p->H, a->sms);
   a->w.queue = reinterpret_cast<int *>(take(sizeof(int) * 2 * ((size_t)a->ranges + 2)));
   a->w.slots = reinterpret_cast<float *>(take((backward ? 2 : 1) * ((size_t)a->ranges + 1) * p->D * p->D * 4));
+  if (p->dtype == KDA_DTYPE_F16) a->w.cuts = reinterpret_cast<float2 *>(take((backward ? 2 : 1) * ((size_t)a->ranges + 1) * 8 * sizeof(float2)));
   a->w.gam = reinterpret_cast<float *>(take(cells * 512));
   a->w.beta = reinterpret_cast<float *>(take(cells * 256));
   if (p->dtype == KDA_DTYPE_F16) a->w.unit = reinterpret_cast<float *>(take(cells * kda::delta::kUnits * 4));

@@ -528,9 +528,10 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
   // and of what half the tokens added to it; the second sizing warp's part of the inputs' sizes
   __shared__ float2 sizes[2][8];
   __shared__ uint2 part_size[2];
-  __shared__ float units[2][2];     // fp16: a chunk's unit and its inverse
+  __shared__ float units[2][3];     // fp16: a chunk's unit, its inverse, what its dO adds to dS at most
   int *queue = a.w.queue + (REV ? a.ranges + 2 : 0);
   float *slots = a.w.slots + (REV ? (size_t)(a.ranges + 1) * D * D : 0);
+  float2 *cuts = BF ? nullptr : a.w.cuts + (REV ? 8 * (a.ranges + 1) : 0);
   const uint32_t sb = smem_u32(smem);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -627,10 +628,10 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       uint32_t vcol[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) vcol[i] = (uint32_t)((dv >> 6) * 8192 + i * 128 + ((((dv >> 3) ^ i) & 7) << 4) + (dv & 7) * 2);
-      // what chunk i's unit goes by: what is left of the state before the chunk, what half of its tokens added
-      auto tell_size = [&](int i, float left, float grown) {
+      // what chunk i's unit goes by: what is left of the state before the last chunk, what half of its tokens added
+      auto tell_size = [&](int i, float2 z) {
         if (lane == 0) {
-          sizes[i & 1][half * Q + quad] = make_float2(left, grown);
+          sizes[i & 1][half * Q + quad] = z;
           mbar_arrive(smem_u32(&bars.state_sized[i & 1]));
         }
       };
@@ -649,11 +650,15 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           wait_full(pos);
           const float last = fac[st].last[0];
           if (!BF && pos == p0) {  // fp16: how large a piece's first state is
-            uint32_t m = 0;
-            if (src != nullptr)
+            if (pc.p0 > 0) {  // what the chunk before said of it: units do not depend on where streams are cut
+              tell_size(it, __ldcg(cuts + 8 * range + half * Q + quad));
+            } else {
+              uint32_t m = 0;
+              if (src != nullptr)
 #pragma unroll 8
-              for (int j = 0; j < W; ++j) m = max(m, abs_bits(__ldcg(src + own + (size_t)j * D)));
-            tell_size(it, __uint_as_float(__reduce_max_sync(0xffffffffu, m)), 0.f);
+                for (int j = 0; j < W; ++j) m = max(m, abs_bits(__ldcg(src + own + (size_t)j * D)));
+              tell_size(it, make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, m)), 0.f));
+            }
           }
           if (it > 0) {
             if (MODE != kOut) wait(bars.out_free, (it - 1) & 1);
@@ -754,9 +759,12 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
 #pragma unroll
               for (int j = 0; j < 32; ++j) g4[j & 3] += fabsf(x[j]);
               const float g = (g4[0] + g4[1]) + (g4[2] + g4[3]);
+              const float2 z = make_float2(__uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(large))) * last * worth + (REV ? units[st][2] : 0.f),
+                                           __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(g))) * kn * worth);
               if (pos + 1 < p1)
-                tell_size(it + 1, __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(large))) * last * worth,
-                          __uint_as_float(__reduce_max_sync(0xffffffffu, abs_bits(g))) * kn * worth);
+                tell_size(it + 1, z);
+              else if (pc.p1 < pc.nc && lane == 0)
+                __stcg(cuts + 8 * (range + 1) + half * Q + quad, z);
             }
           }
         }
@@ -1047,7 +1055,6 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
       off[i] = (g >> 3) * 8192 + chunk_at(r, g & 7) + 1024 * second;
     }
     while (next_piece()) {
-      float added = 0.f;  // to dS by the dO of the chunk before, at most
       for (int pos = p0; pos < p1; ++pos, ++it) {
         const int st = it & 1, rows = rows_of(pos);  // what lies behind a sequence's end is another's
         wait(bars.full[st], (it >> 1) & 1);
@@ -1083,12 +1090,12 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         const uint32_t left = __reduce_max_sync(0xffffffffu, abs_bits(z.x)), grown = __reduce_max_sync(0xffffffffu, abs_bits(z.y));
         if (lane == 0) {
           float worth;
-          const float bound = __uint_as_float(left) + 2.f * __uint_as_float(grown) + added;
+          const float bound = __uint_as_float(left) + 2.f * __uint_as_float(grown);
           units[st][0] = unit_of(max(abs_bits(bound), abs_bits(inputs)), &worth);
           units[st][1] = worth;
+          if (REV) units[st][2] = 64.f * fabsf(a.p.scale) * x * q;
           mbar_arrive(smem_u32(&bars.unit_ready[st]));
         }
-        if (REV) added = 64.f * fabsf(a.p.scale) * x * q;
         __syncwarp();
       }
     }

@@ -39,6 +39,7 @@ constexpr float kMinGate = -110.f;  // exp() is 0 in fp32 from about -104 on
 struct Work {
   int *queue;      // [2 scans][2 + ranges]: ticket, then a flag a range whose entry state is published; cleared by the preparation
   float *slots;    // [scan][ranges + 1][D][D] states at the ranges' boundaries
+  float2 *cuts;    // fp16: [scan][ranges + 1][8] a warp of the chain each: how large a slot's state is at most, in two parts
   int *bound;      // [nseq + 1] sequence offsets, clamped into order and range (packed sequences only)
   int *first;      // [nseq + 1] first chunk of each sequence
   float *gam;      // [chunk][H][2][64] running sums of the log decay inside the chunk, in units of log 2 and in two

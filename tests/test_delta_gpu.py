@@ -173,6 +173,48 @@ def test_packed_rows_equal_their_own_calls():
     assert torch.isnan(o[:, :, 100:164]).any()
 
 
+def test_fp16_results_do_not_depend_on_where_streams_are_cut():
+    """A stream alone is one work range; among 200 others it is cut between CTAs.  The units that fp16 goes by are the same."""
+    from simpletrain_b200 import gated_delta_chunk
+    x = sized(make(3, 67, 67, 330, 64, torch.float16, torch.float32, seed=19, state=True), do=1e-3, v=3.0)
+    results = []
+    for pick in (slice(None), slice(1, 2)):
+        leaf = [x[n][pick].detach().requires_grad_(True) for n in (*NAMES, "s0")]
+        o, s = gated_delta_chunk(*leaf[:5], initial_state=leaf[5])
+        results.append((o, s, *torch.autograd.grad([o, s], leaf, [x["do"][pick], x["dsT"][pick]])))
+    for a, b in zip(*results):
+        assert torch.equal(a[1:2], b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_zeros(dtype):
+    """Nothing in, nothing out: no unit of zeros makes a NaN."""
+    for zero in (("v", "s0"), ("do", "dsT"), ("q",), ("k",), ("beta",), ("v", "s0", "do", "dsT"), NAMES):
+        x = make(1, 2, 1, 140, 64, dtype, torch.float32, seed=20, state=True)
+        x = {n: torch.zeros_like(t) if n in zero else t for n, t in x.items()}
+        compare(*run_both(x, 64))
+    x = make(1, 2, 1, 140, 64, dtype, torch.float32, seed=20, state=True)
+    compare(*run_both(x, 64, scale=0.0))
+
+
+@pytest.mark.parametrize("value", [torch.nan, torch.inf])
+def test_what_is_not_finite_stays_in_its_chunk_and_behind_in_fp16(value):
+    from simpletrain_b200 import gated_delta_chunk
+    for name in ("q", "k", "v"):
+        x = make(1, 1, 1, 260, 64, torch.float16, torch.float32, seed=21)
+        clean, s_clean = gated_delta_chunk(*(x[n] for n in NAMES))
+        x[name][0, 0, 130, 3] = value
+        leaf = [x[n].detach().requires_grad_(True) for n in NAMES]
+        o, s = gated_delta_chunk(*leaf)
+        assert torch.equal(o[:, :, :128], clean[:, :, :128]) and not torch.isfinite(o[0, 0, 130]).all()
+        if name == "q":
+            assert torch.equal(s, s_clean)
+        else:
+            assert not torch.isfinite(s).all()
+        grads = torch.autograd.grad(o, leaf, x["do"])
+        assert any(not torch.isfinite(g).all() for g in grads)
+
+
 @pytest.mark.parametrize("name", NAMES)
 def test_nan_is_not_swallowed(name):
     """A NaN of any input reaches the outputs from its token on, the state and the gradients."""
