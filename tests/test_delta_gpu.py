@@ -652,6 +652,35 @@ def test_fake_implementations_tell_the_truth(layout):
             assert r.numel() == 0 or [s for s, n in zip(r.stride(), r.shape) if n > 1] == [s for s, n in zip(f.stride(), f.shape) if n > 1]
 
 
+def test_offsets_past_32_bits():
+    """The last head of a long call and the last states of a large pool are what they are on their own."""
+    from simpletrain_b200 import gated_delta_chunk, gated_delta_step
+    H, T, D = 33, 1 << 20, 64
+    gen = torch.Generator(device=DEV).manual_seed(22)
+
+    def rnd(*shape):
+        return torch.randn(*shape, generator=gen, device=DEV, dtype=torch.bfloat16)
+
+    v = rnd(1, H, T, D)
+    assert v.numel() > 1 << 31
+    k = torch.nn.functional.normalize(rnd(1, 1, T, D), dim=-1)
+    q = k.flip(2)
+    g, beta = -torch.rand(1, H, T, generator=gen, device=DEV), torch.rand(1, H, T, generator=gen, device=DEV)
+    o, s = gated_delta_chunk(q, k, v, g, beta)
+    oi, si = gated_delta_chunk(q, k, v[:, -1:], g[:, -1:], beta[:, -1:])
+    assert torch.equal(o[:, -1:], oi) and torch.equal(s[:, -1:], si)
+    del o, v
+    pool = torch.zeros((1 << 31) // (2 * D * D) + 3, 2, D, D, device=DEV)
+    assert pool[-1].storage_offset() > 1 << 31
+    a = step_inputs(2, 2, 1, D, 3, torch.bfloat16)
+    n = pool.shape[0]
+    pool[-1], pool[-3] = a["state"][0], a["state"][1]
+    o1 = gated_delta_step(*(a[m] for m in NAMES), a["state"])
+    o2 = gated_delta_step(*(a[m] for m in NAMES), pool, state_indices=torch.tensor([n - 1, n - 3], device=DEV))
+    assert torch.equal(o1, o2) and torch.equal(pool[-1], a["state"][0]) and torch.equal(pool[-3], a["state"][1])
+    assert not pool[0].any() and not pool[-2].any()
+
+
 def test_prefill_steps_and_scores_agree():
     """Prefill, single steps with the tokens' log probabilities, and the chunked form over the whole
     sequence with its gradient: the three operators as a serving and a training loop use them."""

@@ -213,6 +213,25 @@ def test_rows_of_a_padded_vocabulary_and_odd_bases(dtype):
         check(x, tok, a, b, 1.0, 4)
 
 
+def test_offsets_past_32_bits():
+    from simpletrain_b200.fused_ops import token_logprobs
+    N, V = 70000, 32003  # rows of odd length: every alignment
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x = torch.randn(N, V, generator=gen, device=DEV, dtype=torch.bfloat16)
+    tok = torch.randint(0, V, (N,), generator=gen, device=DEV)
+    up = torch.rand(N, generator=gen, device=DEV)
+    got = []
+    for pick in (slice(None), slice(N - 5, N)):
+        leaf = x[pick].detach().requires_grad_(True)
+        r = token_logprobs(leaf, tok[pick])
+        (dx,) = torch.autograd.grad((r.logprob, r.entropy), leaf, (up[pick], up[pick]))
+        got.append([t[-5:].clone() for t in (r.logprob, r.entropy, dx)])
+        del r, dx
+    # five rows are shared by more CTAs each: sums in another order
+    assert (got[0][0] - got[1][0]).abs().max() <= ABS and (got[0][1] - got[1][1]).abs().max() <= ABS
+    assert (got[0][2].double() - got[1][2].double()).norm() <= (2.0 ** -15 + 2 * half_step(x.dtype)) * got[1][2].double().norm()
+
+
 def test_repeats_are_bitwise_equal_and_captured():
     from simpletrain_b200.fused_ops import token_logprobs
     x, tok, a, b = make(8, 32000, torch.bfloat16)
