@@ -134,7 +134,7 @@ __device__ __forceinline__ void inverse_level(float *As, float *Ti) {
 // Measured: 110 us for 16 x 2048 tokens, 10 heads of 128 (5120 cells, 64 KB of k, q and images each:
 // 3.1 TB/s).  The shared-memory pipe sets that (77% of its cycles taken, the tensor pipe 13%): 128 threads a
 // CTA and six CTAs an SM, persistent CTAs that load the next cell under this one, and half the loads
-// in the inverse's upper level all came to the same time.
+// in the inverse's upper level all came to the same time.  In fp16, with P's unit and the sizes, 117 us.
 constexpr int kPrepThreads = 256;
 
 template <int D, bool BF>
@@ -383,7 +383,7 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 //
 // Warps: 8 walk the dependent chain (a value channel a thread, half the columns each), 4
 // turn finished tiles into output or workspace rows, one starts the loads, one issues the
-// products.  TMA brings the tiles two chunks ahead.
+// products.  TMA brings the tiles two chunks ahead.  In fp16 two more warps find each chunk's unit.
 //
 // Measured at D = 128: 2.5 us a chunk (4600 cycles) with outputs, whatever the number of streams up
 // to one an SM (28 streams of 32768 tokens: 1.29 ms).  It is latency: three dependent products with a
@@ -392,6 +392,9 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // (503 MB, 4.3 TB/s), states and u rows 148 us (755 MB, 5.1 TB/s), reverse 199 us (983 MB, 4.9 TB/s; its start
 // under the end of the one before is in that).  dO becomes an operand in the chain's wait for its
 // product with T: in the output warps that took 2000 to 3000 cycles a chunk and made them the slowest.
+// fp16's units cost a chunk 1000 cycles of the chain (its maximum as the state is converted, the wait for
+// the unit): 28 streams of 32768 tokens 1.55 ms, and 172, 174 and 297 us in place of 118, 148 and 199.
+// With the sizes found by the chain itself (the state read twice, a barrier) the former took 1.63 ms.
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
 template <bool BF>

@@ -16,7 +16,9 @@
 // a copy's rate; one row of 8 heads of 64 takes 2.7 us, a launch and two dependent loads.
 //
 // Rows that name the same state are applied one after the other, in row order, by
-// the CTA of the first of them: the result does not depend on the launch.
+// the CTA of the first of them: the result does not depend on the launch.  For that each CTA looks through all
+// N indices, under its state's loads: with 24 heads of 128 it costs 4% at 256 rows, 8% at 1024, 42% at
+// 4096 and 74% at 8192 (6.6 against 3.8 ms); rows that all name one state take 1.4 ms at 1024 and 24 ms at 8192.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -6,14 +6,16 @@
 // fp16 (whose exponents need the units below for that), against 8 and 11 in one term.  A product of two such values is issued as
 // hi*hi + hi*lo + lo*hi into one fp32 accumulator.  With single terms the state,
 // which feeds on itself chunk after chunk, was 2.5e-3 from the 64-bit recurrence;
-// with two it is 4e-6, and the tensor pipe is not what bounds these kernels.
+// with two it is 4e-6, and the tensor pipe is not what bounds these kernels.  (Where keys repeat, an error
+// of an operand is multiplied by the row sums of |T|, up to 1 + beta / (1 - |1 - beta|): 1e-5 at beta = 1, 1e-4 at 1.9.)
 //
 // Units (fp16 only).  fp16 ends at 65504, and its two terms have their 22 bits from about 2^-3 up: a
-// gradient of 1e-5, as a loss's mean gives, was 7% off, and a state past 65504 became infinite.  The
+// gradient of 1e-5, as a loss's mean gives, left ds0 7% off, and a state past 65504 became infinite.  The
 // recurrence is linear in (S, V) and its reverse in (dS, dO), so within a chunk everything that is
 // split is carried times a power of two, chosen from the largest elements of both so that they lie at
 // 2^6 to 2^7: 2^9 of room above for what a chunk's products make of them, 2^9 below before a
-// bit is lost.  Products and sums are scaled back in fp32, which is exact.
+// bit is lost.  Products and sums are scaled back in fp32, which is exact.  Results in fp32 are 6e-7 to 1e-6 from the
+// recurrence whatever the sizes (test inputs of 1e-5 to 1e5).
 #pragma once
 
 #include <cuda_runtime.h>

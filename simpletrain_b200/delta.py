@@ -10,7 +10,7 @@ Unlike ``kda_chunk``'s state, which only adds ``k^T v``, the rule first takes
 out what the state already predicts for ``k_t``.  ``gated_delta_chunk`` runs it
 over whole sequences (training, prefill) and ``gated_delta_step`` continues it
 one token a call on a pool of states (serving); both hold the state in fp32 and
-agree on it to a few parts in 1e6.
+agree on it to a few parts in 1e6 (bf16 keys that repeat, at beta 1.9: 1e-4).
 
 ``kda_b200::delta_fwd / delta_bwd / delta_step`` are defined and implemented in
 C++, autograd included (``csrc/torch_ops.cpp``), over the C ABI (``include/kda_sm100.h``): they run
@@ -153,7 +153,8 @@ def gated_delta_chunk(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, 
 
     States and gradients are fp32 whatever the inputs' type, of any size: in fp16 what a chunk
     computes is carried relative to the largest state, value and gradient of that chunk and head, with
-    room for 2^9 times as much inside the chunk (a rule with ``beta |k|^2 <= 2`` stays far below).
+    room for 2^9 times as much inside the chunk (a rule with ``beta |k|^2 <= 2`` stays far below);
+    what is 2^12 times smaller than that keeps its bits, what is smaller still loses them one by one.
     """
     D = v.shape[-1] if v.dim() else 0
     try:
@@ -192,7 +193,7 @@ def gated_delta_step(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tensor, s
     int64), or state n without them.  A negative index marks a padded row: its o
     is zero and no state changes.  An index past the pool does the same and sets a
     bit of ``device_status()``.  Rows that name the same state are applied in row
-    order.  The step has no gradient: differentiate ``gated_delta_chunk``.
+    order (looking for them takes 4% of a call of 256 rows, 74% more at 8192).  The step has no gradient: differentiate ``gated_delta_chunk``.
     """
     D = v.shape[-1] if v.dim() else 0
     try:

@@ -399,8 +399,9 @@ def test_repeated_and_correlated_keys(case, beta, dtype):
         assert err <= (tol(a.dtype) + (grown - 1) * F32_TOL) * norm, f"{name}: {err / norm:.3e}"
 
 
-def test_long_training_sequence_of_wide_heads():
-    x = make(1, 2, 1, 1700, 128, torch.bfloat16, torch.bfloat16, seed=18, state=True, decay=6.0)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_long_training_sequence_of_wide_heads(dtype):
+    x = make(1, 2, 1, 1700, 128, dtype, torch.bfloat16, seed=18, state=True, decay=6.0)
     compare(*run_both(x, 128))
 
 
@@ -511,6 +512,57 @@ def test_repeats_streams_and_capture():
     for want, a, b in zip((first, other), got, outs):
         for w, u, v in zip(want, a, b):
             assert torch.equal(w, u) and torch.equal(w, v)
+
+
+def test_fp16_repeats_and_capture():
+    """The units are found anew in every call: replays on other inputs, and a captured backward, give the eager bits."""
+    from simpletrain_b200 import gated_delta_chunk
+    cu, bounds, T = packed([150, 0, 64, 300])
+    x, y = (make(1, 4, 2, T, 128, torch.float16, torch.float32, seed=s, state=True, n=4) for s in (23, 24))
+    y = sized(y, v=50.0, s0=1e4, do=1e-4, dsT=1e-6)
+    z = {n: t.detach().clone() for n, t in x.items()}
+
+    def step(a):
+        leaf = [a[n].detach().requires_grad_(True) for n in (*NAMES, "s0")]
+        o, s = gated_delta_chunk(*leaf[:5], initial_state=leaf[5], cu_seqlens=cu)
+        return (o.detach(), s.detach(), *torch.autograd.grad([o, s], leaf, [a["do"], a["dsT"]]))
+
+    want = [[t.clone() for t in step(a)] for a in (x, y, x)]
+    assert all(torch.equal(a, b) for a, b in zip(want[0], want[2]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(z)
+    for a, w in ((x, want[0]), (y, want[1]), (x, want[0])):
+        for n in z:
+            z[n].copy_(a[n])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(u, v) for u, v in zip(w, out))
+
+
+def test_compiled_calls():
+    """Traced with fake tensors, forward and backward, the ops are called as they are in eager mode."""
+    from simpletrain_b200 import gated_delta_chunk, gated_delta_step
+    from simpletrain_b200.fused_ops import token_logprobs
+    x = make(2, 4, 2, 130, 64, torch.bfloat16, torch.float32, state=True)
+    head = torch.randn(64, 50, device=DEV, dtype=torch.bfloat16)
+    tok = torch.arange(2 * 4 * 130, device=DEV) % 50
+    leaf = [x[n].detach().requires_grad_(True) for n in (*NAMES, "s0")]
+
+    def loss(*a):
+        o, s = gated_delta_chunk(*a[:5], initial_state=a[5])
+        r = token_logprobs((o @ head).reshape(-1, 50), tok, top_k=2)
+        return r.logprob.mean() + 0.1 * r.entropy.mean() + s.square().mean()
+
+    a = step_inputs(3, 2, 1, 64, 5, torch.bfloat16)
+    states = [a["state"].clone() for _ in range(2)]
+    results = []
+    for i, wrap in enumerate((lambda f: f, lambda f: torch.compile(f, backend="aot_eager", fullgraph=True))):
+        got = wrap(loss)(*leaf)
+        with torch.no_grad():
+            o = wrap(lambda *t: gated_delta_step(*t) * 2)(*(a[n] for n in NAMES), states[i])
+        results.append((got.detach(), *torch.autograd.grad(got, leaf), o, states[i]))
+    assert all(torch.equal(u, v) for u, v in zip(*results))
 
 
 # ------------------------------------------------------------------- step --
