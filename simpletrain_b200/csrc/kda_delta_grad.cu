@@ -508,6 +508,9 @@ using kda::delta::Args;
 
 bool gate_ok(int32_t d) { return d == KDA_DTYPE_BF16 || d == KDA_DTYPE_F16 || d == KDA_DTYPE_F32; }
 
+// Most chunks of a packed row: one more than the whole ones for each sequence that has a token.
+int packed_chunks(const kda_delta_params *p) { return p->T / 64 + (p->nseq < p->T ? p->nseq : p->T); }
+
 int check_sizes(const kda_delta_params *p) {
   if (p == nullptr) return KDA_ERR_NULL_ARGUMENT;
   if (p->B < 0 || p->H < 0 || p->Hk < 0 || p->T < 0) return KDA_ERR_BAD_SHAPE;
@@ -521,7 +524,7 @@ int check_sizes(const kda_delta_params *p) {
   if (p->H > 65535) return KDA_ERR_BAD_SHAPE;  // a grid dimension
   const int64_t nseq = p->cu_seqlens != nullptr ? (int64_t)p->nseq + 1 : p->B;
   if (nseq * p->H * 2 > 0x7fffffff) return KDA_ERR_BAD_SHAPE;
-  const int64_t chunks = p->cu_seqlens != nullptr ? (int64_t)p->T / 64 + p->nseq : (int64_t)p->B * (((int64_t)p->T + 63) / 64);
+  const int64_t chunks = p->cu_seqlens != nullptr ? packed_chunks(p) : (int64_t)p->B * (((int64_t)p->T + 63) / 64);
   if (chunks * p->H > 0x3fffffff) return KDA_ERR_BAD_SHAPE;
   return KDA_OK;
 }
@@ -551,7 +554,7 @@ size_t lay_out(const kda_delta_params *p, bool backward, Args *a) {
   const bool packed = p->cu_seqlens != nullptr;
   a->nseq = packed ? p->nseq : p->B;
   a->per_seq = packed ? 0 : (int)(((int64_t)p->T + 63) / 64);
-  a->max_chunks = packed ? p->T / 64 + p->nseq : p->B * a->per_seq;
+  a->max_chunks = packed ? packed_chunks(p) : p->B * a->per_seq;
   const size_t cells = (size_t)a->max_chunks * p->H;
   char *base = static_cast<char *>(p->workspace);
   size_t at = 0;

@@ -152,11 +152,22 @@ def test_packed_sequences(lens, lead, tail, H, Hk, D, dtype, index):
     ([128] + [0] * 31, 8, 8, 64, torch.bfloat16),  # offsets padded with empty sequences, as a captured graph has them
     ([0] * 15 + [200], 10, 5, 128, torch.float16),
     ([0] * 9 + [129, 0, 0, 70] + [0] * 30, 6, 3, 64, torch.bfloat16),
+    ([1, 0, 0, 2, 0] * 3 + [0] * 185, 2, 1, 64, torch.bfloat16),  # more sequences than tokens
 ])
 def test_packed_with_fewer_chunks_than_ranges(lens, H, Hk, D, dtype):
     cu, bounds, T = packed(lens)
     x = make(1, H, Hk, T, D, dtype, torch.float32, seed=13, state=True, n=len(lens))
     compare(*run_both(x, D, cu, bounds))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_row_without_tokens(dtype):
+    from simpletrain_b200 import gated_delta_chunk
+    x = make(1, 2, 2, 0, 64, dtype, torch.float32, state=True, n=5)
+    leaf = [x[n].detach().requires_grad_(True) for n in (*NAMES, "s0")]
+    o, s = gated_delta_chunk(*leaf[:5], initial_state=leaf[5], cu_seqlens=torch.zeros(6, dtype=torch.int32, device=DEV))
+    assert o.shape == (1, 2, 0, 64) and torch.equal(s, x["s0"])
+    assert torch.equal(torch.autograd.grad(s, leaf[5], x["dsT"])[0], x["dsT"])
 
 
 def test_packed_rows_equal_their_own_calls():

@@ -178,6 +178,16 @@ def test_delta_workspace_sizes():
     assert lib.kda_delta_fwd_workspace_bytes(ctypes.byref(delta_params(D=96))) == 0
 
 
+def test_workspace_of_padded_offsets():
+    """Sequences beyond the tokens are empty: they need an offset each, no chunks."""
+    lib = _ffi.load()
+    for size in (lib.kda_delta_fwd_workspace_bytes, lib.kda_delta_bwd_workspace_bytes):
+        few, many = (size(ctypes.byref(delta_params(H=8, Hk=8, cu_seqlens=0x10000, nseq=n))) for n in (64, 50000))
+        assert 0 < few < many <= few + 2 * 4 * 50000 + 148 * 2 * 64 * 64 * 4 + 65536
+    p = delta_params(H=8, Hk=8, cu_seqlens=0x10000, nseq=100000000)
+    assert lib.kda_delta_fwd_workspace_bytes(ctypes.byref(p)) > 0
+
+
 def step_params(**kw):
     p = _ffi.KdaDeltaStepParams()
     p.N, p.H, p.Hk, p.D, p.num_states, p.scale = 2, 2, 1, 64, 4, 1.0
