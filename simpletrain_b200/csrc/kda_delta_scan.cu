@@ -404,7 +404,7 @@ constexpr int kOutWarp = 8, kLoadWarp = 12, kMmaWarp = 13, kSizeWarp = 14;  // t
 // Per-token factors of a chunk, one array a factor: beta, -beta e^gamma, e^{gamma_63 - gamma}, scale e^gamma.
 struct Factors {
   float beta[64], bg[64], w[64], sg[64];
-  float last[4];  // e^{gamma_63}
+  float last[4];  // e^{gamma_63}; fp16's reverse scan: the power of two that is taken out of it and of bg and sg
   float4 unit;    // fp16: the preparation's four sizes
 };
 
@@ -673,7 +673,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
             wait(bars.unit_ready[st], (it >> 1) & 1);
             unit = units[st][0];
             held = fminf(worth * unit, 0x1p126f);  // beyond that nothing is left of what is held
-            worth = units[st][1];
+            worth = REV ? units[st][1] * fac[st].last[1] : units[st][1];
           }
 #pragma unroll
           for (int c0 = 0; c0 < W; c0 += 32) {
@@ -1005,16 +1005,26 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
         }
       }
       if constexpr (BF) fetch();
+      // All that the reverse scan hands on has a factor e^gamma of its token, at most the first one's (g <= 0): fp16
+      // takes its power of two out before it splits, and back in with the unit.
+      float out = 1.f, rest = 1.f;
+      if constexpr (REV && !BF) {
+        const float most = ex2f(fminf(__shfl_sync(0xffffffffu, gh[0], 0), 0.f));
+        rest = __uint_as_float(max(__float_as_uint(most) >> 23, 67u) << 23);  // 2^-60 at least
+        out = __uint_as_float((254u << 23) - __float_as_uint(rest));
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float G = ex2f(gh[i]);
+        float G = ex2f(gh[i]);
+        if constexpr (REV && !BF) G *= out;
         fac[st].beta[lane + 32 * i] = be[i];
         fac[st].bg[lane + 32 * i] = -be[i] * G;
         fac[st].w[lane + 32 * i] = decay(lh, ll, gh[i], gl[i]);
         fac[st].sg[lane + 32 * i] = a.p.scale * G;
       }
       if (lane == 0) {
-        fac[st].last[0] = ex2f(lh);
+        fac[st].last[0] = REV && !BF ? ex2f(lh) * out : ex2f(lh);
+        if constexpr (REV && !BF) fac[st].last[1] = rest;
         if constexpr (!BF) fac[st].unit = unit;
       }
       mbar_arrive(bar);
@@ -1096,7 +1106,7 @@ __device__ __forceinline__ void scan_cta(const Args &a, const Maps &maps, int bl
           const float bound = __uint_as_float(left) + 2.f * __uint_as_float(grown);
           units[st][0] = unit_of(max(abs_bits(bound), abs_bits(inputs)), &worth);
           units[st][1] = worth;
-          if (REV) units[st][2] = 64.f * fabsf(a.p.scale) * x * q;
+          if (REV) units[st][2] = 128.f * fabsf(a.p.scale) * x * q * fac[st].last[1];
           mbar_arrive(smem_u32(&bars.unit_ready[st]));
         }
         __syncwarp();

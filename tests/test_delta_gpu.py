@@ -379,6 +379,18 @@ def test_sizes_that_change_along_a_sequence(dtype):
         compare_sized(part(got), part(exp))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("g", [-8.0, -20.0, -30.0])
+def test_gradients_behind_strong_decays(g, dtype):
+    """What a strong decay leaves of a state's gradient keeps its bits, however little it is.  (A chunk's first
+    token has the strong gate, all of them, or the second chunk's first.)"""
+    for pick in (slice(0, 1), slice(None), slice(64, 65)):
+        x = make(1, 2, 1, 150, 64, dtype, torch.float32, seed=25, state=True)
+        x["g"][:, :, pick] = g
+        got, exp = run_both(x, 64)
+        compare_sized([*got[:5], *got[6:]], [*exp[:5], *exp[6:]])
+
+
 def test_a_scale_far_from_the_default():
     for scale in (1e-4, 50.0):
         x = make(1, 2, 2, 150, 64, torch.float16, torch.float32, seed=16, state=True)
