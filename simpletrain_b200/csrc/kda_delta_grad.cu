@@ -10,11 +10,12 @@
 //   dK = M K + M^T K + N^T Q - G beta (dX S^T) + w (U dS^T)
 //   dbeta_i = dX_i.v_i - G_i t_i - sum_j (dX U^T)_ij e_ij k_i.k_j,   t_i = k_i.(dX S^T)_i
 // The gradient of gamma_i, row by row, is what those terms give through their e^gamma
-// factors; with y_i = w_i k_i.(U dS^T)_i,
-//   dgamma_i = q_i.dq_i + k_i.(M K)_i - k_i.(M^T K + N^T Q)_i - G_i beta_i t_i
+// factors; with y_i = w_i k_i.(U dS^T)_i and Z_ij = M_ij k_i.k_j + N_ij q_i.k_j (i > j),
+//   dgamma_i = scale G_i q_i.(dO S^T)_i - G_i beta_i t_i + sum_j Z_ij - sum_j Z_ji
 //   dg_t = sum_{i >= t} dgamma_i + sum_{j < t} y_j + e^{gamma_63} <S, dS>
-// (the y_j enter dgamma_j with a minus and dgamma_63 with a plus; summed this way nothing
-// cancels).
+// (the y_j enter dgamma_j with a minus and dgamma_63 with a plus; they do not cancel summed this way).  Z's
+// sums are taken of its elements and not from the rows of the products: those hold the diagonal's N_ii q_i.k_i in
+// both, which has no decay, and what is left of it after the difference was 5e-7 whatever dg is (7% of it at g = -12).
 //
 // A CTA takes (chunk, query/key head) cells in turn, walks the value heads that share the
 // head and sums their dq and dk in registers, in order: no atomics, the result does not
@@ -228,7 +229,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
       float mn[BF ? 1 : 2][8];  // fp16: M, N until their unit is known
       uint32_t size = 0;
       const float y_unit = BF ? 1.f : worth_row();
-      float rs = 0.f;  // sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus
+      float held[2];   // Z's column sums over this warp's rows: the even warps' go to sm_f, then the odd ones'
+      float rs = 0.f;  // k rows: sum_j (dX U^T)_ij e_ij k_i.k_j, with a minus; q rows: Z's part
       {
         const float gh = gam[r64], gl = gam[64 + r64];
 #pragma unroll
@@ -237,7 +239,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           tmem_ld_32x32b_x8_nowait(lane_t + tG1 + 16 * part + 8 * c, xr);
           tmem_ld_32x32b_x8_nowait(lane_t + tG2 + 16 * part + 8 * c, yr);
           tmem_wait_ld_bind(xr, yr);
-          float m8[8];
+          float m8[8], z[8];
 #pragma unroll
           for (int j4 = 0; j4 < 8; j4 += 4) {
             const float4 ch4 = *reinterpret_cast<const float4 *>(gam + 16 * part + 8 * c + j4);
@@ -251,10 +253,29 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
                 const float m = col < r64 ? -y * e : 0.f;
                 rs = col < r64 ? fmaf(m, __uint_as_float(xr[j]), rs) : rs;
                 m8[j] = m * bi;
+                z[j] = m8[j] * __uint_as_float(xr[j]);
               } else {
                 m8[j] = col <= r64 ? a.p.scale * y * e : 0.f;
+                z[j] = col < r64 ? m8[j] * __uint_as_float(xr[j]) : 0.f;
+                rs += z[j];
               }
             }
+          }
+          {  // eight columns over the warp's 32 rows: half of them go to the other half of the lanes, three times over
+            const int lane = tid & 31;
+#pragma unroll
+            for (int n = 4; n > 0; n >>= 1) {
+              const bool hi = lane & (4 * n);
+#pragma unroll
+              for (int j = 0; j < n; ++j) {
+                const float keep = hi ? z[j + n] : z[j], give = hi ? z[j] : z[j + n];
+                z[j] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * n);
+              }
+            }
+            z[0] += __shfl_xor_sync(0xffffffffu, z[0], 2);
+            z[0] += __shfl_xor_sync(0xffffffffu, z[0], 1);
+            if ((row & 32) == 0 && (lane & 3) == 0) sm_f[row >> 6][16 * part + 8 * c + (lane >> 2)] = -z[0];
+            held[c] = z[0];
           }
           if constexpr (BF) {
             split8<BF>(m8, mh[c], ml[c]);
@@ -289,6 +310,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           prefetch_l2(a.w.dS + nx * (size_t)(D * D * 4), D * D * 4);
         }
       }
+      if ((row & 32) && (tid & 3) == 0)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) sm_f[row >> 6][16 * part + 8 * c + ((tid & 31) >> 2)] -= held[c];
       float iMN = 1.f;
       if constexpr (!BF) {
         size = 0;
@@ -343,7 +367,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
             acc[8 * c + j] = fmaf(f, x[8 * c + j], acc[8 * c + j]);
           }
         }
-        f_dot = f * t_dot;
+        f_dot = f * t_dot + (upper ? rs : bi * rs);
         if constexpr (!BF) t_dot *= worth_row();
       }
       mbar_wait(smem_u32(&bar_d), ph, a.p.status, &ctl.abort);
@@ -366,7 +390,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
         load_head(cidx, h + 1, b, t0, rows);
       else if (more)
         load_head(un / a.p.Hk, (un % a.p.Hk) * G_, nb, nt, nrows);
-      float wi = decay(gam[63], gam[127], gam[r64], gam[64 + r64]), c_dot = 0.f;
+      float wi = decay(gam[63], gam[127], gam[r64], gam[64 + r64]);
       if constexpr (!BF) wi *= worth_F() * worth_R();
 #pragma unroll
       for (int c0 = 0; c0 < W; c0 += 16) {
@@ -384,29 +408,25 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const Args a) {
           for (int j = 0; j < 8; ++j) {
             const int i = 8 * c + j;
             if constexpr (!BF) {
-              const float s = upper ? x[i] : x[i] + y[i], d = upper ? x[i] : x[i] - y[i], v = upper ? 0.f : wi * z[i];
-              c_dot = fmaf(k[j], d, c_dot);
+              const float s = upper ? x[i] : x[i] + y[i], v = upper ? 0.f : wi * z[i];
               y_dot = fmaf(k[j], v, y_dot);
               acc[c0 + i] += fmaf(iMN, s, v);
             } else if (upper) {
-              f_dot = fmaf(k[j], x[i], f_dot);
               acc[c0 + i] += x[i];
             } else {
               const float v = wi * z[i];
-              f_dot = fmaf(k[j], x[i] - y[i], f_dot);  // k.(M K) - k.(M^T K + N^T Q)
               y_dot = fmaf(k[j], v, y_dot);
               acc[c0 + i] += (x[i] + y[i]) + v;
             }
           }
         }
       }
-      if constexpr (!BF) f_dot = fmaf(iMN, c_dot, f_dot);
       // the rows' sums, in a fixed order: the quarters of k rows, then those of q rows
       for (int turn = 0; turn < 2; ++turn) {
         if (!upper && (part >> 1) == turn) {
           const int p = part & 1;
           const float z = 0.f;
-          sm_f[p][r64] = (turn ? sm_f[p][r64] : z) + f_dot;
+          sm_f[p][r64] += f_dot;
           sm_t[p][r64] = (turn ? sm_t[p][r64] : z) + t_dot;
           sm_y[p][r64] = (turn ? sm_y[p][r64] : z) + y_dot;
           sm_r[p][r64] = (turn ? sm_r[p][r64] : z) + rs;
