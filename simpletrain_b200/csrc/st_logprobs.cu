@@ -218,9 +218,10 @@ __device__ __forceinline__ void raise(Stat &t, float m) {
 }
 
 __device__ __forceinline__ void add1(Stat &t, float x, float c) {
-  const float y = c * floor1(x);
+  x = floor1(x);
+  const float y = c * x;
   if (y > t.m) raise(t, y);
-  const float d = y - t.m, e = ex2(d);
+  const float d = fmaf(x, c, -t.m), e = ex2(d);  // (y - t.m would be off by y's rounding, as much as the exponents that count)
   t.s += e;
   t.w = fmaf(e, fmaxf(d, kFloor), t.w);
 }

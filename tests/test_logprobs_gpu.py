@@ -128,6 +128,23 @@ def test_gradients_where_the_rows_sum_is_large(dtype, t, offset):
     assert (dx.double().sum(-1).abs() <= 2.0 ** -15 * a.abs().double() / t).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [3, 13, 33])
+@pytest.mark.parametrize("t,offset", [(1e-2, 0.0), (1e-3, 100.0), (0.05, -1e4)])
+def test_short_odd_rows_where_the_rows_sum_is_large(dtype, V, t, offset):
+    """What lies before and behind a row's 16-byte vectors goes into the sums as exactly as the vectors do."""
+    x, tok, a, b = make(64, V, dtype, seed=10, spread=max(3.0 * t, 1e-3))
+    x = (x.float() + offset).to(dtype)
+    ref = x.double()
+    lp, H = logprobs(ref, tok, t)
+    from simpletrain_b200.fused_ops import token_logprobs
+    r = token_logprobs(x, tok, temperature=t, top_k=3)
+    top = torch.log_softmax(ref / t, -1).gather(1, r.top_ids)
+    assert (r.logprob.double() - lp).abs().max() <= ABS * max(1.0, lp.abs().max().item() / 32)
+    assert (r.entropy.double() - H).abs().max() <= ABS
+    assert (r.top_logprobs.double() - top).abs().max() <= ABS * max(1.0, top.abs().max().item() / 32)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("t", [0.5, 1.0, 2.0, 100.0])
 def test_a_masked_logit_has_probability_0_at_every_temperature(dtype, t):
