@@ -23,11 +23,12 @@
 // next head's are brought into L2 meanwhile; 16 warps, a token row and a quarter of the
 // columns a thread, work off the products.
 //
-// Measured: 450 us for 16 x 2048 tokens, 10 heads of 128 (5120 cells of 288 KB: 3.4 TB/s, 25,000
+// Measured: 466 us for 16 x 2048 tokens, 10 heads of 128 (5120 cells of 288 KB: 3.3 TB/s, 26,000
 // cycles a cell).  One value head's tiles are all that fit, so copies, products and what the threads make of them
 // follow one another; what can overlap does (prefetch into L2, terms through the state under
 // the second products).  Holding k and q rows in registers to free room for the next tiles spilled (514 us).
-// In fp16, where M and N wait for their unit, 535 us.
+// In fp16, where M and N wait for their unit, 569 us.  Z's column sums, 18 shuffles a thread, are 16 us of it; all sixteen
+// columns at once took registers that are not there (478 us).
 #include "kda_delta_tc.cuh"
 
 namespace kda {

@@ -393,7 +393,7 @@ __device__ void zero_outside(const Args &a, void *p, int dtype, int h) {
 // under the end of the one before is in that).  dO becomes an operand in the chain's wait for its
 // product with T: in the output warps that took 2000 to 3000 cycles a chunk and made them the slowest.
 // fp16's units cost a chunk 1000 cycles of the chain (its maximum as the state is converted, the wait for
-// the unit): 28 streams of 32768 tokens 1.55 ms, and 172, 174 and 297 us in place of 118, 148 and 199.
+// the unit): 28 streams of 32768 tokens 1.57 ms, and 171, 174 and 305 us in place of 118, 148 and 199.
 // With the sizes found by the chain itself (the state read twice, a barrier) the former took 1.63 ms.
 enum { kOut = 0, kStore = 1, kRev = 2 };  // outputs; state and u rows for the backward; reverse scan
 
